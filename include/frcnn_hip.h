@@ -404,6 +404,71 @@ int frcnn_flip_images(const float* images, const uint8_t* flip, uint64_t seed, i
 int frcnn_fc1_fwd(const float* x, const float* w, const float* bias, int64_t M, int K, int N,
                   int relu, float* out, frcnn_stream_t stream);
 
+/* ---- the head's dense layers on 16-bit inputs, with their gradients ------------------------------
+ * The layers behind the RoI pool (Faster_RCNN/module/model.py:31-38) in float16 / bfloat16:
+ *     pre[M,N] = x[M,K] W[K,N] + bias;    out = act(pre) + residual
+ * Products are exact, sums are float32 (a reduction split over workgroups is joined in a fixed order:
+ * the same call gives the same bits), every output is rounded once.
+ *   dtype      FRCNN_DT_F16 / FRCNN_DT_BF16: x, W, bias, residual, pre and the gradients;
+ *   w_layout   FRCNN_W_KN: W is [K,N] rows of ldw >= N elements (a Keras kernel),
+ *              FRCNN_W_NK: W is stored as [N,K] rows of ldw >= K elements (a torch Linear weight);
+ *   out_dtype  dtype or FRCNN_DT_F32;   d_dtype likewise for d_out;
+ *   ld*        elements between rows, at least the row's length; any alignment is taken (rows of
+ *              16-byte aligned whole 16-byte pieces are the fast layout);
+ *   bias, residual, pre may be NULL (pre: the pre-activations, rounded, which the backward needs
+ *              for an activation other than FRCNN_ACT_NONE).
+ * M = 0 is allowed (no forward output; d_w and d_bias become 0).
+ * Activations: ReLU max(z, 0); GELU z Phi(z), Phi the normal distribution function (relative error
+ * 1.3e-6); SiLU z / (1 + e^-z). */
+#define FRCNN_DT_F32   0
+#define FRCNN_DT_F16   1
+#define FRCNN_DT_BF16  2
+#define FRCNN_ACT_NONE 0
+#define FRCNN_ACT_RELU 1
+#define FRCNN_ACT_GELU 2
+#define FRCNN_ACT_SILU 3
+#define FRCNN_W_KN     0
+#define FRCNN_W_NK     1
+size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N);
+int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int w_layout,
+                    const void* bias, const void* residual, int64_t ldr, int64_t M, int K, int N,
+                    int dtype, int act, void* out, int64_t ldo, int out_dtype, void* pre,
+                    int64_t ldp, void* workspace, size_t workspace_bytes, frcnn_stream_t stream);
+
+/* dz = d_out * act'(pre) (float32, rounded to dtype for the products; the ReLU's is d_out where
+ * pre > 0, else 0);  d_x = dz W^T,  d_w = x^T dz in W's layout,  d_bias = sum of dz over the rows
+ * (of the unrounded float32 values).  d_x, d_w, d_bias: NULL where not wanted, not all three.  The
+ * residual's gradient is d_out itself. */
+size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N);
+int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, const void* x, int64_t ldx,
+                    const void* w, int64_t ldw, int w_layout, const void* pre, int64_t ldp,
+                    int64_t M, int K, int N, int dtype, int act, void* d_x, int64_t lddx,
+                    void* d_w, int64_t lddw, void* d_bias, void* workspace,
+                    size_t workspace_bytes, frcnn_stream_t stream);
+
+/* ---- distillation of the class logits from a teacher's stored top logits --------------------------
+ * No counterpart in the reference; stands beside frcnn_head_loss for a head that learns from a
+ * larger one.  Row r: student logits z [V], teacher logits t_j at labels i_j, j < k (k <= 1,024).
+ * An entry whose label is outside [0,V) (padding: -1) or whose logit is -inf is not there.
+ *     p = softmax(t / T) over the entries that are there, q = softmax(z / T) over all V
+ *     loss = weight T^2 sum_j p_j (log p_j - log q_(i_j))
+ *     d_logits_v = g weight T (q_v - sum_j p_j [i_j = v])
+ * A label listed more than once counts each time.  A row with weight 0 or without an entry takes
+ * no part: loss, lse and gradient 0, its logits (also NaN) are not read.  A student logit of -inf
+ * has q = 0: the loss is +inf where the teacher gives that label weight; a row of -inf alone is NaN.
+ *   dtype   of logits and d_logits: F32, F16 or BF16; t_dtype of top_values: dtype or F32;
+ *   weight  [rows] or NULL (1);  loss, lse [rows] f32, lse = log sum_v e^(z_v / T) for the backward;
+ *   frcnn_distill_loss: d_logits may be NULL, g = grad_scale; frcnn_distill_bwd: g = d_loss [rows].
+ * d_logits must not overlap logits. */
+int frcnn_distill_loss(const void* logits, int64_t ldz, int dtype, const void* top_values,
+                       int t_dtype, const int64_t* top_index, const float* weight, int64_t rows,
+                       int V, int k, float temperature, float grad_scale, float* loss, float* lse,
+                       void* d_logits, int64_t ldg, frcnn_stream_t stream);
+int frcnn_distill_bwd(const float* d_loss, const void* logits, int64_t ldz, int dtype,
+                      const void* top_values, int t_dtype, const int64_t* top_index,
+                      const float* lse, const float* weight, int64_t rows, int V, int k,
+                      float temperature, void* d_logits, int64_t ldg, frcnn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,10 @@ E_BADARG, E_WORKSPACE, E_LAUNCH, E_UNSUPPORTED, E_STATIC_LIMIT = -1, -2, -3, -4,
 NMS_STATIC_BYTES = 16 << 20
 F_VALID, F_POSITIVE, F_NEGATIVE = 1, 2, 4
 S_OK, S_SHORT_BATCH = 0, 1
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
+W_KN, W_NK = 0, 1
+DISTILL_MAX_K = 1024
 
 
 class FrcnnError(RuntimeError):
@@ -79,6 +83,16 @@ _SIGS = {
     "frcnn_pad_gt": (_i, [_p, _p, _p, _p, _i, _u64, _i, _i, _i, _p, _p, _p, _p]),
     "frcnn_flip_images": (_i, [_p, _p, _u64, _i, _i, _i, _i, _i, _p, _p]),
     "frcnn_fc1_fwd": (_i, [_p, _p, _p, _i64, _i, _i, _i, _p, _p]),
+    "frcnn_dense_fwd_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "frcnn_dense_fwd": (_i, [_p, _i64, _p, _i64, _i, _p, _p, _i64, _i64, _i, _i, _i, _i, _p, _i64,
+                             _i, _p, _i64, _p, _sz, _p]),
+    "frcnn_dense_bwd_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "frcnn_dense_bwd": (_i, [_p, _i64, _i, _p, _i64, _p, _i64, _i, _p, _i64, _i64, _i, _i, _i, _i,
+                             _p, _i64, _p, _i64, _p, _p, _sz, _p]),
+    "frcnn_distill_loss": (_i, [_p, _i64, _i, _p, _i, _p, _p, _i64, _i, _i, _f, _f, _p, _p, _p,
+                                _i64, _p]),
+    "frcnn_distill_bwd": (_i, [_p, _p, _i64, _i, _p, _i, _p, _p, _p, _i64, _i, _i, _f, _p, _i64,
+                               _p]),
 }
 
 for _name, (_res, _args) in _SIGS.items():

@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
+from ..capture import guard_leaves
 
 
 class Loss_bbr:
@@ -47,3 +48,39 @@ def frcn_losses(pred_obj, pred_reg, label, gt_mask, gt_coord, tindex, want_grad=
     out = ops.head_loss(pred_obj, pred_reg, tindex, label, gt_mask, gt_coord, want_grad)
     d_reg = out["d_reg"].reshape(pred_reg.shape) if want_grad else None
     return out["loss"][0], out["loss"][1], out["loss"][2], out["d_cls"], d_reg
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_values, top_index, weight, temperature):
+        out = ops.distill_loss(logits, top_values, top_index, weight, temperature, want_grad=False)
+        ctx.save_for_backward(logits, top_values, top_index, weight, out["lse"])
+        ctx.temperature = temperature
+        return out["loss"]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss):
+        logits, top_values, top_index, weight, lse = ctx.saved_tensors
+        return ops.distill_bwd(grad_loss, logits, top_values, top_index, lse, weight,
+                               ctx.temperature), None, None, None, None
+
+
+def distill_loss(logits, top_values, top_index, weight=None, temperature: float = 1.0):
+    """Differentiable distillation loss per row: weight T^2 KL(p || q) with p the softmax of the
+    teacher's stored top logits and q the student's over all its classes, both at temperature T.
+    logits [...,V]; top_values / top_index [...,k] (label -1: no entry); weight [...] or None.
+    The teacher's side gets no gradient."""
+    held = guard_leaves(logits)
+    out = _Distill.apply(logits, top_values, top_index, weight, float(temperature))
+    del held
+    return out
+
+
+def distill_losses(logits, top_values, top_index, weight=None, temperature: float = 1.0,
+                   want_grad=True):
+    """The same as one call in the manner of frcn_losses: (mean loss over the rows, d_logits), the
+    gradient of that mean computed in the pass that computes the loss."""
+    rows = max(1, logits[..., 0].numel())
+    out = ops.distill_loss(logits, top_values, top_index, weight, temperature, want_grad, 1.0 / rows)
+    return out["loss"].sum() / rows, out["d_logits"]

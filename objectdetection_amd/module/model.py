@@ -7,6 +7,7 @@ from typing import Optional
 import torch
 
 from .. import ops
+from ..capture import guard_leaves
 from ..config import PathConfig, REFERENCE
 
 
@@ -113,3 +114,45 @@ def fc1(pooled: torch.Tensor, kernel: torch.Tensor, bias: Optional[torch.Tensor]
     its (h,w,c)-flattened row already, so Flatten is a view.  kernel [7*7*C, units] and bias
     [units] in the Keras layout.  Returns [B,R,units] float32, computed by frcnn_fc1_fwd."""
     return ops.fc1_fwd(pooled, kernel, bias, relu)
+
+
+class _Dense(torch.autograd.Function):
+    """act(x W + b) + residual whose gradients are frcnn_dense_bwd's; the residual's is the
+    upstream gradient itself."""
+
+    @staticmethod
+    def forward(ctx, x, kernel, bias, residual, act, out_dtype):
+        need_pre = act != "none" and any(ctx.needs_input_grad[:3])
+        got = ops.dense_fwd(x, kernel, bias, act, residual, out_dtype=out_dtype, want_pre=need_pre)
+        out, pre = got if need_pre else (got, None)
+        ctx.save_for_backward(x, kernel, pre)
+        ctx.act = act
+        ctx.residual_dtype = None if residual is None else residual.dtype
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        x, kernel, pre = ctx.saved_tensors
+        dx, dw, db, dr = ctx.needs_input_grad[:4]
+        g = dict(d_x=None, d_weight=None, d_bias=None)
+        if dx or dw or db:
+            g = ops.dense_bwd(grad_out, x, kernel, pre, ctx.act, dx, dw, db)
+        return (g["d_x"], g["d_weight"], g["d_bias"],
+                grad_out.to(ctx.residual_dtype) if dr else None, None, None)
+
+
+def dense(x: torch.Tensor, kernel: torch.Tensor, bias: Optional[torch.Tensor] = None,
+          activation: str = "none", residual: Optional[torch.Tensor] = None,
+          out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """A dense layer of the head (module/model.py:32-38) in float16 / bfloat16, with gradients:
+    activation(x @ kernel + bias) + residual, one fused product (frcnn_dense_fwd / _bwd).
+
+    x [..., K] or the pooled tensor [B,R,7,7,C]; kernel [K, units] in the Keras layout, or a
+    Linear module's weight as `weight.t()` (read as it lies); activation "none", "relu", "gelu",
+    "silu"; out_dtype float32 for class logits.  fc1 is the float32 layer.  Under graph capture no
+    autograd graph of the same leaves that was built on another stream may be alive (refused)."""
+    held = guard_leaves(x, kernel, bias, residual)
+    out = _Dense.apply(x, kernel, bias, residual, activation, out_dtype)
+    del held
+    return out

@@ -5,7 +5,9 @@ computation happens in libfrcnn_hip.so.  Tensors must live on a ROCm device.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
+import math
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -17,6 +19,8 @@ __all__ = [
     "anchors", "iou_assign", "rpn_sample", "encode", "decode_clip", "topk", "nms",
     "nms_workspace_bytes", "roi_crop_pool_fwd", "roi_crop_pool_bwd", "label_proposals",
     "sample_proposals", "detect_postprocess", "fc1_fwd",
+    "dense_fwd", "dense_bwd", "dense_fwd_workspace_bytes", "dense_bwd_workspace_bytes",
+    "distill_loss", "distill_bwd",
 ]
 
 
@@ -551,3 +555,285 @@ def fc1_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] 
         check("frcnn_fc1_fwd", lib.frcnn_fc1_fwd(_ptr(xx), _ptr(w), _ptr(b), M, K, N, int(bool(relu)),
                                                  _ptr(out), _stream(xx)))
     return out.view(*lead, N)
+
+
+# ---- dense layers on 16-bit inputs, distillation ------------------------------------------------
+ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
+               "silu": _lib.ACT_SILU}
+_DT = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
+_DT16 = (torch.float16, torch.bfloat16)
+
+
+def _raw_stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _on(dev: torch.device):
+    """A guard that makes `dev` current (nothing to do when it is: the usual call)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _same_dev(t: torch.Tensor, dev: torch.device, name: str) -> None:
+    if t.device != dev:
+        raise RuntimeError(f"{name}: on {t.device}, the other tensors are on {dev} "
+                           "(the HIP kernels are the only path)")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[n,m] with unit column stride and rows that do not overlap; a copy only where it is not."""
+    n, m = t.shape
+    if (t.stride(1) == 1 or m == 1) and (t.stride(0) >= m or n <= 1):
+        return t
+    return t.contiguous()
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _dense_x(x: torch.Tensor, name: str):
+    """x [..., K] (the pooled tensor [B,R,ph,pw,C] as [B,R,ph*pw*C]) -> (rows [M,K], leading dims)."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor")
+    if not x.is_cuda:
+        raise RuntimeError(f"{name}: must be on a ROCm device (the HIP kernels are the only path)")
+    if x.dtype not in _DT16:
+        raise TypeError(f"{name}: expected torch.float16 or torch.bfloat16, got {x.dtype}"
+                        " (fc1_fwd is the float32 layer)")
+    if x.dim() == 2:
+        return _rows(x), x.shape[:1]
+    if x.dim() == 5:
+        return _rows(x.reshape(x.shape[0] * x.shape[1], x.shape[2] * x.shape[3] * x.shape[4])), x.shape[:2]
+    if x.dim() < 1 or x.dim() == 0:
+        raise ValueError(f"{name}: needs at least one dimension")
+    return _rows(x.reshape(math.prod(x.shape[:-1]), x.shape[-1])), x.shape[:-1]
+
+
+def _dense_w(w: torch.Tensor, x: torch.Tensor, K: int):
+    """weight [K,N] -> (tensor, layout, row stride): rows of N (Keras) or, as the transposed view of
+    a Linear module's [N,K], rows of K; anything else is copied to rows of N."""
+    if not isinstance(w, torch.Tensor):
+        raise TypeError("weight: expected a torch.Tensor")
+    if w.dtype != x.dtype:
+        raise TypeError(f"weight: expected {x.dtype}, got {w.dtype}")
+    _same_dev(w, x.device, "weight")
+    if w.dim() != 2 or w.shape[1] == 0:
+        raise ValueError("weight must be [K,N]")
+    if w.shape[0] != K or K == 0:
+        raise ValueError(f"x has {K} features per row, weight expects {w.shape[0]}")
+    N = w.shape[1]
+    s0, s1 = w.stride()
+    if s1 == 1 and s0 >= N:
+        return w, _lib.W_KN, s0
+    if s0 == 1 and s1 >= K:
+        return w, _lib.W_NK, s1
+    w = w.contiguous()
+    return w, _lib.W_KN, N
+
+
+def _dense_rows(t: Optional[torch.Tensor], name: str, lead, M: int, N: int, dev, dtypes):
+    """A [..., N] operand with the call's leading dimensions -> rows [M,N]."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    _same_dev(t, dev, name)
+    if tuple(t.shape) != (*lead, N):
+        raise ValueError(f"{name} must be {[*lead, N]}, got {list(t.shape)}")
+    return _rows(t if t.dim() == 2 else t.reshape(M, N))
+
+
+def _act_code(act: str) -> int:
+    if act not in ACTIVATIONS:
+        raise ValueError(f"act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
+    return ACTIVATIONS[act]
+
+
+def _dense_out(out, name, shape2, lead, N, dtype, dev):
+    if out is None:
+        return torch.empty(shape2, dtype=dtype, device=dev)
+    if not isinstance(out, torch.Tensor) or out.dtype != dtype or not out.is_contiguous() \
+            or tuple(out.shape) != (*lead, N):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {[*lead, N]}")
+    _same_dev(out, dev, name)
+    return out.view(shape2)
+
+
+def _scratch(ws: Optional[torch.Tensor], need: int, dev) -> Optional[torch.Tensor]:
+    if need == 0:
+        return None
+    if ws is None:
+        return torch.empty(need, dtype=torch.uint8, device=dev)
+    _same_dev(_cont(ws, "workspace", torch.uint8), dev, "workspace")
+    if not ws.is_contiguous() or ws.numel() < need:
+        raise ValueError(f"workspace: {need} bytes are needed")
+    return ws
+
+
+def dense_fwd_workspace_bytes(M: int, K: int, N: int) -> int:
+    return int(lib.frcnn_dense_fwd_workspace_bytes(M, K, N))
+
+
+def dense_bwd_workspace_bytes(M: int, K: int, N: int) -> int:
+    return int(lib.frcnn_dense_bwd_workspace_bytes(M, K, N))
+
+
+def dense_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+              act: str = "none", residual: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+              want_pre: bool = False, workspace: Optional[torch.Tensor] = None):
+    """act(x @ weight + bias) + residual on float16 / bfloat16 (frcnn_dense_fwd).
+
+    x [..., K] (the pooled tensor [B,R,ph,pw,C] is taken as [B,R,ph*pw*C]); weight [K,N], rows of N
+    or the transposed view of a Linear weight [N,K] (both are read as they lie); bias [N]; residual
+    [..., N].  act: "none", "relu", "gelu" (exact), "silu".  out_dtype float32 keeps the sums (class
+    logits).  Returns out [..., N], with want_pre (out, pre): the pre-activations dense_bwd needs.
+    workspace: uint8 of dense_fwd_workspace_bytes(M, K, N), kept by callers that allocate nothing."""
+    xx, lead = _dense_x(x, "x")
+    M, K = xx.shape
+    dev, dt = xx.device, xx.dtype
+    w, layout, ldw = _dense_w(weight, xx, K)
+    N = w.shape[1]
+    code = _act_code(act)
+    if bias is not None:
+        if not isinstance(bias, torch.Tensor) or bias.dtype != dt:
+            raise TypeError(f"bias: expected a {dt} tensor")
+        _same_dev(bias, dev, "bias")
+        if tuple(bias.shape) != (N,):
+            raise ValueError(f"bias must be [{N}]")
+        bias = bias.contiguous()
+    res = None if residual is None else _dense_rows(residual, "residual", lead, M, N, dev, (dt,))
+    odt = dt if out_dtype is None else out_dtype
+    if odt not in (dt, torch.float32):
+        raise TypeError(f"out_dtype: expected {dt} or torch.float32, got {odt}")
+    o = _dense_out(out, "out", (M, N), lead, N, odt, dev)
+    pre = torch.empty((M, N), dtype=dt, device=dev) if want_pre else None
+    ws = _scratch(workspace, lib.frcnn_dense_fwd_workspace_bytes(M, K, N), dev)
+    with _on(dev):
+        check("frcnn_dense_fwd", lib.frcnn_dense_fwd(
+            xx.data_ptr(), _ld(xx), w.data_ptr(), ldw, layout, None if bias is None else bias.data_ptr(),
+            None if res is None else res.data_ptr(), 0 if res is None else _ld(res), M, K, N, _DT[dt], code,
+            o.data_ptr(), N, _DT[odt], None if pre is None else pre.data_ptr(), N,
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _raw_stream(dev)))
+    if len(lead) != 1:
+        o = o.view(*lead, N)
+        pre = None if pre is None else pre.view(*lead, N)
+    return (o, pre) if want_pre else o
+
+
+def dense_bwd(d_out: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+              pre: Optional[torch.Tensor] = None, act: str = "none", want_dx: bool = True,
+              want_dw: bool = True, want_db: bool = True,
+              workspace: Optional[torch.Tensor] = None):
+    """Gradients of dense_fwd (frcnn_dense_bwd): dict(d_x [..., K] of x's shape, d_weight [K,N] in
+    weight's memory layout, d_bias [N]); None where not wanted.  d_out [..., N] in x's type or
+    float32; pre as dense_fwd returned it (not needed for act "none").  The residual's gradient is
+    d_out itself.  workspace: uint8 of dense_bwd_workspace_bytes(M, K, N)."""
+    xx, lead = _dense_x(x, "x")
+    M, K = xx.shape
+    dev, dt = xx.device, xx.dtype
+    w, layout, ldw = _dense_w(weight, xx, K)
+    N = w.shape[1]
+    code = _act_code(act)
+    if not (want_dx or want_dw or want_db):
+        raise ValueError("nothing wanted: set want_dx, want_dw or want_db")
+    d = _dense_rows(d_out, "d_out", lead, M, N, dev, (dt, torch.float32))
+    z = None
+    if code != _lib.ACT_NONE:
+        if pre is None:
+            raise ValueError(f"pre: the forward's pre-activations are needed for act {act!r}")
+        z = _dense_rows(pre, "pre", lead, M, N, dev, (dt,))
+    d_x = torch.empty((M, K), dtype=dt, device=dev) if want_dx else None
+    d_w = torch.empty((K, N) if layout == _lib.W_KN else (N, K), dtype=dt, device=dev) if want_dw else None
+    d_b = torch.empty(N, dtype=dt, device=dev) if want_db else None
+    ws = _scratch(workspace, lib.frcnn_dense_bwd_workspace_bytes(M, K, N), dev)
+    with _on(dev):
+        check("frcnn_dense_bwd", lib.frcnn_dense_bwd(
+            d.data_ptr(), _ld(d), _DT[d.dtype], xx.data_ptr(), _ld(xx), w.data_ptr(), ldw, layout,
+            None if z is None else z.data_ptr(), 0 if z is None else _ld(z), M, K, N, _DT[dt], code,
+            None if d_x is None else d_x.data_ptr(), K, None if d_w is None else d_w.data_ptr(),
+            N if layout == _lib.W_KN else K, None if d_b is None else d_b.data_ptr(),
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _raw_stream(dev)))
+    if d_w is not None and layout == _lib.W_NK:
+        d_w = d_w.t()
+    return dict(d_x=None if d_x is None else d_x.view(x.shape), d_weight=d_w, d_bias=d_b)
+
+
+def _distill_args(logits, top_values, top_index, weight, temperature):
+    if not isinstance(logits, torch.Tensor):
+        raise TypeError("logits: expected a torch.Tensor")
+    if not logits.is_cuda:
+        raise RuntimeError("logits: must be on a ROCm device (the HIP kernels are the only path)")
+    if logits.dtype not in _DT:
+        raise TypeError(f"logits: expected float32, float16 or bfloat16, got {logits.dtype}")
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise ValueError("logits must be [..., V]")
+    lead, V, dev = logits.shape[:-1], logits.shape[-1], logits.device
+    rows = math.prod(lead)
+    if not isinstance(top_values, torch.Tensor) or top_values.dtype not in (logits.dtype, torch.float32):
+        raise TypeError(f"top_values: expected a tensor of {logits.dtype} or float32")
+    if not isinstance(top_index, torch.Tensor) or top_index.dtype != torch.int64:
+        raise TypeError("top_index: expected an int64 tensor")
+    k = top_values.shape[-1] if top_values.dim() else 0
+    if k == 0 or tuple(top_values.shape) != (*lead, k) or top_index.shape != top_values.shape:
+        raise ValueError(f"top_values and top_index must be {[*lead, 'k']}")
+    _same_dev(top_values, dev, "top_values")
+    _same_dev(top_index, dev, "top_index")
+    if weight is not None:
+        if not isinstance(weight, torch.Tensor) or weight.dtype != torch.float32:
+            raise TypeError("weight: expected a float32 tensor")
+        _same_dev(weight, dev, "weight")
+        if weight.shape != lead:
+            raise ValueError(f"weight must be {list(lead)}")
+        weight = weight.contiguous()
+    if not (0.0 < float(temperature) < 3.0e38):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    z = _rows(logits if logits.dim() == 2 else logits.reshape(rows, V))
+    return z, top_values.contiguous(), top_index.contiguous(), weight, lead, rows, V, k
+
+
+def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torch.Tensor,
+                 weight: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                 want_grad: bool = True, grad_scale: float = 1.0):
+    """Distillation from a teacher's stored top logits (frcnn_distill_loss).
+
+    logits [..., V] (float32, float16 or bfloat16), top_values [..., k] (the same type or float32)
+    and top_index [..., k] int64: the teacher's logits and their labels (-1, any label outside
+    [0,V) and a logit of -inf: no entry), weight [...] float32 or None (0: the row takes no part).
+    With p the teacher's softmax over its entries and q the student's over all V, both at
+    `temperature` T, returns dict(loss [...] = weight T^2 KL(p || q), lse [...], d_logits: the
+    gradient of grad_scale * loss.sum() in logits, None unless want_grad)."""
+    z, tv, ti, wt, lead, rows, V, k = _distill_args(logits, top_values, top_index, weight, temperature)
+    dev = z.device
+    loss = torch.empty(lead, dtype=torch.float32, device=dev)
+    lse = torch.empty(lead, dtype=torch.float32, device=dev)
+    grad = torch.empty(logits.shape, dtype=z.dtype, device=dev) if want_grad else None
+    with _on(dev):
+        check("frcnn_distill_loss", lib.frcnn_distill_loss(
+            z.data_ptr(), _ld(z), _DT[z.dtype], tv.data_ptr(), _DT[tv.dtype], ti.data_ptr(),
+            None if wt is None else wt.data_ptr(), rows, V, k, temperature, grad_scale, loss.data_ptr(),
+            lse.data_ptr(), None if grad is None else grad.data_ptr(), V, _raw_stream(dev)))
+    return dict(loss=loss, lse=lse, d_logits=grad)
+
+
+def distill_bwd(d_loss: torch.Tensor, logits: torch.Tensor, top_values: torch.Tensor,
+                top_index: torch.Tensor, lse: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                temperature: float = 1.0) -> torch.Tensor:
+    """Gradient of distill_loss in logits for upstream gradients d_loss [...] (frcnn_distill_bwd);
+    lse [...] as distill_loss returned it."""
+    z, tv, ti, wt, lead, rows, V, k = _distill_args(logits, top_values, top_index, weight, temperature)
+    dev = z.device
+    for t, name in ((d_loss, "d_loss"), (lse, "lse")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
+            raise TypeError(f"{name}: expected a float32 tensor")
+        _same_dev(t, dev, name)
+        if t.shape != lead:
+            raise ValueError(f"{name} must be {list(lead)}")
+    d_loss, lse = d_loss.contiguous(), lse.contiguous()
+    grad = torch.empty(logits.shape, dtype=z.dtype, device=dev)
+    with _on(dev):
+        check("frcnn_distill_bwd", lib.frcnn_distill_bwd(
+            d_loss.data_ptr(), z.data_ptr(), _ld(z), _DT[z.dtype], tv.data_ptr(), _DT[tv.dtype], ti.data_ptr(),
+            lse.data_ptr(), None if wt is None else wt.data_ptr(), rows, V, k, temperature, grad.data_ptr(), V,
+            _raw_stream(dev)))
+    return grad

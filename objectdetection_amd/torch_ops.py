@@ -3,8 +3,9 @@
 Registered with torch.library.custom_op: the dispatcher, fake tensors (shape propagation under
 torch.compile / torch.export / FakeTensorMode) and autograd see the kernels as operators, while
 the implementation stays the C ABI of libfrcnn_hip.so (through `ops.py`).  The fused RoI crop +
-max-pool carries its adjoint (frcnn_roi_crop_pool_bwd) as the registered autograd formula; every
-other operator produces indices, labels or targets and has no gradient, like the TensorFlow ops
+max-pool carries its adjoint (frcnn_roi_crop_pool_bwd) as the registered autograd formula, the
+dense layer and the distillation loss carry frcnn_dense_bwd and frcnn_distill_bwd; every other
+operator produces indices, labels or targets and has no gradient, like the TensorFlow ops
 it replaces (tf.math.top_k indices, combined_non_max_suppression, tf.where ...).
 
 OP_ENTRY_POINTS maps each operator to the entry points of include/frcnn_hip.h it calls;
@@ -41,11 +42,16 @@ OP_ENTRY_POINTS = {
     "pad_gt": ("frcnn_pad_gt",),
     "flip_images": ("frcnn_flip_images",),
     "fc1": ("frcnn_fc1_fwd",),
+    "dense": ("frcnn_dense_fwd",),
+    "dense_backward": ("frcnn_dense_bwd",),
+    "distill_loss": ("frcnn_distill_loss",),
+    "distill_loss_backward": ("frcnn_distill_bwd",),
 }
 HELPER_ENTRY_POINTS = (
     "frcnn_abi_version", "frcnn_status_string", "frcnn_set_tuning", "frcnn_get_tuning",
     "frcnn_topk_sort_workspace_bytes", "frcnn_nms_workspace_bytes", "frcnn_roi_fwd_workspace_bytes",
-    "frcnn_roi_fwd_plan", "frcnn_topk_sort_plan",
+    "frcnn_roi_fwd_plan", "frcnn_topk_sort_plan", "frcnn_dense_fwd_workspace_bytes",
+    "frcnn_dense_bwd_workspace_bytes",
     # stream-ordered halves / allocation-free variants used by RegionProposalPath and serving
     # loops directly; as operators they would be the ones above
     "frcnn_roi_fwd_prepare", "frcnn_roi_crop_pool_fwd_prepared", "frcnn_nms_static",
@@ -340,5 +346,103 @@ def _(x, weight, bias, relu):
     lead = tuple(x.shape[:2]) if x.dim() == 5 else tuple(x.shape[:-1])
     return _e(x, lead + (weight.shape[1],))
 
+
+# ---- dense layers on 16-bit inputs, distillation ------------------------------------------------
+@_op("dense")
+def dense(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], act: str,
+          want_pre: bool) -> Tuple[Tensor, Tensor]:
+    """act(x W + bias) + residual -> out, pre (float16 / bfloat16; ops.dense_fwd).  pre is empty
+    unless want_pre, which the gradient of an activation needs."""
+    if want_pre:
+        return ops.dense_fwd(x, weight, bias, act, residual, want_pre=True)
+    return ops.dense_fwd(x, weight, bias, act, residual), x.new_empty(0)
+
+
+@dense.register_fake
+def _(x, weight, bias, residual, act, want_pre):
+    lead = tuple(x.shape[:2]) if x.dim() == 5 else tuple(x.shape[:-1])
+    shape = lead + (weight.shape[1],)
+    return _e(x, shape), _e(x, shape if want_pre else (0,))
+
+
+@_op("dense_backward")
+def dense_backward(d_out: Tensor, x: Tensor, weight: Tensor, pre: Optional[Tensor], act: str
+                   ) -> Tuple[Tensor, Tensor, Tensor]:
+    """-> d_x (of x's shape), d_weight [K,N] in weight's memory layout, d_bias [N]
+    (ops.dense_bwd)."""
+    o = ops.dense_bwd(d_out, x, weight, pre, act)
+    return o["d_x"], o["d_weight"], o["d_bias"]
+
+
+@dense_backward.register_fake
+def _(d_out, x, weight, pre, act):
+    K, N = weight.shape
+    s0, s1 = weight.stride()
+    rows_of_k = not (s1 == 1 and s0 >= N) and s0 == 1 and s1 >= K
+    return (_e(x, x.shape), _e(x, (N, K)).t() if rows_of_k else _e(x, (K, N)), _e(x, (N,)))
+
+
+def _dense_setup(ctx, inputs, output):
+    x, weight, bias, residual, act, want_pre = inputs
+    ctx.save_for_backward(x, weight, output[1])
+    ctx.act, ctx.has_bias, ctx.has_residual = act, bias is not None, residual is not None
+    ctx.want_pre = want_pre
+    ctx.mark_non_differentiable(output[1])
+
+
+def _dense_backward(ctx, grad_out, grad_pre):
+    if ctx.act != "none" and not ctx.want_pre:
+        raise RuntimeError(f"frcnn::dense: the gradient of act {ctx.act!r} needs want_pre=True")
+    x, weight, pre = ctx.saved_tensors
+    d_x, d_w, d_b = torch.ops.frcnn.dense_backward(grad_out, x, weight, pre if ctx.want_pre else None,
+                                                   ctx.act)
+    return (d_x, d_w, d_b if ctx.has_bias else None, grad_out if ctx.has_residual else None, None,
+            None)
+
+
+dense.register_autograd(_dense_backward, setup_context=_dense_setup)
+
+
+@_op("distill_loss")
+def distill_loss(logits: Tensor, top_values: Tensor, top_index: Tensor, weight: Optional[Tensor],
+                 temperature: float) -> Tuple[Tensor, Tensor]:
+    """logits [...,V], the teacher's top logits and labels [...,k], weight [...] -> loss [...] and
+    the log-sum-exp its gradient needs (ops.distill_loss)."""
+    o = ops.distill_loss(logits, top_values, top_index, weight, temperature, want_grad=False)
+    return o["loss"], o["lse"]
+
+
+@distill_loss.register_fake
+def _(logits, top_values, top_index, weight, temperature):
+    return _e(logits, logits.shape[:-1], torch.float32), _e(logits, logits.shape[:-1], torch.float32)
+
+
+@_op("distill_loss_backward")
+def distill_loss_backward(d_loss: Tensor, logits: Tensor, top_values: Tensor, top_index: Tensor,
+                          lse: Tensor, weight: Optional[Tensor], temperature: float) -> Tensor:
+    """Gradient in logits (ops.distill_bwd)."""
+    return ops.distill_bwd(d_loss, logits, top_values, top_index, lse, weight, temperature)
+
+
+@distill_loss_backward.register_fake
+def _(d_loss, logits, top_values, top_index, lse, weight, temperature):
+    return _e(logits, logits.shape)
+
+
+def _distill_setup(ctx, inputs, output):
+    logits, top_values, top_index, weight, temperature = inputs
+    ctx.save_for_backward(logits, top_values, top_index, output[1], weight)
+    ctx.temperature = temperature
+    ctx.mark_non_differentiable(output[1])
+
+
+def _distill_backward(ctx, grad_loss, grad_lse):
+    logits, top_values, top_index, lse, weight = ctx.saved_tensors
+    g = torch.ops.frcnn.distill_loss_backward(grad_loss, logits, top_values, top_index, lse, weight,
+                                              ctx.temperature)
+    return g, None, None, None, None
+
+
+distill_loss.register_autograd(_distill_backward, setup_context=_distill_setup)
 
 OPS = tuple(OP_ENTRY_POINTS)

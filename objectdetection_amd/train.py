@@ -72,22 +72,45 @@ class RPNModel(nn.Module):
 
 class FRCNModel(nn.Module):
     """construct_frcn (module/model.py:29-41) without its first layer (the 2x2 max-pool is fused
-    into the crop): flatten (h,w,c) -> fc -> fc -> softmax classes, 4 x classes box deltas."""
+    into the crop): flatten (h,w,c) -> fc -> fc -> softmax classes, 4 x classes box deltas.
+
+    dtype float16 / bfloat16: the four layers run on the fused dense kernels (module.model.dense)
+    in that type, from the same float32 parameters; class logits and box deltas come out in
+    float32.  None (default): plain float32 modules."""
 
     def __init__(self, channels: int = 512, pooled: int = 7, hidden: int = 4096,
-                 num_classes: int = 21):
+                 num_classes: int = 21, dtype: Optional[torch.dtype] = None):
         super().__init__()
+        if dtype not in (None, torch.float16, torch.bfloat16):
+            raise ValueError(f"dtype must be None, torch.float16 or torch.bfloat16, got {dtype}")
+        self.dtype = dtype
         self.fc1 = nn.Linear(pooled * pooled * channels, hidden)
         self.fc2 = nn.Linear(hidden, hidden)
         self.cls = nn.Linear(hidden, num_classes)
         self.reg = nn.Linear(hidden, 4 * num_classes)
 
-    def forward(self, pooled: torch.Tensor):
-        """pooled [B,R,ph,pw,C] -> pred_reg [B,R,4K], pred_obj [B,R,K]."""
+    def _layer(self, m: nn.Linear, x: torch.Tensor, act: str, out_dtype=None) -> torch.Tensor:
+        from .module.model import dense
+        return dense(x, m.weight.to(self.dtype).t(), m.bias.to(self.dtype), act, out_dtype=out_dtype)
+
+    def logits(self, pooled: torch.Tensor):
+        """pooled [B,R,ph,pw,C] -> pred_reg [B,R,4K], class logits [B,R,K]."""
         B, R = pooled.shape[:2]
         x = pooled.reshape(B * R, -1)
-        x = torch.relu(self.fc2(torch.relu(self.fc1(x))))
-        return self.reg(x).reshape(B, R, -1), torch.softmax(self.cls(x), -1).reshape(B, R, -1)
+        if self.dtype is None:
+            x = torch.relu(self.fc2(torch.relu(self.fc1(x))))
+            reg, cls = self.reg(x), self.cls(x)
+        else:
+            x = self._layer(self.fc1, x.to(self.dtype), "relu")
+            x = self._layer(self.fc2, x, "relu")
+            reg = self._layer(self.reg, x, "none", torch.float32)
+            cls = self._layer(self.cls, x, "none", torch.float32)
+        return reg.reshape(B, R, -1), cls.reshape(B, R, -1)
+
+    def forward(self, pooled: torch.Tensor):
+        """pooled [B,R,ph,pw,C] -> pred_reg [B,R,4K], pred_obj [B,R,K]."""
+        reg, cls = self.logits(pooled)
+        return reg, torch.softmax(cls, -1)
 
 
 class _KernelLoss(torch.autograd.Function):
@@ -146,6 +169,10 @@ class HipPathOps:
         two_cls, lreg = _KernelLoss.apply(cls_prob, reg, 2.0 * out["loss"][0], out["loss"][1],
                                           out["d_cls"], out["d_reg"].reshape(reg.shape))
         return two_cls, lreg, out["partial"][:, 2].sum()
+
+    def distill_loss(self, logits, top_values, top_index, temperature):
+        from .module.loss import distill_loss
+        return distill_loss(logits, top_values, top_index, None, temperature).mean()
 
 
 class GradBuckets:
@@ -226,8 +253,14 @@ class TrainStep:
 
     def __init__(self, rpn: RPNModel, frcn: FRCNModel, cfg: PathConfig, path_ops, dist=None,
                  rank: int = 0, world: int = 1, lr: float = 1e-5, roi_grad: bool = True,
-                 bucket_bytes: int = 64 << 20):
+                 bucket_bytes: int = 64 << 20, teacher: Optional[nn.Module] = None,
+                 distill_k: int = 8, distill_temperature: float = 2.0, distill_weight: float = 1.0):
+        """teacher: a trained head (its `logits(pooled)` is called without gradients) whose
+        distill_k largest class logits per RoI the head also learns from: the mean distillation
+        loss at distill_temperature is added, times distill_weight."""
         self.rpn, self.frcn, self.cfg, self.ops = rpn, frcn, cfg, path_ops
+        self.teacher, self.distill_k = teacher, min(distill_k, cfg.num_classes)
+        self.distill_temperature, self.distill_weight = distill_temperature, distill_weight
         self.dist = dist if world > 1 else None
         self.rank, self.world, self.roi_grad = rank, world, roi_grad
         params = list(rpn.parameters()) + list(frcn.parameters())
@@ -254,7 +287,17 @@ class TrainStep:
                              self.rank * B)
         rpn_cls2, rpn_reg, rpn_pos = self.ops.rpn_loss(pred_obj, pred_reg, t)
         pooled = self.ops.roi_pool(fmap if self.roi_grad else fmap.detach(), t["proposed"])
-        head_reg_out, head_cls_out = self.frcn(pooled)
+        distill = None
+        if self.teacher is None:
+            head_reg_out, head_cls_out = self.frcn(pooled)
+        else:
+            head_reg_out, head_logits = self.frcn.logits(pooled)
+            head_cls_out = torch.softmax(head_logits, -1)
+            with torch.no_grad():
+                _, t_logits = self.teacher.logits(pooled.detach())
+                top_values, top_index = torch.topk(t_logits.float(), self.distill_k, -1)
+            distill = self.distill_weight * self.ops.distill_loss(
+                head_logits, top_values, top_index, self.distill_temperature)
         head_cls2, head_reg, head_pos = self.ops.head_loss(head_cls_out, head_reg_out, t)
         # global normalisation: the class terms are means over world*B*S samples, the box terms
         # means over the positives of ALL ranks
@@ -262,11 +305,16 @@ class TrainStep:
         gpos = self._global(pos)
         w_reg = torch.where(gpos > 0, pos / gpos.clamp(min=1.0), torch.zeros_like(pos))
         local = (rpn_cls2 + head_cls2) / self.world + w_reg[0] * rpn_reg + w_reg[1] * head_reg
+        if distill is not None:
+            local = local + distill / self.world
         local.backward()
         self.buckets.finish()
-        losses = torch.stack([rpn_cls2 / self.world, w_reg[0] * rpn_reg, head_cls2 / self.world,
-                              w_reg[1] * head_reg]).detach()
-        return self._global(losses)        # [2*rpn_cls, rpn_reg, 2*head_cls, head_reg], global
+        terms = [rpn_cls2 / self.world, w_reg[0] * rpn_reg, head_cls2 / self.world,
+                 w_reg[1] * head_reg]
+        if distill is not None:
+            terms.append(distill / self.world)
+        # [2*rpn_cls, rpn_reg, 2*head_cls, head_reg (, distillation)], global
+        return self._global(torch.stack(terms).detach())
 
     def step(self, images, gt, label, seed: int = 0):
         losses = self.forward_backward(images, gt, label, seed)

@@ -1,0 +1,307 @@
+"""The head's dense layer on 16-bit inputs (ops.dense_fwd / ops.dense_bwd) against the same formulas
+in float64, element by element.
+
+Tolerances are first-order rounding bounds, derived before any run:
+  sums     a float32 sum of n products in any order is off by at most n * 2^-23 * sum|x w| (products of
+           16-bit values are exact; 2^-23 also covers additions that truncate);
+  GELU     Phi is within 2e-6 relative (1.3e-6 polynomial, exp2 and rcp 1 ulp each), SiLU's sigmoid
+           within 1e-6; both activations have slopes of at most 1.13, their derivatives are
+           within 1e-5 * |d_out| absolute;
+  output   one rounding to nearest: eps / 2 * |value|, at least half a step of float16's subnormals
+           (2^-25); bfloat16 has float32's exponent range;
+  dz       is rounded once more before the two products (GELU and SiLU only; the others' dz is
+           d_out or 0): eps / 2 * |dz| through the absolute operand.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def make(rng, dev, M, K, N, dt, layout="kn", bias=True, residual=False):
+    t = lambda a: torch.from_numpy(a.astype(np.float32)).to(dev).to(dt)
+    x = t(np.maximum(rng.standard_normal((M, K)), -0.3))
+    w = rng.standard_normal((K, N)) / math.sqrt(K)
+    w = t(w) if layout == "kn" else t(np.ascontiguousarray(w.T)).t()
+    return (x, w, t(rng.standard_normal(N)) if bias else None,
+            t(rng.standard_normal((M, N))) if residual else None)
+
+
+def f64(t):
+    return None if t is None else t.detach().to("cpu").double()
+
+
+def act64(z, act):
+    return {"none": lambda: z, "relu": lambda: z.clamp(min=0), "gelu": lambda: z * torch.special.ndtr(z),
+            "silu": lambda: z * torch.sigmoid(z)}[act]()
+
+
+def grad64(z, act):
+    if act == "none":
+        return torch.ones_like(z)
+    if act == "relu":
+        return (z > 0).double()
+    if act == "gelu":
+        return torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    s = torch.sigmoid(z)
+    return s * (1 + z * (1 - s))
+
+
+def within(got, ref, tol, what):
+    got = f64(got)
+    assert got.shape == ref.shape, what
+    off = (got - ref).abs()
+    bad = ~(off <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} values off, the worst by " \
+        f"{float((off / tol).nan_to_num(nan=9e9).max()):.3g} times its tolerance"
+
+
+def rounding(v, dt):
+    return torch.finfo(dt).eps / 2 * v.abs() * 1.001 + (2.0 ** -25 if dt == torch.float16 else 1e-37)
+
+
+def check_fwd(x, w, b, res, act, out, pre=None, odt=None):
+    X, W, K = f64(x.reshape(-1, w.shape[0])), f64(w), w.shape[0]
+    z = X @ W + (0 if b is None else f64(b))
+    err = K * 2.0 ** -23 * (X.abs() @ W.abs() + (0 if b is None else f64(b).abs())) + 2.0 ** -23 * z.abs()
+    dt = x.dtype
+    if pre is not None:
+        within(pre.reshape(z.shape), z, err + rounding(z, dt), "pre")
+    ref = act64(z, act)
+    err = 1.13 * err + 4e-6 * z.abs()
+    if res is not None:
+        r = f64(res).reshape(z.shape)
+        ref = ref + r
+        err = err + 2.0 ** -23 * (ref.abs() + r.abs())
+    within(out.reshape(z.shape), ref, err + (rounding(ref, dt) if odt is None else 2.0 ** -23 * ref.abs()), "out")
+
+
+def check_bwd(x, w, d, pre, act, g):
+    X, W, D = f64(x.reshape(-1, w.shape[0])), f64(w), f64(d.reshape(-1, w.shape[1]))
+    M, N, dt = X.shape[0], W.shape[1], x.dtype
+    dz = D * (1 if act == "none" else grad64(f64(pre).reshape(D.shape), act))
+    edz = 1e-5 * D.abs() if act in ("gelu", "silu") else torch.zeros_like(D)
+    erd = edz + (rounding(dz, dt) if act in ("gelu", "silu") or d.dtype != dt else 0)
+    if g["d_x"] is not None:
+        ref = dz @ W.t()
+        tol = erd @ W.abs().t() + N * 2.0 ** -23 * (dz.abs() + erd) @ W.abs().t() + rounding(ref, dt)
+        within(g["d_x"].reshape(M, -1), ref, tol * 1.01, "d_x")
+    if g["d_weight"] is not None:
+        ref = X.t() @ dz
+        tol = X.abs().t() @ erd + M * 2.0 ** -23 * X.abs().t() @ (dz.abs() + erd) + rounding(ref, dt)
+        within(g["d_weight"], ref, tol * 1.01, "d_weight")
+    if g["d_bias"] is not None:
+        ref = dz.sum(0)
+        tol = edz.sum(0) + M * 2.0 ** -23 * dz.abs().sum(0) + rounding(ref, dt)
+        within(g["d_bias"], ref, tol * 1.01, "d_bias")
+
+
+SIZES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (17, 64, 16), (1, 4096, 520), (16, 1536, 256), (33, 96, 21),
+         (130, 200, 84), (257, 1003, 331), (128, 128, 128), (300, 72, 1032), (1030, 264, 136), (2, 7, 2050)]
+
+
+@pytest.mark.parametrize("M,K,N", SIZES)
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+def test_forward_sizes_and_layouts(dev, M, K, N, layout):
+    from objectdetection_amd import ops
+    for n, (name, act) in enumerate((("bf16", "relu"), ("f16", "gelu"), ("bf16", "none"), ("f16", "silu"))):
+        x, w, b, res = make(np.random.default_rng(M + K + N + n), dev, M, K, N, TYPES[name], layout, n != 2, n > 0)
+        out, pre = ops.dense_fwd(x, w, b, act=act, residual=res, want_pre=True)
+        assert out.dtype == x.dtype and pre.dtype == x.dtype
+        check_fwd(x, w, b, res, act, out, pre)
+
+
+@pytest.mark.parametrize("M,K,N", SIZES + [(5001, 40, 24), (2048, 16, 84)])
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+def test_backward_sizes_and_layouts(dev, M, K, N, layout):
+    from objectdetection_amd import ops
+    for n, (name, act) in enumerate((("bf16", "none"), ("f16", "gelu"), ("bf16", "relu"), ("f16", "silu"))):
+        rng = np.random.default_rng(M + 2 * K + N + n)
+        x, w, b, d = make(rng, dev, M, K, N, TYPES[name], layout, True, True)
+        pre = ops.dense_fwd(x, w, b, want_pre=True)[1]
+        g = ops.dense_bwd(d, x, w, pre=pre, act=act)
+        assert g["d_weight"].stride() == w.contiguous().stride() if layout == "kn" else True
+        check_bwd(x, w, d, pre, act, g)
+
+
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+def test_float32_output_and_float32_upstream_gradient(dev, name):
+    from objectdetection_amd import ops
+    x, w, b, _ = make(np.random.default_rng(3), dev, 70, 520, 21, TYPES[name], "nk")
+    out = ops.dense_fwd(x, w, b, out_dtype=torch.float32)
+    assert out.dtype == torch.float32
+    check_fwd(x, w, b, None, "none", out, odt=torch.float32)
+    d = torch.randn((70, 21), device=dev)
+    check_bwd(x, w, d, None, "none", ops.dense_bwd(d, x, w))
+
+
+def test_rows_with_strides_slices_and_pooled_shape(dev):
+    """Column slices (strided rows, odd alignments), sliced weights, an expanded gradient, 5-D and 3-D x."""
+    from objectdetection_amd import ops
+    rng = np.random.default_rng(5)
+    big, _, b, _ = make(rng, dev, 90, 260, 45, torch.bfloat16)
+    wide = make(rng, dev, 200, 200, 64, torch.bfloat16)[1]
+    for c0, k in ((0, 128), (1, 131), (8, 200)):
+        x, w = big[:, c0:c0 + k], wide[:k, 3:48]
+        check_fwd(x, w, b, None, "relu", ops.dense_fwd(x, w, b, act="relu"))
+        d = big[:, 7:52]
+        check_bwd(x, w, d, None, "none", ops.dense_bwd(d, x, w))
+        one = torch.ones((1, 1), dtype=torch.bfloat16, device=dev).expand(90, 45)       # .sum()'s gradient
+        check_bwd(x, w, one, None, "none", ops.dense_bwd(one, x, w))
+    x, w, b, res = make(rng, dev, 12, 7 * 7 * 8, 40, torch.float16, "nk", True, True)
+    out = ops.dense_fwd(x.view(3, 4, 7, 7, 8), w, b, "silu", res.view(3, 4, 40))
+    assert out.shape == (3, 4, 40)
+    check_fwd(x, w, b, res, "silu", out)
+    assert torch.equal(out.view(12, 40), ops.dense_fwd(x, w, b, "silu", res))
+    g = ops.dense_bwd(res.view(3, 4, 40), x.view(3, 4, 7, 7, 8), w)
+    assert g["d_x"].shape == (3, 4, 7, 7, 8)
+    check_bwd(x, w, res, None, "none", g)
+    assert ops.dense_fwd(x.view(2, 2, 3, 392), w).shape == (2, 2, 3, 40)
+    x1, x3 = x[:, 0].contiguous(), x[:, 3:4]                     # one feature; a [K] vector as one row
+    assert torch.equal(ops.dense_fwd(x3, w[3:4]), ops.dense_fwd(x3.contiguous(), w[3:4].contiguous()))
+    check_fwd(x1.view(1, 12), w[:12], None, None, "none", ops.dense_fwd(x1, w[:12]))
+
+
+def test_no_rows(dev):
+    from objectdetection_amd import ops
+    x, w, b, _ = make(np.random.default_rng(5), dev, 4, 24, 9, torch.bfloat16)
+    out, pre = ops.dense_fwd(x[:0], w, b, act="gelu", want_pre=True)
+    assert out.shape == (0, 9) and pre.shape == (0, 9)
+    for ww in (w, w.t().contiguous().t()):
+        g = ops.dense_bwd(out, x[:0], ww, pre=pre, act="gelu")
+        assert g["d_x"].shape == (0, 24) and not g["d_weight"].any() and not g["d_bias"].any()
+        assert g["d_weight"].shape == (24, 9)
+
+
+def test_rows_and_columns_outside_the_result_stay(dev):
+    """`out` as the rows of a larger buffer: what lies behind the last row and value is not written."""
+    from objectdetection_amd import ops
+    for M, K, N in ((5, 40, 13), (131, 520, 130), (1, 4096, 24)):
+        x, w, b, _ = make(np.random.default_rng(M), dev, M, K, N, torch.bfloat16)
+        buf = torch.full((M * N + 300,), 7.0, dtype=torch.bfloat16, device=dev)
+        ops.dense_fwd(x, w, b, out=buf[:M * N].view(M, N))
+        check_fwd(x, w, b, None, "none", buf[:M * N].view(M, N))
+        assert (buf[M * N:] == 7).all()
+
+
+def test_infinities_and_nan(dev):
+    from objectdetection_amd import ops
+    inf, nan = math.inf, math.nan
+    eye = torch.eye(8, device=dev, dtype=torch.bfloat16)
+    row = torch.tensor([[0.0, 1, -1, 3e38, -3e38, 5, -5, 0.5]], device=dev).bfloat16()
+    for act in ("relu", "gelu", "silu"):
+        got = ops.dense_fwd(row, eye, act=act)
+        ref = act64(f64(row), act)
+        assert torch.allclose(got.double().cpu(), ref, rtol=2 ** -7, atol=1e-7), act
+    bias = torch.tensor([inf, -inf, nan, 0, 1, -1, 2, -2], device=dev).bfloat16()
+    z = torch.zeros((1, 8), device=dev, dtype=torch.bfloat16)
+    got = ops.dense_fwd(z, eye, bias, act="relu").float().cpu()
+    assert got[0, 0] == inf and got[0, 1] == 0 and got[0, 2].isnan() and not got[0, 3:].isnan().any()
+    g = ops.dense_bwd(torch.full((1, 8), inf, device=dev).bfloat16(), z, eye, pre=bias[None], act="relu")
+    assert g["d_bias"].float().cpu().tolist() == [inf, 0, 0, 0, inf, 0, inf, 0]
+    # a NaN row or column reaches its own results only, also where tiles are padded
+    x, w, b, _ = make(np.random.default_rng(1), dev, 19, 70, 37, torch.float16)
+    x[7] = nan
+    w = w.clone()
+    w[:, 5] = inf
+    out = ops.dense_fwd(x, w, b)
+    bad = ~out.isfinite()
+    ref = torch.zeros_like(bad)
+    ref[7] = True
+    ref[:, 5] = True
+    assert torch.equal(bad, ref)
+
+
+def test_same_bits_every_time_and_on_another_stream(dev):
+    from objectdetection_amd import ops
+    x, w, b, d = make(np.random.default_rng(9), dev, 40, 4104, 84, torch.bfloat16, "nk", True, True)
+    out, g = ops.dense_fwd(x, w, b), ops.dense_bwd(d, x, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            assert torch.equal(out, ops.dense_fwd(x, w, b))
+            h = ops.dense_bwd(d, x, w)
+            assert all(torch.equal(g[k], h[k]) for k in g)
+    torch.cuda.current_stream().wait_stream(side)
+
+
+def test_captured_forward_and_backward_replay(dev):
+    """Two graphs of the same calls with a workspace each, replayed with other work between."""
+    from objectdetection_amd import ops
+    M, K, N = 24, 2056, 136
+    x, w, b, d = make(np.random.default_rng(11), dev, M, K, N, torch.bfloat16, "kn", True, True)
+    ws = [torch.empty(max(ops.dense_fwd_workspace_bytes(M, K, N), ops.dense_bwd_workspace_bytes(M, K, N)),
+                      dtype=torch.uint8, device=dev) for _ in range(2)]
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    for n in range(2):
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out, pre = ops.dense_fwd(x, w, b, act="gelu", want_pre=True, workspace=ws[n])
+            g = ops.dense_bwd(d, x, w, pre=pre, act="gelu", workspace=ws[n])
+        graphs.append(graph)
+        outs.append((out, g))
+    for step in range(4):
+        x.copy_(torch.randn_like(x))
+        for n in range(2):
+            graphs[n].replay()
+        torch.cuda.synchronize()
+        ref, pre = ops.dense_fwd(x, w, b, act="gelu", want_pre=True)
+        gref = ops.dense_bwd(d, x, w, pre=pre, act="gelu")
+        for out, g in outs:
+            assert torch.equal(out, ref) and all(torch.equal(g[k], gref[k]) for k in g), step
+
+
+def test_gradients_against_differences(dev):
+    """d_x, d_weight, d_bias of sum(d_out * out) against central differences in float64 of the formula,
+    through act' at the saved pre-activations."""
+    from objectdetection_amd import ops
+    rng = np.random.default_rng(2)
+    for act in ("gelu", "silu"):
+        x, w, b, d = make(rng, dev, 6, 16, 8, torch.float16, "kn", True, True)
+        out, pre = ops.dense_fwd(x, w, b, act=act, want_pre=True)
+        g = ops.dense_bwd(d, x, w, pre=pre, act=act)
+        X, W, B, D = f64(x), f64(w), f64(b), f64(d)
+        f = lambda X, W, B: float((D * act64(X @ W + B, act)).sum())
+        h = 1e-4
+        for t, got, call in ((X, g["d_x"], lambda t: f(t, W, B)), (W, g["d_weight"], lambda t: f(X, t, B)),
+                             (B, g["d_bias"], lambda t: f(X, W, t))):
+            num = torch.zeros_like(t)
+            for i in range(t.numel()):
+                p, m = t.clone().view(-1), t.clone().view(-1)
+                p[i] += h
+                m[i] -= h
+                num.view(-1)[i] = (call(p.view(t.shape)) - call(m.view(t.shape))) / (2 * h)
+            # float16: pre, dz and the result are rounded (2^-11 each, relative to the absolute sums)
+            assert (f64(got) - num).abs().max() <= 4 * 2.0 ** -11 * max(1.0, float(num.abs().max())) * 4
+
+
+def test_refusals(dev):
+    from objectdetection_amd import ops
+    x, w, b, d = make(np.random.default_rng(1), dev, 4, 24, 8, torch.bfloat16, "kn", True, True)
+    for bad, err in (
+            (lambda: ops.dense_fwd(x.float(), w.float()), TypeError),
+            (lambda: ops.dense_fwd(x, w.half()), TypeError),
+            (lambda: ops.dense_fwd(x, w[:20]), ValueError),
+            (lambda: ops.dense_fwd(x, w[0]), ValueError),
+            (lambda: ops.dense_fwd(x, w, b.float()), TypeError),
+            (lambda: ops.dense_fwd(x, w, b[:7]), ValueError),
+            (lambda: ops.dense_fwd(x, w, act="tanh"), ValueError),
+            (lambda: ops.dense_fwd(x, w, residual=d[:1]), ValueError),
+            (lambda: ops.dense_fwd(x, w, residual=d.float()), TypeError),
+            (lambda: ops.dense_fwd(x, w, out=torch.empty((4, 8), device=dev)), ValueError),
+            (lambda: ops.dense_fwd(x, w, out_dtype=torch.float16), TypeError),
+            (lambda: ops.dense_fwd(x.cpu(), w), RuntimeError),
+            (lambda: ops.dense_fwd(x, w.cpu()), RuntimeError),
+            (lambda: ops.dense_bwd(d, x, w, act="relu"), ValueError),
+            (lambda: ops.dense_bwd(d[:3], x, w), ValueError),
+            (lambda: ops.dense_bwd(d, x, w, want_dx=False, want_dw=False, want_db=False), ValueError),
+            (lambda: ops.dense_bwd(d, x, w, workspace=torch.empty(16, dtype=torch.uint8, device=dev)), ValueError)):
+        with pytest.raises(err):
+            bad()

@@ -1,0 +1,188 @@
+"""The head's dense layers and the distillation loss together, as a program runs them: module
+functions with autograd, the operators under torch.ops, a training step with a teacher."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def f64(t):
+    return t.detach().double().cpu()
+
+
+def head64(x, ps, t, idx, T):
+    """pooled rows -> two ReLU layers, a residual SiLU layer, logits, mean distillation loss: float64."""
+    h = x
+    for n, (w, b) in enumerate(ps[:-1]):
+        z = h @ w.t() + b
+        h = torch.relu(z) if n < 2 else z * torch.sigmoid(z) + h
+    z = (h @ ps[-1][0].t() + ps[-1][1]) / T
+    p = torch.softmax(t / T, -1)
+    log_q = torch.log_softmax(z, -1).gather(-1, idx)
+    return (T * T * p * (torch.log(p) - log_q)).sum(-1).mean()
+
+
+def test_a_head_is_trained_by_distillation(dev):
+    """Four layers and the loss: the loss and the gradients of every weight agree with float64.
+
+    Tolerance: each of the four layers rounds its output and (SiLU) its pre-activation and dz once,
+    relative 2^-8 each in bfloat16, so about ten independent roundings of up to 2^-8 reach every
+    gradient: in the 2-norm at most 10 * 2^-8 = 0.04 of it, the loss likewise."""
+    from objectdetection_amd.module import dense, distill_loss
+    torch.manual_seed(3)
+    B, R, C, H, K, T = 2, 40, 8, 96, 21, 2.0
+    pooled = torch.relu(torch.randn((B, R, 7, 7, C), device=dev)).bfloat16()
+    ps = [(torch.randn((n, k), device=dev) / k ** 0.5, 0.1 * torch.randn(n, device=dev))
+          for k, n in ((49 * C, H), (H, H), (H, H), (H, K))]
+    ps = [(w.bfloat16().requires_grad_(True), b.bfloat16().requires_grad_(True)) for w, b in ps]
+    t, idx = torch.topk(3 * torch.randn((B, R, K), device=dev), 6, -1)
+    h = dense(pooled, ps[0][0].t(), ps[0][1], "relu")
+    h = dense(h, ps[1][0].t(), ps[1][1], "relu")
+    h = dense(h, ps[2][0].t(), ps[2][1], "silu", residual=h)
+    z = dense(h, ps[3][0].t(), ps[3][1], out_dtype=torch.float32)
+    assert z.dtype == torch.float32 and z.shape == (B, R, K)
+    loss = distill_loss(z, t, idx, None, T).mean()
+    loss.backward()
+    qs = [(f64(w).requires_grad_(True), f64(b).requires_grad_(True)) for w, b in ps]
+    ref = head64(f64(pooled).view(B, R, -1), qs, f64(t), idx.cpu(), T)
+    ref.backward()
+    assert abs(float(loss) - float(ref)) <= 0.04 * float(ref)
+    for (w, b), (u, v) in zip(ps, qs):
+        for got, want in ((w.grad, u.grad), (b.grad, v.grad)):
+            assert got.shape == want.shape
+            assert float((f64(got) - want).norm()) <= 0.04 * float(want.norm())
+
+
+def test_module_functions_give_only_the_gradients_asked_for(dev):
+    from objectdetection_amd import ops
+    from objectdetection_amd.module import dense, distill_loss, distill_losses
+    x = torch.randn((6, 24), device=dev).half().requires_grad_(True)
+    w, b = torch.randn((24, 10), device=dev).half(), torch.randn(10, device=dev).half().requires_grad_(True)
+    r = torch.randn((6, 10), device=dev).half().requires_grad_(True)
+    out = dense(x, w, b, "gelu", r, torch.float32)
+    d = torch.randn_like(out)
+    gx, gb, gr = torch.autograd.grad(out, (x, b, r), d)
+    ref = ops.dense_bwd(d, x.detach(), w, ops.dense_fwd(x.detach(), w, b.detach(), want_pre=True)[1], "gelu")
+    assert torch.equal(gx, ref["d_x"]) and torch.equal(gb, ref["d_bias"]) and torch.equal(gr, d.half())
+    gr, = torch.autograd.grad(dense(x.detach(), w, None, "none", r).sum(), r)     # the residual alone
+    assert (gr == 1).all()
+    with torch.no_grad():
+        assert not dense(x, w, b, "gelu").requires_grad
+    z = torch.randn((2, 5, 21), device=dev).requires_grad_(True)
+    t, i = torch.topk(torch.randn((2, 5, 21), device=dev), 4, -1)
+    g, = torch.autograd.grad(distill_loss(z, t, i, None, 2.0).mean(), z)
+    mean, fused = distill_losses(z.detach(), t, i, None, 2.0)
+    assert torch.allclose(g, fused, rtol=2.0 ** -20, atol=1e-8)
+    assert torch.allclose(mean, distill_loss(z.detach(), t, i, None, 2.0).mean(), rtol=1e-6)
+    assert distill_losses(z.detach(), t, i, want_grad=False)[1] is None
+
+
+def test_operators_through_the_dispatcher(dev):
+    from objectdetection_amd import ops, torch_ops  # noqa: F401
+    F = torch.ops.frcnn
+    x = torch.randn((5, 40), device=dev).bfloat16()
+    for w in (torch.randn((40, 24), device=dev).bfloat16(), torch.randn((24, 40), device=dev).bfloat16().t()):
+        b = torch.randn(24, device=dev).bfloat16()
+        xs, ws, bs = (v.clone(memory_format=torch.preserve_format).requires_grad_(True) for v in (x, w, b))
+        out, pre = F.dense(xs, ws, bs, None, "silu", True)
+        ref, rpre = ops.dense_fwd(x, w, b, "silu", want_pre=True)
+        assert torch.equal(out, ref) and torch.equal(pre, rpre)
+        d = torch.randn_like(out)
+        g = torch.autograd.grad(out, (xs, ws, bs), d)
+        r = ops.dense_bwd(d, x, w, rpre, "silu")
+        assert all(torch.equal(a, c) for a, c in zip(g, (r["d_x"], r["d_weight"], r["d_bias"])))
+        torch.library.opcheck(F.dense.default, (xs, ws, bs, None, "silu", True),
+                              test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))
+        torch.library.opcheck(F.dense_backward.default, (d.detach(), x, w, rpre, "silu"),
+                              test_utils=("test_schema", "test_faketensor"))
+    with pytest.raises(RuntimeError):
+        F.dense(xs, ws, bs, None, "silu", False)[0].sum().backward()
+    z = torch.randn((5, 30), device=dev).requires_grad_(True)
+    t, i = torch.topk(torch.randn((5, 30), device=dev), 3, -1)
+    loss, lse = F.distill_loss(z, t, i, None, 1.5)
+    up = torch.rand(5, device=dev)
+    g, = torch.autograd.grad(loss, z, up)
+    assert torch.equal(g, ops.distill_bwd(up, z.detach(), t, i, lse.detach(), None, 1.5))
+    torch.library.opcheck(F.distill_loss.default, (z, t, i, None, 1.5),
+                          test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))
+
+    @torch.compile(backend="eager", fullgraph=True)
+    def fn(a, b, c):
+        o, _ = torch.ops.frcnn.dense(a, b, c, None, "relu", False)
+        return o + 1
+
+    assert torch.equal(fn(x, w, b), ops.dense_fwd(x, w, b, "relu") + 1)
+
+
+def test_forward_and_backward_captured_with_autograd(dev):
+    """A step captured into a graph through torch.autograd.grad, replayed against the eager step.
+    While an eager graph of the same leaves, built on another stream, is alive the call is refused
+    before anything is captured (the runtime would end the process in the backward)."""
+    from objectdetection_amd.module import dense, distill_loss
+    torch.manual_seed(1)
+    x = torch.randn((32, 64), device=dev).bfloat16()
+    w1 = torch.randn((48, 64), device=dev).bfloat16().requires_grad_(True)
+    w2 = torch.randn((21, 48), device=dev).bfloat16().requires_grad_(True)
+    t, i = torch.topk(torch.randn((32, 21), device=dev), 5, -1)
+
+    def step():
+        h = dense(x, w1.t(), None, "gelu")
+        z = dense(h, w2.t(), out_dtype=torch.float32)
+        loss = distill_loss(z, t, i, None, 2.0)
+        return (loss, *torch.autograd.grad(loss, (w1, w2), torch.ones_like(loss)))
+
+    side = torch.cuda.Stream()
+    for leaf in (torch.randn((8, 64), device=dev).requires_grad_(True),
+                 torch.randn((8, 64), device=dev).bfloat16().requires_grad_(True)):
+        alive = dense(x, leaf.bfloat16().t())       # a view, or a cast and a view, away from its leaf
+        with pytest.raises(RuntimeError, match="capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                dense(x, leaf.bfloat16().t())
+        alive.sum().backward()
+        del alive
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = step()
+    for n in range(4):
+        x.copy_(torch.randn_like(x))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step())), n
+
+
+@pytest.mark.parametrize("dtype", [None, torch.bfloat16, torch.float16])
+def test_training_step_with_a_teacher_and_a_16_bit_head(dev, dtype):
+    """The joint step runs with a 16-bit head and a teacher, every parameter gets a finite gradient,
+    and the head's 16-bit outputs are those of the float32 modules to its roundings."""
+    from objectdetection_amd.config import PathConfig
+    from objectdetection_amd.train import FRCNModel, HipPathOps, RPNModel, TrainStep
+    torch.manual_seed(0)
+    cfg = PathConfig(H=9, W=11, pre_k=500, post_n=150, G=8)
+    rpn = RPNModel(cfg.A, 0.125).to(dev)
+    frcn = FRCNModel(rpn.channels, cfg.crop[0] // cfg.pool, 64, cfg.num_classes, dtype=dtype).to(dev)
+    plain = FRCNModel(rpn.channels, cfg.crop[0] // cfg.pool, 64, cfg.num_classes).to(dev)
+    plain.load_state_dict(frcn.state_dict())
+    teacher = FRCNModel(rpn.channels, cfg.crop[0] // cfg.pool, 128, cfg.num_classes, dtype=dtype).to(dev)
+    pooled = torch.relu(torch.randn((2, 150, 7, 7, rpn.channels), device=dev))
+    with torch.no_grad():
+        for a, b in zip(frcn.logits(pooled), plain.logits(pooled)):
+            assert a.dtype == torch.float32
+            # four roundings of 2^-8 (bfloat16; float16 2^-11) on the way, in the 2-norm
+            assert float((a - b).norm()) <= (0 if dtype is None else 4 * 2.0 ** -8) * float(b.norm())
+    step = TrainStep(rpn, frcn, cfg, HipPathOps(cfg, 2, rpn.channels, dev), teacher=teacher)
+    images = torch.rand((2, 3, cfg.H * 16 + 8, cfg.W * 16 + 8), device=dev)
+    c = torch.rand((2, cfg.G, 2), device=dev) * 0.6 + 0.2
+    half = torch.rand((2, cfg.G, 2), device=dev) * 0.15 + 0.05
+    gt = torch.cat([c - half, c + half], -1)
+    label = torch.randint(0, cfg.num_classes - 1, (2, cfg.G), device=dev)
+    before = [p.detach().clone() for p in frcn.parameters()]
+    losses = step.step(images, gt, label, seed=1)
+    assert losses.shape == (5,) and losses.isfinite().all() and float(losses[4]) > 0
+    for p, q in zip(frcn.parameters(), before):
+        assert p.grad.isfinite().all() and p.grad.any() and not torch.equal(p, q)
+    assert all(p.grad is None for p in teacher.parameters())

@@ -25,6 +25,7 @@ typedef short dn_s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 dn_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 dn_f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) dn_s16x4 dn_lds_s16x4;
+typedef __attribute__((address_space(3))) const dn_s16x8 dn_lds_s16x8;
 
 constexpr int DN_BK = 64;                       // k per LDS tile
 constexpr int DN_TARGET_WG = 256;               // compute units
@@ -140,37 +141,38 @@ struct DnGemm {
     DnEpilogue e;
 };
 
-// four neighbouring outputs of one row
-template <typename T>
-__device__ __forceinline__ void dn_epilogue4(const DnEpilogue& e, long long i, long long j, int valid, dn_f32x4 acc) {
-    float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+// W neighbouring outputs of one row, `valid` of them inside, from their float32 sums
+template <typename T, int W>
+__device__ __forceinline__ void dn_epilogue(const DnEpilogue& e, long long i, long long j, int valid, float* v) {
     if (e.bias) {
-        float b[4];
-        dn_load<T, 4>((const T*)e.bias + j, valid, b);
+        float b[W];
+        dn_load<T, W>((const T*)e.bias + j, valid, b);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] += b[r];
+        for (int r = 0; r < W; ++r) v[r] += b[r];
     }
-    if (e.pre) dn_store<T, 4>((T*)e.pre + i * e.ldp + j, valid, v);
+    if (e.pre) dn_store<T, W>((T*)e.pre + i * e.ldp + j, valid, v);
     if (e.act != FRCNN_ACT_NONE) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = dn_act(v[r], e.act);
+        for (int r = 0; r < W; ++r) v[r] = dn_act(v[r], e.act);
     }
     if (e.residual) {
-        float b[4];
-        dn_load<T, 4>((const T*)e.residual + i * e.ldr + j, valid, b);
+        float b[W];
+        dn_load<T, W>((const T*)e.residual + i * e.ldr + j, valid, b);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] += b[r];
+        for (int r = 0; r < W; ++r) v[r] += b[r];
     }
-    if (e.out_f32) dn_store<float, 4>((float*)e.out + i * e.ldo + j, valid, v);
-    else dn_store<T, 4>((T*)e.out + i * e.ldo + j, valid, v);
+    if (e.out_f32) dn_store<float, W>((float*)e.out + i * e.ldo + j, valid, v);
+    else dn_store<T, W>((T*)e.out + i * e.ldo + j, valid, v);
 }
 
 // ---- LDS tiles -------------------------------------------------------------------------------------
-// position (in 16-byte pieces) of piece `c` of row `r`; its own inverse in c
-template <bool KC, int R>
+// position (in 16-byte pieces) of piece `c` of row `r`; its own inverse in c.  Sixteen lanes that read
+// 16 rows of a k-contiguous tile, or four rows of 32 bytes twice in an outer-contiguous one, touch every
+// bank once (no conflict counted)
+template <bool KC, int R, int BK>
 __device__ __forceinline__ int dn_swizzle(int r, int c) {
-    if constexpr (KC) return c ^ (r & 7);                                     // [R][8 pieces of 8 k]
-    constexpr int m = R >= 128 ? 7 : R / 16 - 1;                              // [64][R / 8 pieces]
+    if constexpr (KC) return c ^ ((r >> 1) & 7);                              // [R][8 pieces of 8 k]
+    constexpr int m = R >= 128 ? 7 : R / 16 - 1;                              // [BK][R / 8 pieces]
     return c ^ ((((r & 3) | ((r >> 1) & 4)) & m) << 1);
 }
 
@@ -201,24 +203,24 @@ struct DnStage {
             const int idx = (int)threadIdx.x + NT * i;
             constexpr int P = KC ? 8 : R / 8;
             const int r = idx / P, c = idx % P;
-            lds[r * P + dn_swizzle<KC, R>(r, c)] = v[i];
+            lds[r * P + dn_swizzle<KC, R, DN_BK>(r, c)] = v[i];
         }
     }
 };
 
 // fragment of outer rows o0 .. o0 + 15 (o0 a multiple of 16), k = 32 kk .. 32 kk + 31: lane l holds
 // row l % 16, k 8 (l / 16) .. + 7
-template <bool KC, int R>
+template <bool KC, int R, int BK>
 __device__ __forceinline__ dn_s16x8 dn_fragment(const dn_s16x8* lds, int o0, int kk) {
     const int lane = lane_id(), g = lane >> 4, l = lane & 15;
     if constexpr (KC) {
         const int r = o0 + l;
-        return lds[r * 8 + dn_swizzle<true, R>(r, kk * 4 + g)];
+        return lds[r * (BK / 8) + dn_swizzle<true, R, BK>(r, kk * 4 + g)];
     } else {
         const int k = kk * 32 + g * 8 + (l >> 2), c = o0 / 8 + ((l & 3) >> 1);
         const short* base = reinterpret_cast<const short*>(lds);
-        const short* p0 = base + (k * (R / 8) + dn_swizzle<false, R>(k, c)) * 8 + (l & 1) * 4;
-        const short* p1 = base + ((k + 4) * (R / 8) + dn_swizzle<false, R>(k + 4, c)) * 8 + (l & 1) * 4;
+        const short* p0 = base + (k * (R / 8) + dn_swizzle<false, R, BK>(k, c)) * 8 + (l & 1) * 4;
+        const short* p1 = base + ((k + 4) * (R / 8) + dn_swizzle<false, R, BK>(k + 4, c)) * 8 + (l & 1) * 4;
         const dn_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((dn_lds_s16x4*)p0);
         const dn_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((dn_lds_s16x4*)p1);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -239,13 +241,52 @@ __device__ __forceinline__ void dn_tile(const DnGemm& p, int& ti, int& tj, int& 
     tj = (t - g * group) / rows;
 }
 
+// A wave's results, (16 FI) x (16 FJ) at (i0, j0): the float32 partial sums of a slice, or the outputs.
+// Sixteen rows at a time turn round through LDS (the wave's own DN_TURN bytes), so that a lane holds eight
+// neighbouring outputs and the lanes of a row store whole 128-byte lines.
+template <int FJ> constexpr int dn_turn_bytes() { return 16 * (FJ * 64 + 16); }
+template <typename T, int FI, int FJ>
+__device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&acc)[FI][FJ], int slice, long long i0,
+                                             long long j0, char* turn) {
+    constexpr int S = FJ * 64 + 16, Q = 2 * FJ, RP = 64 / Q;      // bytes per row, pieces of 8 per row, rows per pass
+    const int lane = lane_id();
+    const long long Jp = (p.J + 3) / 4 * 4, gj = j0 + 8 * (lane % Q), left = p.J - gj;
+    const int valid = left > 8 ? 8 : (int)left;
+#pragma unroll
+    for (int i = 0; i < FI; ++i) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < FJ; ++j)
+            *reinterpret_cast<dn_f32x4*>(turn + (lane & 15) * S + j * 64 + (lane >> 4) * 16) = acc[i][j];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 16; r += RP) {
+            const int row = r + lane / Q;
+            const long long gi = i0 + 16 * i + row;
+            if (gi >= p.I || valid <= 0) continue;
+            const float* src = reinterpret_cast<const float*>(turn + row * S + (lane % Q) * 32);
+            float v[8];
+            __builtin_memcpy(v, src, 32);
+            if (p.partial) {    // columns J .. Jp-1 may be written and are never read as results
+                float* to = p.partial + (slice * p.I + gi) * Jp + gj;
+                __builtin_memcpy(to, v, 16);
+                if (valid > 4) __builtin_memcpy(to + 4, v + 4, 16);
+            } else {
+                dn_epilogue<T, 8>(p.e, gi, gj, valid, v);
+            }
+        }
+    }
+}
+
 // WI x WJ waves, each (BI / WI) x (BJ / WJ) outputs.  The MFMA's rows are j and its columns i, so that
 // a lane ends with four neighbouring outputs of one row.
 template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
 __global__ void __launch_bounds__(64 * WI * WJ)
 dense_gemm_kernel(DnGemm p) {
     constexpr int NT = 64 * WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
-    __shared__ dn_s16x8 lds_a[BI * 8], lds_b[BJ * 8];
+    extern __shared__ __attribute__((aligned(16))) char dn_lds[];
+    dn_s16x8* lds_a = reinterpret_cast<dn_s16x8*>(dn_lds);
+    dn_s16x8* lds_b = lds_a + BI * 8;
     int ti, tj, slice;
     dn_tile(p, ti, tj, slice);
     const long long i0 = (long long)ti * BI, j0 = (long long)tj * BJ;
@@ -276,9 +317,9 @@ dense_gemm_kernel(DnGemm p) {
         for (int kk = 0; kk < DN_BK / 32; ++kk) {
             dn_s16x8 fa[FI], fb[FJ];
 #pragma unroll
-            for (int i = 0; i < FI; ++i) fa[i] = dn_fragment<AKC, BI>(lds_a, wi + 16 * i, kk);
+            for (int i = 0; i < FI; ++i) fa[i] = dn_fragment<AKC, BI, DN_BK>(lds_a, wi + 16 * i, kk);
 #pragma unroll
-            for (int j = 0; j < FJ; ++j) fb[j] = dn_fragment<BKC, BJ>(lds_b, wj + 16 * j, kk);
+            for (int j = 0; j < FJ; ++j) fb[j] = dn_fragment<BKC, BJ, DN_BK>(lds_b, wj + 16 * j, kk);
 #pragma unroll
             for (int i = 0; i < FI; ++i)
 #pragma unroll
@@ -287,23 +328,227 @@ dense_gemm_kernel(DnGemm p) {
         __syncthreads();
     }
 
-    const int lane = lane_id();
-    const long long Jp = (p.J + 3) / 4 * 4;
+    dn_write_out<T, FI, FJ>(p, acc, slice, i0 + wi, j0 + wj, dn_lds + wave * dn_turn_bytes<FJ>());
+}
+
+// ---- the product on aligned operands ----------------------------------------------------------------
+// Tiles go from memory to LDS directly (global_load_lds, 16 bytes per lane, the swizzle applied to the
+// source address because the destination is linear in the lane).  The reduction is walked in steps of 32 k:
+// while the fragments of step s, already in registers, are multiplied, those of step s + 1 are read from
+// LDS and later ones are in flight.  An outer-contiguous operand is copied a step at a time into a ring of
+// four, at step s that of s + 4; a k-contiguous one two steps at a time (64 k: whole 128-byte lines, copies
+// of half lines took L2 twice the requests: 1,282 -> TFLOP/s) into a ring of two, at every odd s those of
+// s + 3 and s + 4.  A handover says that the copies step s + 1 needs have arrived (the newer ones stay in
+// flight) and that every wave has read step s, whose place is then filled again.  Rows outside the
+// operand repeat its last row (their results are not stored); k outside reads a page of zeros.
+constexpr int DN_SK = 32, DN_RING = 4;
+__device__ const __attribute__((aligned(16))) uint32_t dn_zeros[4] = {0, 0, 0, 0};
+
+__device__ __forceinline__ void dn_dma(uint32_t lds, const void* base, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(lds), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void dn_dma(uint32_t lds, const void* p) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :: "s"(lds), "v"(p) : "memory");
+}
+// all but the newest N copies of this wave have arrived and its LDS reads are done; then the same of all waves
+template <int N>
+__device__ __forceinline__ void dn_handover() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <typename T, bool KC, int R, int NT>
+struct DnCopy {
+    static constexpr int CK = KC ? 2 * DN_SK : DN_SK;             // k per copy
+    static constexpr int P = KC ? CK / 8 : R / 8, NP = R * CK / 8 / NT;   // pieces per LDS row, per thread
+    static constexpr uint32_t BYTES = R * CK * 2;
+    uint32_t off[NP];
+    const char* base;          // at (outer0, k)
+    long long step;            // bytes per copy
+    __device__ __forceinline__ void init(const T* p, long long ld, long long outer0, long long outer_end,
+                                         long long k0) {
+        const long long ld2 = ld * 2, left = outer_end - outer0;
+        base = reinterpret_cast<const char*>(p) + (KC ? outer0 * ld2 + k0 * 2 : k0 * ld2 + outer0 * 2);
+        step = KC ? CK * 2 : CK * ld2;
 #pragma unroll
-    for (int i = 0; i < FI; ++i) {
-        const long long gi = i0 + wi + 16 * i + (lane & 15);
-        if (gi >= p.I) continue;
-#pragma unroll
-        for (int j = 0; j < FJ; ++j) {
-            const long long gj = j0 + wj + 16 * j + 4 * (lane >> 4);
-            const long long left = p.J - gj;
-            if (left <= 0) continue;
-            if (p.partial)      // columns J .. Jp-1 hold zeros: the operand's tile is zero there
-                *reinterpret_cast<dn_f32x4*>(p.partial + (slice * p.I + gi) * Jp + gj) = acc[i][j];
-            else
-                dn_epilogue4<T>(p.e, gi, gj, left > 4 ? 4 : (int)left, acc[i][j]);
+        for (int i = 0; i < NP; ++i) {
+            const int idx = (int)threadIdx.x + NT * i;
+            int r = idx / P, c = dn_swizzle<KC, R, CK>(r, idx % P);
+            if constexpr (KC) r = r < left ? r : (int)left - 1;
+            else c = 8 * c + 8 <= left ? c : (int)(left / 8) - 1;
+            off[i] = (uint32_t)r * (uint32_t)ld2 + (uint32_t)c * 16u;
         }
     }
+    // the k at `base` to LDS byte address `lds` (of this wave's first piece); base moves on
+    __device__ __forceinline__ void issue(uint32_t lds) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) dn_dma(lds + (uint32_t)(NT * i * 16), base, off[i]);
+        base += step;
+    }
+    // the same where only the first `valid` k are inside
+    __device__ __forceinline__ void issue(uint32_t lds, int valid) {
+        if (valid >= CK) return issue(lds);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int idx = (int)threadIdx.x + NT * i, r = idx / P;
+            const int k = KC ? 8 * dn_swizzle<KC, R, CK>(r, idx % P) : r;
+            dn_dma(lds + (uint32_t)(NT * i * 16), k < valid ? base + off[i] : reinterpret_cast<const char*>(dn_zeros));
+        }
+        base += step;
+    }
+};
+
+// A wave's fragments of 16 outer rows from `o0` on, of any step in the ring, from one LDS address per lane:
+// fragment f is a constant further where k is contiguous, and at the address with f in its swizzled
+// bits where it is not; the place in the ring is a constant offset of the instruction (an operand's ring
+// lies within 64 KB, its first byte on a multiple of 2 KB).
+template <bool KC, int R>
+struct DnReader {
+    uint32_t at;
+    __device__ __forceinline__ void init(uint32_t lds, int o0) {
+        const int lane = lane_id(), g = lane >> 4, l = lane & 15;
+        if constexpr (KC) {
+            at = lds + (uint32_t)((o0 + l) * 8 + dn_swizzle<true, R, 64>(l, g)) * 16u;
+        } else {
+            const int k = g * 8 + (l >> 2);
+            at = lds + (uint32_t)(k * (R / 8) + dn_swizzle<false, R, DN_SK>(k, o0 / 8 + ((l & 3) >> 1))) * 16u +
+                 (uint32_t)(l & 1) * 8u;
+        }
+    }
+    // keeps the compiler from holding an address per fragment in registers
+    __device__ __forceinline__ void renew() { asm volatile("" : "+v"(at)); }
+    __device__ __forceinline__ dn_s16x8 read(int f, int step) const {
+        const uint32_t ring = (uint32_t)(step % DN_RING);
+        if constexpr (KC) {     // the odd step is the second half of the row: pieces 4 .. 7
+            const uint32_t a = (at ^ ((ring & 1u) * 64u)) + (ring >> 1) * (R * 128u);
+            return *(dn_lds_s16x8*)(uintptr_t)(a + (uint32_t)f * 2048u);
+        } else {
+            const uint32_t a = (at ^ ((uint32_t)f * 32u)) + ring * (R * 64u);
+            const dn_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((dn_lds_s16x4*)(uintptr_t)a);
+            const dn_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((dn_lds_s16x4*)(uintptr_t)(a + 8u * R));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+};
+
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
+__global__ void __launch_bounds__(64 * WI * WJ)
+dense_gemm_lds_kernel(DnGemm p) {
+    constexpr int NT = 64 * WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
+    constexpr int READS = FI * (AKC ? 1 : 2) + FJ * (BKC ? 1 : 2);  // LDS reads per wave and step
+    extern __shared__ __attribute__((aligned(16))) char dn_lds[];    // A's ring, then B's
+    int ti, tj, slice;
+    dn_tile(p, ti, tj, slice);
+    const long long i0 = (long long)ti * BI, j0 = (long long)tj * BJ;
+    const long long k0 = slice * p.k_slice;
+    const long long k_end = k0 + p.k_slice < p.K ? k0 + p.k_slice : p.K;
+    const int wave = __builtin_amdgcn_readfirstlane(wave_id());
+    const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
+
+    dn_f32x4 acc[FI][FJ];
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) acc[i][j] = dn_f32x4{0.f, 0.f, 0.f, 0.f};
+
+    using CopyA = DnCopy<T, AKC, BI, NT>;
+    using CopyB = DnCopy<T, BKC, BJ, NT>;
+    // copies per thread: of the operands that are copied every step, of those copied every other step
+    constexpr int EVERY = (AKC ? 0 : CopyA::NP) + (BKC ? 0 : CopyB::NP);
+    constexpr int OTHER = (AKC ? CopyA::NP : 0) + (BKC ? CopyB::NP : 0);
+    CopyA ca;
+    CopyB cb;
+    ca.init((const T*)p.a, p.lda, i0, p.I, k0);
+    cb.init((const T*)p.b, p.ldb, j0, p.J, k0);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dn_lds;
+    const uint32_t la = lds0 + (uint32_t)wave * 1024u, lb = la + BI * DN_SK * 2 * DN_RING;
+    DnReader<AKC, BI> qa;
+    DnReader<BKC, BJ> qb;
+    qa.init(lds0, wi);
+    qb.init(lds0 + BI * DN_SK * 2 * DN_RING, wj);
+    const int n = (int)((k_end - k0 + DN_SK - 1) / DN_SK);
+    dn_s16x8 fa[2][FI], fb[2][FJ];
+    auto read = [&](int s, dn_s16x8 (&ra)[FI], dn_s16x8 (&rb)[FJ]) {
+        qa.renew();
+        qb.renew();
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) rb[j] = qb.read(j, s);
+#pragma unroll
+        for (int i = 0; i < FI; ++i) ra[i] = qa.read(i, s);
+    };
+    auto multiply = [&](const dn_s16x8 (&ra)[FI], const dn_s16x8 (&rb)[FJ]) {
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) acc[i][j] = dn_mfma(rb[j], ra[i], acc[i][j], T());
+    };
+    // the copies for step s: every-step operands (EV), and with an even s every-other-step ones (OT)
+    auto issue = [&](int s, bool ev, bool ot) {
+        if (s >= n) return;
+        const long long left = k_end - k0 - (long long)s * DN_SK;
+        const int valid = left < 2 * DN_SK ? (int)left : 2 * DN_SK;
+        const uint32_t ring = (uint32_t)(s % DN_RING);
+        if (AKC ? ot : ev) ca.issue(la + ring * (BI * 64u), valid);
+        if (BKC ? ot : ev) cb.issue(lb + ring * (BJ * 64u), valid);
+    };
+    issue(0, true, true);
+    issue(1, true, false);
+    issue(2, true, true);
+    issue(3, true, false);
+    if (n >= DN_RING) dn_handover<OTHER + 2 * EVERY>();      // steps 0 and 1
+    else dn_handover<0>();
+    read(0, fa[0], fb[0]);
+    int s = 0;
+    // whole steps, four at a time so that every LDS address is a constant; no branch inside
+#pragma unroll 1
+    for (; s + 2 * DN_RING < n; s += DN_RING) {
+#pragma unroll
+        for (int u = 0; u < DN_RING; ++u) {
+            if (u & 1) {
+                dn_handover<2 * EVERY>();
+                if (AKC) ca.issue(la + ((u + 3) % DN_RING) * (BI * 64u));
+                if (BKC) cb.issue(lb + ((u + 3) % DN_RING) * (BJ * 64u));
+            } else if (EVERY) {
+                dn_handover<OTHER + 2 * EVERY>();
+            }
+            if (!AKC) ca.issue(la + u * (BI * 64u));
+            if (!BKC) cb.issue(lb + u * (BJ * 64u));
+            read(u + 1, fa[(u + 1) & 1], fb[(u + 1) & 1]);
+            multiply(fa[u & 1], fb[u & 1]);
+            // the reads of the next step between the products of this one, early
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+#pragma unroll
+            for (int q = 0; q < READS; ++q) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, FI * FJ, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // the last steps: up to eight, the last one maybe cut short
+    auto step = [&](const dn_s16x8 (&ra)[FI], const dn_s16x8 (&rb)[FJ], dn_s16x8 (&na)[FI], dn_s16x8 (&nb)[FJ]) {
+        if (s + 1 < n) {
+            if (s + 3 >= n) dn_handover<0>();
+            else if (s & 1) dn_handover<2 * EVERY>();
+            else dn_handover<OTHER + 2 * EVERY>();
+            if (s & 1) issue(s + 3, false, true);
+            issue(s + 4, true, false);
+            read(s + 1, na, nb);
+        }
+        multiply(ra, rb);
+        ++s;
+    };
+#pragma unroll 1
+    while (s < n) {
+        step(fa[0], fb[0], fa[1], fb[1]);
+        if (s < n) step(fa[1], fb[1], fa[0], fb[0]);
+    }
+    dn_handover<0>();
+    dn_write_out<T, FI, FJ>(p, acc, slice, i0 + wi, j0 + wj, dn_lds + wave * dn_turn_bytes<FJ>());
 }
 
 // sums of a split product's slices, in slice order, and the epilogue; four outputs per thread
@@ -320,7 +565,8 @@ dense_join_kernel(const float* __restrict__ partial, int splits, long long I, lo
         for (int r = 0; r < 4; ++r) v[r] += w[r];
     }
     const long long left = J - j;
-    dn_epilogue4<T>(e, i, j, left > 4 ? 4 : (int)left, v);
+    float o[4] = {v[0], v[1], v[2], v[3]};
+    dn_epilogue<T, 4>(e, i, j, left > 4 ? 4 : (int)left, o);
 }
 
 // ---- dz = d_out * act'(pre), and column sums per block of rows ----------------------------------------
@@ -389,11 +635,12 @@ struct DnPlan { int bi, bj, splits; long long k_slice, tiles_i, tiles_j; size_t 
 
 static DnPlan dn_plan(long long I, long long J, long long K) {
     DnPlan p{};
-    p.bi = p.bj = 128;
+    const long long big = ((I + 255) / 256) * ((J + 255) / 256);
+    p.bi = p.bj = big >= DN_TARGET_WG / 2 ? 256 : 128;
     p.tiles_i = (I + p.bi - 1) / p.bi;
     p.tiles_j = (J + p.bj - 1) / p.bj;
     const long long tiles = p.tiles_i * p.tiles_j, steps = (K + DN_BK - 1) / DN_BK;
-    long long splits = tiles >= DN_TARGET_WG ? 1 : 2 * DN_TARGET_WG / tiles;
+    long long splits = tiles >= DN_TARGET_WG || p.bi == 256 ? 1 : 2 * DN_TARGET_WG / tiles;
     if (splits > steps / 4) splits = steps / 4;        // four k steps per slice at least
     if (splits > 32) splits = 32;
     if (splits < 1) splits = 1;
@@ -405,11 +652,34 @@ static DnPlan dn_plan(long long I, long long J, long long K) {
     return p;
 }
 
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
+static int dn_launch_lds(const DnGemm& g, unsigned blocks, hipStream_t stream) {
+    constexpr int lds = DN_RING * (BI + BJ) * DN_SK * 2;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(dense_gemm_lds_kernel<T, AKC, BKC, BI, BJ, WI, WJ>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+        return FRCNN_E_LAUNCH;
+    FRCNN_LAUNCH((dense_gemm_lds_kernel<T, AKC, BKC, BI, BJ, WI, WJ>), dim3(blocks), dim3(64 * WI * WJ), lds, stream,
+                 g);
+    return FRCNN_OK;
+}
+
+// whether an operand can be copied to LDS in 16-byte pieces: rows that start on 16 bytes, whole pieces in
+// its contiguous dimension, and a tile whose rows are within 2 GiB of each other
+static bool dn_whole_pieces(const void* p, long long ld, bool kc, long long outer, long long K) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && (kc ? K : outer) % 8 == 0 && ld <= (1ll << 21);
+}
+
 template <typename T, bool AKC, bool BKC>
 static int dn_launch_gemm(const DnPlan& pl, const DnGemm& g, hipStream_t stream) {
     const long long blocks = pl.tiles_i * pl.tiles_j * pl.splits;
     if (blocks > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
-    FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, 128, 128, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
+    const bool whole = dn_whole_pieces(g.a, g.lda, AKC, g.I, g.K) && dn_whole_pieces(g.b, g.ldb, BKC, g.J, g.K);
+    if (whole && pl.bi == 256) return dn_launch_lds<T, AKC, BKC, 256, 256, 2, 4>(g, (unsigned)blocks, stream);
+    if (whole) return dn_launch_lds<T, AKC, BKC, 128, 128, 2, 2>(g, (unsigned)blocks, stream);
+    if (pl.bi == 256)
+        FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, 256, 256, 2, 4>), dim3((unsigned)blocks), dim3(512), 65536, stream, g);
+    else
+        FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, 128, 128, 2, 2>), dim3((unsigned)blocks), dim3(256), 32768, stream, g);
     return FRCNN_OK;
 }
 

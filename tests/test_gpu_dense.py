@@ -128,6 +128,22 @@ def test_backward_sizes_and_layouts(dev, M, K, N, layout):
         check_bwd(x, w, d, pre, act, g)
 
 
+@pytest.mark.parametrize("M,K,N", [(4100, 200, 2056), (2304, 96, 3000), (2049, 64, 2880), (4097, 33, 2051), (3900, 32, 4104)])
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+def test_large_tiles(dev, M, K, N, layout):
+    """Enough output for the largest workgroup tiles, ragged at their edges, short and odd in k: the
+    forward, and as d_weight's and d_x's sizes the backward."""
+    from objectdetection_amd import ops
+    rng = np.random.default_rng(M + K)
+    x, w, b, res = make(rng, dev, M, K, N, torch.bfloat16, layout, True, True)
+    out, pre = ops.dense_fwd(x, w, b, act="silu", residual=res, want_pre=True)
+    check_fwd(x, w, b, res, "silu", out, pre)
+    xt, wt, _, d = make(rng, dev, K, M, N, torch.float16, layout, False, True)       # d_weight [M,N]
+    check_bwd(xt, wt, d, None, "none", ops.dense_bwd(d, xt, wt))
+    xb, wb, _, d = make(rng, dev, M, N, K, torch.bfloat16, layout, False, True)      # d_x [M,N]
+    check_bwd(xb, wb, d, None, "none", ops.dense_bwd(d, xb, wb))
+
+
 @pytest.mark.parametrize("name", ["bf16", "f16"])
 def test_float32_output_and_float32_upstream_gradient(dev, name):
     from objectdetection_amd import ops

@@ -454,16 +454,19 @@ int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, const void* x, 
  *     loss = weight T^2 sum_j p_j (log p_j - log q_(i_j))
  *     d_logits_v = g weight T (q_v - sum_j p_j [i_j = v])
  * A label listed more than once counts each time.  A row with weight 0 or without an entry takes
- * no part: loss, lse and gradient 0, its logits (also NaN) are not read.  A student logit of -inf
+ * no part: loss, lse and gradient 0 whatever its logits are (also NaN).  A student logit of -inf
  * has q = 0: the loss is +inf where the teacher gives that label weight; a row of -inf alone is NaN.
  *   dtype   of logits and d_logits: F32, F16 or BF16; t_dtype of top_values: dtype or F32;
  *   weight  [rows] or NULL (1);  loss, lse [rows] f32, lse = log sum_v e^(z_v / T) for the backward;
  *   frcnn_distill_loss: d_logits may be NULL, g = grad_scale; frcnn_distill_bwd: g = d_loss [rows].
- * d_logits must not overlap logits. */
+ * d_logits must not overlap logits.  The workspace (0 bytes for most sizes) joins the parts of few
+ * or very long rows. */
+size_t frcnn_distill_workspace_bytes(int64_t rows, int V, int k, int dtype);
 int frcnn_distill_loss(const void* logits, int64_t ldz, int dtype, const void* top_values,
                        int t_dtype, const int64_t* top_index, const float* weight, int64_t rows,
                        int V, int k, float temperature, float grad_scale, float* loss, float* lse,
-                       void* d_logits, int64_t ldg, frcnn_stream_t stream);
+                       void* d_logits, int64_t ldg, void* workspace, size_t workspace_bytes,
+                       frcnn_stream_t stream);
 int frcnn_distill_bwd(const float* d_loss, const void* logits, int64_t ldz, int dtype,
                       const void* top_values, int t_dtype, const int64_t* top_index,
                       const float* lse, const float* weight, int64_t rows, int V, int k,

@@ -89,8 +89,9 @@ _SIGS = {
     "frcnn_dense_bwd_workspace_bytes": (_sz, [_i64, _i, _i]),
     "frcnn_dense_bwd": (_i, [_p, _i64, _i, _p, _i64, _p, _i64, _i, _p, _i64, _i64, _i, _i, _i, _i,
                              _p, _i64, _p, _i64, _p, _p, _sz, _p]),
+    "frcnn_distill_workspace_bytes": (_sz, [_i64, _i, _i, _i]),
     "frcnn_distill_loss": (_i, [_p, _i64, _i, _p, _i, _p, _p, _i64, _i, _i, _f, _f, _p, _p, _p,
-                                _i64, _p]),
+                                _i64, _p, _sz, _p]),
     "frcnn_distill_bwd": (_i, [_p, _p, _i64, _i, _p, _i, _p, _p, _p, _i64, _i, _i, _f, _p, _i64,
                                _p]),
 }

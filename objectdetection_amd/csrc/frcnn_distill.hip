@@ -4,20 +4,27 @@
 // logit is -inf is not there) and student logits z_v (v < V), temperature T:
 //     p = softmax(t / T) over the entries that are there,   q = softmax(z / T) over all V,
 //     loss = w T^2 sum_j p_j (log p_j - log q_(i_j)),   d loss / d z_v = w T (q_v - sum_j p_j [i_j = v]).
-// A row with w = 0 or no entry takes no part: its loss, lse and gradient are 0 and its logits are not read.
+// A row with w = 0 or no entry takes no part: its loss, lse and gradient are 0 whatever its logits are
+// (with w = 0 they are not read).
 //
-// All sums are float32, taken relative to the row's maximum; log q is kept as (z - max)/T - log(sum), so
-// the two large terms of z - lse never cancel.  The gradient is written as q first and the few listed
-// labels are written again with their p subtracted; a label listed twice gets both.
+// All sums are float32, relative to the row's maximum; log q is kept as (z - max) / T - log(sum), so the
+// two large terms of z - lse never cancel.  The gradient is written as c q first and the few listed labels
+// are written again with their p subtracted; a label listed twice gets both.
+//
+// Memory is the bound: a logit is read once and its gradient written once.  A workgroup holds a whole row
+// in registers, as it lies in memory, between the three walks over it (maximum, sum, gradient).  Rows too
+// long for that, and few long rows, are split: one launch leaves a maximum and a sum per chunk, a second one
+// joins them in every workgroup and writes the chunk's gradient.  Rows of up to 64 classes share a wave.
 #include "frcnn_common.h"
 
 namespace frcnn {
 
 constexpr int DS_MAX_K = 1024;
+constexpr float DS_LOG2E = 1.4426950408889634f;
 
 struct DsArgs {
     const void* z; long long ldz;        // [rows,V]
-    const void* t;                       // [rows,k]
+    const void* t; int t_f32;            // [rows,k], float32 or the logits' type
     const int64_t* idx;                  // [rows,k]
     const float* weight;                 // [rows] or null
     const float* d_loss;                 // [rows] or null: the backward's upstream gradient
@@ -26,136 +33,486 @@ struct DsArgs {
     float temperature;
     long long rows; int V, k;
     float* loss; float* lse; void* grad; long long ldg;
+    float2* part; int chunks;            // maximum and sum of each chunk of a split row
 };
 
-template <int BLOCK>
-__device__ __forceinline__ float ds_block_max(float v, float* sh) {
+typedef unsigned int ds_u32x4 __attribute__((ext_vector_type(4)));
+
+// sixteen bytes of a row, as they lie in memory: 4 float32 or 8 16-bit values
+template <typename T>
+struct DsVec {
+    static constexpr int W = 16 / sizeof(T);
+    ds_u32x4 b;
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (W == 4) {
+            return __uint_as_float(b[i]);
+        } else {
+            const unsigned short h = (unsigned short)(b[i / 2] >> (16 * (i & 1)));
+            return (float)__builtin_bit_cast(T, h);
+        }
+    }
+    // keeps the compiler from holding the converted values from one walk over the row to the next
+    __device__ __forceinline__ void renew() { asm volatile("" : "+v"(b)); }
+    __device__ __forceinline__ void load(const T* p, int valid) {          // -inf behind the row's end
+        if (valid >= W) {
+            __builtin_memcpy(&b, p, 16);
+        } else {
+            T v[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = i < valid ? p[i] : (T)-__builtin_inff();
+            __builtin_memcpy(&b, v, 16);
+        }
+    }
+    __device__ __forceinline__ void set(const float* f) {
+        T v[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = (T)f[i];
+        __builtin_memcpy(&b, v, 16);
+    }
+    __device__ __forceinline__ void store(T* p, int valid) const {
+        if (valid >= W) {
+            __builtin_memcpy(p, &b, 16);
+        } else {
+            T v[W];
+            __builtin_memcpy(v, &b, 16);
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (i < valid) p[i] = v[i];
+        }
+    }
+};
+
+__device__ __forceinline__ float ds_wave_max(float v) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    if constexpr (BLOCK > 64) {
-        __syncthreads();
-        if (lane_id() == 0) sh[wave_id()] = v;
-        __syncthreads();
-        v = sh[0];
-        for (int w = 1; w < BLOCK / 64; ++w) v = fmaxf(v, sh[w]);
-    }
     return v;
 }
-template <int BLOCK>
-__device__ __forceinline__ float ds_block_sum(float v, float* sh) {
+__device__ __forceinline__ float ds_wave_sum(float v) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    if constexpr (BLOCK > 64) {
-        __syncthreads();
+    return v;
+}
+// over the workgroup, the same order for every thread; `sh` of BLOCK / 64 floats is used once per call
+template <int BLOCK, bool MAX>
+__device__ __forceinline__ float ds_block(float v, float* sh) {
+    v = MAX ? ds_wave_max(v) : ds_wave_sum(v);
+    if constexpr (BLOCK == 64) {
+        return v;
+    } else {
         if (lane_id() == 0) sh[wave_id()] = v;
         __syncthreads();
         v = sh[0];
-        for (int w = 1; w < BLOCK / 64; ++w) v += sh[w];
+#pragma unroll
+        for (int w = 1; w < BLOCK / 64; ++w) v = MAX ? fmaxf(v, sh[w]) : v + sh[w];
+        return v;
     }
-    return v;
 }
 
-constexpr float DS_LOG2E = 1.4426950408889634f;
-__device__ __forceinline__ float ds_exp(float x) { return __builtin_amdgcn_exp2f(x * DS_LOG2E); }
+// ---- the teacher's side of a row, by one wave ----------------------------------------------------------
+// LDS: per entry its label (-1: not there), t / T relative to the largest one, the student's logit there
+struct DsTeacher {
+    int* label; float* t; float* z;
+    __device__ __forceinline__ DsTeacher(void* lds, int k)
+        : label((int*)lds), t((float*)lds + k), z((float*)lds + 2 * k) {}
+};
+struct DsTeacherSum { float log_sum; bool any; };      // log of the sum of e^t; whether an entry is there
 
-// One workgroup per row.  FORWARD: maximum, sum, loss, lse and (grad given) the gradient; else the
-// gradient alone, from the forward's lse.
-template <typename T, typename U, bool FORWARD, int BLOCK>
-__global__ void __launch_bounds__(BLOCK)
-distill_row_kernel(DsArgs a) {
-    __shared__ float sh[BLOCK / 64 + 1];
-    __shared__ float tp[DS_MAX_K];                   // the teacher's entries: t / T, then p
-    __shared__ int ti[DS_MAX_K];
+template <typename T>
+__device__ __forceinline__ float ds_teacher_logit(const DsArgs& a, long long at) {
+    return a.t_f32 ? ((const float*)a.t)[at] : (float)((const T*)a.t)[at];
+}
+
+template <typename T>
+__device__ DsTeacherSum ds_teacher(const DsArgs& a, long long row, DsTeacher e, float inv_t, bool want_z) {
+    const int lane = lane_id();
+    const T* z = (const T*)a.z + row * a.ldz;
+    float top = -__builtin_inff();
+    bool any = false;
+    for (int j = lane; j < a.k; j += 64) {
+        const int64_t i = a.idx[row * a.k + j];
+        const float t = ds_teacher_logit<T>(a, row * a.k + j) * inv_t;
+        const bool there = i >= 0 && i < a.V && !(t == -__builtin_inff());
+        e.label[j] = there ? (int)i : -1;
+        e.t[j] = t;
+        if (there) {
+            any = true;
+            top = fmaxf(top, t);
+            if (want_z) e.z[j] = (float)z[i];
+        }
+    }
+    top = ds_wave_max(top);
+    any = __ballot(any) != 0;
+    float s = 0.f;
+    for (int j = lane; j < a.k; j += 64) {
+        const float t = e.t[j] - top;
+        e.t[j] = t;
+        if (e.label[j] >= 0) s += __builtin_amdgcn_exp2f(t * DS_LOG2E);
+    }
+    return {logf(ds_wave_sum(s)), any};
+}
+
+// sum_j p_j (log p_j - log q_j) with log q = (z - z_max) / T - log_s, by the same wave
+__device__ __forceinline__ float ds_row_loss(const DsArgs& a, DsTeacher e, float log_sum, float inv_t, float z_max,
+                                             float log_s) {
+    float l = 0.f;
+    for (int j = lane_id(); j < a.k; j += 64) {
+        if (e.label[j] < 0) continue;
+        const float log_p = e.t[j] - log_sum, p = __builtin_amdgcn_exp2f(log_p * DS_LOG2E);
+        const float log_q = (e.z[j] - z_max) * inv_t - log_s;
+        if (!(p == 0.f)) l += p * (log_p - log_q);
+    }
+    return ds_wave_sum(l);
+}
+
+// writes the gradient at the listed labels in [v0, v1): the first entry of a label takes all of them
+template <typename T, typename Q>
+__device__ __forceinline__ void ds_listed(const DsArgs& a, DsTeacher e, float log_sum, float c, T* grad, long long v0,
+                                          long long v1, int tid, int block, Q q_of) {
+    for (int j = tid; j < a.k; j += block) {
+        const int i = e.label[j];
+        if (i < v0 || i >= v1) continue;
+        bool first = true;
+        float p = 0.f;
+        for (int n = 0; n < a.k; ++n) {
+            if (e.label[n] != i) continue;
+            if (n < j) { first = false; break; }
+            p += __builtin_amdgcn_exp2f((e.t[n] - log_sum) * DS_LOG2E);
+        }
+        if (first) grad[i] = (T)(c * (q_of(e.z[j]) - p));
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void ds_zero(T* grad, long long v0, long long v1, int tid, int block) {
+    DsVec<T> o;
+    o.b = ds_u32x4{0, 0, 0, 0};
+    for (long long v = v0 + tid * DsVec<T>::W; v < v1; v += block * DsVec<T>::W)
+        o.store(grad + v, v1 - v > DsVec<T>::W ? DsVec<T>::W : (int)(v1 - v));
+}
+
+// ---- rows of up to 64 classes and 64 entries: G lanes per row ------------------------------------------
+template <typename T, bool FORWARD, int G>
+__global__ void __launch_bounds__(256) distill_small_kernel(DsArgs a) {
+    const int l = threadIdx.x & (G - 1), first = lane_id() & ~(G - 1);
+    const long long row = (long long)blockIdx.x * (256 / G) + threadIdx.x / G;
+    if (row >= a.rows) return;                         // whole groups of lanes leave
+    const float inv_t = 1.0f / a.temperature, ninf = -__builtin_inff();
+    const float w = a.weight ? a.weight[row] : 1.0f;
+    const bool mine = l < a.V;
+    const float z = mine && w != 0.f ? (float)((const T*)a.z)[row * a.ldz + l] : ninf;
+    int label = -1;
+    float t = ninf;
+    if (l < a.k) {
+        const int64_t i = a.idx[row * a.k + l];
+        t = ds_teacher_logit<T>(a, row * a.k + l) * inv_t;
+        if (i >= 0 && i < a.V && !(t == ninf)) label = (int)i;
+    }
+    float top = label >= 0 ? t : ninf, m = z;
+    int any = label >= 0;
+#pragma unroll
+    for (int d = G / 2; d; d >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, d));
+        m = fmaxf(m, __shfl_xor(m, d));
+        any |= __shfl_xor(any, d);
+    }
+    const float te = label >= 0 ? __builtin_amdgcn_exp2f((t - top) * DS_LOG2E) : 0.f;
+    float ts = te, s = mine ? __builtin_amdgcn_exp2f((z - m) * (inv_t * DS_LOG2E)) : 0.f;
+#pragma unroll
+    for (int d = G / 2; d; d >>= 1) {
+        ts += __shfl_xor(ts, d);
+        s += __shfl_xor(s, d);
+    }
+    const bool part = w != 0.f && any;
+    const float log_sum = logf(ts), log_s = logf(s);
+    const float log_p = t - top - log_sum, p = label >= 0 ? __builtin_amdgcn_exp2f(log_p * DS_LOG2E) : 0.f;
+    const float zi = __shfl(z, first + (label >= 0 ? label : 0));
+    if (FORWARD) {
+        float loss = label >= 0 && !(p == 0.f) ? p * (log_p - ((zi - m) * inv_t - log_s)) : 0.f;
+#pragma unroll
+        for (int d = G / 2; d; d >>= 1) loss += __shfl_xor(loss, d);
+        if (l == 0) {
+            a.loss[row] = part ? w * (a.temperature * a.temperature) * loss : 0.f;
+            a.lse[row] = part ? m * inv_t + log_s : 0.f;
+        }
+        if (!a.grad) return;
+    }
+    float listed = 0.f;                                // the p of the entries that name this lane's class
+    for (int j = 0; j < a.k; ++j) {
+        const int i = __shfl(label, first + j);
+        const float pj = __shfl(p, first + j);
+        if (i == l) listed += pj;
+    }
+    const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale);
+    const float log_q = FORWARD ? (z - m) * inv_t - log_s : z * inv_t - a.lse_in[row];
+    if (mine)
+        ((T*)a.grad)[row * a.ldg + l] = (T)(part ? c * (__builtin_amdgcn_exp2f(log_q * DS_LOG2E) - listed) : 0.f);
+}
+
+// ---- a whole row in the registers of one workgroup: up to BLOCK * NV vectors ------------------------------
+template <typename T, int BLOCK, int NV>
+__global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char ds_lds[];
+    __shared__ float sh_m[BLOCK / 64], sh_s[BLOCK / 64], sh_t;
+    __shared__ int sh_any;
+    constexpr int W = DsVec<T>::W;
     const int tid = threadIdx.x;
     const long long row = blockIdx.x;
     const T* z = (const T*)a.z + row * a.ldz;
     T* grad = a.grad ? (T*)a.grad + row * a.ldg : nullptr;
-    const float w = a.weight ? a.weight[row] : 1.0f;
-    const float inv_t = 1.0f / a.temperature;
-
-    float tm = -__builtin_inff();
-    bool nan_seen = false;
-    if (w != 0.f) {
-        for (int j = tid; j < a.k; j += BLOCK) {
-            const int64_t i = a.idx[row * a.k + j];
-            const float t = (float)((const U*)a.t)[row * a.k + j] * inv_t;
-            const bool there = i >= 0 && i < a.V && !(t == -__builtin_inff());
-            ti[j] = there ? (int)i : -1;
-            tp[j] = t;
-            if (there) { tm = fmaxf(tm, t); nan_seen |= t != t; }
-        }
-        tm = ds_block_max<BLOCK>(tm, sh);
-        nan_seen = __syncthreads_or(nan_seen);
-    }
-    if (w == 0.f || (tm == -__builtin_inff() && !nan_seen)) {
-        if (FORWARD && tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
-        if (grad) for (int v = tid; v < a.V; v += BLOCK) grad[v] = (T)0.f;
+    const float w = a.weight ? a.weight[row] : 1.0f, inv_t = 1.0f / a.temperature;
+    if (w == 0.f) {
+        if (tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
+        if (grad) ds_zero(grad, 0, a.V, tid, BLOCK);
         return;
     }
-    float ts = 0.f;
-    for (int j = tid; j < a.k; j += BLOCK)
-        if (ti[j] >= 0) ts += ds_exp(tp[j] - tm);
-    ts = ds_block_sum<BLOCK>(ts, sh);
-    const float log_ts = logf(ts);
-
-    float m, log_s;                                  // log q_v = z_v / T - m - log_s
-    if constexpr (FORWARD) {
-        m = -__builtin_inff();
-        for (int v = tid; v < a.V; v += BLOCK) m = fmaxf(m, (float)z[v] * inv_t);
-        m = ds_block_max<BLOCK>(m, sh);
-        float s = 0.f;
-        for (int v = tid; v < a.V; v += BLOCK) s += ds_exp((float)z[v] * inv_t - m);
-        s = ds_block_sum<BLOCK>(s, sh);
-        log_s = logf(s);
-        float l = 0.f;
-        for (int j = tid; j < a.k; j += BLOCK) {
-            if (ti[j] < 0) continue;
-            const float log_p = tp[j] - tm - log_ts, p = ds_exp(log_p);
-            const float log_q = (float)z[ti[j]] * inv_t - m - log_s;
-            if (!(p == 0.f)) l += p * (log_p - log_q);
-        }
-        l = ds_block_sum<BLOCK>(l, sh);
+    DsVec<T> x[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v = (tid + BLOCK * i) * W;
+        x[i].load(z + v, a.V - v);
+    }
+    const DsTeacher e(ds_lds, a.k);
+    DsTeacherSum te{0.f, false};
+    if (wave_id() == 0) {                              // while the row arrives
+        te = ds_teacher<T>(a, row, e, inv_t, true);
+        if (tid == 0) { sh_t = te.log_sum; sh_any = te.any; }
+    }
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) m = fmaxf(m, x[i][j]);
+    m = ds_block<BLOCK, true>(m, sh_m);
+    if constexpr (BLOCK == 64) __syncthreads();
+    if (!sh_any) {
+        if (tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
+        if (grad) ds_zero(grad, 0, a.V, tid, BLOCK);
+        return;
+    }
+    const float f = inv_t * DS_LOG2E;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float part = 0.f;
+        x[i].renew();
+#pragma unroll
+        for (int j = 0; j < W; ++j) part += __builtin_amdgcn_exp2f((x[i][j] - m) * f);
+        s += part;
+    }
+    s = ds_block<BLOCK, false>(s, sh_s);
+    const float log_s = logf(s);
+    if (wave_id() == 0) {
+        const float l = ds_row_loss(a, e, te.log_sum, inv_t, m, log_s);
         if (tid == 0) {
             a.loss[row] = w * (a.temperature * a.temperature) * l;
-            a.lse[row] = m + log_s;
+            a.lse[row] = m * inv_t + log_s;
         }
-    } else {
-        m = a.lse_in[row];
-        log_s = 0.f;
     }
     if (!grad) return;
-    const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale);
-    for (int v = tid; v < a.V; v += BLOCK) grad[v] = (T)(c * ds_exp((float)z[v] * inv_t - m - log_s));
-    __syncthreads();
-    for (int j = tid; j < a.k; j += BLOCK) {
-        const int i = ti[j];
-        if (i < 0) continue;
-        bool first = true;
-        float p = 0.f;
-        for (int n = 0; n < a.k; ++n) {
-            if (ti[n] != i) continue;
-            if (n < j) { first = false; break; }
-            p += ds_exp(tp[n] - tm - log_ts);
-        }
-        if (first) grad[i] = (T)(c * (ds_exp((float)z[i] * inv_t - m - log_s) - p));
+    const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale), cq = c / s;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v = (tid + BLOCK * i) * W;
+        float q[W];
+        x[i].renew();
+#pragma unroll
+        for (int j = 0; j < W; ++j) q[j] = cq * __builtin_amdgcn_exp2f((x[i][j] - m) * f);
+        x[i].set(q);
+        x[i].store(grad + v, a.V - v);
     }
+    __syncthreads();                                   // the stores of c q come before those of the listed labels
+    ds_listed(a, e, sh_t, c, grad, 0, a.V, tid, BLOCK,
+              [&](float zi) { return __builtin_amdgcn_exp2f((zi - m) * f) / s; });
 }
 
-template <typename T, typename U, bool FORWARD>
-static int ds_launch(const DsArgs& a, hipStream_t s) {
+// ---- a chunk of a row per workgroup --------------------------------------------------------------------
+constexpr int DS_CHUNK_BLOCK = 256, DS_CHUNK_NV = 4;
+template <typename T> constexpr int ds_chunk() { return DS_CHUNK_BLOCK * DS_CHUNK_NV * DsVec<T>::W; }
+
+template <typename T>
+__global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_part_kernel(DsArgs a) {
+    __shared__ float sh_m[DS_CHUNK_BLOCK / 64], sh_s[DS_CHUNK_BLOCK / 64];
+    constexpr int W = DsVec<T>::W;
+    const int tid = threadIdx.x, chunk = blockIdx.x;
+    const long long row = blockIdx.y;
+    if (a.weight && a.weight[row] == 0.f) return;
+    const T* z = (const T*)a.z + row * a.ldz;
+    const long long v0 = (long long)chunk * ds_chunk<T>();
+    DsVec<T> x[DS_CHUNK_NV];
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < DS_CHUNK_NV; ++i) {
+        const long long v = v0 + (tid + DS_CHUNK_BLOCK * i) * W, left = a.V - v;
+        x[i].load(z + v, left > W ? W : (int)left);
+    }
+#pragma unroll
+    for (int i = 0; i < DS_CHUNK_NV; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) m = fmaxf(m, x[i][j]);
+    m = ds_block<DS_CHUNK_BLOCK, true>(m, sh_m);
+    const float f = DS_LOG2E / a.temperature;
+    const float base = m == -__builtin_inff() ? 0.f : m;    // a chunk of -inf alone has the sum 0
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < DS_CHUNK_NV; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) s += __builtin_amdgcn_exp2f((x[i][j] - base) * f);
+    s = ds_block<DS_CHUNK_BLOCK, false>(s, sh_s);
+    if (tid == 0) a.part[row * a.chunks + chunk] = float2{m, s};
+}
+
+// FORWARD: joins the row's partial sums; chunk 0 writes loss and lse; else q comes from the forward's lse
+template <typename T, bool FORWARD>
+__global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_chunk_kernel(DsArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char ds_lds[];
+    __shared__ float sh_t, sh_m, sh_s;
+    __shared__ int sh_any;
+    constexpr int W = DsVec<T>::W;
+    const int tid = threadIdx.x, chunk = blockIdx.x;
+    const long long row = blockIdx.y;
+    const T* z = (const T*)a.z + row * a.ldz;
+    T* grad = a.grad ? (T*)a.grad + row * a.ldg : nullptr;
+    const long long v0 = (long long)chunk * ds_chunk<T>(), v1 = v0 + ds_chunk<T>() < a.V ? v0 + ds_chunk<T>() : a.V;
+    const float w = a.weight ? a.weight[row] : 1.0f, inv_t = 1.0f / a.temperature;
+    if (w == 0.f) {
+        if (FORWARD && chunk == 0 && tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
+        if (grad) ds_zero(grad, v0, v1, tid, DS_CHUNK_BLOCK);
+        return;
+    }
+    DsVec<T> x[DS_CHUNK_NV];
+    if (grad) {
+#pragma unroll
+        for (int i = 0; i < DS_CHUNK_NV; ++i) {
+            const long long v = v0 + (tid + DS_CHUNK_BLOCK * i) * W, left = a.V - v;
+            x[i].load(z + v, left > W ? W : (int)left);
+        }
+    }
+    const DsTeacher e(ds_lds, a.k);
+    DsTeacherSum te{0.f, false};
+    if (wave_id() == 0) {
+        te = ds_teacher<T>(a, row, e, inv_t, true);
+        if (tid == 0) { sh_t = te.log_sum; sh_any = te.any; }
+    }
+    if constexpr (FORWARD) {
+        if (wave_id() == 1) {                          // every workgroup joins the chunks in the same order
+            float m = -__builtin_inff(), s = 0.f;
+            for (int c = lane_id(); c < a.chunks; c += 64) m = fmaxf(m, a.part[row * a.chunks + c].x);
+            m = ds_wave_max(m);
+            for (int c = lane_id(); c < a.chunks; c += 64) {
+                const float2 q = a.part[row * a.chunks + c];
+                const float d = q.x == m ? 0.f : q.x - m;      // also where both are infinite
+                s += q.y * __builtin_amdgcn_exp2f(d * (inv_t * DS_LOG2E));
+            }
+            s = ds_wave_sum(s);
+            if (lane_id() == 0) { sh_m = m; sh_s = m == -__builtin_inff() ? __builtin_nanf("") : s; }
+        }
+    }
+    __syncthreads();
+    if (!sh_any) {
+        if (FORWARD && chunk == 0 && tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
+        if (grad) ds_zero(grad, v0, v1, tid, DS_CHUNK_BLOCK);
+        return;
+    }
+    const float m = FORWARD ? sh_m : 0.f, s = FORWARD ? sh_s : 1.f, lse = FORWARD ? 0.f : a.lse_in[row];
+    if (FORWARD && chunk == 0 && wave_id() == 0) {
+        const float log_s = logf(s), l = ds_row_loss(a, e, te.log_sum, inv_t, m, log_s);
+        if (tid == 0) {
+            a.loss[row] = w * (a.temperature * a.temperature) * l;
+            a.lse[row] = m * inv_t + log_s;
+        }
+    }
+    if (!grad) return;
+    const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale), cq = FORWARD ? c / s : c;
+    const float f = inv_t * DS_LOG2E;
+    auto relative = [&](float zi) {
+        return __builtin_amdgcn_exp2f(FORWARD ? (zi - m) * f : (zi * inv_t - lse) * DS_LOG2E);
+    };
+#pragma unroll
+    for (int i = 0; i < DS_CHUNK_NV; ++i) {
+        const long long v = v0 + (tid + DS_CHUNK_BLOCK * i) * W, left = a.V - v;
+        float q[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) q[j] = cq * relative(x[i][j]);
+        x[i].set(q);
+        x[i].store(grad + v, left > W ? W : (int)left);
+    }
+    __syncthreads();
+    ds_listed(a, e, sh_t, c, grad, v0, v1, tid, DS_CHUNK_BLOCK, [&](float zi) { return relative(zi) / s; });
+}
+
+// ---- host --------------------------------------------------------------------------------------------
+// rows that one workgroup can hold, and long rows of which there are too few to fill the chip
+static long long ds_vectors(int V, int dtype) { return (V + (dtype == FRCNN_DT_F32 ? 4 : 8) - 1) / (dtype == FRCNN_DT_F32 ? 4 : 8); }
+static long long ds_chunks(int V, int dtype) {
+    return (ds_vectors(V, dtype) + DS_CHUNK_BLOCK * DS_CHUNK_NV - 1) / (DS_CHUNK_BLOCK * DS_CHUNK_NV);
+}
+static bool ds_split(long long rows, int V, int dtype) {
+    const long long chunks = ds_chunks(V, dtype);
+    return ds_vectors(V, dtype) > 16384 || (chunks >= 4 && rows * chunks <= 1024);
+}
+static int ds_group(int V, int k) {
+    int g = 1;
+    while (g < V || g < k) g *= 2;
+    return g;
+}
+
+template <typename T, bool FORWARD, int G>
+static int ds_launch_small(const DsArgs& a, hipStream_t s) {
+    const long long blocks = (a.rows + 256 / G - 1) / (256 / G);
+    if (blocks > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
+    FRCNN_LAUNCH((distill_small_kernel<T, FORWARD, G>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    return FRCNN_OK;
+}
+template <typename T, int BLOCK, int NV>
+static int ds_launch_row(const DsArgs& a, hipStream_t s) {
     if (a.rows > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
-    FRCNN_LAUNCH((distill_row_kernel<T, U, FORWARD, 256>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+    FRCNN_LAUNCH((distill_row_kernel<T, BLOCK, NV>), dim3((unsigned)a.rows), dim3(BLOCK), (size_t)a.k * 12, s, a);
+    return FRCNN_OK;
+}
+
+template <typename T, bool FORWARD>
+static int ds_run(DsArgs a, int dtype, hipStream_t s) {
+    const int g = ds_group(a.V, a.k);
+    if (g <= 8) return ds_launch_small<T, FORWARD, 8>(a, s);
+    if (g <= 16) return ds_launch_small<T, FORWARD, 16>(a, s);
+    if (g <= 32) return ds_launch_small<T, FORWARD, 32>(a, s);
+    if (g <= 64) return ds_launch_small<T, FORWARD, 64>(a, s);
+    const long long n = ds_vectors(a.V, dtype);
+    a.chunks = (int)ds_chunks(a.V, dtype);
+    if (FORWARD && !ds_split(a.rows, a.V, dtype)) {
+        if (n <= 64) return ds_launch_row<T, 64, 1>(a, s);
+        if (n <= 256) return ds_launch_row<T, 64, 4>(a, s);
+        if (n <= 1024) return ds_launch_row<T, 256, 4>(a, s);
+        if (n <= 4096) return ds_launch_row<T, 1024, 4>(a, s);
+        if (n <= 8192) return ds_launch_row<T, 1024, 8>(a, s);
+        return ds_launch_row<T, 1024, 16>(a, s);
+    }
+    // rows along the grid's second dimension, at most 65,535 in a launch
+    for (long long r = 0; r < a.rows; r += 65535) {
+        DsArgs b = a;
+        b.rows = a.rows - r < 65535 ? a.rows - r : 65535;
+        b.z = (const T*)a.z + r * a.ldz;
+        b.t = (const char*)a.t + r * a.k * (a.t_f32 ? 4 : (long long)sizeof(T));
+        b.idx = a.idx + r * a.k;
+        if (a.weight) b.weight = a.weight + r;
+        if (a.d_loss) b.d_loss = a.d_loss + r;
+        if (a.lse_in) b.lse_in = a.lse_in + r;
+        if (a.loss) { b.loss = a.loss + r; b.lse = a.lse + r; }
+        if (a.grad) b.grad = (T*)a.grad + r * a.ldg;
+        if (a.part) b.part = a.part + r * a.chunks;
+        const dim3 grid((unsigned)a.chunks, (unsigned)b.rows);
+        if (FORWARD) FRCNN_LAUNCH((distill_part_kernel<T>), grid, dim3(DS_CHUNK_BLOCK), 0, s, b);
+        const dim3 gg(a.grad ? (unsigned)a.chunks : 1u, (unsigned)b.rows);      // without a gradient: the loss alone
+        FRCNN_LAUNCH((distill_chunk_kernel<T, FORWARD>), gg, dim3(DS_CHUNK_BLOCK), (size_t)a.k * 12, s, b);
+    }
     return FRCNN_OK;
 }
 
 template <bool FORWARD>
-static int ds_dispatch(const DsArgs& a, int dtype, int t_dtype, hipStream_t s) {
-    if (dtype == FRCNN_DT_F32) return ds_launch<float, float, FORWARD>(a, s);
-    if (dtype == FRCNN_DT_F16)
-        return t_dtype == FRCNN_DT_F32 ? ds_launch<_Float16, float, FORWARD>(a, s)
-                                       : ds_launch<_Float16, _Float16, FORWARD>(a, s);
-    return t_dtype == FRCNN_DT_F32 ? ds_launch<__bf16, float, FORWARD>(a, s)
-                                   : ds_launch<__bf16, __bf16, FORWARD>(a, s);
+static int ds_dispatch(const DsArgs& a, int dtype, hipStream_t s) {
+    if (dtype == FRCNN_DT_F32) return ds_run<float, FORWARD>(a, dtype, s);
+    if (dtype == FRCNN_DT_F16) return ds_run<_Float16, FORWARD>(a, dtype, s);
+    return ds_run<__bf16, FORWARD>(a, dtype, s);
 }
 
 static int ds_check(const void* z, int64_t ldz, int dtype, const void* t, int t_dtype, const int64_t* idx,
@@ -178,18 +535,27 @@ static int ds_check(const void* z, int64_t ldz, int dtype, const void* t, int t_
 
 using namespace frcnn;
 
+extern "C" size_t frcnn_distill_workspace_bytes(int64_t rows, int V, int k, int dtype) {
+    if (rows <= 0 || V <= 0 || k <= 0 || ds_group(V, k) <= 64 || !ds_split(rows, V, dtype)) return 0;
+    return (size_t)rows * (size_t)ds_chunks(V, dtype) * sizeof(float2);
+}
+
 extern "C" int frcnn_distill_loss(const void* logits, int64_t ldz, int dtype, const void* top_values, int t_dtype,
                                   const int64_t* top_index, const float* weight, int64_t rows, int V, int k,
                                   float temperature, float grad_scale, float* loss, float* lse, void* d_logits,
-                                  int64_t ldg, frcnn_stream_t stream) {
+                                  int64_t ldg, void* workspace, size_t workspace_bytes, frcnn_stream_t stream) {
     const int rc = ds_check(logits, ldz, dtype, top_values, t_dtype, top_index, rows, V, k, temperature);
     if (rc != FRCNN_OK || rows == 0) return rc;
     if (!loss || !lse || (d_logits && ldg < V)) return FRCNN_E_BADARG;
+    const size_t need = frcnn_distill_workspace_bytes(rows, V, k, dtype);
+    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8))
+        return FRCNN_E_WORKSPACE;
     DsArgs a{};
     a.z = logits; a.ldz = ldz; a.t = top_values; a.idx = top_index; a.weight = weight; a.scale = grad_scale;
     a.temperature = temperature; a.rows = rows; a.V = V; a.k = k;
-    a.loss = loss; a.lse = lse; a.grad = d_logits; a.ldg = ldg;
-    return ds_dispatch<true>(a, dtype, t_dtype, (hipStream_t)stream);
+    a.loss = loss; a.lse = lse; a.grad = d_logits; a.ldg = ldg; a.t_f32 = t_dtype == FRCNN_DT_F32;
+    a.part = (float2*)workspace;
+    return ds_dispatch<true>(a, dtype, (hipStream_t)stream);
 }
 
 extern "C" int frcnn_distill_bwd(const float* d_loss, const void* logits, int64_t ldz, int dtype,
@@ -202,6 +568,6 @@ extern "C" int frcnn_distill_bwd(const float* d_loss, const void* logits, int64_
     DsArgs a{};
     a.z = logits; a.ldz = ldz; a.t = top_values; a.idx = top_index; a.weight = weight; a.d_loss = d_loss;
     a.lse_in = lse; a.temperature = temperature; a.rows = rows; a.V = V; a.k = k;
-    a.grad = d_logits; a.ldg = ldg;
-    return ds_dispatch<false>(a, dtype, t_dtype, (hipStream_t)stream);
+    a.grad = d_logits; a.ldg = ldg; a.t_f32 = t_dtype == FRCNN_DT_F32;
+    return ds_dispatch<false>(a, dtype, (hipStream_t)stream);
 }

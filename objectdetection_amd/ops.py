@@ -20,7 +20,7 @@ __all__ = [
     "nms_workspace_bytes", "roi_crop_pool_fwd", "roi_crop_pool_bwd", "label_proposals",
     "sample_proposals", "detect_postprocess", "fc1_fwd",
     "dense_fwd", "dense_bwd", "dense_fwd_workspace_bytes", "dense_bwd_workspace_bytes",
-    "distill_loss", "distill_bwd",
+    "distill_loss", "distill_bwd", "distill_workspace_bytes",
 ]
 
 
@@ -792,9 +792,14 @@ def _distill_args(logits, top_values, top_index, weight, temperature):
     return z, top_values.contiguous(), top_index.contiguous(), weight, lead, rows, V, k
 
 
+def distill_workspace_bytes(rows: int, V: int, k: int, dtype: torch.dtype) -> int:
+    return int(lib.frcnn_distill_workspace_bytes(rows, V, k, _DT[dtype]))
+
+
 def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torch.Tensor,
                  weight: Optional[torch.Tensor] = None, temperature: float = 1.0,
-                 want_grad: bool = True, grad_scale: float = 1.0):
+                 want_grad: bool = True, grad_scale: float = 1.0,
+                 workspace: Optional[torch.Tensor] = None):
     """Distillation from a teacher's stored top logits (frcnn_distill_loss).
 
     logits [..., V] (float32, float16 or bfloat16), top_values [..., k] (the same type or float32)
@@ -802,17 +807,20 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torc
     [0,V) and a logit of -inf: no entry), weight [...] float32 or None (0: the row takes no part).
     With p the teacher's softmax over its entries and q the student's over all V, both at
     `temperature` T, returns dict(loss [...] = weight T^2 KL(p || q), lse [...], d_logits: the
-    gradient of grad_scale * loss.sum() in logits, None unless want_grad)."""
+    gradient of grad_scale * loss.sum() in logits, None unless want_grad).  workspace: uint8 of
+    distill_workspace_bytes(rows, V, k, dtype)."""
     z, tv, ti, wt, lead, rows, V, k = _distill_args(logits, top_values, top_index, weight, temperature)
     dev = z.device
     loss = torch.empty(lead, dtype=torch.float32, device=dev)
     lse = torch.empty(lead, dtype=torch.float32, device=dev)
     grad = torch.empty(logits.shape, dtype=z.dtype, device=dev) if want_grad else None
+    ws = _scratch(workspace, lib.frcnn_distill_workspace_bytes(rows, V, k, _DT[z.dtype]), dev)
     with _on(dev):
         check("frcnn_distill_loss", lib.frcnn_distill_loss(
             z.data_ptr(), _ld(z), _DT[z.dtype], tv.data_ptr(), _DT[tv.dtype], ti.data_ptr(),
             None if wt is None else wt.data_ptr(), rows, V, k, temperature, grad_scale, loss.data_ptr(),
-            lse.data_ptr(), None if grad is None else grad.data_ptr(), V, _raw_stream(dev)))
+            lse.data_ptr(), None if grad is None else grad.data_ptr(), V,
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _raw_stream(dev)))
     return dict(loss=loss, lse=lse, d_logits=grad)
 
 

@@ -59,8 +59,8 @@ def test_dense_workspaces(L):
 
 
 def loss(L, z=ONE, ldz=50, dt=0, t=ONE, tdt=0, idx=ONE, w=None, rows=3, V=50, k=4, T=1.0, g=1.0, l=ONE, lse=ONE,
-         d=None, ldg=50):
-    return L.lib.frcnn_distill_loss(z, ldz, dt, t, tdt, idx, w, rows, V, k, T, g, l, lse, d, ldg, None)
+         d=None, ldg=50, ws=None, wsb=0):
+    return L.lib.frcnn_distill_loss(z, ldz, dt, t, tdt, idx, w, rows, V, k, T, g, l, lse, d, ldg, ws, wsb, None)
 
 
 @pytest.mark.parametrize("bad", [
@@ -80,6 +80,13 @@ def test_distillation_refuses(L, bad):
 
 def test_distillation_limits(L):
     assert loss(L, k=L.DISTILL_MAX_K + 1) == L.E_UNSUPPORTED
+    need = L.lib.frcnn_distill_workspace_bytes
+    assert need(128000, 21, 8, 0) == 0 and need(4096, 65536, 64, 2) == 0 and need(0, 1 << 20, 8, 0) == 0
+    big = need(1, 131072, 64, 0)
+    assert big > 0
+    wide = dict(rows=1, V=131072, k=64, ldz=131072)
+    assert loss(L, **wide) == L.E_WORKSPACE and loss(L, ws=ONE, wsb=big - 1, **wide) == L.E_WORKSPACE
+    assert loss(L, ws=ctypes.c_void_p(20), wsb=big, **wide) == L.E_WORKSPACE
     assert loss(L, rows=0, z=None, t=None, idx=None) == L.OK
 
 

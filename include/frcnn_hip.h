@@ -413,8 +413,12 @@ int frcnn_fc1_fwd(const float* x, const float* w, const float* bias, int64_t M, 
  *   w_layout   FRCNN_W_KN: W is [K,N] rows of ldw >= N elements (a Keras kernel),
  *              FRCNN_W_NK: W is stored as [N,K] rows of ldw >= K elements (a torch Linear weight);
  *   out_dtype  dtype or FRCNN_DT_F32;   d_dtype likewise for d_out;
- *   ld*        elements between rows, at least the row's length; any alignment is taken (rows of
- *              16-byte aligned whole 16-byte pieces are the fast layout);
+ *   ld*        elements between rows, at least the row's length; any alignment is taken: an operand
+ *              of a product whose rows are not whole 16-byte pieces starting on 16 bytes is copied
+ *              to the workspace first (not for calls of up to 32 rows);
+ *   aligned    of the workspace sizes: bit 0 x, bit 1 W starts on 16 bytes with a row stride of a
+ *              multiple of 8 up to 2,097,152; bit 2 (backward) d_out does, is of type dtype and act
+ *              is FRCNN_ACT_NONE.  A bit left out asks for more than needed;
  *   bias, residual, pre may be NULL (pre: the pre-activations, rounded, which the backward needs
  *              for an activation other than FRCNN_ACT_NONE).
  * M = 0 is allowed (no forward output; d_w and d_bias become 0).
@@ -429,7 +433,7 @@ int frcnn_fc1_fwd(const float* x, const float* w, const float* bias, int64_t M, 
 #define FRCNN_ACT_SILU 3
 #define FRCNN_W_KN     0
 #define FRCNN_W_NK     1
-size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N);
+size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned);
 int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int w_layout,
                     const void* bias, const void* residual, int64_t ldr, int64_t M, int K, int N,
                     int dtype, int act, void* out, int64_t ldo, int out_dtype, void* pre,
@@ -439,7 +443,7 @@ int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int 
  * pre > 0, else 0);  d_x = dz W^T,  d_w = x^T dz in W's layout,  d_bias = sum of dz over the rows
  * (of the unrounded float32 values).  d_x, d_w, d_bias: NULL where not wanted, not all three.  The
  * residual's gradient is d_out itself. */
-size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N);
+size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned);
 int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, const void* x, int64_t ldx,
                     const void* w, int64_t ldw, int w_layout, const void* pre, int64_t ldp,
                     int64_t M, int K, int N, int dtype, int act, void* d_x, int64_t lddx,

@@ -83,10 +83,10 @@ _SIGS = {
     "frcnn_pad_gt": (_i, [_p, _p, _p, _p, _i, _u64, _i, _i, _i, _p, _p, _p, _p]),
     "frcnn_flip_images": (_i, [_p, _p, _u64, _i, _i, _i, _i, _i, _p, _p]),
     "frcnn_fc1_fwd": (_i, [_p, _p, _p, _i64, _i, _i, _i, _p, _p]),
-    "frcnn_dense_fwd_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "frcnn_dense_fwd_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i]),
     "frcnn_dense_fwd": (_i, [_p, _i64, _p, _i64, _i, _p, _p, _i64, _i64, _i, _i, _i, _i, _p, _i64,
                              _i, _p, _i64, _p, _sz, _p]),
-    "frcnn_dense_bwd_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "frcnn_dense_bwd_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i]),
     "frcnn_dense_bwd": (_i, [_p, _i64, _i, _p, _i64, _p, _i64, _i, _p, _i64, _i64, _i, _i, _i, _i,
                              _p, _i64, _p, _i64, _p, _p, _sz, _p]),
     "frcnn_distill_workspace_bytes": (_sz, [_i64, _i, _i, _i]),

@@ -16,6 +16,7 @@
 // added in slice order, so a call always gives the same bits.  The epilogue works on the float32
 // sums: each output is rounded once.
 #include "frcnn_common.h"
+#include <atomic>
 
 namespace frcnn {
 
@@ -135,6 +136,7 @@ struct DnEpilogue {
 struct DnGemm {
     const void *a, *b;
     long long lda, ldb, I, J, K;
+    long long outer_a, outer_b;   // I, J rounded up to whole pieces where the operand's rows are that long
     long long k_slice;        // k per slice, a multiple of DN_BK
     int splits, tiles_i, tiles_j;
     float* partial;           // [splits][I][Jp], Jp = J rounded up to 4, when splits > 1
@@ -174,57 +176,6 @@ __device__ __forceinline__ int dn_swizzle(int r, int c) {
     if constexpr (KC) return c ^ ((r >> 1) & 7);                              // [R][8 pieces of 8 k]
     constexpr int m = R >= 128 ? 7 : R / 16 - 1;                              // [BK][R / 8 pieces]
     return c ^ ((((r & 3) | ((r >> 1) & 4)) & m) << 1);
-}
-
-// One operand's tile, `outer0 ..` by `k0 ..`, from memory into registers (zeros outside) and on into LDS.
-template <typename T, bool KC, int R, int NT>
-struct DnStage {
-    static constexpr int NP = R * 8 / NT;       // 16-byte pieces per thread
-    dn_s16x8 v[NP];
-    __device__ __forceinline__ void load(const T* p, long long ld, long long outer0, long long outer_end,
-                                         long long k0, long long k_end) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int idx = (int)threadIdx.x + NT * i;
-            if constexpr (KC) {
-                const long long o = outer0 + idx / 8, k = k0 + 8 * (idx % 8);
-                const long long left = o < outer_end ? k_end - k : 0;
-                v[i] = dn_load8(p + o * ld + k, left > 8 ? 8 : (int)left);
-            } else {
-                const long long k = k0 + idx / (R / 8), o = outer0 + 8 * (idx % (R / 8));
-                const long long left = k < k_end ? outer_end - o : 0;
-                v[i] = dn_load8(p + k * ld + o, left > 8 ? 8 : (int)left);
-            }
-        }
-    }
-    __device__ __forceinline__ void store(dn_s16x8* lds) const {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int idx = (int)threadIdx.x + NT * i;
-            constexpr int P = KC ? 8 : R / 8;
-            const int r = idx / P, c = idx % P;
-            lds[r * P + dn_swizzle<KC, R, DN_BK>(r, c)] = v[i];
-        }
-    }
-};
-
-// fragment of outer rows o0 .. o0 + 15 (o0 a multiple of 16), k = 32 kk .. 32 kk + 31: lane l holds
-// row l % 16, k 8 (l / 16) .. + 7
-template <bool KC, int R, int BK>
-__device__ __forceinline__ dn_s16x8 dn_fragment(const dn_s16x8* lds, int o0, int kk) {
-    const int lane = lane_id(), g = lane >> 4, l = lane & 15;
-    if constexpr (KC) {
-        const int r = o0 + l;
-        return lds[r * (BK / 8) + dn_swizzle<true, R, BK>(r, kk * 4 + g)];
-    } else {
-        const int k = kk * 32 + g * 8 + (l >> 2), c = o0 / 8 + ((l & 3) >> 1);
-        const short* base = reinterpret_cast<const short*>(lds);
-        const short* p0 = base + (k * (R / 8) + dn_swizzle<false, R, BK>(k, c)) * 8 + (l & 1) * 4;
-        const short* p1 = base + ((k + 4) * (R / 8) + dn_swizzle<false, R, BK>(k + 4, c)) * 8 + (l & 1) * 4;
-        const dn_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((dn_lds_s16x4*)p0);
-        const dn_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((dn_lds_s16x4*)p1);
-        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
 }
 
 // workgroup id -> tile: every XCD (id % 8) gets a contiguous run of tiles, and a run walks groups of
@@ -278,60 +229,7 @@ __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&a
     }
 }
 
-// WI x WJ waves, each (BI / WI) x (BJ / WJ) outputs.  The MFMA's rows are j and its columns i, so that
-// a lane ends with four neighbouring outputs of one row.
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
-__global__ void __launch_bounds__(64 * WI * WJ)
-dense_gemm_kernel(DnGemm p) {
-    constexpr int NT = 64 * WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
-    extern __shared__ __attribute__((aligned(16))) char dn_lds[];
-    dn_s16x8* lds_a = reinterpret_cast<dn_s16x8*>(dn_lds);
-    dn_s16x8* lds_b = lds_a + BI * 8;
-    int ti, tj, slice;
-    dn_tile(p, ti, tj, slice);
-    const long long i0 = (long long)ti * BI, j0 = (long long)tj * BJ;
-    const long long k0 = slice * p.k_slice;
-    const long long k_end = k0 + p.k_slice < p.K ? k0 + p.k_slice : p.K;
-    const int wave = wave_id(), wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
-
-    dn_f32x4 acc[FI][FJ];
-#pragma unroll
-    for (int i = 0; i < FI; ++i)
-#pragma unroll
-        for (int j = 0; j < FJ; ++j) acc[i][j] = dn_f32x4{0.f, 0.f, 0.f, 0.f};
-
-    DnStage<T, AKC, BI, NT> sa;
-    DnStage<T, BKC, BJ, NT> sb;
-    sa.load((const T*)p.a, p.lda, i0, p.I, k0, k_end);
-    sb.load((const T*)p.b, p.ldb, j0, p.J, k0, k_end);
-#pragma unroll 1
-    for (long long k = k0; k < k_end; k += DN_BK) {
-        sa.store(lds_a);
-        sb.store(lds_b);
-        __syncthreads();
-        if (k + DN_BK < k_end) {
-            sa.load((const T*)p.a, p.lda, i0, p.I, k + DN_BK, k_end);
-            sb.load((const T*)p.b, p.ldb, j0, p.J, k + DN_BK, k_end);
-        }
-#pragma unroll
-        for (int kk = 0; kk < DN_BK / 32; ++kk) {
-            dn_s16x8 fa[FI], fb[FJ];
-#pragma unroll
-            for (int i = 0; i < FI; ++i) fa[i] = dn_fragment<AKC, BI, DN_BK>(lds_a, wi + 16 * i, kk);
-#pragma unroll
-            for (int j = 0; j < FJ; ++j) fb[j] = dn_fragment<BKC, BJ, DN_BK>(lds_b, wj + 16 * j, kk);
-#pragma unroll
-            for (int i = 0; i < FI; ++i)
-#pragma unroll
-                for (int j = 0; j < FJ; ++j) acc[i][j] = dn_mfma(fb[j], fa[i], acc[i][j], T());
-        }
-        __syncthreads();
-    }
-
-    dn_write_out<T, FI, FJ>(p, acc, slice, i0 + wi, j0 + wj, dn_lds + wave * dn_turn_bytes<FJ>());
-}
-
-// ---- the product on aligned operands ----------------------------------------------------------------
+// ---- the product -----------------------------------------------------------------------------------------
 // Tiles go from memory to LDS directly (global_load_lds, 16 bytes per lane, the swizzle applied to the
 // source address because the destination is linear in the lane).  The reduction is walked in steps of 32 k:
 // while the fragments of step s, already in registers, are multiplied, those of step s + 1 are read from
@@ -436,7 +334,7 @@ struct DnReader {
 
 template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
 __global__ void __launch_bounds__(64 * WI * WJ)
-dense_gemm_lds_kernel(DnGemm p) {
+dense_gemm_kernel(DnGemm p) {
     constexpr int NT = 64 * WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
     constexpr int READS = FI * (AKC ? 1 : 2) + FJ * (BKC ? 1 : 2);  // LDS reads per wave and step
     extern __shared__ __attribute__((aligned(16))) char dn_lds[];    // A's ring, then B's
@@ -461,8 +359,8 @@ dense_gemm_lds_kernel(DnGemm p) {
     constexpr int OTHER = (AKC ? CopyA::NP : 0) + (BKC ? CopyB::NP : 0);
     CopyA ca;
     CopyB cb;
-    ca.init((const T*)p.a, p.lda, i0, p.I, k0);
-    cb.init((const T*)p.b, p.ldb, j0, p.J, k0);
+    ca.init((const T*)p.a, p.lda, i0, AKC ? p.I : p.outer_a, k0);
+    cb.init((const T*)p.b, p.ldb, j0, BKC ? p.J : p.outer_b, k0);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dn_lds;
     const uint32_t la = lds0 + (uint32_t)wave * 1024u, lb = la + BI * DN_SK * 2 * DN_RING;
     DnReader<AKC, BI> qa;
@@ -551,15 +449,165 @@ dense_gemm_lds_kernel(DnGemm p) {
     dn_write_out<T, FI, FJ>(p, acc, slice, i0 + wi, j0 + wj, dn_lds + wave * dn_turn_bytes<FJ>());
 }
 
+// ---- few rows ------------------------------------------------------------------------------------------
+// Up to 32 rows (I): the product reads B once and little else, so what counts is how soon and how wide the
+// loads of B leave.  A workgroup owns 16 (k contiguous) or 32 (outer contiguous) columns and its eight waves
+// share out the reduction in pieces of 64 k: a wave's load covers whole 128-byte lines of 16 rows of B, or
+// 64-byte pieces of 16 k, and the next piece is loaded while the present one is multiplied.  A fragment of A
+// comes straight from memory (every workgroup reads the same few rows: L2).  An outer-contiguous piece is
+// turned round by the transposing LDS read in the wave's own LDS.  The eight sums are added in wave order.
+// The MFMA's k order is free as long as both operands agree: lane group g takes k 16 g .. 16 g + 15 of a
+// piece in two instructions (k contiguous), or 8 g .. 8 g + 7 of each half.
+constexpr int DN_FEW = 32, DN_FW = 8;           // most rows; waves
+
+template <typename T, bool BKC, int MB>
+__global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
+    constexpr int JB = BKC ? 1 : 2, NL = BKC ? 2 : 4;             // 16-column blocks; loads of B per piece and lane
+    __shared__ dn_f32x4 sums[DN_FW][JB * MB][64];
+    __shared__ dn_s16x8 turn[BKC ? 1 : DN_FW][BKC ? 1 : 256];     // [64 k][4 pieces of 8 columns] per wave
+    const int lane = lane_id(), wave = wave_id(), g = lane >> 4, l = lane & 15;
+    const long long j0 = (long long)blockIdx.x * (16 * JB);
+    const int slice = blockIdx.y;
+    const long long k0 = slice * p.k_slice, k_end = k0 + p.k_slice < p.K ? k0 + p.k_slice : p.K;
+    const T* A = (const T*)p.a;
+    const T* B = (const T*)p.b;
+    const T* rows[MB];
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+        const long long i = 16 * m + l;
+        rows[m] = A + (i < p.I ? i : p.I - 1) * p.lda;
+    }
+    const long long jl = j0 + l < p.J ? j0 + l : p.J - 1;         // k contiguous: this lane's row of B
+    const bool inner = BKC || j0 + 16 * JB <= p.J;                // whole pieces in every lane
+    const int jv = (int)(p.J - j0 - 8 * (lane & 3) < 8 ? p.J - j0 - 8 * (lane & 3) : 8);
+
+    dn_s16x8 b[NL], a[MB][2], nb[NL], na[MB][2];
+    auto load = [&](long long k, dn_s16x8 (&rb)[NL], dn_s16x8 (&ra)[MB][2]) {
+        if (k + 64 <= k_end && inner) {                // no guard at all: the loads leave back to back
+#pragma unroll
+            for (int h = 0; h < NL; ++h) {
+                const T* q = BKC ? B + jl * p.ldb + k + 16 * g + 8 * h
+                                 : B + (k + 16 * h + (lane >> 2)) * p.ldb + j0 + 8 * (lane & 3);
+                __builtin_memcpy(&rb[h], q, 16);
+            }
+#pragma unroll
+            for (int m = 0; m < MB; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    __builtin_memcpy(&ra[m][h], rows[m] + k + (BKC ? 16 * g + 8 * h : 32 * h + 8 * g), 16);
+            return;
+        }
+        auto at = [&](const T* q, long long kk) {
+            const long long left = k_end - kk;
+            return dn_load8(q + kk, left > 8 ? 8 : (int)left);
+        };
+#pragma unroll
+        for (int h = 0; h < NL; ++h) {
+            if constexpr (BKC) {
+                rb[h] = at(B + jl * p.ldb, k + 16 * g + 8 * h);
+            } else {
+                const long long kk = k + 16 * h + (lane >> 2);
+                rb[h] = dn_load8(B + kk * p.ldb + j0 + 8 * (lane & 3), kk < k_end ? jv : 0);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) ra[m][h] = at(rows[m], k + (BKC ? 16 * g + 8 * h : 32 * h + 8 * g));
+    };
+    dn_f32x4 acc[JB][MB];
+#pragma unroll
+    for (int j = 0; j < JB; ++j)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) acc[j][m] = dn_f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](dn_s16x8 (&rb)[NL], dn_s16x8 (&ra)[MB][2]) {
+        if constexpr (BKC) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int m = 0; m < MB; ++m) acc[0][m] = dn_mfma(rb[h], ra[m][h], acc[0][m], T());
+        } else {
+            // row k, 32-byte half c / 2 exchanged where k has bit 3: two lane groups meet no bank twice
+            dn_s16x8* lds = turn[wave];
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int h = 0; h < NL; ++h) {
+                const int k = 16 * h + (lane >> 2), c = lane & 3;
+                lds[k * 4 + (c ^ ((k >> 2) & 2))] = rb[h];
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < JB; ++j) {
+                    const int k = 32 * h + 8 * g + (l >> 2), c = (2 * j + ((l & 3) >> 1)) ^ ((k >> 2) & 2);
+                    const short* q = reinterpret_cast<const short*>(lds) + (k * 4 + c) * 8 + (l & 1) * 4;
+                    const dn_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((dn_lds_s16x4*)q);
+                    const dn_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((dn_lds_s16x4*)(q + 4 * 32));
+                    const dn_s16x8 f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                    for (int m = 0; m < MB; ++m) acc[j][m] = dn_mfma(f, ra[m][h], acc[j][m], T());
+                }
+        }
+    };
+    long long k = k0 + 64 * wave;
+    if (k < k_end) load(k, b, a);
+#pragma unroll 1
+    while (k < k_end) {
+        const long long next = k + 64 * DN_FW;
+        if (next < k_end) load(next, nb, na);
+        multiply(b, a);
+#pragma unroll
+        for (int h = 0; h < NL; ++h) b[h] = nb[h];
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) a[m][h] = na[m][h];
+        k = next;
+    }
+#pragma unroll
+    for (int j = 0; j < JB; ++j)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) sums[wave][j * MB + m][lane] = acc[j][m];
+    __syncthreads();
+    if (wave >= JB * MB) return;
+    dn_f32x4 v = sums[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < DN_FW; ++w) {
+        const dn_f32x4 o = sums[w][wave][lane];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += o[r];
+    }
+    const long long i = 16 * (wave % MB) + l, j = j0 + 16 * (wave / MB) + 4 * g, left = p.J - j;
+    if (i >= p.I || left <= 0) return;
+    if (p.partial) {
+        const long long Jp = (p.J + 3) / 4 * 4;
+        *reinterpret_cast<dn_f32x4*>(p.partial + (slice * p.I + i) * Jp + j) = v;
+    } else {
+        float o[4] = {v[0], v[1], v[2], v[3]};
+        dn_epilogue<T, 4>(p.e, i, j, left > 4 ? 4 : (int)left, o);
+    }
+}
+
 // sums of a split product's slices, in slice order, and the epilogue; four outputs per thread
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(64)
 dense_join_kernel(const float* __restrict__ partial, int splits, long long I, long long J, DnEpilogue e) {
-    const long long q = (J + 3) / 4, id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long q = (J + 3) / 4, id = (long long)blockIdx.x * 64 + threadIdx.x;
     if (id >= I * q) return;
     const long long i = id / q, j = (id - i * q) * 4, stride = I * q * 4;
     dn_f32x4 v = *reinterpret_cast<const dn_f32x4*>(partial + id * 4);
-    for (int s = 1; s < splits; ++s) {
+    int s = 1;
+    for (; s + 8 <= splits; s += 8) {                  // eight slices on their way at once
+        dn_f32x4 w[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) w[q] = *reinterpret_cast<const dn_f32x4*>(partial + (s + q) * stride + id * 4);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += w[q][r];
+    }
+    for (; s < splits; ++s) {
         const dn_f32x4 w = *reinterpret_cast<const dn_f32x4*>(partial + s * stride + id * 4);
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] += w[r];
@@ -567,6 +615,20 @@ dense_join_kernel(const float* __restrict__ partial, int splits, long long I, lo
     const long long left = J - j;
     float o[4] = {v[0], v[1], v[2], v[3]};
     dn_epilogue<T, 4>(e, i, j, left > 4 ? 4 : (int)left, o);
+}
+
+// ---- operands whose rows are not whole 16-byte pieces --------------------------------------------------
+// are copied once to rows that are, with zeros behind their end; one launch for both of a product's
+struct DnPack { const void* src; void* dst; long long rows, cols, ld, pieces; };   // pieces of 8 per row of dst
+template <typename T>
+__global__ void __launch_bounds__(256) dense_pack_kernel(DnPack a, DnPack b, long long blocks_a) {
+    const bool first = (long long)blockIdx.x < blocks_a;
+    const DnPack p = first ? a : b;
+    const long long id = ((long long)blockIdx.x - (first ? 0 : blocks_a)) * 256 + threadIdx.x;
+    if (id >= p.rows * p.pieces) return;
+    const long long r = id / p.pieces, c = 8 * (id - r * p.pieces), left = p.cols - c;
+    const dn_s16x8 v = dn_load8((const T*)p.src + r * p.ld + c, left > 8 ? 8 : (int)left);
+    reinterpret_cast<dn_s16x8*>(p.dst)[id] = v;
 }
 
 // ---- dz = d_out * act'(pre), and column sums per block of rows ----------------------------------------
@@ -633,8 +695,25 @@ __global__ void __launch_bounds__(256) dense_zero_kernel(T* p, long long rows, l
 // ---- host ------------------------------------------------------------------------------------------
 struct DnPlan { int bi, bj, splits; long long k_slice, tiles_i, tiles_j; size_t partial_bytes; };
 
-static DnPlan dn_plan(long long I, long long J, long long K) {
+// akc: A is k-contiguous (the forward and d_x); only those products have few rows
+static DnPlan dn_plan(long long I, long long J, long long K, bool akc, bool bkc) {
     DnPlan p{};
+    if (akc && I <= DN_FEW) {
+        // one workgroup per 16 or 32 columns; a long reduction is split where that leaves compute units idle
+        p.bi = 0;
+        p.bj = bkc ? 16 : 32;
+        p.tiles_i = 1;
+        p.tiles_j = (J + p.bj - 1) / p.bj;
+        const long long pieces = (K + 64 * DN_FW - 1) / (64 * DN_FW);
+        long long splits = pieces >= 16 ? DN_TARGET_WG / p.tiles_j : 1;
+        if (splits > pieces / 4) splits = pieces / 4;
+        if (splits < 1) splits = 1;
+        const long long per = (pieces + splits - 1) / splits;
+        p.k_slice = per * 64 * DN_FW;
+        p.splits = (int)((pieces + per - 1) / per);
+        p.partial_bytes = p.splits > 1 ? (size_t)p.splits * (size_t)I * (size_t)((J + 3) / 4 * 4) * 4 : 0;
+        return p;
+    }
     const long long big = ((I + 255) / 256) * ((J + 255) / 256);
     p.bi = p.bj = big >= DN_TARGET_WG / 2 ? 256 : 128;
     p.tiles_i = (I + p.bi - 1) / p.bi;
@@ -647,50 +726,93 @@ static DnPlan dn_plan(long long I, long long J, long long K) {
     const long long per = (steps + splits - 1) / splits;
     p.k_slice = per * DN_BK;
     p.splits = (int)((steps + per - 1) / per);         // no empty slice
-    if (p.splits < 1) p.splits = 1;
     p.partial_bytes = p.splits > 1 ? (size_t)p.splits * (size_t)I * (size_t)((J + 3) / 4 * 4) * 4 : 0;
     return p;
 }
 
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
-static int dn_launch_lds(const DnGemm& g, unsigned blocks, hipStream_t stream) {
-    constexpr int lds = DN_RING * (BI + BJ) * DN_SK * 2;
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(dense_gemm_lds_kernel<T, AKC, BKC, BI, BJ, WI, WJ>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
-        return FRCNN_E_LAUNCH;
-    FRCNN_LAUNCH((dense_gemm_lds_kernel<T, AKC, BKC, BI, BJ, WI, WJ>), dim3(blocks), dim3(64 * WI * WJ), lds, stream,
-                 g);
-    return FRCNN_OK;
+// lets a kernel use `bytes` of LDS on the current device; said once per kernel and device
+static bool dn_raise_lds(const void* kernel, int bytes, std::atomic<uint64_t>& raised) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return false;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (raised.load(std::memory_order_relaxed) & bit)) return true;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+    raised.fetch_or(bit, std::memory_order_relaxed);
+    return true;
 }
 
-// whether an operand can be copied to LDS in 16-byte pieces: rows that start on 16 bytes, whole pieces in
-// its contiguous dimension, and a tile whose rows are within 2 GiB of each other
-static bool dn_whole_pieces(const void* p, long long ld, bool kc, long long outer, long long K) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && (kc ? K : outer) % 8 == 0 && ld <= (1ll << 21);
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
+static int dn_launch_tiles(const DnGemm& g, unsigned blocks, hipStream_t stream) {
+    constexpr int lds = DN_RING * (BI + BJ) * DN_SK * 2;
+    static std::atomic<uint64_t> raised{0};
+    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ>), lds, raised))
+        return FRCNN_E_LAUNCH;
+    FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ>), dim3(blocks), dim3(64 * WI * WJ), lds, stream, g);
+    return FRCNN_OK;
 }
 
 template <typename T, bool AKC, bool BKC>
 static int dn_launch_gemm(const DnPlan& pl, const DnGemm& g, hipStream_t stream) {
+    if (pl.bi == 0) {
+        if (pl.tiles_j > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
+        if constexpr (AKC) {
+            const dim3 grid((unsigned)pl.tiles_j, (unsigned)pl.splits);
+            if (g.I <= 16) FRCNN_LAUNCH((dense_few_rows_kernel<T, BKC, 1>), grid, dim3(64 * DN_FW), 0, stream, g);
+            else FRCNN_LAUNCH((dense_few_rows_kernel<T, BKC, 2>), grid, dim3(64 * DN_FW), 0, stream, g);
+        }
+        return FRCNN_OK;
+    }
     const long long blocks = pl.tiles_i * pl.tiles_j * pl.splits;
     if (blocks > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
-    const bool whole = dn_whole_pieces(g.a, g.lda, AKC, g.I, g.K) && dn_whole_pieces(g.b, g.ldb, BKC, g.J, g.K);
-    if (whole && pl.bi == 256) return dn_launch_lds<T, AKC, BKC, 256, 256, 2, 4>(g, (unsigned)blocks, stream);
-    if (whole) return dn_launch_lds<T, AKC, BKC, 128, 128, 2, 2>(g, (unsigned)blocks, stream);
-    if (pl.bi == 256)
-        FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, 256, 256, 2, 4>), dim3((unsigned)blocks), dim3(512), 65536, stream, g);
-    else
-        FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, 128, 128, 2, 2>), dim3((unsigned)blocks), dim3(256), 32768, stream, g);
-    return FRCNN_OK;
+    if (pl.bi == 256) return dn_launch_tiles<T, AKC, BKC, 256, 256, 2, 4>(g, (unsigned)blocks, stream);
+    return dn_launch_tiles<T, AKC, BKC, 128, 128, 2, 2>(g, (unsigned)blocks, stream);
 }
 
+static size_t dn_up(size_t b) { return (b + 255) / 256 * 256; }
+
+// A matrix in memory as rows of `cols` values.  padded: its rows are whole pieces with zeros behind `cols`.
+struct DnMatrix { const void* p; long long rows, cols, ld; bool padded; };
+static long long dn_pieces(long long n) { return (n + 7) / 8; }
+// rows that start on 16 bytes, of whole 16-byte pieces, and a tile whose rows lie within 2 GiB of each other
+static bool dn_whole(const DnMatrix& m) {
+    return reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.ld % 8 == 0 && (m.padded || m.cols % 8 == 0) &&
+           m.ld <= (1ll << 21);
+}
+static size_t dn_pack_bytes(long long rows, long long cols) {
+    return dn_up((size_t)rows * (size_t)dn_pieces(cols) * 16);
+}
+
+// D = A B^T: `a` holds A as [I][K] (akc) or [K][I], `b` B as [J][K] (bkc) or [K][J].  Workspace: the packed
+// copies of the operands that need one, then the partial sums of a split reduction.
 template <typename T>
-static int dn_product(const void* a, long long lda, bool akc, const void* b, long long ldb, bool bkc, long long I,
-                      long long J, long long K, const DnEpilogue& e, void* ws, hipStream_t stream) {
-    const DnPlan pl = dn_plan(I, J, K);
-    DnGemm g{};
-    g.a = a; g.b = b; g.lda = lda; g.ldb = ldb; g.I = I; g.J = J; g.K = K;
-    g.k_slice = pl.k_slice; g.splits = pl.splits;
+static int dn_product(DnMatrix a, bool akc, DnMatrix b, bool bkc, const DnEpilogue& e, char* ws, hipStream_t stream) {
+    const long long I = akc ? a.rows : a.cols, K = akc ? a.cols : a.rows, J = bkc ? b.rows : b.cols;
+    const DnPlan pl = dn_plan(I, J, K, akc, bkc);
     if (pl.tiles_i > 0x7FFFFF || pl.tiles_j > 0x7FFFFF) return FRCNN_E_UNSUPPORTED;
+    if (pl.bi) {
+        DnPack pack[2] = {};
+        long long blocks[2] = {0, 0};
+        int n = 0;
+        for (DnMatrix* m : {&a, &b}) {
+            if (dn_whole(*m)) continue;
+            if (dn_pieces(m->cols) * 8 > (1ll << 21)) return FRCNN_E_UNSUPPORTED;
+            pack[n] = DnPack{m->p, ws, m->rows, m->cols, m->ld, dn_pieces(m->cols)};
+            blocks[n] = (m->rows * pack[n].pieces + 255) / 256;
+            ws += dn_pack_bytes(m->rows, m->cols);
+            *m = DnMatrix{pack[n].dst, m->rows, m->cols, pack[n].pieces * 8, true};
+            ++n;
+        }
+        if (n) {
+            if (blocks[0] + blocks[1] > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
+            FRCNN_LAUNCH(dense_pack_kernel<T>, dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), 0, stream, pack[0],
+                         pack[1], blocks[0]);
+        }
+    }
+    DnGemm g{};
+    g.a = a.p; g.b = b.p; g.lda = a.ld; g.ldb = b.ld; g.I = I; g.J = J; g.K = K;
+    g.outer_a = a.padded ? dn_pieces(I) * 8 : I;
+    g.outer_b = b.padded ? dn_pieces(J) * 8 : J;
+    g.k_slice = pl.k_slice; g.splits = pl.splits;
     g.tiles_i = (int)pl.tiles_i; g.tiles_j = (int)pl.tiles_j;
     g.partial = pl.splits > 1 ? (float*)ws : nullptr;
     g.e = e;
@@ -699,34 +821,40 @@ static int dn_product(const void* a, long long lda, bool akc, const void* b, lon
     else if (akc) rc = dn_launch_gemm<T, true, false>(pl, g, stream);
     else rc = dn_launch_gemm<T, false, false>(pl, g, stream);
     if (rc != FRCNN_OK || pl.splits == 1) return rc;
-    const long long groups = (I * ((J + 3) / 4) + 255) / 256;
+    const long long groups = (I * ((J + 3) / 4) + 63) / 64;
     if (groups > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
-    FRCNN_LAUNCH(dense_join_kernel<T>, dim3((unsigned)groups), dim3(256), 0, stream, (const float*)ws, pl.splits, I,
-                 J, e);
+    FRCNN_LAUNCH(dense_join_kernel<T>, dim3((unsigned)groups), dim3(64), 0, stream, (const float*)g.partial, pl.splits,
+                 I, J, e);
     return FRCNN_OK;
 }
 
-static size_t dn_up(size_t b) { return (b + 255) / 256 * 256; }
+// the workspace of one product whose operands are [ra][ca] and [rb][cb]
+enum DnRows { DN_ANY, DN_ALIGNED, DN_PADDED };         // rows anywhere; on 16 bytes; padded to whole pieces as well
+static size_t dn_product_bytes(long long ra, long long ca, bool akc, long long rb, long long cb, bool bkc,
+                               DnRows a_rows, DnRows b_rows) {
+    const DnPlan pl = dn_plan(akc ? ra : ca, bkc ? rb : cb, akc ? ca : ra, akc, bkc);
+    size_t bytes = dn_up(pl.partial_bytes);
+    if (pl.bi && !(a_rows == DN_PADDED || (a_rows == DN_ALIGNED && ca % 8 == 0))) bytes += dn_pack_bytes(ra, ca);
+    if (pl.bi && !(b_rows == DN_PADDED || (b_rows == DN_ALIGNED && cb % 8 == 0))) bytes += dn_pack_bytes(rb, cb);
+    return bytes;
+}
 
-// the backward's workspace: dz, its column sums, then the partial sums of one product at a time
-struct DnBwdPlan { bool copy; long long ldz; int rows; long long blocks; size_t dz_bytes, sum_bytes, partial_bytes; };
+// the backward's workspace: dz, its column sums, then what one product at a time needs
+struct DnBwdPlan { bool copy; long long ldz; int rows; long long blocks; size_t dz_bytes, sum_bytes; };
 
-static DnBwdPlan dn_bwd_plan(long long M, int K, int N, int act, int d_dtype, int dtype, bool aligned) {
+static DnBwdPlan dn_bwd_plan(long long M, int N, bool copy) {
     DnBwdPlan p{};
     if (M == 0) return p;                              // nothing to multiply: zeros are stored
-    p.copy = act != FRCNN_ACT_NONE || d_dtype != dtype || !aligned;
-    p.ldz = (N + 7) / 8 * 8;
+    p.copy = copy;
+    p.ldz = dn_pieces(N) * 8;
     p.rows = 64;
     p.blocks = (M + p.rows - 1) / p.rows;
     if (p.blocks > 4096) {                             // long batches: up to 4,096 partial sums per column
         p.rows = (int)(((M + 4095) / 4096 + 63) / 64 * 64);
         p.blocks = (M + p.rows - 1) / p.rows;
     }
-    p.dz_bytes = p.copy ? dn_up((size_t)M * (size_t)p.ldz * 2) : 0;
+    p.dz_bytes = copy ? dn_up((size_t)M * (size_t)p.ldz * 2) : 0;
     p.sum_bytes = dn_up((size_t)p.blocks * (size_t)N * 4);
-    const size_t x = dn_plan(M, K, N).partial_bytes, w = dn_plan(K, N, M).partial_bytes;
-    const size_t wt = dn_plan(N, K, M).partial_bytes;
-    p.partial_bytes = dn_up(x > w ? (x > wt ? x : wt) : (w > wt ? w : wt));
     return p;
 }
 
@@ -769,7 +897,7 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
     }
     void* dz = p.copy ? ws : nullptr;
     float* sums = d_bias ? reinterpret_cast<float*>(ws + p.dz_bytes) : nullptr;
-    void* partial = ws + p.dz_bytes + p.sum_bytes;
+    char* rest = ws + p.dz_bytes + p.sum_bytes;
     if (sums || (dz && (d_x || d_w))) {
         rc = d_dtype == FRCNN_DT_F32 ? dn_launch_dz<T, float>(d_out, ldd, pre, ldp, M, N, act, p, dz, sums, s)
                                      : dn_launch_dz<T, T>(d_out, ldd, pre, ldp, M, N, act, p, dz, sums, s);
@@ -778,18 +906,18 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
     if (sums)
         FRCNN_LAUNCH(dense_bias_grad_kernel<T>, dim3((unsigned)((N + 63) / 64)), dim3(256), 0, s, sums,
                      (int)p.blocks, N, (T*)d_bias);
-    const void* z = dz ? dz : d_out;
-    const long long ldz = dz ? p.ldz : ldd;
+    const DnMatrix z = dz ? DnMatrix{dz, M, N, p.ldz, true} : DnMatrix{d_out, M, N, ldd, false};
+    const DnMatrix mx{x, M, K, ldx, false};
     DnEpilogue e{};
     if (d_x) {
         e.out = d_x; e.ldo = lddx;
-        rc = dn_product<T>(z, ldz, true, w, ldw, kn, M, K, N, e, partial, s);
+        const DnMatrix mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
+        rc = dn_product<T>(z, true, mw, kn, e, rest, s);
         if (rc != FRCNN_OK) return rc;
     }
     if (d_w) {
         e.out = d_w; e.ldo = lddw;
-        rc = kn ? dn_product<T>(x, ldx, false, z, ldz, false, K, N, M, e, partial, s)
-                : dn_product<T>(z, ldz, false, x, ldx, false, N, K, M, e, partial, s);
+        rc = kn ? dn_product<T>(mx, false, z, false, e, rest, s) : dn_product<T>(z, false, mx, false, e, rest, s);
     }
     return rc;
 }
@@ -798,9 +926,16 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
 
 using namespace frcnn;
 
-extern "C" size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N) {
+extern "C" size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
     if (!dn_sizes(M, K, N) || M == 0) return 0;
-    return dn_plan(M, N, K).partial_bytes;
+    const DnRows x = aligned & 1 ? DN_ALIGNED : DN_ANY, w = aligned & 2 ? DN_ALIGNED : DN_ANY;
+    return w_layout == FRCNN_W_KN ? dn_product_bytes(M, K, true, K, N, false, x, w)
+                                  : dn_product_bytes(M, K, true, N, K, true, x, w);
+}
+
+static int dn_aligned(const void* x, int64_t ldx, const void* w, int64_t ldw) {
+    return (dn_even(x, 16) && ldx % 8 == 0 && ldx <= (1 << 21) ? 1 : 0) |
+           (dn_even(w, 16) && ldw % 8 == 0 && ldw <= (1 << 21) ? 2 : 0);
 }
 
 extern "C" int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int w_layout, const void* bias,
@@ -818,20 +953,27 @@ extern "C" int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_
     if (!dn_even(x, 2) || !dn_even(w, 2) || !dn_even(bias, 2) || !dn_even(residual, 2) || !dn_even(pre, 2) ||
         !dn_even(out, out_dtype == FRCNN_DT_F32 ? 4 : 2))
         return FRCNN_E_BADARG;
-    const size_t need = frcnn_dense_fwd_workspace_bytes(M, K, N);
+    const size_t need = frcnn_dense_fwd_workspace_bytes(M, K, N, w_layout, dn_aligned(x, ldx, w, ldw));
     if (need && (!workspace || workspace_bytes < need || !dn_even(workspace, 16))) return FRCNN_E_WORKSPACE;
     DnEpilogue e{};
     e.bias = bias; e.residual = residual; e.pre = pre; e.out = out;
     e.ldr = ldr; e.ldp = ldp; e.ldo = ldo; e.act = act; e.out_f32 = out_dtype == FRCNN_DT_F32;
+    const DnMatrix mx{x, M, K, ldx, false}, mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
     return dtype == FRCNN_DT_BF16
-               ? dn_product<__bf16>(x, ldx, true, w, ldw, !kn, M, N, K, e, workspace, (hipStream_t)stream)
-               : dn_product<_Float16>(x, ldx, true, w, ldw, !kn, M, N, K, e, workspace, (hipStream_t)stream);
+               ? dn_product<__bf16>(mx, true, mw, !kn, e, (char*)workspace, (hipStream_t)stream)
+               : dn_product<_Float16>(mx, true, mw, !kn, e, (char*)workspace, (hipStream_t)stream);
 }
 
-extern "C" size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N) {
+extern "C" size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
     if (!dn_sizes(M, K, N) || M == 0) return 0;
-    const DnBwdPlan p = dn_bwd_plan(M, K, N, FRCNN_ACT_RELU, FRCNN_DT_F32, FRCNN_DT_F16, false);
-    return p.dz_bytes + p.sum_bytes + p.partial_bytes;
+    const DnBwdPlan p = dn_bwd_plan(M, N, !(aligned & 4) || N % 8 != 0);
+    const bool kn = w_layout == FRCNN_W_KN;
+    const DnRows x = aligned & 1 ? DN_ALIGNED : DN_ANY, w = aligned & 2 ? DN_ALIGNED : DN_ANY;
+    const size_t dx = kn ? dn_product_bytes(M, N, true, K, N, true, DN_PADDED, w)
+                         : dn_product_bytes(M, N, true, N, K, false, DN_PADDED, w);
+    const size_t dw = kn ? dn_product_bytes(M, K, false, M, N, false, x, DN_PADDED)
+                         : dn_product_bytes(M, N, false, M, K, false, DN_PADDED, x);
+    return p.dz_bytes + p.sum_bytes + (dx > dw ? dx : dw);
 }
 
 extern "C" int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, const void* x, int64_t ldx, const void* w,
@@ -848,16 +990,19 @@ extern "C" int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, cons
     if (!dn_even(d_out, d_dtype == FRCNN_DT_F32 ? 4 : 2) || !dn_even(x, 2) || !dn_even(w, 2) || !dn_even(pre, 2) ||
         !dn_even(d_x, 2) || !dn_even(d_w, 2) || !dn_even(d_bias, 2))
         return FRCNN_E_BADARG;
+    // dz is d_out itself where that is whole pieces in the products' type and no activation changes it
+    const bool copy = act != FRCNN_ACT_NONE || d_dtype != dtype || !dn_whole(DnMatrix{d_out, M, N, ldd, false});
     if (M > 0) {
         if (!d_out || ldd < N) return FRCNN_E_BADARG;
         if (act != FRCNN_ACT_NONE && (!pre || ldp < N)) return FRCNN_E_BADARG;
         if (d_x && (!w || ldw < (kn ? N : K) || lddx < K)) return FRCNN_E_BADARG;
         if (d_w && (!x || ldx < K)) return FRCNN_E_BADARG;
-        const size_t need = frcnn_dense_bwd_workspace_bytes(M, K, N);
+        const int aligned = dn_aligned(d_x ? w : nullptr, d_x ? ldw : 0, d_w ? x : nullptr, d_w ? ldx : 0);
+        const size_t need = frcnn_dense_bwd_workspace_bytes(M, K, N, w_layout, (aligned & 1) * 2 | aligned >> 1 |
+                                                            (copy ? 0 : 4));
         if (!workspace || workspace_bytes < need || !dn_even(workspace, 16)) return FRCNN_E_WORKSPACE;
     }
-    const bool aligned = ldd % 8 == 0 && dn_even(d_out, 16);
-    const DnBwdPlan p = dn_bwd_plan(M, K, N, act, d_dtype, dtype, aligned);
+    const DnBwdPlan p = dn_bwd_plan(M, N, copy);
     return dtype == FRCNN_DT_BF16
                ? dn_backward<__bf16>(d_out, ldd, d_dtype, x, ldx, w, ldw, w_layout, pre, ldp, M, K, N, dtype, act,
                                      d_x, lddx, d_w, lddw, d_bias, (char*)workspace, p, (hipStream_t)stream)

@@ -5,8 +5,8 @@ computation happens in libfrcnn_hip.so.  Tensors must live on a ROCm device.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import functools
 import math
 from typing import Optional, Sequence, Tuple
 
@@ -558,87 +558,129 @@ def fc1_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] 
 
 
 # ---- dense layers on 16-bit inputs, distillation ------------------------------------------------
+# These calls may last a few microseconds on the GPU, so the host side is kept short: sizes are
+# remembered per shape, devices compared by index, the device guard entered only where needed.
 ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
                "silu": _lib.ACT_SILU}
 _DT = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
 _DT16 = (torch.float16, torch.bfloat16)
+_W_KN, _W_NK, _OK = _lib.W_KN, _lib.W_NK, _lib.OK
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
-def _raw_stream(dev: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+@functools.lru_cache(maxsize=4096)
+def dense_fwd_workspace_bytes(M: int, K: int, N: int, layout: int = _W_KN, aligned: int = 0) -> int:
+    """Bytes dense_fwd needs for rows [M,K] and a weight [K,N].  layout: rows of N (0) or the view of a
+    Linear weight (1).  aligned: 1 if x, 2 if weight starts on 16 bytes with a row stride of a multiple
+    of 8 (contiguous tensors with K and N multiples of 8 do: 3); 0 covers every call."""
+    return int(lib.frcnn_dense_fwd_workspace_bytes(M, K, N, layout, aligned))
 
 
-def _on(dev: torch.device):
-    """A guard that makes `dev` current (nothing to do when it is: the usual call)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+@functools.lru_cache(maxsize=4096)
+def dense_bwd_workspace_bytes(M: int, K: int, N: int, layout: int = _W_KN, aligned: int = 0) -> int:
+    """Bytes dense_bwd needs; aligned as above, plus 4 if d_out is aligned too, has x's type and act is
+    "none"."""
+    return int(lib.frcnn_dense_bwd_workspace_bytes(M, K, N, layout, aligned))
 
 
-def _same_dev(t: torch.Tensor, dev: torch.device, name: str) -> None:
-    if t.device != dev:
-        raise RuntimeError(f"{name}: on {t.device}, the other tensors are on {dev} "
-                           "(the HIP kernels are the only path)")
+@functools.lru_cache(maxsize=4096)
+def distill_workspace_bytes(rows: int, V: int, k: int, dtype: torch.dtype) -> int:
+    return int(lib.frcnn_distill_workspace_bytes(rows, V, k, _DT[dtype]))
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """[n,m] with unit column stride and rows that do not overlap; a copy only where it is not."""
+def _aligned(ptr: int, ld: int) -> bool:
+    return not (ptr & 15 or ld & 7 or ld > 2097152)
+
+
+def _call(name: str, fn, dev: int, args) -> None:
+    """fn(*args, current stream of device `dev`), with that device current."""
+    if _current_device() == dev:
+        status = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _raw_stream(dev))
+    if status != _OK:
+        check(name, status)
+
+
+def _other_device(t: torch.Tensor, dev: int, name: str):
+    return RuntimeError(f"{name}: on {t.device}, the other tensors are on cuda:{dev} "
+                        "(the HIP kernels are the only path)")
+
+
+def _rows(t: torch.Tensor):
+    """[n,m] -> (tensor with unit column stride and rows that do not overlap, row stride); a copy
+    only where it is not."""
     n, m = t.shape
-    if (t.stride(1) == 1 or m == 1) and (t.stride(0) >= m or n <= 1):
-        return t
-    return t.contiguous()
+    s0, s1 = t.stride()
+    if s1 == 1 or m == 1:
+        if n <= 1:
+            return t, m
+        if s0 >= m:
+            return t, s0
+    return t.contiguous(), m
 
 
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-
-
-def _dense_x(x: torch.Tensor, name: str):
-    """x [..., K] (the pooled tensor [B,R,ph,pw,C] as [B,R,ph*pw*C]) -> (rows [M,K], leading dims)."""
+def _dense_x(x: torch.Tensor):
+    """x [..., K] (the pooled tensor [B,R,ph,pw,C] as [B,R,ph*pw*C]) -> rows [M,K], row stride,
+    leading dimensions, device index."""
     if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{name}: expected a torch.Tensor")
-    if not x.is_cuda:
-        raise RuntimeError(f"{name}: must be on a ROCm device (the HIP kernels are the only path)")
+        raise TypeError("x: expected a torch.Tensor")
+    dev = x.get_device() if x.is_cuda else -1
+    if dev < 0:
+        raise RuntimeError("x: must be on a ROCm device (the HIP kernels are the only path)")
     if x.dtype not in _DT16:
-        raise TypeError(f"{name}: expected torch.float16 or torch.bfloat16, got {x.dtype}"
+        raise TypeError(f"x: expected torch.float16 or torch.bfloat16, got {x.dtype}"
                         " (fc1_fwd is the float32 layer)")
-    if x.dim() == 2:
-        return _rows(x), x.shape[:1]
-    if x.dim() == 5:
-        return _rows(x.reshape(x.shape[0] * x.shape[1], x.shape[2] * x.shape[3] * x.shape[4])), x.shape[:2]
-    if x.dim() < 1 or x.dim() == 0:
-        raise ValueError(f"{name}: needs at least one dimension")
-    return _rows(x.reshape(math.prod(x.shape[:-1]), x.shape[-1])), x.shape[:-1]
+    shape = x.shape
+    if len(shape) == 2:
+        lead = shape[:1]
+    elif len(shape) == 5:
+        lead = shape[:2]
+        x = x.reshape(lead[0] * lead[1], shape[2] * shape[3] * shape[4])
+    elif len(shape) == 0:
+        raise ValueError("x: needs at least one dimension")
+    else:
+        lead = shape[:-1]
+        x = x.reshape(math.prod(lead), shape[-1])
+    x, ld = _rows(x)
+    return x, ld, lead, dev
 
 
-def _dense_w(w: torch.Tensor, x: torch.Tensor, K: int):
-    """weight [K,N] -> (tensor, layout, row stride): rows of N (Keras) or, as the transposed view of
-    a Linear module's [N,K], rows of K; anything else is copied to rows of N."""
+def _dense_w(w: torch.Tensor, dtype: torch.dtype, dev: int, K: int):
+    """weight [K,N] -> (tensor, layout, row stride, N): rows of N (Keras) or, as the transposed view
+    of a Linear module's [N,K], rows of K; anything else is copied to rows of N."""
     if not isinstance(w, torch.Tensor):
         raise TypeError("weight: expected a torch.Tensor")
-    if w.dtype != x.dtype:
-        raise TypeError(f"weight: expected {x.dtype}, got {w.dtype}")
-    _same_dev(w, x.device, "weight")
-    if w.dim() != 2 or w.shape[1] == 0:
+    if w.dtype != dtype:
+        raise TypeError(f"weight: expected {dtype}, got {w.dtype}")
+    if w.get_device() != dev:
+        raise _other_device(w, dev, "weight")
+    if w.dim() != 2:
         raise ValueError("weight must be [K,N]")
-    if w.shape[0] != K or K == 0:
-        raise ValueError(f"x has {K} features per row, weight expects {w.shape[0]}")
-    N = w.shape[1]
+    k, N = w.shape
+    if N == 0 or k == 0:
+        raise ValueError("weight must be [K,N]")
+    if k != K:
+        raise ValueError(f"x has {K} features per row, weight expects {k}")
     s0, s1 = w.stride()
     if s1 == 1 and s0 >= N:
-        return w, _lib.W_KN, s0
+        return w, _W_KN, s0, N
     if s0 == 1 and s1 >= K:
-        return w, _lib.W_NK, s1
-    w = w.contiguous()
-    return w, _lib.W_KN, N
+        return w, _W_NK, s1, N
+    return w.contiguous(), _W_KN, N, N
 
 
-def _dense_rows(t: Optional[torch.Tensor], name: str, lead, M: int, N: int, dev, dtypes):
-    """A [..., N] operand with the call's leading dimensions -> rows [M,N]."""
+def _dense_rows(t: Optional[torch.Tensor], name: str, lead, M: int, N: int, dev: int, dtypes):
+    """A [..., N] operand with the call's leading dimensions -> rows [M,N] and their stride."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
-    _same_dev(t, dev, name)
-    if tuple(t.shape) != (*lead, N):
+    if t.get_device() != dev:
+        raise _other_device(t, dev, name)
+    if t.shape != (*lead, N):
         raise ValueError(f"{name} must be {[*lead, N]}, got {list(t.shape)}")
     return _rows(t if t.dim() == 2 else t.reshape(M, N))
 
@@ -649,33 +691,20 @@ def _act_code(act: str) -> int:
     return ACTIVATIONS[act]
 
 
-def _dense_out(out, name, shape2, lead, N, dtype, dev):
-    if out is None:
-        return torch.empty(shape2, dtype=dtype, device=dev)
-    if not isinstance(out, torch.Tensor) or out.dtype != dtype or not out.is_contiguous() \
-            or tuple(out.shape) != (*lead, N):
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {[*lead, N]}")
-    _same_dev(out, dev, name)
-    return out.view(shape2)
-
-
-def _scratch(ws: Optional[torch.Tensor], need: int, dev) -> Optional[torch.Tensor]:
+def _scratch(ws: Optional[torch.Tensor], need: int, like: torch.Tensor, dev: int):
+    """(pointer, bytes, tensor that keeps them) of a workspace of `need` bytes."""
     if need == 0:
-        return None
+        return None, 0, None
     if ws is None:
-        return torch.empty(need, dtype=torch.uint8, device=dev)
-    _same_dev(_cont(ws, "workspace", torch.uint8), dev, "workspace")
-    if not ws.is_contiguous() or ws.numel() < need:
-        raise ValueError(f"workspace: {need} bytes are needed")
-    return ws
-
-
-def dense_fwd_workspace_bytes(M: int, K: int, N: int) -> int:
-    return int(lib.frcnn_dense_fwd_workspace_bytes(M, K, N))
-
-
-def dense_bwd_workspace_bytes(M: int, K: int, N: int) -> int:
-    return int(lib.frcnn_dense_bwd_workspace_bytes(M, K, N))
+        ws = like.new_empty(need, dtype=torch.uint8)
+    else:
+        if not isinstance(ws, torch.Tensor) or ws.dtype != torch.uint8:
+            raise TypeError("workspace: expected a torch.uint8 tensor")
+        if ws.get_device() != dev:
+            raise _other_device(ws, dev, "workspace")
+        if not ws.is_contiguous() or ws.numel() < need:
+            raise ValueError(f"workspace: {need} contiguous bytes are needed")
+    return ws.data_ptr(), ws.numel(), ws
 
 
 def dense_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -688,37 +717,47 @@ def dense_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
     or the transposed view of a Linear weight [N,K] (both are read as they lie); bias [N]; residual
     [..., N].  act: "none", "relu", "gelu" (exact), "silu".  out_dtype float32 keeps the sums (class
     logits).  Returns out [..., N], with want_pre (out, pre): the pre-activations dense_bwd needs.
-    workspace: uint8 of dense_fwd_workspace_bytes(M, K, N), kept by callers that allocate nothing."""
-    xx, lead = _dense_x(x, "x")
+    workspace: uint8 of dense_fwd_workspace_bytes(M, K, N, ...), kept by callers that allocate nothing."""
+    xx, ldx, lead, dev = _dense_x(x)
     M, K = xx.shape
-    dev, dt = xx.device, xx.dtype
-    w, layout, ldw = _dense_w(weight, xx, K)
-    N = w.shape[1]
+    dt = xx.dtype
+    w, layout, ldw, N = _dense_w(weight, dt, dev, K)
     code = _act_code(act)
+    pb = pr = pp = None
+    ldr = 0
     if bias is not None:
         if not isinstance(bias, torch.Tensor) or bias.dtype != dt:
             raise TypeError(f"bias: expected a {dt} tensor")
-        _same_dev(bias, dev, "bias")
-        if tuple(bias.shape) != (N,):
+        if bias.get_device() != dev:
+            raise _other_device(bias, dev, "bias")
+        if bias.shape != (N,):
             raise ValueError(f"bias must be [{N}]")
         bias = bias.contiguous()
-    res = None if residual is None else _dense_rows(residual, "residual", lead, M, N, dev, (dt,))
+        pb = bias.data_ptr()
+    if residual is not None:
+        residual, ldr = _dense_rows(residual, "residual", lead, M, N, dev, (dt,))
+        pr = residual.data_ptr()
     odt = dt if out_dtype is None else out_dtype
-    if odt not in (dt, torch.float32):
+    if odt != dt and odt != torch.float32:
         raise TypeError(f"out_dtype: expected {dt} or torch.float32, got {odt}")
-    o = _dense_out(out, "out", (M, N), lead, N, odt, dev)
-    pre = torch.empty((M, N), dtype=dt, device=dev) if want_pre else None
-    ws = _scratch(workspace, lib.frcnn_dense_fwd_workspace_bytes(M, K, N), dev)
-    with _on(dev):
-        check("frcnn_dense_fwd", lib.frcnn_dense_fwd(
-            xx.data_ptr(), _ld(xx), w.data_ptr(), ldw, layout, None if bias is None else bias.data_ptr(),
-            None if res is None else res.data_ptr(), 0 if res is None else _ld(res), M, K, N, _DT[dt], code,
-            o.data_ptr(), N, _DT[odt], None if pre is None else pre.data_ptr(), N,
-            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _raw_stream(dev)))
-    if len(lead) != 1:
-        o = o.view(*lead, N)
-        pre = None if pre is None else pre.view(*lead, N)
-    return (o, pre) if want_pre else o
+    if out is None:
+        out = xx.new_empty((*lead, N), dtype=odt)
+    elif not isinstance(out, torch.Tensor) or out.dtype != odt or not out.is_contiguous() \
+            or out.shape != (*lead, N):
+        raise ValueError(f"out must be a contiguous {odt} tensor of shape {[*lead, N]}")
+    elif out.get_device() != dev:
+        raise _other_device(out, dev, "out")
+    pre = None
+    if want_pre:
+        pre = xx.new_empty((*lead, N))
+        pp = pre.data_ptr()
+    px, pw = xx.data_ptr(), w.data_ptr()
+    aligned = 3 if M <= 32 else _aligned(px, ldx) + 2 * _aligned(pw, ldw)
+    pws, nws, ws = _scratch(workspace, dense_fwd_workspace_bytes(M, K, N, layout, aligned), xx, dev)
+    _call("frcnn_dense_fwd", lib.frcnn_dense_fwd, dev, (
+        px, ldx, pw, ldw, layout, pb, pr, ldr, M, K, N, _DT[dt], code, out.data_ptr(), N,
+        _DT[odt], pp, N, pws, nws))
+    return (out, pre) if want_pre else out
 
 
 def dense_bwd(d_out: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
@@ -728,72 +767,91 @@ def dense_bwd(d_out: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     """Gradients of dense_fwd (frcnn_dense_bwd): dict(d_x [..., K] of x's shape, d_weight [K,N] in
     weight's memory layout, d_bias [N]); None where not wanted.  d_out [..., N] in x's type or
     float32; pre as dense_fwd returned it (not needed for act "none").  The residual's gradient is
-    d_out itself.  workspace: uint8 of dense_bwd_workspace_bytes(M, K, N)."""
-    xx, lead = _dense_x(x, "x")
+    d_out itself.  workspace: uint8 of
+    dense_bwd_workspace_bytes(M, K, N, ...)."""
+    xx, ldx, lead, dev = _dense_x(x)
     M, K = xx.shape
-    dev, dt = xx.device, xx.dtype
-    w, layout, ldw = _dense_w(weight, xx, K)
-    N = w.shape[1]
+    dt = xx.dtype
+    w, layout, ldw, N = _dense_w(weight, dt, dev, K)
     code = _act_code(act)
     if not (want_dx or want_dw or want_db):
         raise ValueError("nothing wanted: set want_dx, want_dw or want_db")
-    d = _dense_rows(d_out, "d_out", lead, M, N, dev, (dt, torch.float32))
-    z = None
+    d, ldd = _dense_rows(d_out, "d_out", lead, M, N, dev, (dt, torch.float32))
+    pz, ldz = None, 0
     if code != _lib.ACT_NONE:
         if pre is None:
             raise ValueError(f"pre: the forward's pre-activations are needed for act {act!r}")
-        z = _dense_rows(pre, "pre", lead, M, N, dev, (dt,))
-    d_x = torch.empty((M, K), dtype=dt, device=dev) if want_dx else None
-    d_w = torch.empty((K, N) if layout == _lib.W_KN else (N, K), dtype=dt, device=dev) if want_dw else None
-    d_b = torch.empty(N, dtype=dt, device=dev) if want_db else None
-    ws = _scratch(workspace, lib.frcnn_dense_bwd_workspace_bytes(M, K, N), dev)
-    with _on(dev):
-        check("frcnn_dense_bwd", lib.frcnn_dense_bwd(
-            d.data_ptr(), _ld(d), _DT[d.dtype], xx.data_ptr(), _ld(xx), w.data_ptr(), ldw, layout,
-            None if z is None else z.data_ptr(), 0 if z is None else _ld(z), M, K, N, _DT[dt], code,
-            None if d_x is None else d_x.data_ptr(), K, None if d_w is None else d_w.data_ptr(),
-            N if layout == _lib.W_KN else K, None if d_b is None else d_b.data_ptr(),
-            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _raw_stream(dev)))
-    if d_w is not None and layout == _lib.W_NK:
-        d_w = d_w.t()
-    return dict(d_x=None if d_x is None else d_x.view(x.shape), d_weight=d_w, d_bias=d_b)
+        pre, ldz = _dense_rows(pre, "pre", lead, M, N, dev, (dt,))
+        pz = pre.data_ptr()
+    d_x = d_w = d_b = px = pw = pb = None
+    if want_dx:
+        d_x = xx.new_empty(x.shape)
+        px = d_x.data_ptr()
+    ldo = N
+    if want_dw:
+        if layout == _W_KN:
+            d_w = xx.new_empty((K, N))
+        else:
+            ldo = K
+            d_w = xx.new_empty((N, K)).t()
+        pw = d_w.data_ptr()
+    if want_db:
+        d_b = xx.new_empty(N)
+        pb = d_b.data_ptr()
+    pd, pix, piw = d.data_ptr(), xx.data_ptr(), w.data_ptr()
+    aligned = _aligned(pix, ldx) + 2 * _aligned(piw, ldw)
+    if code == _lib.ACT_NONE and d.dtype == dt:
+        aligned += 4 * _aligned(pd, ldd)
+    pws, nws, ws = _scratch(workspace, dense_bwd_workspace_bytes(M, K, N, layout, aligned), xx, dev)
+    _call("frcnn_dense_bwd", lib.frcnn_dense_bwd, dev, (
+        pd, ldd, _DT[d.dtype], pix, ldx, piw, ldw, layout, pz, ldz, M, K, N, _DT[dt],
+        code, px, K, pw, ldo, pb, pws, nws))
+    return {"d_x": d_x, "d_weight": d_w, "d_bias": d_b}
 
 
 def _distill_args(logits, top_values, top_index, weight, temperature):
     if not isinstance(logits, torch.Tensor):
         raise TypeError("logits: expected a torch.Tensor")
-    if not logits.is_cuda:
+    dev = logits.get_device() if logits.is_cuda else -1
+    if dev < 0:
         raise RuntimeError("logits: must be on a ROCm device (the HIP kernels are the only path)")
-    if logits.dtype not in _DT:
-        raise TypeError(f"logits: expected float32, float16 or bfloat16, got {logits.dtype}")
-    if logits.dim() < 1 or logits.shape[-1] == 0:
+    dt = logits.dtype
+    if dt not in _DT:
+        raise TypeError(f"logits: expected float32, float16 or bfloat16, got {dt}")
+    shape = logits.shape
+    if len(shape) < 1 or shape[-1] == 0:
         raise ValueError("logits must be [..., V]")
-    lead, V, dev = logits.shape[:-1], logits.shape[-1], logits.device
-    rows = math.prod(lead)
-    if not isinstance(top_values, torch.Tensor) or top_values.dtype not in (logits.dtype, torch.float32):
-        raise TypeError(f"top_values: expected a tensor of {logits.dtype} or float32")
+    lead, V = shape[:-1], shape[-1]
+    if not isinstance(top_values, torch.Tensor) or top_values.dtype not in (dt, torch.float32):
+        raise TypeError(f"top_values: expected a tensor of {dt} or float32")
     if not isinstance(top_index, torch.Tensor) or top_index.dtype != torch.int64:
         raise TypeError("top_index: expected an int64 tensor")
-    k = top_values.shape[-1] if top_values.dim() else 0
-    if k == 0 or tuple(top_values.shape) != (*lead, k) or top_index.shape != top_values.shape:
+    ts = top_values.shape
+    k = ts[-1] if len(ts) else 0
+    if k == 0 or ts[:-1] != lead or top_index.shape != ts:
         raise ValueError(f"top_values and top_index must be {[*lead, 'k']}")
-    _same_dev(top_values, dev, "top_values")
-    _same_dev(top_index, dev, "top_index")
+    if top_values.get_device() != dev:
+        raise _other_device(top_values, dev, "top_values")
+    if top_index.get_device() != dev:
+        raise _other_device(top_index, dev, "top_index")
+    pw = None
     if weight is not None:
         if not isinstance(weight, torch.Tensor) or weight.dtype != torch.float32:
             raise TypeError("weight: expected a float32 tensor")
-        _same_dev(weight, dev, "weight")
+        if weight.get_device() != dev:
+            raise _other_device(weight, dev, "weight")
         if weight.shape != lead:
             raise ValueError(f"weight must be {list(lead)}")
         weight = weight.contiguous()
-    if not (0.0 < float(temperature) < 3.0e38):
+        pw = weight.data_ptr()
+    if not 0.0 < temperature < 3.0e38:
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
-    z = _rows(logits if logits.dim() == 2 else logits.reshape(rows, V))
-    return z, top_values.contiguous(), top_index.contiguous(), weight, lead, rows, V, k
-
-
-def distill_workspace_bytes(rows: int, V: int, k: int, dtype: torch.dtype) -> int:
-    return int(lib.frcnn_distill_workspace_bytes(rows, V, k, _DT[dtype]))
+    rows = lead[0] if len(lead) == 1 else math.prod(lead)
+    z, ldz = _rows(logits if len(lead) == 1 else logits.reshape(rows, V))
+    top_values, top_index = top_values.contiguous(), top_index.contiguous()
+    head = (z.data_ptr(), ldz, _DT[dt], top_values.data_ptr(), _DT[top_values.dtype], top_index.data_ptr())
+    # the tensors behind the pointers, kept until the call is made
+    return head, pw, lead, rows, V, k, dev, (z, top_values, top_index, weight)
 
 
 def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torch.Tensor,
@@ -809,19 +867,18 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torc
     `temperature` T, returns dict(loss [...] = weight T^2 KL(p || q), lse [...], d_logits: the
     gradient of grad_scale * loss.sum() in logits, None unless want_grad).  workspace: uint8 of
     distill_workspace_bytes(rows, V, k, dtype)."""
-    z, tv, ti, wt, lead, rows, V, k = _distill_args(logits, top_values, top_index, weight, temperature)
-    dev = z.device
-    loss = torch.empty(lead, dtype=torch.float32, device=dev)
-    lse = torch.empty(lead, dtype=torch.float32, device=dev)
-    grad = torch.empty(logits.shape, dtype=z.dtype, device=dev) if want_grad else None
-    ws = _scratch(workspace, lib.frcnn_distill_workspace_bytes(rows, V, k, _DT[z.dtype]), dev)
-    with _on(dev):
-        check("frcnn_distill_loss", lib.frcnn_distill_loss(
-            z.data_ptr(), _ld(z), _DT[z.dtype], tv.data_ptr(), _DT[tv.dtype], ti.data_ptr(),
-            None if wt is None else wt.data_ptr(), rows, V, k, temperature, grad_scale, loss.data_ptr(),
-            lse.data_ptr(), None if grad is None else grad.data_ptr(), V,
-            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _raw_stream(dev)))
-    return dict(loss=loss, lse=lse, d_logits=grad)
+    head, pw, lead, rows, V, k, dev, kept = _distill_args(logits, top_values, top_index, weight, temperature)
+    z = kept[0]
+    loss = z.new_empty(lead, dtype=torch.float32)
+    lse = torch.empty_like(loss)
+    grad = pg = None
+    if want_grad:
+        grad = z.new_empty(logits.shape)
+        pg = grad.data_ptr()
+    pws, nws, ws = _scratch(workspace, distill_workspace_bytes(rows, V, k, z.dtype), z, dev)
+    _call("frcnn_distill_loss", lib.frcnn_distill_loss, dev, (
+        *head, pw, rows, V, k, temperature, grad_scale, loss.data_ptr(), lse.data_ptr(), pg, V, pws, nws))
+    return {"loss": loss, "lse": lse, "d_logits": grad}
 
 
 def distill_bwd(d_loss: torch.Tensor, logits: torch.Tensor, top_values: torch.Tensor,
@@ -829,19 +886,16 @@ def distill_bwd(d_loss: torch.Tensor, logits: torch.Tensor, top_values: torch.Te
                 temperature: float = 1.0) -> torch.Tensor:
     """Gradient of distill_loss in logits for upstream gradients d_loss [...] (frcnn_distill_bwd);
     lse [...] as distill_loss returned it."""
-    z, tv, ti, wt, lead, rows, V, k = _distill_args(logits, top_values, top_index, weight, temperature)
-    dev = z.device
+    head, pw, lead, rows, V, k, dev, kept = _distill_args(logits, top_values, top_index, weight, temperature)
     for t, name in ((d_loss, "d_loss"), (lse, "lse")):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
             raise TypeError(f"{name}: expected a float32 tensor")
-        _same_dev(t, dev, name)
+        if t.get_device() != dev:
+            raise _other_device(t, dev, name)
         if t.shape != lead:
             raise ValueError(f"{name} must be {list(lead)}")
     d_loss, lse = d_loss.contiguous(), lse.contiguous()
-    grad = torch.empty(logits.shape, dtype=z.dtype, device=dev)
-    with _on(dev):
-        check("frcnn_distill_bwd", lib.frcnn_distill_bwd(
-            d_loss.data_ptr(), z.data_ptr(), _ld(z), _DT[z.dtype], tv.data_ptr(), _DT[tv.dtype], ti.data_ptr(),
-            lse.data_ptr(), None if wt is None else wt.data_ptr(), rows, V, k, temperature, grad.data_ptr(), V,
-            _raw_stream(dev)))
+    grad = kept[0].new_empty(logits.shape)
+    _call("frcnn_distill_bwd", lib.frcnn_distill_bwd, dev, (
+        d_loss.data_ptr(), *head, lse.data_ptr(), pw, rows, V, k, temperature, grad.data_ptr(), V))
     return grad

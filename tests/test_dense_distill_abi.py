@@ -46,14 +46,23 @@ def test_dense_backward_refuses(L, bad):
 
 def test_dense_workspaces(L):
     f, b = L.lib.frcnn_dense_fwd_workspace_bytes, L.lib.frcnn_dense_bwd_workspace_bytes
-    assert f(0, 8, 8) == 0 and b(0, 8, 8) == 0 and f(4, 0, 8) == 0 and f(-1, 8, 8) == 0
-    assert f(16000, 4096, 4096) == 0                       # enough tiles: no split
-    need = f(2, 25088, 4096)
-    assert need > 0
-    assert fwd(L, M=2, K=25088, ldx=25088, N=4096, ldw=4096, ldo=4096) == L.E_WORKSPACE
-    assert fwd(L, M=2, K=25088, ldx=25088, N=4096, ldw=4096, ldo=4096, ws=ONE, wsb=need - 1) == L.E_WORKSPACE
-    assert b(100, 64, 32) >= 100 * 32 * 2
-    assert bwd(L, ws=None) == L.E_WORKSPACE and bwd(L, wsb=b(4, 64, 32) - 1) == L.E_WORKSPACE
+    assert f(0, 8, 8, 0, 0) == 0 and b(0, 8, 8, 0, 0) == 0 and f(4, 0, 8, 0, 0) == 0 and f(-1, 8, 8, 0, 0) == 0
+    assert f(16000, 4096, 4096, 0, 3) == 0                 # enough tiles: no split; aligned: no copy
+    copy = lambda rows, cols: (rows * ((cols + 7) // 8) * 16 + 255) // 256 * 256
+    assert f(16000, 4096, 4096, 0, 2) == copy(16000, 4096) and f(16000, 4096, 4096, 1, 1) == copy(4096, 4096)
+    assert f(16000, 4095, 4096, 0, 3) == copy(16000, 4095)
+    assert f(16000, 4095, 4095, 0, 0) == copy(16000, 4095) + copy(4095, 4095)
+    for layout, ldw in ((0, 64), (1, 25088)):
+        need = f(2, 25088, 64, layout, 0)
+        assert need > 0 and need == f(2, 25088, 64, layout, 3)     # few rows: partial sums, no copy
+        small = dict(M=2, K=25088, ldx=25088, N=64, layout=layout, ldw=ldw, ldo=64)
+        assert fwd(L, **small) == L.E_WORKSPACE and fwd(L, ws=ONE, wsb=need - 1, **small) == L.E_WORKSPACE
+    odd = dict(M=100, ldx=65)                              # a stride that is no multiple of 8: x is copied
+    assert fwd(L, ws=ONE, wsb=f(100, 64, 32, 0, 2) - 1, **odd) == L.E_WORKSPACE
+    assert b(100, 64, 32, 0, 0) >= 100 * 32 * 2 + copy(100, 64)
+    assert b(100, 64, 33, 0, 3) - b(100, 64, 33, 0, 1) == copy(64, 33) * 0      # 33: W is copied either way
+    assert b(100, 64, 32, 0, 7) < b(100, 64, 32, 0, 3) <= b(100, 64, 32, 0, 0)
+    assert bwd(L, ws=None) == L.E_WORKSPACE and bwd(L, wsb=b(4, 64, 32, 0, 7) - 1) == L.E_WORKSPACE
     assert bwd(L, ws=ctypes.c_void_p(24)) == L.E_WORKSPACE
     assert fwd(L, M=0, x=None, out=None) == L.OK           # no rows: nothing to do, nothing launched
 

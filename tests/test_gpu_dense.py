@@ -101,7 +101,8 @@ def check_bwd(x, w, d, pre, act, g):
 
 
 SIZES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (17, 64, 16), (1, 4096, 520), (16, 1536, 256), (33, 96, 21),
-         (130, 200, 84), (257, 1003, 331), (128, 128, 128), (300, 72, 1032), (1030, 264, 136), (2, 7, 2050)]
+         (130, 200, 84), (257, 1003, 331), (128, 128, 128), (300, 72, 1032), (1030, 264, 136), (2, 7, 2050), (32, 1000, 100), (31, 9001, 40),
+         (5, 25088, 24), (1, 8200, 33), (33, 4104, 48)]
 
 
 @pytest.mark.parametrize("M,K,N", SIZES)

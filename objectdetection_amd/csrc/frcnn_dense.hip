@@ -193,38 +193,113 @@ __device__ __forceinline__ void dn_tile(const DnGemm& p, int& ti, int& tj, int& 
 }
 
 // A wave's results, (16 FI) x (16 FJ) at (i0, j0): the float32 partial sums of a slice, or the outputs.
-// Sixteen rows at a time turn round through LDS (the wave's own DN_TURN bytes), so that a lane holds eight
-// neighbouring outputs and the lanes of a row store whole 128-byte lines.
+// Sixteen rows at a time turn round through LDS (the wave's own dn_turn_bytes), so that a lane holds eight
+// neighbouring outputs and the lanes of a row store whole 128-byte lines.  Inside the matrix nothing is
+// guarded, the bias is loaded once (a lane's columns stay the same) and the residual of the next sixteen
+// rows is on its way before the stores of these: memory operations finish in order, and a load waited for
+// behind stores, or a guarded one, costs their whole way to memory (6 us per 256 x 256 tile).
 template <int FJ> constexpr int dn_turn_bytes() { return 16 * (FJ * 64 + 16); }
-template <typename T, int FI, int FJ>
+
+template <typename T, int FI, int FJ, bool FULL>
 __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&acc)[FI][FJ], int slice, long long i0,
                                              long long j0, char* turn) {
     constexpr int S = FJ * 64 + 16, Q = 2 * FJ, RP = 64 / Q;      // bytes per row, pieces of 8 per row, rows per pass
+    constexpr int NP = 16 / RP;                                   // passes per sixteen rows
     const int lane = lane_id();
-    const long long Jp = (p.J + 3) / 4 * 4, gj = j0 + 8 * (lane % Q), left = p.J - gj;
-    const int valid = left > 8 ? 8 : (int)left;
+    if (p.partial) {            // columns J .. Jp-1 may be written and are never read as results
+        const long long Jp = (p.J + 3) / 4 * 4;
 #pragma unroll
-    for (int i = 0; i < FI; ++i) {
-        __builtin_amdgcn_wave_barrier();
+        for (int i = 0; i < FI; ++i) {
+            const long long gi = i0 + 16 * i + (lane & 15);
+            if (gi >= p.I) continue;
 #pragma unroll
-        for (int j = 0; j < FJ; ++j)
-            *reinterpret_cast<dn_f32x4*>(turn + (lane & 15) * S + j * 64 + (lane >> 4) * 16) = acc[i][j];
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int r = 0; r < 16; r += RP) {
-            const int row = r + lane / Q;
-            const long long gi = i0 + 16 * i + row;
-            if (gi >= p.I || valid <= 0) continue;
-            const float* src = reinterpret_cast<const float*>(turn + row * S + (lane % Q) * 32);
-            float v[8];
-            __builtin_memcpy(v, src, 32);
-            if (p.partial) {    // columns J .. Jp-1 may be written and are never read as results
-                float* to = p.partial + (slice * p.I + gi) * Jp + gj;
-                __builtin_memcpy(to, v, 16);
-                if (valid > 4) __builtin_memcpy(to + 4, v + 4, 16);
-            } else {
-                dn_epilogue<T, 8>(p.e, gi, gj, valid, v);
+            for (int j = 0; j < FJ; ++j) {
+                const long long gj = j0 + 16 * j + 4 * (lane >> 4);
+                if (gj < Jp) *reinterpret_cast<dn_f32x4*>(p.partial + (slice * p.I + gi) * Jp + gj) = acc[i][j];
             }
+        }
+        return;
+    }
+    const long long row0 = i0 + lane / Q, gj = j0 + 8 * (lane % Q), left = p.J - gj;
+    char* put = turn + (lane & 15) * S + (lane >> 4) * 16;
+    const char* get = turn + (lane / Q) * S + (lane % Q) * 32;
+    auto turn_in = [&](const dn_f32x4 (&a)[FJ]) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) *reinterpret_cast<dn_f32x4*>(put + j * 64) = a[j];
+        __builtin_amdgcn_wave_barrier();
+    };
+    auto turn_out = [&](int pass, float (&v)[8]) { __builtin_memcpy(v, get + pass * RP * S, 32); };
+    if (j0 + 16 * FJ <= p.J && !(FULL && p.e.out_f32)) {
+        T* out = (T*)p.e.out + row0 * p.e.ldo + gj;
+        if constexpr (!FULL) {
+#pragma unroll
+            for (int i = 0; i < FI; ++i) {
+                turn_in(acc[i]);
+#pragma unroll
+                for (int r = 0; r < NP; ++r) {
+                    float v[8];
+                    turn_out(r, v);
+                    if (row0 + 16 * i + r * RP < p.I) dn_store<T, 8>(out + (16 * i + r * RP) * p.e.ldo, 8, v);
+                }
+            }
+        } else {
+            const bool has_res = p.e.residual != nullptr, has_pre = p.e.pre != nullptr;
+            const int act = p.e.act;
+            T* pre = (T*)p.e.pre + (has_pre ? row0 * p.e.ldp + gj : 0);
+            const T* res = (const T*)p.e.residual + (has_res ? gj : 0);
+            float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (p.e.bias) dn_load<T, 8>((const T*)p.e.bias + gj, 8, bias);
+            dn_s16x8 now[NP] = {}, next[NP] = {};
+            auto fetch = [&](int i, dn_s16x8 (&to)[NP]) {
+#pragma unroll
+                for (int r = 0; r < NP; ++r) {
+                    const long long gi = row0 + 16 * i + r * RP;
+                    __builtin_memcpy(&to[r], res + (gi < p.I ? gi : p.I - 1) * p.e.ldr, 16);
+                }
+            };
+            if (has_res) fetch(0, now);
+#pragma unroll
+            for (int i = 0; i < FI; ++i) {
+                turn_in(acc[i]);
+                if (has_res && i + 1 < FI) fetch(i + 1, next);
+#pragma unroll
+                for (int r = 0; r < NP; ++r) {
+                    const bool inside = row0 + 16 * i + r * RP < p.I;
+                    float v[8];
+                    turn_out(r, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += bias[e];
+                    if (has_pre && inside) dn_store<T, 8>(pre + (16 * i + r * RP) * p.e.ldp, 8, v);
+                    if (act != FRCNN_ACT_NONE) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = dn_act(v[e], act);
+                    }
+                    if (has_res) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] += (float)__builtin_bit_cast(T, (short)now[r][e]);
+                    }
+                    if (inside) dn_store<T, 8>(out + (16 * i + r * RP) * p.e.ldo, 8, v);
+                }
+#pragma unroll
+                for (int r = 0; r < NP; ++r) now[r] = next[r];
+            }
+        }
+        return;
+    }
+    // a tile at the matrix' right edge, or float32 outputs
+#pragma unroll 1
+    for (int i = 0; i < FI; ++i) {
+#pragma unroll
+        for (int c = 0; c < FI; ++c)
+            if (i == c) turn_in(acc[c]);
+#pragma unroll 1
+        for (int r = 0; r < NP; ++r) {
+            const long long gi = row0 + 16 * i + r * RP;
+            if (gi >= p.I || left <= 0) continue;
+            float v[8];
+            turn_out(r, v);
+            dn_epilogue<T, 8>(p.e, gi, gj, left > 8 ? 8 : (int)left, v);
         }
     }
 }
@@ -332,7 +407,8 @@ struct DnReader {
     }
 };
 
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
+// FULL: with bias, pre, activation, residual or a float32 output in the epilogue (the forward)
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, bool FULL>
 __global__ void __launch_bounds__(64 * WI * WJ)
 dense_gemm_kernel(DnGemm p) {
     constexpr int NT = 64 * WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
@@ -446,7 +522,7 @@ dense_gemm_kernel(DnGemm p) {
         if (s < n) step(fa[1], fb[1], fa[0], fb[0]);
     }
     dn_handover<0>();
-    dn_write_out<T, FI, FJ>(p, acc, slice, i0 + wi, j0 + wj, dn_lds + wave * dn_turn_bytes<FJ>());
+    dn_write_out<T, FI, FJ, FULL>(p, acc, slice, i0 + wi, j0 + wj, dn_lds + wave * dn_turn_bytes<FJ>());
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------
@@ -637,26 +713,40 @@ __global__ void __launch_bounds__(256) dense_pack_kernel(DnPack a, DnPack b, lon
 template <typename T, typename D>
 __global__ void __launch_bounds__(256)
 dense_dz_kernel(const D* __restrict__ d_out, long long ldd, const T* __restrict__ pre, long long ldp, long long M,
-                int N, int act, int rows, int cg, T* __restrict__ dz, long long ldz, float* __restrict__ sums) {
+                int N, int act, long long rows, int cg, T* __restrict__ dz, long long ldz, float* __restrict__ sums) {
     __shared__ float part[256][9];
     const int tid = threadIdx.x, c = tid % cg, rl = tid / cg, rn = 256 / cg;
     const long long col = ((long long)blockIdx.y * cg + c) * 8, r0 = (long long)blockIdx.x * rows;
     const long long r1 = r0 + rows < M ? r0 + rows : M;
     const int valid = N - col > 8 ? 8 : (int)(N - col);
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    auto row = [&](long long r, const float (&d)[8], const float (&z)[8]) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < valid ? dn_act_grad(d[e], z[e], act) : 0.f;
+        if (dz) dn_store<T, 8>(dz + r * ldz + col, 8, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += v[e];
+    };
     if (valid > 0) {
-        for (long long r = r0 + rl; r < r1; r += rn) {
-            float d[8];
-            dn_load<D, 8>(d_out + r * ldd + col, valid, d);
-            if (act != FRCNN_ACT_NONE) {
-                float z[8];
-                dn_load<T, 8>(pre + r * ldp + col, valid, z);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) d[e] = e < valid ? dn_act_grad(d[e], z[e], act) : 0.f;
+        const bool act_any = act != FRCNN_ACT_NONE;
+        long long r = r0 + rl;
+        for (; r + rn < r1; r += 2 * rn) {             // two rows on their way
+            float d0[8], d1[8], z0[8] = {}, z1[8] = {};
+            dn_load<D, 8>(d_out + r * ldd + col, valid, d0);
+            dn_load<D, 8>(d_out + (r + rn) * ldd + col, valid, d1);
+            if (act_any) {
+                dn_load<T, 8>(pre + r * ldp + col, valid, z0);
+                dn_load<T, 8>(pre + (r + rn) * ldp + col, valid, z1);
             }
-            if (dz) dn_store<T, 8>(dz + r * ldz + col, 8, d);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] += d[e];
+            row(r, d0, z0);
+            row(r + rn, d1, z1);
+        }
+        if (r < r1) {
+            float d0[8], z0[8] = {};
+            dn_load<D, 8>(d_out + r * ldd + col, valid, d0);
+            if (act_any) dn_load<T, 8>(pre + r * ldp + col, valid, z0);
+            row(r, d0, z0);
         }
     }
     if (!sums) return;
@@ -671,19 +761,28 @@ dense_dz_kernel(const D* __restrict__ d_out, long long ldd, const T* __restrict_
     }
 }
 
-// column sums of `blocks` rows of float32 partial sums: 64 columns per workgroup, 4 threads each
+// column sums of `blocks` rows of float32 partial sums: 16 columns per workgroup, 16 threads each, four
+// rows on their way per thread
 template <typename T>
 __global__ void __launch_bounds__(256)
 dense_bias_grad_kernel(const float* __restrict__ sums, int blocks, int N, T* __restrict__ d_bias) {
-    __shared__ float part[4][64];
-    const int c = threadIdx.x & 63, q = threadIdx.x >> 6;
-    const int col = blockIdx.x * 64 + c;
-    float s = 0.f;
+    __shared__ float part[16][17];
+    const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
+    const int col = blockIdx.x * 16 + c;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (col < N)
-        for (int b = q; b < blocks; b += 4) s += sums[(long long)b * N + col];
-    part[q][c] = s;
+        for (int b = q; b < blocks; b += 64)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (b + 16 * u < blocks) s[u] += sums[(long long)(b + 16 * u) * N + col];
+    part[q][c] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
-    if (q == 0 && col < N) d_bias[col] = (T)(part[0][c] + part[1][c] + part[2][c] + part[3][c]);
+    if (q == 0 && col < N) {
+        float v = part[0][c];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) v += part[r][c];
+        d_bias[col] = (T)v;
+    }
 }
 
 template <typename T>
@@ -741,14 +840,22 @@ static bool dn_raise_lds(const void* kernel, int bytes, std::atomic<uint64_t>& r
     return true;
 }
 
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
-static int dn_launch_tiles(const DnGemm& g, unsigned blocks, hipStream_t stream) {
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, bool FULL>
+static int dn_launch_kernel(const DnGemm& g, unsigned blocks, hipStream_t stream) {
     constexpr int lds = DN_RING * (BI + BJ) * DN_SK * 2;
     static std::atomic<uint64_t> raised{0};
-    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ>), lds, raised))
+    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, FULL>), lds, raised))
         return FRCNN_E_LAUNCH;
-    FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ>), dim3(blocks), dim3(64 * WI * WJ), lds, stream, g);
+    FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, FULL>), dim3(blocks), dim3(64 * WI * WJ), lds, stream, g);
     return FRCNN_OK;
+}
+
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
+static int dn_launch_tiles(const DnGemm& g, unsigned blocks, hipStream_t stream) {
+    const bool full = !g.partial && (g.e.bias || g.e.pre || g.e.residual || g.e.act != FRCNN_ACT_NONE || g.e.out_f32);
+    if constexpr (AKC)          // d_weight's product has none of it
+        if (full) return dn_launch_kernel<T, AKC, BKC, BI, BJ, WI, WJ, true>(g, blocks, stream);
+    return dn_launch_kernel<T, AKC, BKC, BI, BJ, WI, WJ, false>(g, blocks, stream);
 }
 
 template <typename T, bool AKC, bool BKC>
@@ -840,19 +947,23 @@ static size_t dn_product_bytes(long long ra, long long ca, bool akc, long long r
 }
 
 // the backward's workspace: dz, its column sums, then what one product at a time needs
-struct DnBwdPlan { bool copy; long long ldz; int rows; long long blocks; size_t dz_bytes, sum_bytes; };
+struct DnBwdPlan { bool copy; long long ldz; int cg; long long rows, blocks; size_t dz_bytes, sum_bytes; };
 
 static DnBwdPlan dn_bwd_plan(long long M, int N, bool copy) {
     DnBwdPlan p{};
     if (M == 0) return p;                              // nothing to multiply: zeros are stored
     p.copy = copy;
     p.ldz = dn_pieces(N) * 8;
-    p.rows = 64;
+    // a workgroup takes 256 / cg rows at a time of 8 cg columns: two to eight such walks, as many workgroups
+    // as fill the chip four times, at most 4,096 partial sums per column
+    p.cg = 1;
+    while (p.cg < 32 && p.cg < dn_pieces(N)) p.cg *= 2;
+    const long long walk = 256 / p.cg, columns = (dn_pieces(N) + p.cg - 1) / p.cg;
+    long long walks = M * columns / (walk * 4 * DN_TARGET_WG);
+    walks = walks < 2 ? 2 : walks > 8 ? 8 : walks;
+    while ((M + walk * walks - 1) / (walk * walks) > 4096) walks *= 2;
+    p.rows = walk * walks;
     p.blocks = (M + p.rows - 1) / p.rows;
-    if (p.blocks > 4096) {                             // long batches: up to 4,096 partial sums per column
-        p.rows = (int)(((M + 4095) / 4096 + 63) / 64 * 64);
-        p.blocks = (M + p.rows - 1) / p.rows;
-    }
     p.dz_bytes = copy ? dn_up((size_t)M * (size_t)p.ldz * 2) : 0;
     p.sum_bytes = dn_up((size_t)p.blocks * (size_t)N * 4);
     return p;
@@ -873,13 +984,10 @@ static int dn_zero(void* p, long long rows, long long cols, long long ld, hipStr
 template <typename T, typename D>
 static int dn_launch_dz(const void* d_out, long long ldd, const void* pre, long long ldp, long long M, int N, int act,
                         const DnBwdPlan& p, void* dz, float* sums, hipStream_t s) {
-    const int pieces = (N + 7) / 8;
-    int cg = 1;
-    while (cg < 32 && cg < pieces) cg *= 2;
-    const long long gy = (pieces + cg - 1) / cg;
+    const long long gy = (dn_pieces(N) + p.cg - 1) / p.cg;
     if (p.blocks > 0x7FFFFFFFll || gy > 65535) return FRCNN_E_UNSUPPORTED;
     FRCNN_LAUNCH((dense_dz_kernel<T, D>), dim3((unsigned)p.blocks, (unsigned)gy), dim3(256), 0, s, (const D*)d_out,
-                 ldd, (const T*)pre, ldp, M, N, act, p.rows, cg, (T*)dz, p.ldz, sums);
+                 ldd, (const T*)pre, ldp, M, N, act, p.rows, p.cg, (T*)dz, p.ldz, sums);
     return FRCNN_OK;
 }
 
@@ -904,7 +1012,7 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
         if (rc != FRCNN_OK) return rc;
     }
     if (sums)
-        FRCNN_LAUNCH(dense_bias_grad_kernel<T>, dim3((unsigned)((N + 63) / 64)), dim3(256), 0, s, sums,
+        FRCNN_LAUNCH(dense_bias_grad_kernel<T>, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, s, sums,
                      (int)p.blocks, N, (T*)d_bias);
     const DnMatrix z = dz ? DnMatrix{dz, M, N, p.ldz, true} : DnMatrix{d_out, M, N, ldd, false};
     const DnMatrix mx{x, M, K, ldx, false};

@@ -28,8 +28,7 @@ typedef _Float16 dn_f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) dn_s16x4 dn_lds_s16x4;
 typedef __attribute__((address_space(3))) const dn_s16x8 dn_lds_s16x8;
 
-constexpr int DN_BK = 64;                       // k per LDS tile
-constexpr int DN_TARGET_WG = 256;               // compute units
+constexpr int DN_CUS = 256;                     // compute units
 
 __device__ __forceinline__ dn_f32x4 dn_mfma(dn_s16x8 a, dn_s16x8 b, dn_f32x4 c, __bf16) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dn_bf16x8, a),
@@ -137,7 +136,7 @@ struct DnGemm {
     const void *a, *b;
     long long lda, ldb, I, J, K;
     long long outer_a, outer_b;   // I, J rounded up to whole pieces where the operand's rows are that long
-    long long k_slice;        // k per slice, a multiple of DN_BK
+    long long k_slice;        // k per slice: an even number of steps
     int splits, tiles_i, tiles_j;
     float* partial;           // [splits][I][Jp], Jp = J rounded up to 4, when splits > 1
     DnEpilogue e;
@@ -794,6 +793,19 @@ __global__ void __launch_bounds__(256) dense_zero_kernel(T* p, long long rows, l
 // ---- host ------------------------------------------------------------------------------------------
 struct DnPlan { int bi, bj, splits; long long k_slice, tiles_i, tiles_j; size_t partial_bytes; };
 
+// Workgroup tiles: what a step of 32 k takes in us on a compute unit that is full of such workgroups (with
+// W as [N,K], both operands k-contiguous: step_kc), and for one alone; the rest of a workgroup (start, first
+// copies, results) and how many are resident.  Measured with every tile and split on products from 300 x 512 x
+// 512 to 16,000 x 25,088 x 4,096; what follows takes the pair with the shortest sum (rounds over the chip, at
+// least the operands' bytes at 4.6 TB/s from all compute units, plus the join of a split).  Large products want the large tile
+// (1.45 PFLOP/s; 1.2 from 128 x 128), 2,000 x 25,088 x 4,096 two slices of it (295 us; 391 from 128 x 128
+// unsplit), 1,024 cubed the small one (10.5 us; 15.6 from 128 x 256).
+struct DnTile { int bi, bj; double step, step_kc, alone, fixed; int resident; };
+constexpr DnTile DN_TILES[] = {{256, 256, 0.69, 0.69, 0.69, 5.5, 1},
+                               {128, 256, 0.374, 0.50, 0.374, 5.0, 1},
+                               {128, 128, 0.215, 0.215, 0.26, 4.0, 2},
+                               {64, 128, 0.18, 0.18, 0.22, 3.0, 3}};
+
 // akc: A is k-contiguous (the forward and d_x); only those products have few rows
 static DnPlan dn_plan(long long I, long long J, long long K, bool akc, bool bkc) {
     DnPlan p{};
@@ -804,7 +816,7 @@ static DnPlan dn_plan(long long I, long long J, long long K, bool akc, bool bkc)
         p.tiles_i = 1;
         p.tiles_j = (J + p.bj - 1) / p.bj;
         const long long pieces = (K + 64 * DN_FW - 1) / (64 * DN_FW);
-        long long splits = pieces >= 16 ? DN_TARGET_WG / p.tiles_j : 1;
+        long long splits = pieces >= 16 ? DN_CUS / p.tiles_j : 1;
         if (splits > pieces / 4) splits = pieces / 4;
         if (splits < 1) splits = 1;
         const long long per = (pieces + splits - 1) / splits;
@@ -813,18 +825,29 @@ static DnPlan dn_plan(long long I, long long J, long long K, bool akc, bool bkc)
         p.partial_bytes = p.splits > 1 ? (size_t)p.splits * (size_t)I * (size_t)((J + 3) / 4 * 4) * 4 : 0;
         return p;
     }
-    const long long big = ((I + 255) / 256) * ((J + 255) / 256);
-    p.bi = p.bj = big >= DN_TARGET_WG / 2 ? 256 : 128;
-    p.tiles_i = (I + p.bi - 1) / p.bi;
-    p.tiles_j = (J + p.bj - 1) / p.bj;
-    const long long tiles = p.tiles_i * p.tiles_j, steps = (K + DN_BK - 1) / DN_BK;
-    long long splits = tiles >= DN_TARGET_WG || p.bi == 256 ? 1 : 2 * DN_TARGET_WG / tiles;
-    if (splits > steps / 4) splits = steps / 4;        // four k steps per slice at least
-    if (splits > 32) splits = 32;
-    if (splits < 1) splits = 1;
-    const long long per = (steps + splits - 1) / splits;
-    p.k_slice = per * DN_BK;
-    p.splits = (int)((steps + per - 1) / per);         // no empty slice
+    const long long steps = (K + DN_SK - 1) / DN_SK;
+    const double bytes = 2.0 * ((double)I * K + (double)J * K + (double)I * J);
+    double best = 0.0;
+    for (const DnTile& t : DN_TILES) {
+        const long long ti = (I + t.bi - 1) / t.bi, tj = (J + t.bj - 1) / t.bj;
+        const double sat = bkc && akc ? t.step_kc : t.step;
+        for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+            if (want > 1 && steps < 8 * want) break;       // eight steps per slice at least
+            const long long per = ((steps + want - 1) / want + 1) / 2 * 2, splits = (steps + per - 1) / per;
+            const double groups = (double)(ti * tj) * (double)splits;
+            const double waves = groups <= DN_CUS ? 1.0 : __builtin_ceil(groups / DN_CUS);
+            double us = per * (waves * sat > t.alone ? waves * sat : t.alone) + t.fixed * __builtin_ceil(waves / t.resident);
+            const double stream = bytes / (4.6e6 * (groups < DN_CUS ? groups / DN_CUS : 1.0));
+            if (us < stream) us = stream;
+            if (splits > 1) us += 5.0 + (double)splits * I * J * 8.0 / 1.0e7;
+            // in doubt the larger tile and fewer slices
+            if (p.bi && us > 0.97 * best) continue;
+            best = us;
+            p.bi = t.bi; p.bj = t.bj;
+            p.tiles_i = ti; p.tiles_j = tj;
+            p.splits = (int)splits; p.k_slice = per * DN_SK;
+        }
+    }
     p.partial_bytes = p.splits > 1 ? (size_t)p.splits * (size_t)I * (size_t)((J + 3) / 4 * 4) * 4 : 0;
     return p;
 }
@@ -872,7 +895,9 @@ static int dn_launch_gemm(const DnPlan& pl, const DnGemm& g, hipStream_t stream)
     const long long blocks = pl.tiles_i * pl.tiles_j * pl.splits;
     if (blocks > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
     if (pl.bi == 256) return dn_launch_tiles<T, AKC, BKC, 256, 256, 2, 4>(g, (unsigned)blocks, stream);
-    return dn_launch_tiles<T, AKC, BKC, 128, 128, 2, 2>(g, (unsigned)blocks, stream);
+    if (pl.bj == 256) return dn_launch_tiles<T, AKC, BKC, 128, 256, 2, 4>(g, (unsigned)blocks, stream);
+    if (pl.bi == 128) return dn_launch_tiles<T, AKC, BKC, 128, 128, 2, 2>(g, (unsigned)blocks, stream);
+    return dn_launch_tiles<T, AKC, BKC, 64, 128, 1, 4>(g, (unsigned)blocks, stream);
 }
 
 static size_t dn_up(size_t b) { return (b + 255) / 256 * 256; }
@@ -959,7 +984,7 @@ static DnBwdPlan dn_bwd_plan(long long M, int N, bool copy) {
     p.cg = 1;
     while (p.cg < 32 && p.cg < dn_pieces(N)) p.cg *= 2;
     const long long walk = 256 / p.cg, columns = (dn_pieces(N) + p.cg - 1) / p.cg;
-    long long walks = M * columns / (walk * 4 * DN_TARGET_WG);
+    long long walks = M * columns / (walk * 4 * DN_CUS);
     walks = walks < 2 ? 2 : walks > 8 ? 8 : walks;
     while ((M + walk * walks - 1) / (walk * walks) > 4096) walks *= 2;
     p.rows = walk * walks;

@@ -109,12 +109,14 @@ __device__ __forceinline__ float ds_block(float v, float* sh) {
 }
 
 // ---- the teacher's side of a row, by one wave ----------------------------------------------------------
-// LDS: per entry its label (-1: not there), t / T relative to the largest one, the student's logit there
+// LDS: per entry its label (-1: not there), t / T relative to the largest one, the student's logit there,
+// and what its label gets: the sum of its entries' p at the first of them, -1 at the others
 struct DsTeacher {
-    int* label; float* t; float* z;
+    int* label; float* t; float* z; float* p;
     __device__ __forceinline__ DsTeacher(void* lds, int k)
-        : label((int*)lds), t((float*)lds + k), z((float*)lds + 2 * k) {}
+        : label((int*)lds), t((float*)lds + k), z((float*)lds + 2 * k), p((float*)lds + 3 * k) {}
 };
+constexpr int DS_ENTRY_BYTES = 16;
 struct DsTeacherSum { float log_sum; bool any; };      // log of the sum of e^t; whether an entry is there
 
 template <typename T>
@@ -164,21 +166,39 @@ __device__ __forceinline__ float ds_row_loss(const DsArgs& a, DsTeacher e, float
     return ds_wave_sum(l);
 }
 
-// writes the gradient at the listed labels in [v0, v1): the first entry of a label takes all of them
-template <typename T, typename Q>
-__device__ __forceinline__ void ds_listed(const DsArgs& a, DsTeacher e, float log_sum, float c, T* grad, long long v0,
-                                          long long v1, int tid, int block, Q q_of) {
-    for (int j = tid; j < a.k; j += block) {
-        const int i = e.label[j];
-        if (i < v0 || i >= v1) continue;
-        bool first = true;
-        float p = 0.f;
-        for (int n = 0; n < a.k; ++n) {
-            if (e.label[n] != i) continue;
-            if (n < j) { first = false; break; }
-            p += __builtin_amdgcn_exp2f((e.t[n] - log_sum) * DS_LOG2E);
+// e.p for the entries of one wave in every `waves`: 64 entries in its lanes against all entries one by one
+// (from a register of another lane: an LDS read per comparison costs the whole row its latency)
+__device__ __forceinline__ void ds_listed_sums(DsTeacher e, int k, float log_sum, int wave, int waves) {
+    const int lane = lane_id();
+    for (int j0 = 64 * wave; j0 < k; j0 += 64 * waves) {
+        const int mine = j0 + lane < k ? e.label[j0 + lane] : -1;
+        float sum = 0.f;
+        bool first = mine >= 0;
+        for (int n0 = 0; n0 < k; n0 += 64) {
+            const int label = n0 + lane < k ? e.label[n0 + lane] : -1;
+            const float p = n0 + lane < k ? __builtin_amdgcn_exp2f((e.t[n0 + lane] - log_sum) * DS_LOG2E) : 0.f;
+            const int end = k - n0 < 64 ? k - n0 : 64;
+            for (int n = 0; n < end; ++n) {
+                const int other = __builtin_amdgcn_readlane(label, n);
+                const float q = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), n));
+                if (other == mine) {
+                    sum += q;
+                    if (n0 + n < j0 + lane) first = false;
+                }
+            }
         }
-        if (first) grad[i] = (T)(c * (q_of(e.z[j]) - p));
+        if (j0 + lane < k) e.p[j0 + lane] = first ? sum : -1.0f;
+    }
+}
+
+// writes the gradient at the listed labels in [v0, v1)
+template <typename T, typename Q>
+__device__ __forceinline__ void ds_listed(DsTeacher e, int k, float c, T* grad, long long v0, long long v1, int tid,
+                                          int block, Q q_of) {
+    for (int j = tid; j < k; j += block) {
+        const int i = e.label[j];
+        const float p = e.p[j];
+        if (i >= v0 && i < v1 && !(p < 0.f)) grad[i] = (T)(c * (q_of(e.z[j]) - p));      // also a NaN
     }
 }
 
@@ -299,6 +319,7 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
         for (int j = 0; j < W; ++j) part += __builtin_amdgcn_exp2f((x[i][j] - m) * f);
         s += part;
     }
+    if (grad) ds_listed_sums(e, a.k, sh_t, wave_id(), BLOCK / 64);
     s = ds_block<BLOCK, false>(s, sh_s);
     const float log_s = logf(s);
     if (wave_id() == 0) {
@@ -321,15 +342,16 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
         x[i].store(grad + v, a.V - v);
     }
     __syncthreads();                                   // the stores of c q come before those of the listed labels
-    ds_listed(a, e, sh_t, c, grad, 0, a.V, tid, BLOCK,
+    ds_listed(e, a.k, c, grad, 0, a.V, tid, BLOCK,
               [&](float zi) { return __builtin_amdgcn_exp2f((zi - m) * f) / s; });
 }
 
 // ---- a chunk of a row per workgroup --------------------------------------------------------------------
-constexpr int DS_CHUNK_BLOCK = 256, DS_CHUNK_NV = 4;
-template <typename T> constexpr int ds_chunk() { return DS_CHUNK_BLOCK * DS_CHUNK_NV * DsVec<T>::W; }
+// of 4 vectors per thread, of one where the rows are few and their chunks would not fill the chip
+constexpr int DS_CHUNK_BLOCK = 256;
+template <typename T, int NV> constexpr int ds_chunk() { return DS_CHUNK_BLOCK * NV * DsVec<T>::W; }
 
-template <typename T>
+template <typename T, int NV>
 __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_part_kernel(DsArgs a) {
     __shared__ float sh_m[DS_CHUNK_BLOCK / 64], sh_s[DS_CHUNK_BLOCK / 64];
     constexpr int W = DsVec<T>::W;
@@ -337,16 +359,16 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_part_kernel(DsArgs a) 
     const long long row = blockIdx.y;
     if (a.weight && a.weight[row] == 0.f) return;
     const T* z = (const T*)a.z + row * a.ldz;
-    const long long v0 = (long long)chunk * ds_chunk<T>();
-    DsVec<T> x[DS_CHUNK_NV];
+    const long long v0 = (long long)chunk * ds_chunk<T, NV>();
+    DsVec<T> x[NV];
     float m = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < DS_CHUNK_NV; ++i) {
+    for (int i = 0; i < NV; ++i) {
         const long long v = v0 + (tid + DS_CHUNK_BLOCK * i) * W, left = a.V - v;
         x[i].load(z + v, left > W ? W : (int)left);
     }
 #pragma unroll
-    for (int i = 0; i < DS_CHUNK_NV; ++i)
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < W; ++j) m = fmaxf(m, x[i][j]);
     m = ds_block<DS_CHUNK_BLOCK, true>(m, sh_m);
@@ -354,7 +376,7 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_part_kernel(DsArgs a) 
     const float base = m == -__builtin_inff() ? 0.f : m;    // a chunk of -inf alone has the sum 0
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < DS_CHUNK_NV; ++i)
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < W; ++j) s += __builtin_amdgcn_exp2f((x[i][j] - base) * f);
     s = ds_block<DS_CHUNK_BLOCK, false>(s, sh_s);
@@ -362,7 +384,7 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_part_kernel(DsArgs a) 
 }
 
 // FORWARD: joins the row's partial sums; chunk 0 writes loss and lse; else q comes from the forward's lse
-template <typename T, bool FORWARD>
+template <typename T, bool FORWARD, int NV>
 __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_chunk_kernel(DsArgs a) {
     extern __shared__ __attribute__((aligned(16))) char ds_lds[];
     __shared__ float sh_t, sh_m, sh_s;
@@ -372,17 +394,17 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_chunk_kernel(DsArgs a)
     const long long row = blockIdx.y;
     const T* z = (const T*)a.z + row * a.ldz;
     T* grad = a.grad ? (T*)a.grad + row * a.ldg : nullptr;
-    const long long v0 = (long long)chunk * ds_chunk<T>(), v1 = v0 + ds_chunk<T>() < a.V ? v0 + ds_chunk<T>() : a.V;
+    const long long v0 = (long long)chunk * ds_chunk<T, NV>(), v1 = v0 + ds_chunk<T, NV>() < a.V ? v0 + ds_chunk<T, NV>() : a.V;
     const float w = a.weight ? a.weight[row] : 1.0f, inv_t = 1.0f / a.temperature;
     if (w == 0.f) {
         if (FORWARD && chunk == 0 && tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
         if (grad) ds_zero(grad, v0, v1, tid, DS_CHUNK_BLOCK);
         return;
     }
-    DsVec<T> x[DS_CHUNK_NV];
+    DsVec<T> x[NV];
     if (grad) {
 #pragma unroll
-        for (int i = 0; i < DS_CHUNK_NV; ++i) {
+        for (int i = 0; i < NV; ++i) {
             const long long v = v0 + (tid + DS_CHUNK_BLOCK * i) * W, left = a.V - v;
             x[i].load(z + v, left > W ? W : (int)left);
         }
@@ -422,13 +444,14 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_chunk_kernel(DsArgs a)
         }
     }
     if (!grad) return;
+    ds_listed_sums(e, a.k, sh_t, wave_id(), DS_CHUNK_BLOCK / 64);
     const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale), cq = FORWARD ? c / s : c;
     const float f = inv_t * DS_LOG2E;
     auto relative = [&](float zi) {
         return __builtin_amdgcn_exp2f(FORWARD ? (zi - m) * f : (zi * inv_t - lse) * DS_LOG2E);
     };
 #pragma unroll
-    for (int i = 0; i < DS_CHUNK_NV; ++i) {
+    for (int i = 0; i < NV; ++i) {
         const long long v = v0 + (tid + DS_CHUNK_BLOCK * i) * W, left = a.V - v;
         float q[W];
 #pragma unroll
@@ -437,18 +460,23 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_chunk_kernel(DsArgs a)
         x[i].store(grad + v, left > W ? W : (int)left);
     }
     __syncthreads();
-    ds_listed(a, e, sh_t, c, grad, v0, v1, tid, DS_CHUNK_BLOCK, [&](float zi) { return relative(zi) / s; });
+    ds_listed(e, a.k, c, grad, v0, v1, tid, DS_CHUNK_BLOCK, [&](float zi) { return relative(zi) / s; });
 }
 
 // ---- host --------------------------------------------------------------------------------------------
 // rows that one workgroup can hold, and long rows of which there are too few to fill the chip
 static long long ds_vectors(int V, int dtype) { return (V + (dtype == FRCNN_DT_F32 ? 4 : 8) - 1) / (dtype == FRCNN_DT_F32 ? 4 : 8); }
-static long long ds_chunks(int V, int dtype) {
-    return (ds_vectors(V, dtype) + DS_CHUNK_BLOCK * DS_CHUNK_NV - 1) / (DS_CHUNK_BLOCK * DS_CHUNK_NV);
+static int ds_chunk_vectors(long long rows, int V, int dtype) {
+    const long long four = (ds_vectors(V, dtype) + DS_CHUNK_BLOCK * 4 - 1) / (DS_CHUNK_BLOCK * 4);
+    return rows * four <= 256 ? 1 : 4;
+}
+static long long ds_chunks(long long rows, int V, int dtype) {
+    const long long c = (long long)DS_CHUNK_BLOCK * ds_chunk_vectors(rows, V, dtype);
+    return (ds_vectors(V, dtype) + c - 1) / c;
 }
 static bool ds_split(long long rows, int V, int dtype) {
-    const long long chunks = ds_chunks(V, dtype);
-    return ds_vectors(V, dtype) > 16384 || (chunks >= 4 && rows * chunks <= 1024);
+    const long long n = ds_vectors(V, dtype);
+    return n > 16384 || (n >= 4 * 1024 && rows * ((n + 1023) / 1024) <= 1024);
 }
 static int ds_group(int V, int k) {
     int g = 1;
@@ -466,7 +494,7 @@ static int ds_launch_small(const DsArgs& a, hipStream_t s) {
 template <typename T, int BLOCK, int NV>
 static int ds_launch_row(const DsArgs& a, hipStream_t s) {
     if (a.rows > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
-    FRCNN_LAUNCH((distill_row_kernel<T, BLOCK, NV>), dim3((unsigned)a.rows), dim3(BLOCK), (size_t)a.k * 12, s, a);
+    FRCNN_LAUNCH((distill_row_kernel<T, BLOCK, NV>), dim3((unsigned)a.rows), dim3(BLOCK), (size_t)a.k * DS_ENTRY_BYTES, s, a);
     return FRCNN_OK;
 }
 
@@ -478,13 +506,15 @@ static int ds_run(DsArgs a, int dtype, hipStream_t s) {
     if (g <= 32) return ds_launch_small<T, FORWARD, 32>(a, s);
     if (g <= 64) return ds_launch_small<T, FORWARD, 64>(a, s);
     const long long n = ds_vectors(a.V, dtype);
-    a.chunks = (int)ds_chunks(a.V, dtype);
+    const int nv = ds_chunk_vectors(a.rows, a.V, dtype);
+    a.chunks = (int)ds_chunks(a.rows, a.V, dtype);
     if (FORWARD && !ds_split(a.rows, a.V, dtype)) {
         if (n <= 64) return ds_launch_row<T, 64, 1>(a, s);
         if (n <= 256) return ds_launch_row<T, 64, 4>(a, s);
         if (n <= 1024) return ds_launch_row<T, 256, 4>(a, s);
-        if (n <= 4096) return ds_launch_row<T, 1024, 4>(a, s);
-        if (n <= 8192) return ds_launch_row<T, 1024, 8>(a, s);
+        if (n <= 2048) return ds_launch_row<T, 256, 8>(a, s);
+        if (n <= 4096) return ds_launch_row<T, 512, 8>(a, s);
+        if (n <= 8192) return ds_launch_row<T, 512, 16>(a, s);
         return ds_launch_row<T, 1024, 16>(a, s);
     }
     // rows along the grid's second dimension, at most 65,535 in a launch
@@ -501,9 +531,12 @@ static int ds_run(DsArgs a, int dtype, hipStream_t s) {
         if (a.grad) b.grad = (T*)a.grad + r * a.ldg;
         if (a.part) b.part = a.part + r * a.chunks;
         const dim3 grid((unsigned)a.chunks, (unsigned)b.rows);
-        if (FORWARD) FRCNN_LAUNCH((distill_part_kernel<T>), grid, dim3(DS_CHUNK_BLOCK), 0, s, b);
+        if (FORWARD && nv == 1) FRCNN_LAUNCH((distill_part_kernel<T, 1>), grid, dim3(DS_CHUNK_BLOCK), 0, s, b);
+        else if (FORWARD) FRCNN_LAUNCH((distill_part_kernel<T, 4>), grid, dim3(DS_CHUNK_BLOCK), 0, s, b);
         const dim3 gg(a.grad ? (unsigned)a.chunks : 1u, (unsigned)b.rows);      // without a gradient: the loss alone
-        FRCNN_LAUNCH((distill_chunk_kernel<T, FORWARD>), gg, dim3(DS_CHUNK_BLOCK), (size_t)a.k * 12, s, b);
+        const size_t lds = (size_t)a.k * DS_ENTRY_BYTES;
+        if (nv == 1) FRCNN_LAUNCH((distill_chunk_kernel<T, FORWARD, 1>), gg, dim3(DS_CHUNK_BLOCK), lds, s, b);
+        else FRCNN_LAUNCH((distill_chunk_kernel<T, FORWARD, 4>), gg, dim3(DS_CHUNK_BLOCK), lds, s, b);
     }
     return FRCNN_OK;
 }
@@ -537,7 +570,7 @@ using namespace frcnn;
 
 extern "C" size_t frcnn_distill_workspace_bytes(int64_t rows, int V, int k, int dtype) {
     if (rows <= 0 || V <= 0 || k <= 0 || ds_group(V, k) <= 64 || !ds_split(rows, V, dtype)) return 0;
-    return (size_t)rows * (size_t)ds_chunks(V, dtype) * sizeof(float2);
+    return (size_t)rows * (size_t)ds_chunks(rows, V, dtype) * sizeof(float2);
 }
 
 extern "C" int frcnn_distill_loss(const void* logits, int64_t ldz, int dtype, const void* top_values, int t_dtype,

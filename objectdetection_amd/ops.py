@@ -873,7 +873,7 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torc
     lse = torch.empty_like(loss)
     grad = pg = None
     if want_grad:
-        grad = z.new_empty(logits.shape)
+        grad = torch.empty_like(logits) if logits.is_contiguous() else z.new_empty(logits.shape)
         pg = grad.data_ptr()
     pws, nws, ws = _scratch(workspace, distill_workspace_bytes(rows, V, k, z.dtype), z, dev)
     _call("frcnn_distill_loss", lib.frcnn_distill_loss, dev, (

@@ -17,6 +17,7 @@
 // sums: each output is rounded once.
 #include "frcnn_common.h"
 #include <atomic>
+#include <type_traits>
 
 namespace frcnn {
 
@@ -123,6 +124,21 @@ __device__ __forceinline__ void dn_store(T* p, int valid, const float* v) {
     }
 }
 
+// the first `valid` of eight values, without a branch where all are known to be wanted
+template <bool ALL, typename T>
+__device__ __forceinline__ void dn_store_some(T* p, int valid, const float (&v)[8]) {
+    T t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = (T)v[e];
+    if constexpr (ALL) {
+        __builtin_memcpy(p, t, 8 * sizeof(T));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < valid) p[e] = t[e];
+    }
+}
+
 // ---- the product's arguments -------------------------------------------------------------------------
 struct DnEpilogue {
     const void* bias;         // [N'] or null
@@ -219,88 +235,95 @@ __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&a
         }
         return;
     }
-    const long long row0 = i0 + lane / Q, gj = j0 + 8 * (lane % Q), left = p.J - gj;
+    if (j0 >= p.J) return;
+    const long long row0 = i0 + lane / Q, gj = j0 + 8 * (lane % Q);
+    const int valid = p.J - gj > 8 ? 8 : (int)(p.J - gj);
     char* put = turn + (lane & 15) * S + (lane >> 4) * 16;
     const char* get = turn + (lane / Q) * S + (lane % Q) * 32;
-    auto turn_in = [&](const dn_f32x4 (&a)[FJ]) {
-        __builtin_amdgcn_wave_barrier();
+    const DnEpilogue& ep = p.e;
+    const bool has_res = FULL && ep.residual, has_pre = FULL && ep.pre, f32 = FULL && ep.out_f32;
+    // INNER: whole pieces in all lanes; else value by value, loads at clamped places instead of under a guard
+    auto body = [&](auto inner) {
+        constexpr bool INNER = decltype(inner)::value;
+        auto load = [&](const T* row, short (&to)[8]) {
+            if constexpr (INNER) {
+                __builtin_memcpy(to, row + gj, 16);
+            } else {
 #pragma unroll
-        for (int j = 0; j < FJ; ++j) *reinterpret_cast<dn_f32x4*>(put + j * 64) = a[j];
-        __builtin_amdgcn_wave_barrier();
-    };
-    auto turn_out = [&](int pass, float (&v)[8]) { __builtin_memcpy(v, get + pass * RP * S, 32); };
-    if (j0 + 16 * FJ <= p.J && !(FULL && p.e.out_f32)) {
-        T* out = (T*)p.e.out + row0 * p.e.ldo + gj;
-        if constexpr (!FULL) {
-#pragma unroll
-            for (int i = 0; i < FI; ++i) {
-                turn_in(acc[i]);
-#pragma unroll
-                for (int r = 0; r < NP; ++r) {
-                    float v[8];
-                    turn_out(r, v);
-                    if (row0 + 16 * i + r * RP < p.I) dn_store<T, 8>(out + (16 * i + r * RP) * p.e.ldo, 8, v);
+                for (int e = 0; e < 8; ++e) {
+                    const long long j = gj + e < p.J ? gj + e : p.J - 1;
+                    __builtin_memcpy(&to[e], row + j, 2);
                 }
             }
-        } else {
-            const bool has_res = p.e.residual != nullptr, has_pre = p.e.pre != nullptr;
-            const int act = p.e.act;
-            T* pre = (T*)p.e.pre + (has_pre ? row0 * p.e.ldp + gj : 0);
-            const T* res = (const T*)p.e.residual + (has_res ? gj : 0);
-            float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (p.e.bias) dn_load<T, 8>((const T*)p.e.bias + gj, 8, bias);
-            dn_s16x8 now[NP] = {}, next[NP] = {};
-            auto fetch = [&](int i, dn_s16x8 (&to)[NP]) {
+        };
+        auto store = [&](auto* to, const float (&v)[8]) { dn_store_some<INNER>(to, valid, v); };
+        float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        short now[NP][8] = {}, next[NP][8] = {};
+        auto fetch = [&](int i, short (&to)[NP][8]) {
 #pragma unroll
-                for (int r = 0; r < NP; ++r) {
-                    const long long gi = row0 + 16 * i + r * RP;
-                    __builtin_memcpy(&to[r], res + (gi < p.I ? gi : p.I - 1) * p.e.ldr, 16);
-                }
-            };
+            for (int r = 0; r < NP; ++r) {
+                const long long gi = row0 + 16 * i + r * RP;
+                load((const T*)ep.residual + (gi < p.I ? gi : p.I - 1) * ep.ldr, to[r]);
+            }
+        };
+        if constexpr (FULL) {
+            if (ep.bias) {
+                short t[8];
+                load((const T*)ep.bias, t);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) bias[e] = (float)__builtin_bit_cast(T, t[e]);
+            }
             if (has_res) fetch(0, now);
+        }
+        // a loop, not FI copies: code that runs once per workgroup is fetched from beyond the instruction cache
+#pragma unroll 1
+        for (int i = 0; i < FI; ++i) {
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int i = 0; i < FI; ++i) {
-                turn_in(acc[i]);
-                if (has_res && i + 1 < FI) fetch(i + 1, next);
+            for (int c = 0; c < FI; ++c)
+                if (i == c) {
+                    asm volatile("; rows %0" ::"n"(c));           // keeps the branches apart: acc stays in registers
 #pragma unroll
-                for (int r = 0; r < NP; ++r) {
-                    const bool inside = row0 + 16 * i + r * RP < p.I;
-                    float v[8];
-                    turn_out(r, v);
+                    for (int j = 0; j < FJ; ++j) {
+                        dn_f32x4 a = acc[c][j];
+                        asm volatile("" : "+v"(a));
+                        *reinterpret_cast<dn_f32x4*>(put + j * 64) = a;
+                    }
+                }
+            __builtin_amdgcn_wave_barrier();
+            if (has_res && i + 1 < FI) fetch(i + 1, next);
+#pragma unroll
+            for (int r = 0; r < NP; ++r) {
+                const long long gi = row0 + 16 * i + r * RP;
+                const bool inside = gi < p.I;
+                float v[8];
+                __builtin_memcpy(v, get + r * RP * S, 32);
+                if constexpr (FULL) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] += bias[e];
-                    if (has_pre && inside) dn_store<T, 8>(pre + (16 * i + r * RP) * p.e.ldp, 8, v);
-                    if (act != FRCNN_ACT_NONE) {
+                    if (has_pre && inside) store((T*)ep.pre + gi * ep.ldp + gj, v);
+                    if (ep.act != FRCNN_ACT_NONE) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = dn_act(v[e], act);
+                        for (int e = 0; e < 8; ++e) v[e] = dn_act(v[e], ep.act);
                     }
                     if (has_res) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] += (float)__builtin_bit_cast(T, (short)now[r][e]);
+                        for (int e = 0; e < 8; ++e) v[e] += (float)__builtin_bit_cast(T, now[r][e]);
                     }
-                    if (inside) dn_store<T, 8>(out + (16 * i + r * RP) * p.e.ldo, 8, v);
                 }
-#pragma unroll
-                for (int r = 0; r < NP; ++r) now[r] = next[r];
+                if (inside) {
+                    if (f32) store((float*)ep.out + gi * ep.ldo + gj, v);
+                    else store((T*)ep.out + gi * ep.ldo + gj, v);
+                }
             }
-        }
-        return;
-    }
-    // a tile at the matrix' right edge, or float32 outputs
-#pragma unroll 1
-    for (int i = 0; i < FI; ++i) {
 #pragma unroll
-        for (int c = 0; c < FI; ++c)
-            if (i == c) turn_in(acc[c]);
-#pragma unroll 1
-        for (int r = 0; r < NP; ++r) {
-            const long long gi = row0 + 16 * i + r * RP;
-            if (gi >= p.I || left <= 0) continue;
-            float v[8];
-            turn_out(r, v);
-            dn_epilogue<T, 8>(p.e, gi, gj, left > 8 ? 8 : (int)left, v);
+            for (int r = 0; r < NP; ++r)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) now[r][e] = next[r][e];
         }
-    }
+    };
+    if (j0 + 16 * FJ <= p.J) body(std::true_type());
+    else body(std::false_type());
 }
 
 // ---- the product -----------------------------------------------------------------------------------------
@@ -796,20 +819,24 @@ struct DnPlan { int bi, bj, splits; long long k_slice, tiles_i, tiles_j; size_t 
 // Workgroup tiles: what a step of 32 k takes in us on a compute unit that is full of such workgroups (with
 // W as [N,K], both operands k-contiguous: step_kc), and for one alone; the rest of a workgroup (start, first
 // copies, results) and how many are resident.  Measured with every tile and split on products from 300 x 512 x
-// 512 to 16,000 x 25,088 x 4,096; what follows takes the pair with the shortest sum (rounds over the chip, at
-// least the operands' bytes at 4.6 TB/s from all compute units, plus the join of a split).  Large products want the large tile
-// (1.45 PFLOP/s; 1.2 from 128 x 128), 2,000 x 25,088 x 4,096 two slices of it (295 us; 391 from 128 x 128
-// unsplit), 1,024 cubed the small one (10.5 us; 15.6 from 128 x 256).
+// 512 to 16,000 x 25,088 x 4,096; what follows takes the pair with the shortest sum: rounds over the chip, at
+// least the operands' bytes at 4.6 TB/s and what tiles copy again at 20 TB/s (all compute units), plus the
+// join of a split.  Large products want the large tile (1.45 PFLOP/s; 1.2 from 128 x 128), 2,000 x 25,088 x
+// 4,096 two slices of it (295 us; 391 from 128 x 128 unsplit), 128 x 25,088 x 4,096 eight slices of 128 x 128
+// (51 us; 67 from four of 64 x 128), 1,024 cubed the small one (10.5 us; 15.6 from 128 x 256).
 struct DnTile { int bi, bj; double step, step_kc, alone, fixed; int resident; };
 constexpr DnTile DN_TILES[] = {{256, 256, 0.69, 0.69, 0.69, 5.5, 1},
                                {128, 256, 0.374, 0.50, 0.374, 5.0, 1},
                                {128, 128, 0.215, 0.215, 0.26, 4.0, 2},
                                {64, 128, 0.18, 0.18, 0.22, 3.0, 3}};
 
+// a product of few rows reads its operands as they are
+static bool dn_few(long long rows) { return rows <= DN_FEW; }
+
 // akc: A is k-contiguous (the forward and d_x); only those products have few rows
 static DnPlan dn_plan(long long I, long long J, long long K, bool akc, bool bkc) {
     DnPlan p{};
-    if (akc && I <= DN_FEW) {
+    if (akc && dn_few(I)) {
         // one workgroup per 16 or 32 columns; a long reduction is split where that leaves compute units idle
         p.bi = 0;
         p.bj = bkc ? 16 : 32;
@@ -837,7 +864,10 @@ static DnPlan dn_plan(long long I, long long J, long long K, bool akc, bool bkc)
             const double groups = (double)(ti * tj) * (double)splits;
             const double waves = groups <= DN_CUS ? 1.0 : __builtin_ceil(groups / DN_CUS);
             double us = per * (waves * sat > t.alone ? waves * sat : t.alone) + t.fixed * __builtin_ceil(waves / t.resident);
-            const double stream = bytes / (4.6e6 * (groups < DN_CUS ? groups / DN_CUS : 1.0));
+            // what memory gives, and what L2 gives again
+            const double copied = groups * per * (t.bi + t.bj) * (2.0 * DN_SK);
+            const double stream = (bytes / 4.6e6 + (copied > bytes ? copied - bytes : 0.0) / 2.0e7) *
+                                  (groups < DN_CUS ? DN_CUS / groups : 1.0);
             if (us < stream) us = stream;
             if (splits > 1) us += 5.0 + (double)splits * I * J * 8.0 / 1.0e7;
             // in doubt the larger tile and fewer slices
@@ -914,32 +944,37 @@ static size_t dn_pack_bytes(long long rows, long long cols) {
     return dn_up((size_t)rows * (size_t)dn_pieces(cols) * 16);
 }
 
-// D = A B^T: `a` holds A as [I][K] (akc) or [K][I], `b` B as [J][K] (bkc) or [K][J].  Workspace: the packed
-// copies of the operands that need one, then the partial sums of a split reduction.
+// Copies of the matrices whose rows are not whole pieces, from `ws` on (which moves behind them); a null
+// matrix is left alone.
 template <typename T>
-static int dn_product(DnMatrix a, bool akc, DnMatrix b, bool bkc, const DnEpilogue& e, char* ws, hipStream_t stream) {
+static int dn_pack(DnMatrix* a, DnMatrix* b, char*& ws, hipStream_t stream) {
+    DnPack pack[2] = {};
+    long long blocks[2] = {0, 0};
+    int n = 0;
+    for (DnMatrix* m : {a, b}) {
+        if (!m || dn_whole(*m)) continue;
+        if (dn_pieces(m->cols) * 8 > (1ll << 21)) return FRCNN_E_UNSUPPORTED;
+        pack[n] = DnPack{m->p, ws, m->rows, m->cols, m->ld, dn_pieces(m->cols)};
+        blocks[n] = (m->rows * pack[n].pieces + 255) / 256;
+        ws += dn_pack_bytes(m->rows, m->cols);
+        *m = DnMatrix{pack[n].dst, m->rows, m->cols, pack[n].pieces * 8, true};
+        ++n;
+    }
+    if (!n) return FRCNN_OK;
+    if (blocks[0] + blocks[1] > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
+    FRCNN_LAUNCH(dense_pack_kernel<T>, dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), 0, stream, pack[0], pack[1],
+                 blocks[0]);
+    return FRCNN_OK;
+}
+
+// D = A B^T: `a` holds A as [I][K] (akc) or [K][I], `b` B as [J][K] (bkc) or [K][J], packed where they have
+// to be; the workspace holds the partial sums of a split reduction
+template <typename T>
+static int dn_product(const DnMatrix& a, bool akc, const DnMatrix& b, bool bkc, const DnEpilogue& e, void* ws,
+                      hipStream_t stream) {
     const long long I = akc ? a.rows : a.cols, K = akc ? a.cols : a.rows, J = bkc ? b.rows : b.cols;
     const DnPlan pl = dn_plan(I, J, K, akc, bkc);
     if (pl.tiles_i > 0x7FFFFF || pl.tiles_j > 0x7FFFFF) return FRCNN_E_UNSUPPORTED;
-    if (pl.bi) {
-        DnPack pack[2] = {};
-        long long blocks[2] = {0, 0};
-        int n = 0;
-        for (DnMatrix* m : {&a, &b}) {
-            if (dn_whole(*m)) continue;
-            if (dn_pieces(m->cols) * 8 > (1ll << 21)) return FRCNN_E_UNSUPPORTED;
-            pack[n] = DnPack{m->p, ws, m->rows, m->cols, m->ld, dn_pieces(m->cols)};
-            blocks[n] = (m->rows * pack[n].pieces + 255) / 256;
-            ws += dn_pack_bytes(m->rows, m->cols);
-            *m = DnMatrix{pack[n].dst, m->rows, m->cols, pack[n].pieces * 8, true};
-            ++n;
-        }
-        if (n) {
-            if (blocks[0] + blocks[1] > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
-            FRCNN_LAUNCH(dense_pack_kernel<T>, dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), 0, stream, pack[0],
-                         pack[1], blocks[0]);
-        }
-    }
     DnGemm g{};
     g.a = a.p; g.b = b.p; g.lda = a.ld; g.ldb = b.ld; g.I = I; g.J = J; g.K = K;
     g.outer_a = a.padded ? dn_pieces(I) * 8 : I;
@@ -960,15 +995,14 @@ static int dn_product(DnMatrix a, bool akc, DnMatrix b, bool bkc, const DnEpilog
     return FRCNN_OK;
 }
 
-// the workspace of one product whose operands are [ra][ca] and [rb][cb]
-enum DnRows { DN_ANY, DN_ALIGNED, DN_PADDED };         // rows anywhere; on 16 bytes; padded to whole pieces as well
-static size_t dn_product_bytes(long long ra, long long ca, bool akc, long long rb, long long cb, bool bkc,
-                               DnRows a_rows, DnRows b_rows) {
-    const DnPlan pl = dn_plan(akc ? ra : ca, bkc ? rb : cb, akc ? ca : ra, akc, bkc);
-    size_t bytes = dn_up(pl.partial_bytes);
-    if (pl.bi && !(a_rows == DN_PADDED || (a_rows == DN_ALIGNED && ca % 8 == 0))) bytes += dn_pack_bytes(ra, ca);
-    if (pl.bi && !(b_rows == DN_PADDED || (b_rows == DN_ALIGNED && cb % 8 == 0))) bytes += dn_pack_bytes(rb, cb);
-    return bytes;
+// Whether the operands of a product have to be whole pieces, and what its partial sums and its packed
+// operands take.  DN_ANY: rows anywhere; DN_ALIGNED: on 16 bytes; DN_PADDED: padded to whole pieces as well
+enum DnRows { DN_ANY, DN_ALIGNED, DN_PADDED };
+static size_t dn_copy_bytes(long long rows, long long cols, DnRows r) {
+    return r == DN_PADDED || (r == DN_ALIGNED && cols % 8 == 0) ? 0 : dn_pack_bytes(rows, cols);
+}
+static size_t dn_partial_bytes(long long I, long long J, long long K, bool akc, bool bkc) {
+    return dn_up(dn_plan(I, J, K, akc, bkc).partial_bytes);
 }
 
 // the backward's workspace: dz, its column sums, then what one product at a time needs
@@ -1017,6 +1051,15 @@ static int dn_launch_dz(const void* d_out, long long ldd, const void* pre, long 
 }
 
 template <typename T>
+static int dn_forward(DnMatrix x, DnMatrix w, bool bkc, const DnEpilogue& e, char* ws, hipStream_t s) {
+    if (!dn_few(x.rows)) {
+        const int rc = dn_pack<T>(&x, &w, ws, s);
+        if (rc != FRCNN_OK) return rc;
+    }
+    return dn_product<T>(x, true, w, bkc, e, ws, s);
+}
+
+template <typename T>
 static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void* x, long long ldx, const void* w,
                        long long ldw, int w_layout, const void* pre, long long ldp, long long M, int K, int N,
                        int dtype, int act, void* d_x, long long lddx, void* d_w, long long lddw, void* d_bias,
@@ -1040,11 +1083,12 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
         FRCNN_LAUNCH(dense_bias_grad_kernel<T>, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, s, sums,
                      (int)p.blocks, N, (T*)d_bias);
     const DnMatrix z = dz ? DnMatrix{dz, M, N, p.ldz, true} : DnMatrix{d_out, M, N, ldd, false};
-    const DnMatrix mx{x, M, K, ldx, false};
+    DnMatrix mx{x, M, K, ldx, false}, mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
+    rc = dn_pack<T>(d_x && !dn_few(M) ? &mw : nullptr, d_w ? &mx : nullptr, rest, s);
+    if (rc != FRCNN_OK) return rc;
     DnEpilogue e{};
     if (d_x) {
         e.out = d_x; e.ldo = lddx;
-        const DnMatrix mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
         rc = dn_product<T>(z, true, mw, kn, e, rest, s);
         if (rc != FRCNN_OK) return rc;
     }
@@ -1062,8 +1106,10 @@ using namespace frcnn;
 extern "C" size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
     if (!dn_sizes(M, K, N) || M == 0) return 0;
     const DnRows x = aligned & 1 ? DN_ALIGNED : DN_ANY, w = aligned & 2 ? DN_ALIGNED : DN_ANY;
-    return w_layout == FRCNN_W_KN ? dn_product_bytes(M, K, true, K, N, false, x, w)
-                                  : dn_product_bytes(M, K, true, N, K, true, x, w);
+    const bool kn = w_layout == FRCNN_W_KN;
+    const size_t partial = dn_partial_bytes(M, N, K, true, !kn);
+    if (dn_few(M)) return partial;
+    return dn_copy_bytes(M, K, x) + (kn ? dn_copy_bytes(K, N, w) : dn_copy_bytes(N, K, w)) + partial;
 }
 
 static int dn_aligned(const void* x, int64_t ldx, const void* w, int64_t ldw) {
@@ -1092,9 +1138,8 @@ extern "C" int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_
     e.bias = bias; e.residual = residual; e.pre = pre; e.out = out;
     e.ldr = ldr; e.ldp = ldp; e.ldo = ldo; e.act = act; e.out_f32 = out_dtype == FRCNN_DT_F32;
     const DnMatrix mx{x, M, K, ldx, false}, mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
-    return dtype == FRCNN_DT_BF16
-               ? dn_product<__bf16>(mx, true, mw, !kn, e, (char*)workspace, (hipStream_t)stream)
-               : dn_product<_Float16>(mx, true, mw, !kn, e, (char*)workspace, (hipStream_t)stream);
+    return dtype == FRCNN_DT_BF16 ? dn_forward<__bf16>(mx, mw, !kn, e, (char*)workspace, (hipStream_t)stream)
+                                  : dn_forward<_Float16>(mx, mw, !kn, e, (char*)workspace, (hipStream_t)stream);
 }
 
 extern "C" size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
@@ -1102,11 +1147,10 @@ extern "C" size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N, int w
     const DnBwdPlan p = dn_bwd_plan(M, N, !(aligned & 4) || N % 8 != 0);
     const bool kn = w_layout == FRCNN_W_KN;
     const DnRows x = aligned & 1 ? DN_ALIGNED : DN_ANY, w = aligned & 2 ? DN_ALIGNED : DN_ANY;
-    const size_t dx = kn ? dn_product_bytes(M, N, true, K, N, true, DN_PADDED, w)
-                         : dn_product_bytes(M, N, true, N, K, false, DN_PADDED, w);
-    const size_t dw = kn ? dn_product_bytes(M, K, false, M, N, false, x, DN_PADDED)
-                         : dn_product_bytes(M, N, false, M, K, false, DN_PADDED, x);
-    return p.dz_bytes + p.sum_bytes + (dx > dw ? dx : dw);
+    const size_t dx = dn_partial_bytes(M, K, N, true, kn);
+    const size_t dw = kn ? dn_partial_bytes(K, N, M, false, false) : dn_partial_bytes(N, K, M, false, false);
+    const size_t packed = dn_copy_bytes(M, K, x) + (dn_few(M) ? 0 : kn ? dn_copy_bytes(K, N, w) : dn_copy_bytes(N, K, w));
+    return p.dz_bytes + p.sum_bytes + packed + (dx > dw ? dx : dw);
 }
 
 extern "C" int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, const void* x, int64_t ldx, const void* w,

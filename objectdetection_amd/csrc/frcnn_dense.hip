@@ -687,13 +687,18 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
     }
 }
 
+// a / b for a below 2^40: by 32-bit division where that does (a 64-bit one is a hundred instructions)
+__device__ __forceinline__ long long dn_divide(long long a, long long b) {
+    return a < 0x80000000ll && b < 0x80000000ll ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // sums of a split product's slices, in slice order, and the epilogue; four outputs per thread
 template <typename T>
 __global__ void __launch_bounds__(64)
 dense_join_kernel(const float* __restrict__ partial, int splits, long long I, long long J, DnEpilogue e) {
     const long long q = (J + 3) / 4, id = (long long)blockIdx.x * 64 + threadIdx.x;
     if (id >= I * q) return;
-    const long long i = id / q, j = (id - i * q) * 4, stride = I * q * 4;
+    const long long i = dn_divide(id, q), j = (id - i * q) * 4, stride = I * q * 4;
     dn_f32x4 v = *reinterpret_cast<const dn_f32x4*>(partial + id * 4);
     int s = 1;
     for (; s + 8 <= splits; s += 8) {                  // eight slices on their way at once
@@ -716,94 +721,120 @@ dense_join_kernel(const float* __restrict__ partial, int splits, long long I, lo
 }
 
 // ---- operands whose rows are not whole 16-byte pieces --------------------------------------------------
-// are copied once to rows that are, with zeros behind their end; one launch for both of a product's
+// are copied once to rows that are, with zeros behind their end: a piece per thread, in one launch for all
+// of a call's operands
 struct DnPack { const void* src; void* dst; long long rows, cols, ld, pieces; };   // pieces of 8 per row of dst
+struct DnPacks { DnPack of[2]; long long blocks_first, blocks; };                  // workgroups of 256 pieces
+
 template <typename T>
-__global__ void __launch_bounds__(256) dense_pack_kernel(DnPack a, DnPack b, long long blocks_a) {
-    const bool first = (long long)blockIdx.x < blocks_a;
-    const DnPack p = first ? a : b;
-    const long long id = ((long long)blockIdx.x - (first ? 0 : blocks_a)) * 256 + threadIdx.x;
+__device__ __forceinline__ void dn_pack_piece(const DnPacks& packs, long long block) {
+    const bool first = block < packs.blocks_first;
+    const DnPack p = packs.of[first ? 0 : 1];
+    const long long id = (block - (first ? 0 : packs.blocks_first)) * 256 + threadIdx.x;
     if (id >= p.rows * p.pieces) return;
-    const long long r = id / p.pieces, c = 8 * (id - r * p.pieces), left = p.cols - c;
+    const long long r = dn_divide(id, p.pieces), c = 8 * (id - r * p.pieces), left = p.cols - c;
     const dn_s16x8 v = dn_load8((const T*)p.src + r * p.ld + c, left > 8 ? 8 : (int)left);
     reinterpret_cast<dn_s16x8*>(p.dst)[id] = v;
 }
+template <typename T>
+__global__ void __launch_bounds__(256) dense_pack_kernel(DnPacks packs) {
+    dn_pack_piece<T>(packs, blockIdx.x);
+}
 
-// ---- dz = d_out * act'(pre), and column sums per block of rows ----------------------------------------
-// A workgroup takes `rows` rows of 8 * CG columns; a thread 8 neighbouring columns of every (256 / CG)-th
-// row.  dz (may be null) has rows of ldz elements, a multiple of 8; its columns N .. ldz-1 become 0.
+// ---- dz = d_out * act'(pre) and its column sums ---------------------------------------------------------
+// A workgroup takes `rows` rows of 8 * cg columns; a thread 8 neighbouring columns of every (256 / cg)-th
+// row.  dz (may be null) has rows of ldz elements, a multiple of 8; its columns N .. ldz-1 become 0.  The
+// sums of the unrounded values go to d_bias where one workgroup has all rows, else to `sums`, a row per
+// block of rows.  The workgroups behind the first `blocks` pack the products' operands.
+struct DnDz {
+    const void *d_out, *pre;
+    void *dz, *d_bias;
+    float* sums;
+    long long ldd, ldp, ldz, M, rows, row_blocks, blocks;
+    int N, act, cg;
+};
 template <typename T, typename D>
-__global__ void __launch_bounds__(256)
-dense_dz_kernel(const D* __restrict__ d_out, long long ldd, const T* __restrict__ pre, long long ldp, long long M,
-                int N, int act, long long rows, int cg, T* __restrict__ dz, long long ldz, float* __restrict__ sums) {
-    __shared__ float part[256][9];
-    const int tid = threadIdx.x, c = tid % cg, rl = tid / cg, rn = 256 / cg;
-    const long long col = ((long long)blockIdx.y * cg + c) * 8, r0 = (long long)blockIdx.x * rows;
-    const long long r1 = r0 + rows < M ? r0 + rows : M;
-    const int valid = N - col > 8 ? 8 : (int)(N - col);
+__global__ void __launch_bounds__(256) dense_dz_kernel(DnDz p, DnPacks packs) {
+    __shared__ float part[4][32][9];
+    if ((long long)blockIdx.x >= p.blocks) return dn_pack_piece<T>(packs, blockIdx.x - p.blocks);
+    const D* d_out = (const D*)p.d_out;
+    const T* pre = (const T*)p.pre;
+    T* dz = (T*)p.dz;
+    const int tid = threadIdx.x, c = tid & (p.cg - 1), rl = tid / p.cg, rn = 256 / p.cg;
+    const long long column = dn_divide(blockIdx.x, p.row_blocks), block = blockIdx.x - column * p.row_blocks;
+    const long long col = (column * p.cg + c) * 8, r0 = block * p.rows, r1 = r0 + p.rows < p.M ? r0 + p.rows : p.M;
+    const int valid = p.N - col > 8 ? 8 : (int)(p.N - col);
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     auto row = [&](long long r, const float (&d)[8], const float (&z)[8]) {
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < valid ? dn_act_grad(d[e], z[e], act) : 0.f;
-        if (dz) dn_store<T, 8>(dz + r * ldz + col, 8, v);
+        for (int e = 0; e < 8; ++e) v[e] = e < valid ? dn_act_grad(d[e], z[e], p.act) : 0.f;
+        if (dz) dn_store<T, 8>(dz + r * p.ldz + col, 8, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] += v[e];
     };
     if (valid > 0) {
-        const bool act_any = act != FRCNN_ACT_NONE;
+        const bool act_any = p.act != FRCNN_ACT_NONE;
         long long r = r0 + rl;
         for (; r + rn < r1; r += 2 * rn) {             // two rows on their way
             float d0[8], d1[8], z0[8] = {}, z1[8] = {};
-            dn_load<D, 8>(d_out + r * ldd + col, valid, d0);
-            dn_load<D, 8>(d_out + (r + rn) * ldd + col, valid, d1);
+            dn_load<D, 8>(d_out + r * p.ldd + col, valid, d0);
+            dn_load<D, 8>(d_out + (r + rn) * p.ldd + col, valid, d1);
             if (act_any) {
-                dn_load<T, 8>(pre + r * ldp + col, valid, z0);
-                dn_load<T, 8>(pre + (r + rn) * ldp + col, valid, z1);
+                dn_load<T, 8>(pre + r * p.ldp + col, valid, z0);
+                dn_load<T, 8>(pre + (r + rn) * p.ldp + col, valid, z1);
             }
             row(r, d0, z0);
             row(r + rn, d1, z1);
         }
         if (r < r1) {
             float d0[8], z0[8] = {};
-            dn_load<D, 8>(d_out + r * ldd + col, valid, d0);
-            if (act_any) dn_load<T, 8>(pre + r * ldp + col, valid, z0);
+            dn_load<D, 8>(d_out + r * p.ldd + col, valid, d0);
+            if (act_any) dn_load<T, 8>(pre + r * p.ldp + col, valid, z0);
             row(r, d0, z0);
         }
     }
-    if (!sums) return;
+    if (!p.sums && !p.d_bias) return;
+    for (int d = p.cg; d < 64; d *= 2)                 // the wave's lanes of the same columns, then the four waves
 #pragma unroll
-    for (int e = 0; e < 8; ++e) part[tid][e] = s[e];
+        for (int e = 0; e < 8; ++e) s[e] += __shfl_xor(s[e], d);
+    if (lane_id() < p.cg)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[wave_id()][c][e] = s[e];
     __syncthreads();
-    if (rl == 0 && valid > 0) {
-        for (int r = 1; r < rn; ++r)
+    if (tid >= p.cg || valid <= 0) return;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] += part[r * cg + c][e];
-        for (int e = 0; e < valid; ++e) sums[(long long)blockIdx.x * N + col + e] = s[e];
+    for (int e = 0; e < 8; ++e) s[e] = (part[0][c][e] + part[1][c][e]) + (part[2][c][e] + part[3][c][e]);
+    if (p.d_bias) {
+        for (int e = 0; e < valid; ++e) ((T*)p.d_bias)[col + e] = (T)s[e];
+    } else {
+        for (int e = 0; e < valid; ++e) p.sums[block * p.N + col + e] = s[e];
     }
 }
 
-// column sums of `blocks` rows of float32 partial sums: 16 columns per workgroup, 16 threads each, four
+// column sums of `blocks` rows of float32 partial sums: 16 columns per workgroup, 64 threads each, four
 // rows on their way per thread
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 dense_bias_grad_kernel(const float* __restrict__ sums, int blocks, int N, T* __restrict__ d_bias) {
-    __shared__ float part[16][17];
+    __shared__ float part[64][17];
     const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
     const int col = blockIdx.x * 16 + c;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (col < N)
-        for (int b = q; b < blocks; b += 64)
+        for (int b = q; b < blocks; b += 256)
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (b + 16 * u < blocks) s[u] += sums[(long long)(b + 16 * u) * N + col];
+                if (b + 64 * u < blocks) s[u] += sums[(long long)(b + 64 * u) * N + col];
     part[q][c] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
-    if (q == 0 && col < N) {
-        float v = part[0][c];
+    if (q < 4) {                                       // 16 rows each
+        float v = part[16 * q][c];
 #pragma unroll
-        for (int r = 1; r < 16; ++r) v += part[r][c];
-        d_bias[col] = (T)v;
+        for (int r = 1; r < 16; ++r) v += part[16 * q + r][c];
+        v += __shfl_xor(v, 16);
+        v += __shfl_xor(v, 32);
+        if (q == 0 && col < N) d_bias[col] = (T)v;
     }
 }
 
@@ -865,11 +896,13 @@ static DnPlan dn_plan(long long I, long long J, long long K, bool akc, bool bkc)
             const double waves = groups <= DN_CUS ? 1.0 : __builtin_ceil(groups / DN_CUS);
             double us = per * (waves * sat > t.alone ? waves * sat : t.alone) + t.fixed * __builtin_ceil(waves / t.resident);
             // what memory gives, and what L2 gives again
-            const double copied = groups * per * (t.bi + t.bj) * (2.0 * DN_SK);
+            // (rows outside the operand repeat one row: counted half)
+            const double copied = groups * per * ((I < t.bi ? (I + t.bi) / 2 : t.bi) +
+                                                  (J < t.bj ? (J + t.bj) / 2 : t.bj)) * (2.0 * DN_SK);
             const double stream = (bytes / 4.6e6 + (copied > bytes ? copied - bytes : 0.0) / 2.0e7) *
                                   (groups < DN_CUS ? DN_CUS / groups : 1.0);
             if (us < stream) us = stream;
-            if (splits > 1) us += 5.0 + (double)splits * I * J * 8.0 / 1.0e7;
+            if (splits > 1) us += 3.0 + 0.3 * splits + (double)splits * I * J * 8.0 / 1.0e7;
             // in doubt the larger tile and fewer slices
             if (p.bi && us > 0.97 * best) continue;
             best = us;
@@ -944,26 +977,26 @@ static size_t dn_pack_bytes(long long rows, long long cols) {
     return dn_up((size_t)rows * (size_t)dn_pieces(cols) * 16);
 }
 
-// Copies of the matrices whose rows are not whole pieces, from `ws` on (which moves behind them); a null
-// matrix is left alone.
-template <typename T>
-static int dn_pack(DnMatrix* a, DnMatrix* b, char*& ws, hipStream_t stream) {
-    DnPack pack[2] = {};
-    long long blocks[2] = {0, 0};
+// Copies of the matrices whose rows are not whole pieces, from `ws` on (which moves behind them): what has
+// to be launched; a null matrix is left alone.
+static int dn_pack(DnMatrix* a, DnMatrix* b, char*& ws, DnPacks& packs) {
+    packs = DnPacks{};
     int n = 0;
     for (DnMatrix* m : {a, b}) {
         if (!m || dn_whole(*m)) continue;
         if (dn_pieces(m->cols) * 8 > (1ll << 21)) return FRCNN_E_UNSUPPORTED;
-        pack[n] = DnPack{m->p, ws, m->rows, m->cols, m->ld, dn_pieces(m->cols)};
-        blocks[n] = (m->rows * pack[n].pieces + 255) / 256;
+        packs.of[n] = DnPack{m->p, ws, m->rows, m->cols, m->ld, dn_pieces(m->cols)};
+        packs.blocks += (m->rows * packs.of[n].pieces + 255) / 256;
+        if (n == 0) packs.blocks_first = packs.blocks;
         ws += dn_pack_bytes(m->rows, m->cols);
-        *m = DnMatrix{pack[n].dst, m->rows, m->cols, pack[n].pieces * 8, true};
+        *m = DnMatrix{packs.of[n].dst, m->rows, m->cols, packs.of[n].pieces * 8, true};
         ++n;
     }
-    if (!n) return FRCNN_OK;
-    if (blocks[0] + blocks[1] > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
-    FRCNN_LAUNCH(dense_pack_kernel<T>, dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), 0, stream, pack[0], pack[1],
-                 blocks[0]);
+    return packs.blocks > 0x7FFFFFFFll ? FRCNN_E_UNSUPPORTED : FRCNN_OK;
+}
+template <typename T>
+static int dn_launch_packs(const DnPacks& packs, hipStream_t stream) {
+    if (packs.blocks) FRCNN_LAUNCH(dense_pack_kernel<T>, dim3((unsigned)packs.blocks), dim3(256), 0, stream, packs);
     return FRCNN_OK;
 }
 
@@ -1013,18 +1046,26 @@ static DnBwdPlan dn_bwd_plan(long long M, int N, bool copy) {
     if (M == 0) return p;                              // nothing to multiply: zeros are stored
     p.copy = copy;
     p.ldz = dn_pieces(N) * 8;
-    // a workgroup takes 256 / cg rows at a time of 8 cg columns: two to eight such walks, as many workgroups
-    // as fill the chip four times, at most 4,096 partial sums per column
-    p.cg = 1;
-    while (p.cg < 32 && p.cg < dn_pieces(N)) p.cg *= 2;
-    const long long walk = 256 / p.cg, columns = (dn_pieces(N) + p.cg - 1) / p.cg;
-    long long walks = M * columns / (walk * 4 * DN_CUS);
-    walks = walks < 2 ? 2 : walks > 8 ? 8 : walks;
-    while ((M + walk * walks - 1) / (walk * walks) > 4096) walks *= 2;
-    p.rows = walk * walks;
-    p.blocks = (M + p.rows - 1) / p.rows;
+    if (M <= 256) {
+        // one workgroup has all rows of 16 columns: no second launch for the sums (of 1,111 rows x 333
+        // this took 26 us, the two launches 7.6 + 3.2)
+        p.cg = 2;
+        p.rows = M;
+        p.blocks = 1;
+    } else {
+        // a workgroup takes 256 / cg rows at a time of 8 cg columns: two to eight such walks, as many
+        // workgroups as fill the chip four times, at most 4,096 partial sums per column
+        p.cg = 1;
+        while (p.cg < 32 && p.cg < dn_pieces(N)) p.cg *= 2;
+        const long long walk = 256 / p.cg, columns = (dn_pieces(N) + p.cg - 1) / p.cg;
+        long long walks = M * columns / (walk * 4 * DN_CUS);
+        walks = walks < 2 ? 2 : walks > 8 ? 8 : walks;
+        while ((M + walk * walks - 1) / (walk * walks) > 4096) walks *= 2;
+        p.rows = walk * walks;
+        p.blocks = (M + p.rows - 1) / p.rows;
+    }
     p.dz_bytes = copy ? dn_up((size_t)M * (size_t)p.ldz * 2) : 0;
-    p.sum_bytes = dn_up((size_t)p.blocks * (size_t)N * 4);
+    p.sum_bytes = p.blocks > 1 ? dn_up((size_t)p.blocks * (size_t)N * 4) : 0;
     return p;
 }
 
@@ -1040,20 +1081,12 @@ static int dn_zero(void* p, long long rows, long long cols, long long ld, hipStr
     return FRCNN_OK;
 }
 
-template <typename T, typename D>
-static int dn_launch_dz(const void* d_out, long long ldd, const void* pre, long long ldp, long long M, int N, int act,
-                        const DnBwdPlan& p, void* dz, float* sums, hipStream_t s) {
-    const long long gy = (dn_pieces(N) + p.cg - 1) / p.cg;
-    if (p.blocks > 0x7FFFFFFFll || gy > 65535) return FRCNN_E_UNSUPPORTED;
-    FRCNN_LAUNCH((dense_dz_kernel<T, D>), dim3((unsigned)p.blocks, (unsigned)gy), dim3(256), 0, s, (const D*)d_out,
-                 ldd, (const T*)pre, ldp, M, N, act, p.rows, p.cg, (T*)dz, p.ldz, sums);
-    return FRCNN_OK;
-}
-
 template <typename T>
 static int dn_forward(DnMatrix x, DnMatrix w, bool bkc, const DnEpilogue& e, char* ws, hipStream_t s) {
     if (!dn_few(x.rows)) {
-        const int rc = dn_pack<T>(&x, &w, ws, s);
+        DnPacks packs;
+        int rc = dn_pack(&x, &w, ws, packs);
+        if (rc == FRCNN_OK) rc = dn_launch_packs<T>(packs, s);
         if (rc != FRCNN_OK) return rc;
     }
     return dn_product<T>(x, true, w, bkc, e, ws, s);
@@ -1071,21 +1104,33 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
         if (rc == FRCNN_OK && d_bias) rc = dn_zero<T>(d_bias, 1, N, N, s);
         return rc;
     }
-    void* dz = p.copy ? ws : nullptr;
-    float* sums = d_bias ? reinterpret_cast<float*>(ws + p.dz_bytes) : nullptr;
+    void* dz = p.copy && (d_x || d_w) ? ws : nullptr;
     char* rest = ws + p.dz_bytes + p.sum_bytes;
-    if (sums || (dz && (d_x || d_w))) {
-        rc = d_dtype == FRCNN_DT_F32 ? dn_launch_dz<T, float>(d_out, ldd, pre, ldp, M, N, act, p, dz, sums, s)
-                                     : dn_launch_dz<T, T>(d_out, ldd, pre, ldp, M, N, act, p, dz, sums, s);
-        if (rc != FRCNN_OK) return rc;
-    }
-    if (sums)
-        FRCNN_LAUNCH(dense_bias_grad_kernel<T>, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, s, sums,
-                     (int)p.blocks, N, (T*)d_bias);
     const DnMatrix z = dz ? DnMatrix{dz, M, N, p.ldz, true} : DnMatrix{d_out, M, N, ldd, false};
     DnMatrix mx{x, M, K, ldx, false}, mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
-    rc = dn_pack<T>(d_x && !dn_few(M) ? &mw : nullptr, d_w ? &mx : nullptr, rest, s);
+    DnPacks packs;
+    rc = dn_pack(d_x && !dn_few(M) ? &mw : nullptr, d_w ? &mx : nullptr, rest, packs);
     if (rc != FRCNN_OK) return rc;
+    if (d_bias || dz) {
+        DnDz q{};
+        q.d_out = d_out; q.ldd = ldd; q.pre = pre; q.ldp = ldp; q.dz = dz; q.ldz = p.ldz;
+        q.M = M; q.N = N; q.act = act; q.cg = p.cg; q.rows = p.rows; q.row_blocks = p.blocks;
+        if (p.blocks == 1) q.d_bias = d_bias;
+        else q.sums = d_bias ? reinterpret_cast<float*>(ws + p.dz_bytes) : nullptr;
+        q.blocks = p.blocks * ((dn_pieces(N) + p.cg - 1) / p.cg);
+        const long long blocks = q.blocks + packs.blocks;
+        if (blocks > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
+        if (d_dtype == FRCNN_DT_F32)
+            FRCNN_LAUNCH((dense_dz_kernel<T, float>), dim3((unsigned)blocks), dim3(256), 0, s, q, packs);
+        else
+            FRCNN_LAUNCH((dense_dz_kernel<T, T>), dim3((unsigned)blocks), dim3(256), 0, s, q, packs);
+        if (q.sums)
+            FRCNN_LAUNCH(dense_bias_grad_kernel<T>, dim3((unsigned)((N + 15) / 16)), dim3(1024), 0, s, q.sums,
+                         (int)p.blocks, N, (T*)d_bias);
+    } else {
+        rc = dn_launch_packs<T>(packs, s);
+        if (rc != FRCNN_OK) return rc;
+    }
     DnEpilogue e{};
     if (d_x) {
         e.out = d_x; e.ldo = lddx;
@@ -1177,7 +1222,7 @@ extern "C" int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, cons
         const int aligned = dn_aligned(d_x ? w : nullptr, d_x ? ldw : 0, d_w ? x : nullptr, d_w ? ldx : 0);
         const size_t need = frcnn_dense_bwd_workspace_bytes(M, K, N, w_layout, (aligned & 1) * 2 | aligned >> 1 |
                                                             (copy ? 0 : 4));
-        if (!workspace || workspace_bytes < need || !dn_even(workspace, 16)) return FRCNN_E_WORKSPACE;
+        if (need && (!workspace || workspace_bytes < need || !dn_even(workspace, 16))) return FRCNN_E_WORKSPACE;
     }
     const DnBwdPlan p = dn_bwd_plan(M, N, copy);
     return dtype == FRCNN_DT_BF16

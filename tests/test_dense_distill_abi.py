@@ -62,8 +62,10 @@ def test_dense_workspaces(L):
     assert b(100, 64, 32, 0, 0) >= 100 * 32 * 2 + copy(100, 64)
     assert b(100, 64, 33, 0, 3) - b(100, 64, 33, 0, 1) == copy(64, 33) * 0      # 33: W is copied either way
     assert b(100, 64, 32, 0, 7) < b(100, 64, 32, 0, 3) <= b(100, 64, 32, 0, 0)
-    assert bwd(L, ws=None) == L.E_WORKSPACE and bwd(L, wsb=b(4, 64, 32, 0, 7) - 1) == L.E_WORKSPACE
-    assert bwd(L, ws=ctypes.c_void_p(24)) == L.E_WORKSPACE
+    relu = dict(act=1, pre=ONE, ldp=32)                    # dz is kept in the workspace
+    assert bwd(L, ws=None, **relu) == L.E_WORKSPACE
+    assert bwd(L, wsb=b(4, 64, 32, 0, 3) - 1, **relu) == L.E_WORKSPACE
+    assert bwd(L, ws=ctypes.c_void_p(24), **relu) == L.E_WORKSPACE
     assert fwd(L, M=0, x=None, out=None) == L.OK           # no rows: nothing to do, nothing launched
 
 

@@ -319,6 +319,7 @@ def test_refusals(dev):
             (lambda: ops.dense_bwd(d, x, w, act="relu"), ValueError),
             (lambda: ops.dense_bwd(d[:3], x, w), ValueError),
             (lambda: ops.dense_bwd(d, x, w, want_dx=False, want_dw=False, want_db=False), ValueError),
-            (lambda: ops.dense_bwd(d, x, w, workspace=torch.empty(16, dtype=torch.uint8, device=dev)), ValueError)):
+            (lambda: ops.dense_bwd(d, x, w, pre=d, act="relu", workspace=torch.empty(16, dtype=torch.uint8, device=dev)),
+             ValueError)):
         with pytest.raises(err):
             bad()

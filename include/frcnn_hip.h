@@ -421,7 +421,7 @@ int frcnn_fc1_fwd(const float* x, const float* w, const float* bias, int64_t M, 
  *              is FRCNN_ACT_NONE.  A bit left out asks for more than needed;
  *   bias, residual, pre may be NULL (pre: the pre-activations, rounded, which the backward needs
  *              for an activation other than FRCNN_ACT_NONE).
- * M = 0 is allowed (no forward output; d_w and d_bias become 0).
+ * M = 0 is allowed (no forward output; d_w and d_bias become 0); M up to 2,147,483,647.
  * Activations: ReLU max(z, 0); GELU z Phi(z), Phi the normal distribution function (relative error
  * 1.3e-6); SiLU z / (1 + e^-z). */
 #define FRCNN_DT_F32   0

@@ -193,10 +193,11 @@ __device__ __forceinline__ int dn_swizzle(int r, int c) {
     return c ^ ((((r & 3) | ((r >> 1) & 4)) & m) << 1);
 }
 
-// workgroup id -> tile: every XCD (id % 8) gets a contiguous run of tiles, and a run walks groups of
-// eight tile rows column by column, so that the tiles resident on an XCD share A and B panels in its L2
-__device__ __forceinline__ void dn_tile(const DnGemm& p, int& ti, int& tj, int& slice) {
-    const int n = (int)gridDim.x, id = (int)blockIdx.x, xcd = id & 7, q = n >> 3, r = n & 7;
+// tile number -> tile: every XCD (number % 8) gets a contiguous run of tiles, and a run walks groups of eight
+// tile rows column by column, so that the tiles resident on an XCD share A and B panels in its L2 (groups of
+// four or sixteen: within 1 % on most products, 2 % and 12 % slower with W as [N,K])
+__device__ __forceinline__ void dn_tile(const DnGemm& p, int id, int n, int& ti, int& tj, int& slice) {
+    const int xcd = id & 7, q = n >> 3, r = n & 7;
     int t = xcd * q + (xcd < r ? xcd : r) + (id >> 3);
     const int per = p.tiles_i * p.tiles_j;
     slice = t / per;
@@ -207,20 +208,30 @@ __device__ __forceinline__ void dn_tile(const DnGemm& p, int& ti, int& tj, int& 
     tj = (t - g * group) / rows;
 }
 
+// the thread's number, not known to be the same as before: what is computed from it is computed again where
+// it is needed instead of waiting in registers through the products
+__device__ __forceinline__ int dn_thread() {
+    int t = (int)threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
 // A wave's results, (16 FI) x (16 FJ) at (i0, j0): the float32 partial sums of a slice, or the outputs.
 // Sixteen rows at a time turn round through LDS (the wave's own dn_turn_bytes), so that a lane holds eight
 // neighbouring outputs and the lanes of a row store whole 128-byte lines.  Inside the matrix nothing is
 // guarded, the bias is loaded once (a lane's columns stay the same) and the residual of the next sixteen
 // rows is on its way before the stores of these: memory operations finish in order, and a load waited for
 // behind stores, or a guarded one, costs their whole way to memory (6 us per 256 x 256 tile).
-template <int FJ> constexpr int dn_turn_bytes() { return 16 * (FJ * 64 + 16); }
+// The turned rows' 16-byte pieces are exchanged by the row number instead of padded: the large tile's ring
+// and turns are all of a compute unit's LDS.
+template <int FJ> constexpr int dn_turn_bytes() { return 16 * FJ * 64; }
 
 template <typename T, int FI, int FJ, bool FULL>
 __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&acc)[FI][FJ], int slice, long long i0,
                                              long long j0, char* turn) {
-    constexpr int S = FJ * 64 + 16, Q = 2 * FJ, RP = 64 / Q;      // bytes per row, pieces of 8 per row, rows per pass
+    constexpr int S = FJ * 64, Q = 2 * FJ, RP = 64 / Q;           // bytes per row, pieces of 8 per row, rows per pass
     constexpr int NP = 16 / RP;                                   // passes per sixteen rows
-    const int lane = lane_id();
+    const int lane = dn_thread() & 63;
     if (p.partial) {            // columns J .. Jp-1 may be written and are never read as results
         const long long Jp = (p.J + 3) / 4 * 4;
 #pragma unroll
@@ -238,8 +249,9 @@ __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&a
     if (j0 >= p.J) return;
     const long long row0 = i0 + lane / Q, gj = j0 + 8 * (lane % Q);
     const int valid = p.J - gj > 8 ? 8 : (int)(p.J - gj);
-    char* put = turn + (lane & 15) * S + (lane >> 4) * 16;
-    const char* get = turn + (lane / Q) * S + (lane % Q) * 32;
+    constexpr int X = 4 * FJ - 1;                                 // 16-byte pieces per row, less one
+    char* put = turn + (lane & 15) * S;
+    const char* get = turn + (lane / Q) * S;
     const DnEpilogue& ep = p.e;
     const bool has_res = FULL && ep.residual, has_pre = FULL && ep.pre, f32 = FULL && ep.out_f32;
     // INNER: whole pieces in all lanes; else value by value, loads at clamped places instead of under a guard
@@ -287,7 +299,7 @@ __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&a
                     for (int j = 0; j < FJ; ++j) {
                         dn_f32x4 a = acc[c][j];
                         asm volatile("" : "+v"(a));
-                        *reinterpret_cast<dn_f32x4*>(put + j * 64) = a;
+                        *reinterpret_cast<dn_f32x4*>(put + (((4 * j + (lane >> 4)) ^ lane) & X) * 16) = a;
                     }
                 }
             __builtin_amdgcn_wave_barrier();
@@ -297,7 +309,10 @@ __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&a
                 const long long gi = row0 + 16 * i + r * RP;
                 const bool inside = gi < p.I;
                 float v[8];
-                __builtin_memcpy(v, get + r * RP * S, 32);
+                const int row = r * RP + lane / Q;                // of the sixteen
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    __builtin_memcpy(v + 4 * h, get + r * RP * S + (((2 * (lane % Q) + h) ^ row) & X) * 16, 16);
                 if constexpr (FULL) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] += bias[e];
@@ -366,11 +381,12 @@ struct DnCopy {
     __device__ __forceinline__ void init(const T* p, long long ld, long long outer0, long long outer_end,
                                          long long k0) {
         const long long ld2 = ld * 2, left = outer_end - outer0;
+        const int tid = dn_thread();
         base = reinterpret_cast<const char*>(p) + (KC ? outer0 * ld2 + k0 * 2 : k0 * ld2 + outer0 * 2);
         step = KC ? CK * 2 : CK * ld2;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const int idx = (int)threadIdx.x + NT * i;
+            const int idx = tid + NT * i;
             int r = idx / P, c = dn_swizzle<KC, R, CK>(r, idx % P);
             if constexpr (KC) r = r < left ? r : (int)left - 1;
             else c = 8 * c + 8 <= left ? c : (int)(left / 8) - 1;
@@ -386,9 +402,10 @@ struct DnCopy {
     // the same where only the first `valid` k are inside
     __device__ __forceinline__ void issue(uint32_t lds, int valid) {
         if (valid >= CK) return issue(lds);
+        const int tid = dn_thread();
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const int idx = (int)threadIdx.x + NT * i, r = idx / P;
+            const int idx = tid + NT * i, r = idx / P;
             const int k = KC ? 8 * dn_swizzle<KC, R, CK>(r, idx % P) : r;
             dn_dma(lds + (uint32_t)(NT * i * 16), k < valid ? base + off[i] : reinterpret_cast<const char*>(dn_zeros));
         }
@@ -429,26 +446,19 @@ struct DnReader {
     }
 };
 
-// FULL: with bias, pre, activation, residual or a float32 output in the epilogue (the forward)
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, bool FULL>
+// FULL: with bias, pre, activation, residual or a float32 output in the epilogue (the forward).
+// STAY: the workgroup takes every gridDim.x-th tile; the first copies of the next tile leave before the
+// results of this one are written, and arrive meanwhile.  `tiles`: tiles and slices in all.
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, bool FULL, bool STAY>
 __global__ void __launch_bounds__(64 * WI * WJ)
-dense_gemm_kernel(DnGemm p) {
+dense_gemm_kernel(DnGemm p, int tiles) {
     constexpr int NT = 64 * WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
     constexpr int READS = FI * (AKC ? 1 : 2) + FJ * (BKC ? 1 : 2);  // LDS reads per wave and step
-    extern __shared__ __attribute__((aligned(16))) char dn_lds[];    // A's ring, then B's
-    int ti, tj, slice;
-    dn_tile(p, ti, tj, slice);
-    const long long i0 = (long long)ti * BI, j0 = (long long)tj * BJ;
-    const long long k0 = slice * p.k_slice;
-    const long long k_end = k0 + p.k_slice < p.K ? k0 + p.k_slice : p.K;
+    extern __shared__ __attribute__((aligned(16))) char dn_lds[];    // A's ring, B's, the turns (STAY)
+    constexpr uint32_t RING_A = BI * DN_SK * 2 * DN_RING, RING_B = BJ * DN_SK * 2 * DN_RING;
     const int wave = __builtin_amdgcn_readfirstlane(wave_id());
     const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
-
-    dn_f32x4 acc[FI][FJ];
-#pragma unroll
-    for (int i = 0; i < FI; ++i)
-#pragma unroll
-        for (int j = 0; j < FJ; ++j) acc[i][j] = dn_f32x4{0.f, 0.f, 0.f, 0.f};
+    char* turn = dn_lds + (STAY ? RING_A + RING_B : 0) + wave * dn_turn_bytes<FJ>();
 
     using CopyA = DnCopy<T, AKC, BI, NT>;
     using CopyB = DnCopy<T, BKC, BJ, NT>;
@@ -457,16 +467,12 @@ dense_gemm_kernel(DnGemm p) {
     constexpr int OTHER = (AKC ? CopyA::NP : 0) + (BKC ? CopyB::NP : 0);
     CopyA ca;
     CopyB cb;
-    ca.init((const T*)p.a, p.lda, i0, AKC ? p.I : p.outer_a, k0);
-    cb.init((const T*)p.b, p.ldb, j0, BKC ? p.J : p.outer_b, k0);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dn_lds;
-    const uint32_t la = lds0 + (uint32_t)wave * 1024u, lb = la + BI * DN_SK * 2 * DN_RING;
+    const uint32_t la = lds0 + (uint32_t)wave * 1024u, lb = la + RING_A;
     DnReader<AKC, BI> qa;
     DnReader<BKC, BJ> qb;
     qa.init(lds0, wi);
-    qb.init(lds0 + BI * DN_SK * 2 * DN_RING, wj);
-    const int n = (int)((k_end - k0 + DN_SK - 1) / DN_SK);
-    dn_s16x8 fa[2][FI], fb[2][FJ];
+    qb.init(lds0 + RING_A, wj);
     auto read = [&](int s, dn_s16x8 (&ra)[FI], dn_s16x8 (&rb)[FJ]) {
         qa.renew();
         qb.renew();
@@ -475,12 +481,8 @@ dense_gemm_kernel(DnGemm p) {
 #pragma unroll
         for (int i = 0; i < FI; ++i) ra[i] = qa.read(i, s);
     };
-    auto multiply = [&](const dn_s16x8 (&ra)[FI], const dn_s16x8 (&rb)[FJ]) {
-#pragma unroll
-        for (int i = 0; i < FI; ++i)
-#pragma unroll
-            for (int j = 0; j < FJ; ++j) acc[i][j] = dn_mfma(rb[j], ra[i], acc[i][j], T());
-    };
+    long long i0 = 0, j0 = 0, k0 = 0, k_end = 0;
+    int slice = 0, n = 0;                              // n: steps
     // the copies for step s: every-step operands (EV), and with an even s every-other-step ones (OT)
     auto issue = [&](int s, bool ev, bool ot) {
         if (s >= n) return;
@@ -490,61 +492,97 @@ dense_gemm_kernel(DnGemm p) {
         if (AKC ? ot : ev) ca.issue(la + ring * (BI * 64u), valid);
         if (BKC ? ot : ev) cb.issue(lb + ring * (BJ * 64u), valid);
     };
-    issue(0, true, true);
-    issue(1, true, false);
-    issue(2, true, true);
-    issue(3, true, false);
-    if (n >= DN_RING) dn_handover<OTHER + 2 * EVERY>();      // steps 0 and 1
-    else dn_handover<0>();
-    read(0, fa[0], fb[0]);
-    int s = 0;
-    // whole steps, four at a time so that every LDS address is a constant; no branch inside
-#pragma unroll 1
-    for (; s + 2 * DN_RING < n; s += DN_RING) {
-#pragma unroll
-        for (int u = 0; u < DN_RING; ++u) {
-            if (u & 1) {
-                dn_handover<2 * EVERY>();
-                if (AKC) ca.issue(la + ((u + 3) % DN_RING) * (BI * 64u));
-                if (BKC) cb.issue(lb + ((u + 3) % DN_RING) * (BJ * 64u));
-            } else if (EVERY) {
-                dn_handover<OTHER + 2 * EVERY>();
-            }
-            if (!AKC) ca.issue(la + u * (BI * 64u));
-            if (!BKC) cb.issue(lb + u * (BJ * 64u));
-            read(u + 1, fa[(u + 1) & 1], fb[(u + 1) & 1]);
-            multiply(fa[u & 1], fb[u & 1]);
-            // the reads of the next step between the products of this one, early
-            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-#pragma unroll
-            for (int q = 0; q < READS; ++q) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            }
-            __builtin_amdgcn_sched_group_barrier(0x008, FI * FJ, 0);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-    // the last steps: up to eight, the last one maybe cut short
-    auto step = [&](const dn_s16x8 (&ra)[FI], const dn_s16x8 (&rb)[FJ], dn_s16x8 (&na)[FI], dn_s16x8 (&nb)[FJ]) {
-        if (s + 1 < n) {
-            if (s + 3 >= n) dn_handover<0>();
-            else if (s & 1) dn_handover<2 * EVERY>();
-            else dn_handover<OTHER + 2 * EVERY>();
-            if (s & 1) issue(s + 3, false, true);
-            issue(s + 4, true, false);
-            read(s + 1, na, nb);
-        }
-        multiply(ra, rb);
-        ++s;
+    auto start = [&](int id) {
+        int ti, tj;
+        dn_tile(p, id, tiles, ti, tj, slice);
+        i0 = (long long)ti * BI;
+        j0 = (long long)tj * BJ;
+        k0 = slice * p.k_slice;
+        k_end = k0 + p.k_slice < p.K ? k0 + p.k_slice : p.K;
+        n = (int)((k_end - k0 + DN_SK - 1) / DN_SK);
+        ca.init((const T*)p.a, p.lda, i0, AKC ? p.I : p.outer_a, k0);
+        cb.init((const T*)p.b, p.ldb, j0, BKC ? p.J : p.outer_b, k0);
+        issue(0, true, true);
+        issue(1, true, false);
+        issue(2, true, true);
+        issue(3, true, false);
     };
+
+    int id = (int)blockIdx.x;
+    start(id);
 #pragma unroll 1
-    while (s < n) {
-        step(fa[0], fb[0], fa[1], fb[1]);
-        if (s < n) step(fa[1], fb[1], fa[0], fb[0]);
+    while (true) {
+        dn_f32x4 acc[FI][FJ];
+        dn_s16x8 fa[2][FI], fb[2][FJ];
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) acc[i][j] = dn_f32x4{0.f, 0.f, 0.f, 0.f};
+        auto multiply = [&](const dn_s16x8 (&ra)[FI], const dn_s16x8 (&rb)[FJ]) {
+#pragma unroll
+            for (int i = 0; i < FI; ++i)
+#pragma unroll
+                for (int j = 0; j < FJ; ++j) acc[i][j] = dn_mfma(rb[j], ra[i], acc[i][j], T());
+        };
+        // steps 0 and 1 (behind the last tile's results all but the newest are waited for: no harm)
+        if (n >= DN_RING) dn_handover<OTHER + 2 * EVERY>();
+        else dn_handover<0>();
+        read(0, fa[0], fb[0]);
+        int s = 0;
+        // whole steps, four at a time so that every LDS address is a constant; no branch inside
+#pragma unroll 1
+        for (; s + 2 * DN_RING < n; s += DN_RING) {
+#pragma unroll
+            for (int u = 0; u < DN_RING; ++u) {
+                if (u & 1) {
+                    dn_handover<2 * EVERY>();
+                    if (AKC) ca.issue(la + ((u + 3) % DN_RING) * (BI * 64u));
+                    if (BKC) cb.issue(lb + ((u + 3) % DN_RING) * (BJ * 64u));
+                } else if (EVERY) {
+                    dn_handover<OTHER + 2 * EVERY>();
+                }
+                if (!AKC) ca.issue(la + u * (BI * 64u));
+                if (!BKC) cb.issue(lb + u * (BJ * 64u));
+                read(u + 1, fa[(u + 1) & 1], fb[(u + 1) & 1]);
+                multiply(fa[u & 1], fb[u & 1]);
+                // the reads of the next step between the products of this one, early
+                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+#pragma unroll
+                for (int q = 0; q < READS; ++q) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, FI * FJ, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        // the last steps: up to eight, the last one maybe cut short
+        auto step = [&](const dn_s16x8 (&ra)[FI], const dn_s16x8 (&rb)[FJ], dn_s16x8 (&na)[FI], dn_s16x8 (&nb)[FJ]) {
+            if (s + 1 < n) {
+                if (s + 3 >= n) dn_handover<0>();
+                else if (s & 1) dn_handover<2 * EVERY>();
+                else dn_handover<OTHER + 2 * EVERY>();
+                if (s & 1) issue(s + 3, false, true);
+                issue(s + 4, true, false);
+                read(s + 1, na, nb);
+            }
+            multiply(ra, rb);
+            ++s;
+        };
+#pragma unroll 1
+        while (s < n) {
+            step(fa[0], fb[0], fa[1], fb[1]);
+            if (s < n) step(fa[1], fb[1], fa[0], fb[0]);
+        }
+        dn_handover<0>();                              // every wave has read the last step: the ring is free
+        const long long oi = i0 + wi, oj = j0 + wj;
+        const int os = slice;
+        id += (int)gridDim.x;
+        const bool more = STAY && id < tiles;
+        if (more) start(id);
+        dn_write_out<T, FI, FJ, FULL>(p, acc, os, oi, oj, turn);
+        if (!more) return;
     }
-    dn_handover<0>();
-    dn_write_out<T, FI, FJ, FULL>(p, acc, slice, i0 + wi, j0 + wj, dn_lds + wave * dn_turn_bytes<FJ>());
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------
@@ -927,12 +965,20 @@ static bool dn_raise_lds(const void* kernel, int bytes, std::atomic<uint64_t>& r
 }
 
 template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, bool FULL>
-static int dn_launch_kernel(const DnGemm& g, unsigned blocks, hipStream_t stream) {
-    constexpr int lds = DN_RING * (BI + BJ) * DN_SK * 2;
+static int dn_launch_kernel(const DnGemm& g, unsigned tiles, hipStream_t stream) {
+    // One workgroup of the large tile is all that a compute unit holds: it stays for the tiles of its XCD
+    // (16,384 x 64 x 4,096: 32.8 us; 36.5 with a workgroup per tile).  Not with the full epilogue and not where
+    // both operands are outer-contiguous: there the next tile's addresses do not fit beside the sums in 256
+    // registers, and what is parked in memory costs the products 20 %.
+    constexpr bool STAY = BI == 256 && BJ == 256 && AKC && !FULL;
+    constexpr int lds = DN_RING * (BI + BJ) * DN_SK * 2 + (STAY ? WI * WJ * dn_turn_bytes<BJ / WJ / 16>() : 0);
+    static_assert(lds <= 160 * 1024, "LDS of a compute unit");
+    const unsigned blocks = STAY && tiles > DN_CUS ? DN_CUS : tiles;
     static std::atomic<uint64_t> raised{0};
-    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, FULL>), lds, raised))
+    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, FULL, STAY>), lds, raised))
         return FRCNN_E_LAUNCH;
-    FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, FULL>), dim3(blocks), dim3(64 * WI * WJ), lds, stream, g);
+    FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, FULL, STAY>), dim3(blocks), dim3(64 * WI * WJ), lds, stream, g,
+                 (int)tiles);
     return FRCNN_OK;
 }
 
@@ -1069,7 +1115,8 @@ static DnBwdPlan dn_bwd_plan(long long M, int N, bool copy) {
     return p;
 }
 
-static bool dn_sizes(int64_t M, int K, int N) { return M >= 0 && M <= (1ll << 40) && K > 0 && N > 0; }
+static bool dn_sizes(int64_t M, int K, int N) { return M >= 0 && K > 0 && N > 0; }
+constexpr int64_t DN_MAX_ROWS = 0x7FFFFFFF;
 static bool dn_16bit(int dtype) { return dtype == FRCNN_DT_F16 || dtype == FRCNN_DT_BF16; }
 static bool dn_even(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
@@ -1149,7 +1196,7 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
 using namespace frcnn;
 
 extern "C" size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
-    if (!dn_sizes(M, K, N) || M == 0) return 0;
+    if (!dn_sizes(M, K, N) || M == 0 || M > DN_MAX_ROWS) return 0;
     const DnRows x = aligned & 1 ? DN_ALIGNED : DN_ANY, w = aligned & 2 ? DN_ALIGNED : DN_ANY;
     const bool kn = w_layout == FRCNN_W_KN;
     const size_t partial = dn_partial_bytes(M, N, K, true, !kn);
@@ -1170,6 +1217,7 @@ extern "C" int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_
         return FRCNN_E_BADARG;
     if (act < FRCNN_ACT_NONE || act > FRCNN_ACT_SILU || (w_layout != FRCNN_W_KN && w_layout != FRCNN_W_NK))
         return FRCNN_E_BADARG;
+    if (M > DN_MAX_ROWS) return FRCNN_E_UNSUPPORTED;
     if (M == 0) return FRCNN_OK;
     const bool kn = w_layout == FRCNN_W_KN;
     if (!x || !w || !out || ldx < K || ldw < (kn ? N : K) || ldo < N) return FRCNN_E_BADARG;
@@ -1188,7 +1236,7 @@ extern "C" int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_
 }
 
 extern "C" size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
-    if (!dn_sizes(M, K, N) || M == 0) return 0;
+    if (!dn_sizes(M, K, N) || M == 0 || M > DN_MAX_ROWS) return 0;
     const DnBwdPlan p = dn_bwd_plan(M, N, !(aligned & 4) || N % 8 != 0);
     const bool kn = w_layout == FRCNN_W_KN;
     const DnRows x = aligned & 1 ? DN_ALIGNED : DN_ANY, w = aligned & 2 ? DN_ALIGNED : DN_ANY;
@@ -1208,6 +1256,7 @@ extern "C" int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, cons
         return FRCNN_E_BADARG;
     const bool kn = w_layout == FRCNN_W_KN;
     if (!d_x && !d_w && !d_bias) return FRCNN_E_BADARG;
+    if (M > DN_MAX_ROWS) return FRCNN_E_UNSUPPORTED;
     if (d_w && lddw < (kn ? N : K)) return FRCNN_E_BADARG;
     if (!dn_even(d_out, d_dtype == FRCNN_DT_F32 ? 4 : 2) || !dn_even(x, 2) || !dn_even(w, 2) || !dn_even(pre, 2) ||
         !dn_even(d_x, 2) || !dn_even(d_w, 2) || !dn_even(d_bias, 2))

@@ -421,7 +421,8 @@ int frcnn_fc1_fwd(const float* x, const float* w, const float* bias, int64_t M, 
  *              is FRCNN_ACT_NONE.  A bit left out asks for more than needed;
  *   bias, residual, pre may be NULL (pre: the pre-activations, rounded, which the backward needs
  *              for an activation other than FRCNN_ACT_NONE).
- * M = 0 is allowed (no forward output; d_w and d_bias become 0); M up to 2,147,483,647.
+ * M = 0 is allowed (no forward output; d_w and d_bias become 0); M up to 2,147,483,647,
+ * K and N up to 2,097,152 (a call of up to 32 rows: as memory allows).
  * Activations: ReLU max(z, 0); GELU z Phi(z), Phi the normal distribution function (relative error
  * 1.3e-6); SiLU z / (1 + e^-z). */
 #define FRCNN_DT_F32   0
@@ -461,6 +462,7 @@ int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, const void* x, 
  * no part: loss, lse and gradient 0 whatever its logits are (also NaN).  A student logit of -inf
  * has q = 0: the loss is +inf where the teacher gives that label weight; a row of -inf alone is NaN.
  *   dtype   of logits and d_logits: F32, F16 or BF16; t_dtype of top_values: dtype or F32;
+ *   temperature  1e-18 .. 1e18;
  *   weight  [rows] or NULL (1);  loss, lse [rows] f32, lse = log sum_v e^(z_v / T) for the backward;
  *   frcnn_distill_loss: d_logits may be NULL, g = grad_scale; frcnn_distill_bwd: g = d_loss [rows].
  * d_logits must not overlap logits.  The workspace (0 bytes for most sizes) joins the parts of few

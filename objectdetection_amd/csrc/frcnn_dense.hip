@@ -1013,11 +1013,12 @@ static size_t dn_up(size_t b) { return (b + 255) / 256 * 256; }
 
 // A matrix in memory as rows of `cols` values.  padded: its rows are whole pieces with zeros behind `cols`.
 struct DnMatrix { const void* p; long long rows, cols, ld; bool padded; };
+constexpr long long DN_MAX_LD = 1ll << 21;             // a tile's rows lie within 2 GiB of each other
 static long long dn_pieces(long long n) { return (n + 7) / 8; }
-// rows that start on 16 bytes, of whole 16-byte pieces, and a tile whose rows lie within 2 GiB of each other
+// rows that start on 16 bytes, of whole 16-byte pieces
 static bool dn_whole(const DnMatrix& m) {
     return reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.ld % 8 == 0 && (m.padded || m.cols % 8 == 0) &&
-           m.ld <= (1ll << 21);
+           m.ld <= DN_MAX_LD;
 }
 static size_t dn_pack_bytes(long long rows, long long cols) {
     return dn_up((size_t)rows * (size_t)dn_pieces(cols) * 16);
@@ -1030,7 +1031,7 @@ static int dn_pack(DnMatrix* a, DnMatrix* b, char*& ws, DnPacks& packs) {
     int n = 0;
     for (DnMatrix* m : {a, b}) {
         if (!m || dn_whole(*m)) continue;
-        if (dn_pieces(m->cols) * 8 > (1ll << 21)) return FRCNN_E_UNSUPPORTED;
+        if (dn_pieces(m->cols) * 8 > DN_MAX_LD) return FRCNN_E_UNSUPPORTED;
         packs.of[n] = DnPack{m->p, ws, m->rows, m->cols, m->ld, dn_pieces(m->cols)};
         packs.blocks += (m->rows * packs.of[n].pieces + 255) / 256;
         if (n == 0) packs.blocks_first = packs.blocks;
@@ -1151,6 +1152,7 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
         if (rc == FRCNN_OK && d_bias) rc = dn_zero<T>(d_bias, 1, N, N, s);
         return rc;
     }
+    if ((d_x || d_w) && dn_pieces(N) * 8 > DN_MAX_LD) return FRCNN_E_UNSUPPORTED;
     void* dz = p.copy && (d_x || d_w) ? ws : nullptr;
     char* rest = ws + p.dz_bytes + p.sum_bytes;
     const DnMatrix z = dz ? DnMatrix{dz, M, N, p.ldz, true} : DnMatrix{d_out, M, N, ldd, false};
@@ -1205,8 +1207,8 @@ extern "C" size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N, int w
 }
 
 static int dn_aligned(const void* x, int64_t ldx, const void* w, int64_t ldw) {
-    return (dn_even(x, 16) && ldx % 8 == 0 && ldx <= (1 << 21) ? 1 : 0) |
-           (dn_even(w, 16) && ldw % 8 == 0 && ldw <= (1 << 21) ? 2 : 0);
+    return (dn_even(x, 16) && ldx % 8 == 0 && ldx <= DN_MAX_LD ? 1 : 0) |
+           (dn_even(w, 16) && ldw % 8 == 0 && ldw <= DN_MAX_LD ? 2 : 0);
 }
 
 extern "C" int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int w_layout, const void* bias,

@@ -33,7 +33,7 @@ struct DsArgs {
     float temperature;
     long long rows; int V, k;
     float* loss; float* lse; void* grad; long long ldg;
-    float2* part; int chunks;            // maximum and sum of each chunk of a split row
+    float2* part; int chunks, nv;        // maximum and sum of each chunk of a split row; its vectors per thread
 };
 
 typedef unsigned int ds_u32x4 __attribute__((ext_vector_type(4)));
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
 // ---- a chunk of a row per workgroup --------------------------------------------------------------------
 // of 4 vectors per thread, of one where the rows are few and their chunks would not fill the chip
 constexpr int DS_CHUNK_BLOCK = 256;
-template <typename T, int NV> constexpr int ds_chunk() { return DS_CHUNK_BLOCK * NV * DsVec<T>::W; }
+template <typename T, int BLOCK, int NV> constexpr int ds_chunk() { return BLOCK * NV * DsVec<T>::W; }
 
 template <typename T, int NV>
 __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_part_kernel(DsArgs a) {
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_part_kernel(DsArgs a) 
     const long long row = blockIdx.y;
     if (a.weight && a.weight[row] == 0.f) return;
     const T* z = (const T*)a.z + row * a.ldz;
-    const long long v0 = (long long)chunk * ds_chunk<T, NV>();
+    const long long v0 = (long long)chunk * ds_chunk<T, DS_CHUNK_BLOCK, NV>();
     DsVec<T> x[NV];
     float m = -__builtin_inff();
 #pragma unroll
@@ -384,8 +384,8 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_part_kernel(DsArgs a) 
 }
 
 // FORWARD: joins the row's partial sums; chunk 0 writes loss and lse; else q comes from the forward's lse
-template <typename T, bool FORWARD, int NV>
-__global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_chunk_kernel(DsArgs a) {
+template <typename T, bool FORWARD, int BLOCK, int NV>
+__global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
     extern __shared__ __attribute__((aligned(16))) char ds_lds[];
     __shared__ float sh_t, sh_m, sh_s;
     __shared__ int sh_any;
@@ -394,18 +394,18 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_chunk_kernel(DsArgs a)
     const long long row = blockIdx.y;
     const T* z = (const T*)a.z + row * a.ldz;
     T* grad = a.grad ? (T*)a.grad + row * a.ldg : nullptr;
-    const long long v0 = (long long)chunk * ds_chunk<T, NV>(), v1 = v0 + ds_chunk<T, NV>() < a.V ? v0 + ds_chunk<T, NV>() : a.V;
+    const long long v0 = (long long)chunk * ds_chunk<T, BLOCK, NV>(), v1 = v0 + ds_chunk<T, BLOCK, NV>() < a.V ? v0 + ds_chunk<T, BLOCK, NV>() : a.V;
     const float w = a.weight ? a.weight[row] : 1.0f, inv_t = 1.0f / a.temperature;
     if (w == 0.f) {
         if (FORWARD && chunk == 0 && tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
-        if (grad) ds_zero(grad, v0, v1, tid, DS_CHUNK_BLOCK);
+        if (grad) ds_zero(grad, v0, v1, tid, BLOCK);
         return;
     }
     DsVec<T> x[NV];
     if (grad) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const long long v = v0 + (tid + DS_CHUNK_BLOCK * i) * W, left = a.V - v;
+            const long long v = v0 + (tid + BLOCK * i) * W, left = a.V - v;
             x[i].load(z + v, left > W ? W : (int)left);
         }
     }
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_chunk_kernel(DsArgs a)
     __syncthreads();
     if (!sh_any) {
         if (FORWARD && chunk == 0 && tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
-        if (grad) ds_zero(grad, v0, v1, tid, DS_CHUNK_BLOCK);
+        if (grad) ds_zero(grad, v0, v1, tid, BLOCK);
         return;
     }
     const float m = FORWARD ? sh_m : 0.f, s = FORWARD ? sh_s : 1.f, lse = FORWARD ? 0.f : a.lse_in[row];
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_chunk_kernel(DsArgs a)
         }
     }
     if (!grad) return;
-    ds_listed_sums(e, a.k, sh_t, wave_id(), DS_CHUNK_BLOCK / 64);
+    ds_listed_sums(e, a.k, sh_t, wave_id(), BLOCK / 64);
     const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale), cq = FORWARD ? c / s : c;
     const float f = inv_t * DS_LOG2E;
     auto relative = [&](float zi) {
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_chunk_kernel(DsArgs a)
     };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const long long v = v0 + (tid + DS_CHUNK_BLOCK * i) * W, left = a.V - v;
+        const long long v = v0 + (tid + BLOCK * i) * W, left = a.V - v;
         float q[W];
 #pragma unroll
         for (int j = 0; j < W; ++j) q[j] = cq * relative(x[i][j]);
@@ -460,12 +460,13 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_chunk_kernel(DsArgs a)
         x[i].store(grad + v, left > W ? W : (int)left);
     }
     __syncthreads();
-    ds_listed(e, a.k, c, grad, v0, v1, tid, DS_CHUNK_BLOCK, [&](float zi) { return relative(zi) / s; });
+    ds_listed(e, a.k, c, grad, v0, v1, tid, BLOCK, [&](float zi) { return relative(zi) / s; });
 }
 
 // ---- host --------------------------------------------------------------------------------------------
 // rows that one workgroup can hold, and long rows of which there are too few to fill the chip
 static long long ds_vectors(int V, int dtype) { return (V + (dtype == FRCNN_DT_F32 ? 4 : 8) - 1) / (dtype == FRCNN_DT_F32 ? 4 : 8); }
+// vectors per thread of a chunk
 static int ds_chunk_vectors(long long rows, int V, int dtype) {
     const long long four = (ds_vectors(V, dtype) + DS_CHUNK_BLOCK * 4 - 1) / (DS_CHUNK_BLOCK * 4);
     return rows * four <= 256 ? 1 : 4;
@@ -484,68 +485,90 @@ static int ds_group(int V, int k) {
     return g;
 }
 
+// rows r .. r + n - 1 of a call
+template <typename T>
+static DsArgs ds_rows(const DsArgs& a, long long r, long long n) {
+    DsArgs b = a;
+    b.rows = n;
+    b.z = (const T*)a.z + r * a.ldz;
+    b.t = (const char*)a.t + r * a.k * (a.t_f32 ? 4 : (long long)sizeof(T));
+    b.idx = a.idx + r * a.k;
+    if (a.weight) b.weight = a.weight + r;
+    if (a.d_loss) b.d_loss = a.d_loss + r;
+    if (a.lse_in) b.lse_in = a.lse_in + r;
+    if (a.loss) { b.loss = a.loss + r; b.lse = a.lse + r; }
+    if (a.grad) b.grad = (T*)a.grad + r * a.ldg;
+    if (a.part) b.part = a.part + r * a.chunks;
+    return b;
+}
+
 template <typename T, bool FORWARD, int G>
 static int ds_launch_small(const DsArgs& a, hipStream_t s) {
-    const long long blocks = (a.rows + 256 / G - 1) / (256 / G);
-    if (blocks > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
-    FRCNN_LAUNCH((distill_small_kernel<T, FORWARD, G>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    FRCNN_LAUNCH((distill_small_kernel<T, FORWARD, G>), dim3((unsigned)((a.rows + 256 / G - 1) / (256 / G))), dim3(256),
+                 0, s, a);
     return FRCNN_OK;
 }
 template <typename T, int BLOCK, int NV>
 static int ds_launch_row(const DsArgs& a, hipStream_t s) {
-    if (a.rows > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
-    FRCNN_LAUNCH((distill_row_kernel<T, BLOCK, NV>), dim3((unsigned)a.rows), dim3(BLOCK), (size_t)a.k * DS_ENTRY_BYTES, s, a);
+    FRCNN_LAUNCH((distill_row_kernel<T, BLOCK, NV>), dim3((unsigned)a.rows), dim3(BLOCK), (size_t)a.k * DS_ENTRY_BYTES,
+                 s, a);
+    return FRCNN_OK;
+}
+template <typename T, bool FORWARD, int BLOCK, int NV>
+static int ds_launch_chunk(const DsArgs& a, hipStream_t s) {
+    if constexpr (FORWARD)
+        FRCNN_LAUNCH((distill_part_kernel<T, NV>), dim3((unsigned)a.chunks, (unsigned)a.rows), dim3(BLOCK), 0, s, a);
+    const dim3 grid(a.grad ? (unsigned)a.chunks : 1u, (unsigned)a.rows);           // without a gradient: the loss alone
+    FRCNN_LAUNCH((distill_chunk_kernel<T, FORWARD, BLOCK, NV>), grid, dim3(BLOCK), (size_t)a.k * DS_ENTRY_BYTES, s, a);
     return FRCNN_OK;
 }
 
 template <typename T, bool FORWARD>
-static int ds_run(DsArgs a, int dtype, hipStream_t s) {
+static int ds_run(const DsArgs& a, int dtype, hipStream_t s) {
     const int g = ds_group(a.V, a.k);
     if (g <= 8) return ds_launch_small<T, FORWARD, 8>(a, s);
     if (g <= 16) return ds_launch_small<T, FORWARD, 16>(a, s);
     if (g <= 32) return ds_launch_small<T, FORWARD, 32>(a, s);
     if (g <= 64) return ds_launch_small<T, FORWARD, 64>(a, s);
     const long long n = ds_vectors(a.V, dtype);
-    const int nv = ds_chunk_vectors(a.rows, a.V, dtype);
-    a.chunks = (int)ds_chunks(a.rows, a.V, dtype);
-    if (FORWARD && !ds_split(a.rows, a.V, dtype)) {
-        if (n <= 64) return ds_launch_row<T, 64, 1>(a, s);
-        if (n <= 256) return ds_launch_row<T, 64, 4>(a, s);
-        if (n <= 1024) return ds_launch_row<T, 256, 4>(a, s);
-        if (n <= 2048) return ds_launch_row<T, 256, 8>(a, s);
-        if (n <= 4096) return ds_launch_row<T, 512, 8>(a, s);
-        if (n <= 8192) return ds_launch_row<T, 512, 16>(a, s);
-        return ds_launch_row<T, 1024, 16>(a, s);
+    if constexpr (FORWARD) {
+        if (!a.part) {
+            if (n <= 64) return ds_launch_row<T, 64, 1>(a, s);
+            if (n <= 256) return ds_launch_row<T, 64, 4>(a, s);
+            if (n <= 1024) return ds_launch_row<T, 256, 4>(a, s);
+            if (n <= 2048) return ds_launch_row<T, 256, 8>(a, s);
+            if (n <= 4096) return ds_launch_row<T, 512, 8>(a, s);
+            if (n <= 8192) return ds_launch_row<T, 512, 16>(a, s);
+            return ds_launch_row<T, 1024, 16>(a, s);
+        }
+        return a.nv == 1 ? ds_launch_chunk<T, true, DS_CHUNK_BLOCK, 1>(a, s)
+                         : ds_launch_chunk<T, true, DS_CHUNK_BLOCK, 4>(a, s);
+    } else {
+        // short rows: a wave each
+        if (n <= 64) return ds_launch_chunk<T, false, 64, 1>(a, s);
+        if (n <= 256) return ds_launch_chunk<T, false, 64, 4>(a, s);
+        return a.nv == 1 ? ds_launch_chunk<T, false, DS_CHUNK_BLOCK, 1>(a, s)
+                         : ds_launch_chunk<T, false, DS_CHUNK_BLOCK, 4>(a, s);
     }
-    // rows along the grid's second dimension, at most 65,535 in a launch
-    for (long long r = 0; r < a.rows; r += 65535) {
-        DsArgs b = a;
-        b.rows = a.rows - r < 65535 ? a.rows - r : 65535;
-        b.z = (const T*)a.z + r * a.ldz;
-        b.t = (const char*)a.t + r * a.k * (a.t_f32 ? 4 : (long long)sizeof(T));
-        b.idx = a.idx + r * a.k;
-        if (a.weight) b.weight = a.weight + r;
-        if (a.d_loss) b.d_loss = a.d_loss + r;
-        if (a.lse_in) b.lse_in = a.lse_in + r;
-        if (a.loss) { b.loss = a.loss + r; b.lse = a.lse + r; }
-        if (a.grad) b.grad = (T*)a.grad + r * a.ldg;
-        if (a.part) b.part = a.part + r * a.chunks;
-        const dim3 grid((unsigned)a.chunks, (unsigned)b.rows);
-        if (FORWARD && nv == 1) FRCNN_LAUNCH((distill_part_kernel<T, 1>), grid, dim3(DS_CHUNK_BLOCK), 0, s, b);
-        else if (FORWARD) FRCNN_LAUNCH((distill_part_kernel<T, 4>), grid, dim3(DS_CHUNK_BLOCK), 0, s, b);
-        const dim3 gg(a.grad ? (unsigned)a.chunks : 1u, (unsigned)b.rows);      // without a gradient: the loss alone
-        const size_t lds = (size_t)a.k * DS_ENTRY_BYTES;
-        if (nv == 1) FRCNN_LAUNCH((distill_chunk_kernel<T, FORWARD, 1>), gg, dim3(DS_CHUNK_BLOCK), lds, s, b);
-        else FRCNN_LAUNCH((distill_chunk_kernel<T, FORWARD, 4>), gg, dim3(DS_CHUNK_BLOCK), lds, s, b);
-    }
-    return FRCNN_OK;
 }
 
+// a launch at a time: rows are the grid's second dimension where rows have chunks (65,535 at most), else
+// workgroups of up to 1,024 threads (fewer than 2^32 threads in a launch)
 template <bool FORWARD>
-static int ds_dispatch(const DsArgs& a, int dtype, hipStream_t s) {
-    if (dtype == FRCNN_DT_F32) return ds_run<float, FORWARD>(a, dtype, s);
-    if (dtype == FRCNN_DT_F16) return ds_run<_Float16, FORWARD>(a, dtype, s);
-    return ds_run<__bf16, FORWARD>(a, dtype, s);
+static int ds_dispatch(DsArgs a, int dtype, hipStream_t s) {
+    const bool chunked = ds_group(a.V, a.k) > 64 && (!FORWARD || ds_split(a.rows, a.V, dtype));
+    if (!chunked) a.part = nullptr;
+    a.nv = ds_chunk_vectors(a.rows, a.V, dtype);
+    a.chunks = (int)ds_chunks(a.rows, a.V, dtype);
+    const long long most = chunked ? 65535 : 1 << 21;
+    for (long long r = 0; r < a.rows; r += most) {
+        const long long n = a.rows - r < most ? a.rows - r : most;
+        const int rc = dtype == FRCNN_DT_F32   ? ds_run<float, FORWARD>(ds_rows<float>(a, r, n), dtype, s)
+                       : dtype == FRCNN_DT_F16 ? ds_run<_Float16, FORWARD>(ds_rows<_Float16>(a, r, n), dtype, s)
+                                               : ds_run<__bf16, FORWARD>(ds_rows<__bf16>(a, r, n), dtype, s);
+        if (rc != FRCNN_OK) return rc;
+    }
+    return FRCNN_OK;
 }
 
 static int ds_check(const void* z, int64_t ldz, int dtype, const void* t, int t_dtype, const int64_t* idx,
@@ -553,7 +576,7 @@ static int ds_check(const void* z, int64_t ldz, int dtype, const void* t, int t_
     if (rows < 0 || V <= 0 || k <= 0 || ldz < V) return FRCNN_E_BADARG;
     if (dtype != FRCNN_DT_F32 && dtype != FRCNN_DT_F16 && dtype != FRCNN_DT_BF16) return FRCNN_E_BADARG;
     if (t_dtype != dtype && t_dtype != FRCNN_DT_F32) return FRCNN_E_BADARG;
-    if (!(temperature > 0.f) || temperature > 3.0e38f) return FRCNN_E_BADARG;
+    if (!(temperature >= 1e-18f && temperature <= 1e18f)) return FRCNN_E_BADARG;   // its square is a float32 too
     if (k > DS_MAX_K || V > 0x40000000) return FRCNN_E_UNSUPPORTED;
     if (rows == 0) return FRCNN_OK;
     if (!z || !t || !idx) return FRCNN_E_BADARG;

@@ -844,8 +844,8 @@ def _distill_args(logits, top_values, top_index, weight, temperature):
             raise ValueError(f"weight must be {list(lead)}")
         weight = weight.contiguous()
         pw = weight.data_ptr()
-    if not 0.0 < temperature < 3.0e38:
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-18 <= temperature <= 1e18:
+        raise ValueError(f"temperature must be in 1e-18 .. 1e18, got {temperature}")
     rows = lead[0] if len(lead) == 1 else math.prod(lead)
     z, ldz = _rows(logits if len(lead) == 1 else logits.reshape(rows, V))
     top_values, top_index = top_values.contiguous(), top_index.contiguous()

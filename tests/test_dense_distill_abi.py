@@ -65,6 +65,9 @@ def test_dense_workspaces(L):
     assert bwd(L, ws=None, **relu) == L.E_WORKSPACE
     assert bwd(L, wsb=b(4, 64, 32, 0, 3) - 1, **relu) == L.E_WORKSPACE
     assert bwd(L, ws=ctypes.c_void_p(24), **relu) == L.E_WORKSPACE
+    wide = (1 << 21) + 8                                    # rows that a tile cannot reach over
+    assert fwd(L, M=40, K=wide, ldx=wide, ws=ONE, wsb=1 << 50) == L.E_UNSUPPORTED
+    assert bwd(L, M=40, N=wide, ldd=wide, ldw=wide, lddw=wide, ws=ONE, wsb=1 << 50) == L.E_UNSUPPORTED
     assert fwd(L, M=1 << 31) == L.E_UNSUPPORTED and bwd(L, M=1 << 31) == L.E_UNSUPPORTED
     assert fwd(L, M=0, x=None, out=None) == L.OK           # no rows: nothing to do, nothing launched
 
@@ -77,7 +80,7 @@ def loss(L, z=ONE, ldz=50, dt=0, t=ONE, tdt=0, idx=ONE, w=None, rows=3, V=50, k=
 @pytest.mark.parametrize("bad", [
     dict(z=None), dict(t=None), dict(idx=None), dict(l=None), dict(lse=None), dict(ldz=49), dict(d=ONE, ldg=49),
     dict(dt=3), dict(tdt=1), dict(rows=-1), dict(V=0), dict(k=0), dict(T=0.0), dict(T=-1.0), dict(T=float("nan")),
-    dict(T=float("inf")), dict(z=ctypes.c_void_p(18)), dict(idx=ctypes.c_void_p(20))])
+    dict(T=float("inf")), dict(T=1e-19), dict(T=1e19), dict(z=ctypes.c_void_p(18)), dict(idx=ctypes.c_void_p(20))])
 def test_distillation_refuses(L, bad):
     assert loss(L, **bad) == L.E_BADARG
     b = dict(z=ONE, ldz=50, dt=0, t=ONE, tdt=0, idx=ONE, lse=ONE, w=None, rows=3, V=50, k=4, T=1.0, d=ONE, ldg=50)

@@ -233,6 +233,46 @@ def test_infinities_and_nan(dev):
     assert torch.equal(bad, ref)
 
 
+@pytest.mark.parametrize("M", [3, 70])
+def test_values_below_the_normal_range(dev, M):
+    """float16 subnormals are kept as operands and as results (a factor of two exact)."""
+    from objectdetection_amd import ops
+    x = (2.0 ** -24 * torch.arange(1, M + 1, device=dev)).half()[:, None] * torch.eye(8, device=dev)[0].half()
+    w = torch.full((8, 16), 2.0, device=dev).half()
+    for ww in (w, w.t().contiguous().t()):
+        assert torch.equal(ops.dense_fwd(x, ww), (2.0 ** -23 * torch.arange(1, M + 1, device=dev)).half()[:, None].expand(M, 16))
+        d = torch.zeros((M, 16), device=dev).half()
+        d[:, 3] = 2.0 ** -24
+        assert (ops.dense_bwd(d, x, ww)["d_x"] == 2.0 ** -23).all()
+
+
+def test_a_workspace_is_written_before_it_is_read(dev):
+    """A workspace full of NaN, and one byte more than needed behind it, change nothing."""
+    from objectdetection_amd import ops
+    for M, K, N, layout in ((1, 25088, 24, "kn"), (130, 1003, 333, "nk"), (90, 8200, 84, "kn"), (5000, 40, 84, "nk")):
+        x, w, b, d = make(np.random.default_rng(7), dev, M, K, N, torch.bfloat16, layout, True, True)
+        lay = 0 if layout == "kn" else 1
+        pre = ops.dense_fwd(x, w, b, want_pre=True)[1]
+        nf, nb = ops.dense_fwd_workspace_bytes(M, K, N, lay), ops.dense_bwd_workspace_bytes(M, K, N, lay)
+        ws = torch.full((max(nf, nb) + 256,), 255, dtype=torch.uint8, device=dev)
+        assert torch.equal(ops.dense_fwd(x, w, b, workspace=ws[:nf] if nf else None), ops.dense_fwd(x, w, b))
+        assert (ws[nf:] == 255).all()
+        ws.fill_(255)
+        g, h = ops.dense_bwd(d, x, w, pre, "silu", workspace=ws[:nb]), ops.dense_bwd(d, x, w, pre, "silu")
+        assert all(torch.equal(g[k], h[k]) for k in g) and (ws[nb:] == 255).all()
+
+
+def test_only_the_wanted_gradients(dev):
+    from objectdetection_amd import ops
+    x, w, b, d = make(np.random.default_rng(8), dev, 300, 203, 85, torch.float16, "nk", True, True)
+    pre = ops.dense_fwd(x, w, b, want_pre=True)[1]
+    full = ops.dense_bwd(d, x, w, pre, "gelu")
+    for n in range(1, 8):
+        g = ops.dense_bwd(d, x, w, pre, "gelu", bool(n & 1), bool(n & 2), bool(n & 4))
+        for bit, key in ((1, "d_x"), (2, "d_weight"), (4, "d_bias")):
+            assert torch.equal(g[key], full[key]) if n & bit else g[key] is None
+
+
 def test_same_bits_every_time_and_on_another_stream(dev):
     from objectdetection_amd import ops
     x, w, b, d = make(np.random.default_rng(9), dev, 40, 4104, 84, torch.bfloat16, "nk", True, True)
@@ -247,12 +287,15 @@ def test_same_bits_every_time_and_on_another_stream(dev):
     torch.cuda.current_stream().wait_stream(side)
 
 
-def test_captured_forward_and_backward_replay(dev):
-    """Two graphs of the same calls with a workspace each, replayed with other work between."""
+@pytest.mark.parametrize("M,K,N,layout", [(24, 2056, 136, "kn"), (130, 1003, 333, "nk"), (4100, 72, 2056, "kn"),
+                                          (700, 4096, 84, "nk")])
+def test_captured_forward_and_backward_replay(dev, M, K, N, layout):
+    """Two graphs of the same calls with a workspace each, replayed with other work between: few rows,
+    packed operands, the large tile, a split reduction."""
     from objectdetection_amd import ops
-    M, K, N = 24, 2056, 136
-    x, w, b, d = make(np.random.default_rng(11), dev, M, K, N, torch.bfloat16, "kn", True, True)
-    ws = [torch.empty(max(ops.dense_fwd_workspace_bytes(M, K, N), ops.dense_bwd_workspace_bytes(M, K, N)),
+    x, w, b, d = make(np.random.default_rng(11), dev, M, K, N, torch.bfloat16, layout, True, True)
+    lay = 0 if layout == "kn" else 1
+    ws = [torch.empty(max(16, ops.dense_fwd_workspace_bytes(M, K, N, lay), ops.dense_bwd_workspace_bytes(M, K, N, lay)),
                       dtype=torch.uint8, device=dev) for _ in range(2)]
     side = torch.cuda.Stream()
     graphs, outs = [], []

@@ -76,7 +76,7 @@ def check(got, z, t, idx, wt, T, g=None):
 
 
 SIZES = [(1, 1, 1), (5, 2, 2), (7, 21, 8), (300, 21, 21), (3, 64, 3), (9, 65, 5), (4, 257, 33), (2, 1031, 100),
-         (33, 4096, 64), (3, 20011, 17), (1, 131072, 64), (2, 66000, 1), (5, 40, 40), (2, 2500, 1024)]
+         (33, 4096, 64), (700, 100, 12), (260, 700, 40), (3, 20011, 17), (1, 131072, 64), (2, 66000, 1), (5, 40, 40), (2, 2500, 1024)]
 
 
 @pytest.mark.parametrize("rows,V,k", SIZES)
@@ -109,7 +109,7 @@ def test_grad_scale_strided_logits_and_leading_dimensions(dev):
     check(dict(loss=a["loss"], lse=a["lse"], d_logits=a["d_logits"] * 8), z, t, idx, None, 2.0)
 
 
-@pytest.mark.parametrize("V,k", [(21, 5), (64, 64), (300, 7), (5000, 70)])
+@pytest.mark.parametrize("V,k", [(21, 5), (64, 64), (300, 7), (5000, 70), (21, 100), (70000, 300)])
 def test_label_listed_twice_counts_twice(dev, V, k):
     from objectdetection_amd import ops
     z, t, idx, _ = make(3, dev, 6, V, k, torch.float32)
@@ -118,7 +118,7 @@ def test_label_listed_twice_counts_twice(dev, V, k):
     check(ops.distill_loss(z, t, idx, temperature=1.5), z, t, idx, None, 1.5)
 
 
-@pytest.mark.parametrize("V", [21, 300, 9001])
+@pytest.mark.parametrize("V", [21, 300, 9001, 40000])
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
 def test_masked_rows_infinities_and_nan(dev, V, name):
     """Rows that take no part are not read (NaN there changes nothing) and get zeros; -inf logits of
@@ -242,6 +242,7 @@ def test_refusals(dev):
             (lambda: ops.distill_loss(z, t, idx, temperature=0.0), ValueError),
             (lambda: ops.distill_loss(z, t, idx, temperature=math.nan), ValueError),
             (lambda: ops.distill_loss(z, t, idx, temperature=math.inf), ValueError),
+            (lambda: ops.distill_loss(z, t, idx, temperature=1e-19), ValueError),
             (lambda: ops.distill_loss(z.cpu(), t, idx), RuntimeError),
             (lambda: ops.distill_loss(z, t.cpu(), idx), RuntimeError),
             (lambda: ops.distill_loss(z, t, idx.cpu()), RuntimeError),

@@ -190,16 +190,21 @@ class RegionProposalPath:
         self._validate(fmap, score, coord, gt, label)
         if self.pooled is None and not skip_roi:
             raise ValueError("this path was built with alloc_pooled=False: call run(skip_roi=True)")
+        main = torch.cuda.current_stream(self.device)
+        if self.depth == 2 and self._calls:
+            # what the caller queued behind the call before may still read that call's results:
+            # its set may be rewritten once the caller's stream has passed this point
+            self._sets[(self._calls - 1) % self.depth]["ev"][4].record(main)
         d = self._sets[self._calls % self.depth]
         self._calls += 1
         self._bind(d)
         ev = d["ev"]
-        main = torch.cuda.current_stream(self.device)
         prop = self.prop_stream if self.depth == 2 else main
         st, ps = main.cuda_stream, prop.cuda_stream
         seed &= 0xFFFFFFFFFFFFFFFF
-        # inputs were produced on the caller's stream; this set's previous user (two calls
-        # ago) finished reading it before the point ev[4] marks
+        # inputs were produced on the caller's stream; this set's previous user (two calls ago) and
+        # what the caller queued between that call and the next finished reading it before the
+        # point ev[4] marks
         if inputs_ready is not None:
             ready = inputs_ready
         else:
@@ -288,7 +293,6 @@ class RegionProposalPath:
             roi_events[1].record(main)
         if self.train:
             main.wait_event(ev[2])                     # join: everything is ordered on `main` again
-        ev[4].record(main)                             # this set may be rewritten after here
         return self
 
 

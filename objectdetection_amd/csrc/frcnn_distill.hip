@@ -110,13 +110,21 @@ __device__ __forceinline__ float ds_block(float v, float* sh) {
 
 // ---- the teacher's side of a row, by one wave ----------------------------------------------------------
 // LDS: per entry its label (-1: not there), t / T relative to the largest one, the student's logit there,
-// and what its label gets: the sum of its entries' p at the first of them, -1 at the others
+// and what its label gets: the sum of its entries' p at the first of them, -1 at the others; with more than
+// 64 entries also a table of twice as many places or more, in which entries with the same label meet
+constexpr int ds_slots(int k) {
+    int n = 0;
+    if (k > 64)
+        for (n = 256; n < 2 * k; n *= 2) {}
+    return n;
+}
 struct DsTeacher {
-    int* label; float* t; float* z; float* p;
+    int* label; float* t; float* z; float* p; int* key; int* first;
     __device__ __forceinline__ DsTeacher(void* lds, int k)
-        : label((int*)lds), t((float*)lds + k), z((float*)lds + 2 * k), p((float*)lds + 3 * k) {}
+        : label((int*)lds), t((float*)lds + k), z((float*)lds + 2 * k), p((float*)lds + 3 * k), key((int*)lds + 4 * k),
+          first(key + ds_slots(k)) {}
 };
-constexpr int DS_ENTRY_BYTES = 16;
+static size_t ds_lds_bytes(int k) { return (size_t)k * 16 + (size_t)ds_slots(k) * 8; }
 struct DsTeacherSum { float log_sum; bool any; };      // log of the sum of e^t; whether an entry is there
 
 template <typename T>
@@ -166,28 +174,79 @@ __device__ __forceinline__ float ds_row_loss(const DsArgs& a, DsTeacher e, float
     return ds_wave_sum(l);
 }
 
-// e.p for the entries of one wave in every `waves`: 64 entries in its lanes against all entries one by one
-// (from a register of another lane: an LDS read per comparison costs the whole row its latency)
-__device__ __forceinline__ void ds_listed_sums(DsTeacher e, int k, float log_sum, int wave, int waves) {
-    const int lane = lane_id();
-    for (int j0 = 64 * wave; j0 < k; j0 += 64 * waves) {
-        const int mine = j0 + lane < k ? e.label[j0 + lane] : -1;
+// e.p for the labels in [v0, v1), by the whole workgroup.  Up to 64 entries: one wave compares each with all
+// of them one by one (from a register of another lane: an LDS read per comparison costs the whole row its
+// latency).  More: that would be the square of their number, so each looks for its label's place in
+// the table; the first entry of a label adds up the later ones, in their order.  (4,096 rows x 65,536, 1,024 entries: 416 us; 1,917 by comparing all with all.)
+template <int BLOCK>
+__device__ __forceinline__ void ds_listed_sums(DsTeacher e, int k, float log_sum, long long v0, long long v1) {
+    if (k <= 64) {
+        if (wave_id() != 0) return;
+        const int lane = lane_id();
+        const int mine = lane < k ? e.label[lane] : -1;
+        const float p = lane < k ? __builtin_amdgcn_exp2f((e.t[lane] - log_sum) * DS_LOG2E) : 0.f;
         float sum = 0.f;
         bool first = mine >= 0;
-        for (int n0 = 0; n0 < k; n0 += 64) {
-            const int label = n0 + lane < k ? e.label[n0 + lane] : -1;
-            const float p = n0 + lane < k ? __builtin_amdgcn_exp2f((e.t[n0 + lane] - log_sum) * DS_LOG2E) : 0.f;
-            const int end = k - n0 < 64 ? k - n0 : 64;
-            for (int n = 0; n < end; ++n) {
-                const int other = __builtin_amdgcn_readlane(label, n);
-                const float q = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), n));
-                if (other == mine) {
-                    sum += q;
-                    if (n0 + n < j0 + lane) first = false;
-                }
+        for (int n = 0; n < k; ++n) {
+            const int other = __builtin_amdgcn_readlane(mine, n);
+            const float q = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), n));
+            if (other == mine) {
+                sum += q;
+                if (n < lane) first = false;
             }
         }
-        if (j0 + lane < k) e.p[j0 + lane] = first ? sum : -1.0f;
+        if (lane < k) e.p[lane] = first ? sum : -1.0f;
+        return;
+    }
+    const int tid = threadIdx.x, slots = ds_slots(k), shift = __builtin_clz(slots) + 1;
+    for (int n = tid; n < slots; n += BLOCK) {
+        e.key[n] = -1;
+        e.first[n] = k;
+    }
+    __syncthreads();
+    for (int j = tid; j < k; j += BLOCK) {             // places; e.p: the entry's place
+        const int label = e.label[j];
+        if (label < v0 || label >= v1) {
+            e.p[j] = -1.0f;
+            continue;
+        }
+        int n = (int)(((unsigned)label * 2654435761u) >> shift);
+        while (true) {                                 // ends: there are more places than labels
+            const int held = atomicCAS(&e.key[n], -1, label);
+            if (held == -1 || held == label) break;
+            n = (n + 1) & (slots - 1);
+        }
+        atomicMin(&e.first[n], j);
+        e.p[j] = __int_as_float(n);
+    }
+    __syncthreads();
+    for (int j = tid; j < k; j += BLOCK) {             // the later ones form a chain: key -2 - j, e.p -2 - j of the next
+        if (e.p[j] < 0.f) continue;
+        const int n = __float_as_int(e.p[j]);
+        if (e.first[n] == j) continue;
+        const int held = atomicExch(&e.key[n], -2 - j);
+        e.p[j] = held >= 0 ? -1.0f : (float)held;
+    }
+    __syncthreads();
+    for (int j = tid; j < k; j += BLOCK) {
+        if (e.p[j] < 0.f) continue;
+        const int head = e.key[__float_as_int(e.p[j])], label = e.label[j];
+        float sum = __builtin_amdgcn_exp2f((e.t[j] - log_sum) * DS_LOG2E);
+        int length = 0;
+        for (int n = head; n < -1 && length <= 16; ++length) n = (int)e.p[-2 - n];
+        if (length <= 16) {                            // the chain's order is chance: the smallest number first
+            for (int from = j, m = 0; m < length; ++m) {
+                int next = k;
+                for (int n = head; n < -1; n = (int)e.p[-2 - n])
+                    if (-2 - n > from && -2 - n < next) next = -2 - n;
+                sum += __builtin_amdgcn_exp2f((e.t[next] - log_sum) * DS_LOG2E);
+                from = next;
+            }
+        } else {
+            for (int n = j + 1; n < k; ++n)
+                if (e.label[n] == label) sum += __builtin_amdgcn_exp2f((e.t[n] - log_sum) * DS_LOG2E);
+        }
+        e.p[j] = sum;
     }
 }
 
@@ -319,7 +378,7 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
         for (int j = 0; j < W; ++j) part += __builtin_amdgcn_exp2f((x[i][j] - m) * f);
         s += part;
     }
-    if (grad) ds_listed_sums(e, a.k, sh_t, wave_id(), BLOCK / 64);
+    if (grad) ds_listed_sums<BLOCK>(e, a.k, sh_t, 0, a.V);
     s = ds_block<BLOCK, false>(s, sh_s);
     const float log_s = logf(s);
     if (wave_id() == 0) {
@@ -333,7 +392,11 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
     const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale), cq = c / s;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int v = (tid + BLOCK * i) * W;
+        int t = tid;
+        // a large workgroup has 128 registers per lane: the places are not kept in them from the loads on
+        // (2,048 rows x 131,072 bf16: 253 us; 280 with 68 bytes per lane waiting in memory)
+        if constexpr (BLOCK == 1024) asm volatile("" : "+v"(t));
+        const int v = (t + BLOCK * i) * W;
         float q[W];
         x[i].renew();
 #pragma unroll
@@ -444,7 +507,7 @@ __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
         }
     }
     if (!grad) return;
-    ds_listed_sums(e, a.k, sh_t, wave_id(), BLOCK / 64);
+    ds_listed_sums<BLOCK>(e, a.k, sh_t, v0, v1);
     const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale), cq = FORWARD ? c / s : c;
     const float f = inv_t * DS_LOG2E;
     auto relative = [&](float zi) {
@@ -510,7 +573,7 @@ static int ds_launch_small(const DsArgs& a, hipStream_t s) {
 }
 template <typename T, int BLOCK, int NV>
 static int ds_launch_row(const DsArgs& a, hipStream_t s) {
-    FRCNN_LAUNCH((distill_row_kernel<T, BLOCK, NV>), dim3((unsigned)a.rows), dim3(BLOCK), (size_t)a.k * DS_ENTRY_BYTES,
+    FRCNN_LAUNCH((distill_row_kernel<T, BLOCK, NV>), dim3((unsigned)a.rows), dim3(BLOCK), ds_lds_bytes(a.k),
                  s, a);
     return FRCNN_OK;
 }
@@ -519,7 +582,7 @@ static int ds_launch_chunk(const DsArgs& a, hipStream_t s) {
     if constexpr (FORWARD)
         FRCNN_LAUNCH((distill_part_kernel<T, NV>), dim3((unsigned)a.chunks, (unsigned)a.rows), dim3(BLOCK), 0, s, a);
     const dim3 grid(a.grad ? (unsigned)a.chunks : 1u, (unsigned)a.rows);           // without a gradient: the loss alone
-    FRCNN_LAUNCH((distill_chunk_kernel<T, FORWARD, BLOCK, NV>), grid, dim3(BLOCK), (size_t)a.k * DS_ENTRY_BYTES, s, a);
+    FRCNN_LAUNCH((distill_chunk_kernel<T, FORWARD, BLOCK, NV>), grid, dim3(BLOCK), ds_lds_bytes(a.k), s, a);
     return FRCNN_OK;
 }
 

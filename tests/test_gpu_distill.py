@@ -251,3 +251,49 @@ def test_refusals(dev):
             (lambda: ops.distill_loss(z, t.repeat(1, 400), idx.repeat(1, 400)), RuntimeError)):
         with pytest.raises(err):
             bad()
+
+
+@pytest.mark.parametrize("name,rows,V", [("bf16", 210, 40000), ("f32", 210, 20003), ("f16", 70, 131072), ("f32", 70, 65000)])
+def test_many_long_rows(dev, name, rows, V):
+    """Rows of up to 16,384 pieces of 16 bytes stay in one workgroup when there are many."""
+    from objectdetection_amd import ops
+    assert ops.distill_workspace_bytes(rows, V, 9, TYPES[name]) == 0
+    z, t, idx, wt = make(rows + V, dev, rows, V, 9, TYPES[name], torch.float32, True)
+    check(ops.distill_loss(z, t, idx, weight=wt, temperature=1.5), z, t, idx, wt, 1.5)
+
+
+def test_rows_further_apart_than_32_bits(dev):
+    from objectdetection_amd import ops
+    for rows, V, ld in ((40, 21, 1 << 27), (40, 5003, 1 << 27), (3, 70001, 1 << 31)):
+        z, t, idx, wt = make(rows, dev, rows, V, 5, torch.bfloat16, torch.float32, True)
+        buf = torch.empty(((rows - 1) * ld + V,), dtype=torch.bfloat16, device=dev)
+        far = torch.as_strided(buf, (rows, V), (ld, 1))
+        far.copy_(z)
+        a, b = (ops.distill_loss(q, t, idx, weight=wt, temperature=2.0) for q in (far, z))
+        assert all(torch.equal(a[k], b[k]) for k in a)
+        g = torch.ones(rows, device=dev)
+        assert torch.equal(ops.distill_bwd(g, far, t, idx, a["lse"], wt, 2.0), ops.distill_bwd(g, z, t, idx, a["lse"], wt, 2.0))
+        del buf, far
+
+
+@pytest.mark.parametrize("V,k,labels", [(5000, 65, 30), (5000, 1024, 1), (5000, 1024, 5), (70000, 1024, 400), (300, 700, 300),
+                                        (1000, 130, 129), (40000, 1024, 1024)])
+def test_many_entries_with_the_same_labels(dev, V, k, labels):
+    """More than 64 entries: every label in the list once, a few times, or in all of it; the same bits each time."""
+    rng = np.random.default_rng(V + k + labels)
+    z, t, _, _ = make(V, dev, 5, V, k, torch.float32)
+    of = np.stack([rng.permutation(V)[:labels] for _ in range(5)])
+    idx = np.take_along_axis(of, rng.integers(0, labels, (5, k)) if labels < k else np.tile(rng.permutation(k), (5, 1)), 1)
+    idx[1, ::3] = -1
+    idx[2, 1:] = V
+    idx[3, :] = idx[3, 0]
+    idx = torch.from_numpy(idx).to(dev)
+    from objectdetection_amd import ops
+    got = ops.distill_loss(z, t, idx, temperature=1.5)
+    check(got, z, t, idx, None, 1.5)
+    g = torch.ones(5, device=dev)
+    d = ops.distill_bwd(g, z, t, idx, got["lse"], None, 1.5)
+    check({"d_logits": d}, z, t, idx, None, 1.5)
+    for _ in range(3):
+        assert torch.equal(ops.distill_loss(z, t, idx, temperature=1.5)["d_logits"], got["d_logits"])
+        assert torch.equal(ops.distill_bwd(g, z, t, idx, got["lse"], None, 1.5), d)

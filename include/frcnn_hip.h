@@ -421,8 +421,11 @@ int frcnn_fc1_fwd(const float* x, const float* w, const float* bias, int64_t M, 
  *              is FRCNN_ACT_NONE.  A bit left out asks for more than needed;
  *   bias, residual, pre may be NULL (pre: the pre-activations, rounded, which the backward needs
  *              for an activation other than FRCNN_ACT_NONE).
- * M = 0 is allowed (no forward output; d_w and d_bias become 0); M up to 2,147,483,647,
- * K and N up to 2,097,152 (a call of up to 32 rows: as memory allows).
+ * M = 0 is allowed (no forward output; d_w and d_bias become 0); M up to 1,073,741,760,
+ * K and N up to 2,097,152 (a call of up to 32 rows: as memory allows); what needs a launch of 2^32
+ * threads is refused (FRCNN_E_UNSUPPORTED).  Results overlap neither the inputs nor one another;
+ * only `out` may be the residual (the same type, rows and stride).  A workspace serves one call at
+ * a time: calls on two streams, or two captured graphs, have one each.
  * Activations: ReLU max(z, 0); GELU z Phi(z), Phi the normal distribution function (relative error
  * 1.3e-6); SiLU z / (1 + e^-z). */
 #define FRCNN_DT_F32   0

@@ -354,6 +354,7 @@ __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&a
 constexpr int DN_SK = 32, DN_RING = 4;
 __device__ const __attribute__((aligned(16))) uint32_t dn_zeros[4] = {0, 0, 0, 0};
 
+// (m0 is a reserved register: the compiler sets it before each use of its own)
 __device__ __forceinline__ void dn_dma(uint32_t lds, const void* base, uint32_t offset) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :: "s"(lds), "v"(offset), "s"(base) : "memory");
@@ -899,6 +900,9 @@ constexpr DnTile DN_TILES[] = {{256, 256, 0.69, 0.69, 0.69, 5.5, 1},
                                {128, 128, 0.215, 0.215, 0.26, 4.0, 2},
                                {64, 128, 0.18, 0.18, 0.22, 3.0, 3}};
 
+// a launch has fewer than 2^32 threads
+static bool dn_grid(long long blocks, int threads) { return blocks * threads < 1ll << 32; }
+
 // a product of few rows reads its operands as they are
 static bool dn_few(long long rows) { return rows <= DN_FEW; }
 
@@ -993,7 +997,7 @@ static int dn_launch_tiles(const DnGemm& g, unsigned blocks, hipStream_t stream)
 template <typename T, bool AKC, bool BKC>
 static int dn_launch_gemm(const DnPlan& pl, const DnGemm& g, hipStream_t stream) {
     if (pl.bi == 0) {
-        if (pl.tiles_j > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
+        if (!dn_grid(pl.tiles_j, 64 * DN_FW)) return FRCNN_E_UNSUPPORTED;
         if constexpr (AKC) {
             const dim3 grid((unsigned)pl.tiles_j, (unsigned)pl.splits);
             if (g.I <= 16) FRCNN_LAUNCH((dense_few_rows_kernel<T, BKC, 1>), grid, dim3(64 * DN_FW), 0, stream, g);
@@ -1002,7 +1006,7 @@ static int dn_launch_gemm(const DnPlan& pl, const DnGemm& g, hipStream_t stream)
         return FRCNN_OK;
     }
     const long long blocks = pl.tiles_i * pl.tiles_j * pl.splits;
-    if (blocks > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
+    if (!dn_grid(blocks, pl.bj == 256 ? 512 : 256)) return FRCNN_E_UNSUPPORTED;
     if (pl.bi == 256) return dn_launch_tiles<T, AKC, BKC, 256, 256, 2, 4>(g, (unsigned)blocks, stream);
     if (pl.bj == 256) return dn_launch_tiles<T, AKC, BKC, 128, 256, 2, 4>(g, (unsigned)blocks, stream);
     if (pl.bi == 128) return dn_launch_tiles<T, AKC, BKC, 128, 128, 2, 2>(g, (unsigned)blocks, stream);
@@ -1039,7 +1043,7 @@ static int dn_pack(DnMatrix* a, DnMatrix* b, char*& ws, DnPacks& packs) {
         *m = DnMatrix{packs.of[n].dst, m->rows, m->cols, packs.of[n].pieces * 8, true};
         ++n;
     }
-    return packs.blocks > 0x7FFFFFFFll ? FRCNN_E_UNSUPPORTED : FRCNN_OK;
+    return dn_grid(packs.blocks, 256) ? FRCNN_OK : FRCNN_E_UNSUPPORTED;
 }
 template <typename T>
 static int dn_launch_packs(const DnPacks& packs, hipStream_t stream) {
@@ -1054,7 +1058,7 @@ static int dn_product(const DnMatrix& a, bool akc, const DnMatrix& b, bool bkc, 
                       hipStream_t stream) {
     const long long I = akc ? a.rows : a.cols, K = akc ? a.cols : a.rows, J = bkc ? b.rows : b.cols;
     const DnPlan pl = dn_plan(I, J, K, akc, bkc);
-    if (pl.tiles_i > 0x7FFFFF || pl.tiles_j > 0x7FFFFF) return FRCNN_E_UNSUPPORTED;
+    if (pl.tiles_i > 0xFFFFFFF || pl.tiles_j > 0xFFFFFFF) return FRCNN_E_UNSUPPORTED;
     DnGemm g{};
     g.a = a.p; g.b = b.p; g.lda = a.ld; g.ldb = b.ld; g.I = I; g.J = J; g.K = K;
     g.outer_a = a.padded ? dn_pieces(I) * 8 : I;
@@ -1069,7 +1073,7 @@ static int dn_product(const DnMatrix& a, bool akc, const DnMatrix& b, bool bkc, 
     else rc = dn_launch_gemm<T, false, false>(pl, g, stream);
     if (rc != FRCNN_OK || pl.splits == 1) return rc;
     const long long groups = (I * ((J + 3) / 4) + 63) / 64;
-    if (groups > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
+    if (!dn_grid(groups, 64)) return FRCNN_E_UNSUPPORTED;
     FRCNN_LAUNCH(dense_join_kernel<T>, dim3((unsigned)groups), dim3(64), 0, stream, (const float*)g.partial, pl.splits,
                  I, J, e);
     return FRCNN_OK;
@@ -1117,14 +1121,14 @@ static DnBwdPlan dn_bwd_plan(long long M, int N, bool copy) {
 }
 
 static bool dn_sizes(int64_t M, int K, int N) { return M >= 0 && K > 0 && N > 0; }
-constexpr int64_t DN_MAX_ROWS = 0x7FFFFFFF;
+constexpr int64_t DN_MAX_ROWS = (1ll << 30) - 64;      // rows of 64 each: fewer than 2^24 workgroups of 256 threads
 static bool dn_16bit(int dtype) { return dtype == FRCNN_DT_F16 || dtype == FRCNN_DT_BF16; }
 static bool dn_even(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 template <typename T>
 static int dn_zero(void* p, long long rows, long long cols, long long ld, hipStream_t s) {
     const long long groups = (rows * cols + 255) / 256;
-    if (groups > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
+    if (!dn_grid(groups, 256)) return FRCNN_E_UNSUPPORTED;
     FRCNN_LAUNCH(dense_zero_kernel<T>, dim3((unsigned)groups), dim3(256), 0, s, (T*)p, rows, cols, ld);
     return FRCNN_OK;
 }
@@ -1168,7 +1172,7 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
         else q.sums = d_bias ? reinterpret_cast<float*>(ws + p.dz_bytes) : nullptr;
         q.blocks = p.blocks * ((dn_pieces(N) + p.cg - 1) / p.cg);
         const long long blocks = q.blocks + packs.blocks;
-        if (blocks > 0x7FFFFFFFll) return FRCNN_E_UNSUPPORTED;
+        if (!dn_grid(blocks, 256)) return FRCNN_E_UNSUPPORTED;
         if (d_dtype == FRCNN_DT_F32)
             FRCNN_LAUNCH((dense_dz_kernel<T, float>), dim3((unsigned)blocks), dim3(256), 0, s, q, packs);
         else

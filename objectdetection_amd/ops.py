@@ -707,6 +707,21 @@ def _scratch(ws: Optional[torch.Tensor], need: int, like: torch.Tensor, dev: int
     return ws.data_ptr(), ws.numel(), ws
 
 
+def _no_overlap(out, N, x, ldx, w, layout, ldw, bias, residual, ldr) -> None:
+    """`out` shares no memory with an input, or is the residual itself."""
+    a = out.data_ptr()
+    b = a + out.numel() * out.element_size()
+    same = residual is not None and residual.data_ptr() == a and residual.dtype == out.dtype and \
+        (ldr == N or residual.shape[0] <= 1)
+    for name, t, n, ld in (("x", x, x.shape[0], ldx), ("weight", w, w.shape[layout], ldw), ("bias", bias, 1, 0),
+                           ("residual", None if same else residual, x.shape[0], ldr)):
+        if t is None or t.numel() == 0:
+            continue
+        p = t.data_ptr()
+        if p < b and a < p + 2 * ((n - 1) * ld + t.numel() // n):
+            raise ValueError(f"out overlaps {name}")
+
+
 def dense_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
               act: str = "none", residual: Optional[torch.Tensor] = None,
               out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
@@ -716,7 +731,8 @@ def dense_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
     x [..., K] (the pooled tensor [B,R,ph,pw,C] is taken as [B,R,ph*pw*C]); weight [K,N], rows of N
     or the transposed view of a Linear weight [N,K] (both are read as they lie); bias [N]; residual
     [..., N].  act: "none", "relu", "gelu" (exact), "silu".  out_dtype float32 keeps the sums (class
-    logits).  Returns out [..., N], with want_pre (out, pre): the pre-activations dense_bwd needs.
+    logits).  out: contiguous, shares no memory with the inputs except that it may be the residual.
+    Returns out [..., N], with want_pre (out, pre): the pre-activations dense_bwd needs.
     workspace: uint8 of dense_fwd_workspace_bytes(M, K, N, ...), kept by callers that allocate nothing."""
     xx, ldx, lead, dev = _dense_x(x)
     M, K = xx.shape
@@ -747,6 +763,8 @@ def dense_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
         raise ValueError(f"out must be a contiguous {odt} tensor of shape {[*lead, N]}")
     elif out.get_device() != dev:
         raise _other_device(out, dev, "out")
+    else:
+        _no_overlap(out, N, xx, ldx, w, layout, ldw, bias, residual, ldr)
     pre = None
     if want_pre:
         pre = xx.new_empty((*lead, N))

@@ -139,3 +139,24 @@ def test_head_dtype_is_checked():
     m, n = FRCNModel(8, 7, 16, 21), FRCNModel(8, 7, 16, 21, dtype=torch.bfloat16)
     assert {k: v.shape for k, v in m.state_dict().items()} == {k: v.shape for k, v in n.state_dict().items()}
     assert all(v.dtype == torch.float32 for v in n.state_dict().values())
+
+
+def test_a_launch_has_fewer_than_2_32_threads(L):
+    assert fwd(L, M=(1 << 30) - 63) == L.E_UNSUPPORTED
+    far = dict(M=1 << 29, K=67, ldx=67, ws=ONE, wsb=1 << 62)   # 2^32 pieces would be copied
+    assert fwd(L, ldw=67, layout=1, **far) == L.E_UNSUPPORTED
+    assert bwd(L, ldw=67, layout=1, lddw=67, lddx=67, **far) == L.E_UNSUPPORTED
+    assert bwd(L, M=0, K=2097152, N=4096, ldd=4096, ldw=4096, lddx=2097152, lddw=4096) == L.E_UNSUPPORTED
+
+
+def test_kernels_keep_everything_in_registers():
+    """Nothing of the dense and distillation kernels waits in scratch memory, and eight waves of the
+    large tile fit on a compute unit (256 registers per lane)."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tools"))
+    from kernel_budgets import kernel_budgets
+    own = {n: k for n, k in kernel_budgets().items() if "dense_" in n or "distill_" in n}
+    assert len(own) > 60
+    for name, k in own.items():
+        assert k["scratch"] == 0 and k["vgpr"] <= (256 if k["wg_max"] <= 512 else 128), (name, k)

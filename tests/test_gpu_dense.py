@@ -366,3 +366,74 @@ def test_refusals(dev):
              ValueError)):
         with pytest.raises(err):
             bad()
+
+
+def test_the_output_may_be_the_residual_and_nothing_else(dev):
+    from objectdetection_amd import ops
+    rng = np.random.default_rng(15)
+    for M, K, N in ((5, 40, 13), (300, 136, 136), (3000, 64, 520), (60, 8200, 84)):
+        x, w, b, d = make(rng, dev, M, K, N, torch.bfloat16, "nk", True, True)
+        ref = ops.dense_fwd(x, w, b, "silu", residual=d)
+        assert ops.dense_fwd(x, w, b, "silu", residual=d, out=d) is d and torch.equal(d, ref)
+    x, w, b, d = make(rng, dev, 40, 40, 40, torch.bfloat16, "kn", True, True)
+    for bad in (x, w, w.t(), b):
+        out = torch.as_strided(bad, (40, 40), (40, 1), bad.storage_offset()) if bad is not b else None
+        if out is None:
+            store = torch.zeros(1600, dtype=torch.bfloat16, device=dev)
+            b, out = store[80:120], store.view(40, 40)
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.dense_fwd(x, w, b, out=out)
+    two = torch.zeros((41, 40), dtype=torch.bfloat16, device=dev)
+    with pytest.raises(ValueError, match="overlaps residual"):
+        ops.dense_fwd(x, w, b, residual=two[:40], out=two[1:])
+
+
+def test_rows_further_apart_than_32_bits(dev):
+    """Row strides of 2,097,152 elements: the last rows lie 4.3 GB behind the first."""
+    from objectdetection_amd import ops
+    rng = np.random.default_rng(16)
+    M, K, N, ld = 1030, 72, 40, 1 << 21
+    x, w, b, d = make(rng, dev, M, K, N, torch.bfloat16, "nk", True, True)
+    buf = torch.empty((M * ld,), dtype=torch.bfloat16, device=dev)
+    far = lambda at, n: torch.as_strided(buf, (M, n), (ld, 1), at)
+    far(0, K).copy_(x)
+    far(128, N).copy_(d)
+    for act in ("none", "gelu"):
+        out, pre = ops.dense_fwd(far(0, K), w, b, act, residual=far(128, N), want_pre=True)
+        ref = ops.dense_fwd(x, w, b, act, residual=d, want_pre=True)
+        assert torch.equal(out, ref[0]) and torch.equal(pre, ref[1])
+        g, h = ops.dense_bwd(far(128, N), far(0, K), w, pre, act), ops.dense_bwd(d, x, w, pre, act)
+        assert all(torch.equal(g[k], h[k]) for k in g)
+    # the few rows' kernel, a weight of rows as far apart
+    wide = torch.as_strided(buf, (K, M), (1, ld), 0)          # Linear weight [1030, 72]
+    assert torch.equal(ops.dense_fwd(x[:20], wide), ops.dense_fwd(x[:20], x.t()))
+
+
+def test_two_streams_at_once(dev):
+    """Calls of different sizes queued on two streams give what they give one after the other."""
+    from objectdetection_amd import ops
+    rng = np.random.default_rng(17)
+    cases = [make(rng, dev, *s, torch.bfloat16, "nk", True, True) for s in
+             ((700, 4096, 84), (130, 1003, 333), (4100, 72, 2056), (24, 2056, 136))]
+    z = torch.randn((70, 40000), device=dev)
+    t, i = torch.randn((70, 8), device=dev), torch.randint(0, 40000, (70, 8), device=dev)
+
+    def work(case):
+        x, w, b, d = case
+        out, pre = ops.dense_fwd(x, w, b, "gelu", want_pre=True)
+        g = ops.dense_bwd(d, x, w, pre, "gelu")
+        o = ops.distill_loss(z, t, i, temperature=2.0)
+        return [out, pre, *g.values(), *o.values()]
+
+    want = [work(c) for c in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for n, c in enumerate(cases):
+            with torch.cuda.stream(streams[n % 2]):
+                got.append((n, work(c)))
+    torch.cuda.synchronize()
+    for n, r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want[n])), n

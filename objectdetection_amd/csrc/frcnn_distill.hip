@@ -82,16 +82,35 @@ struct DsVec {
     }
 };
 
-__device__ __forceinline__ float ds_wave_max(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+// Over G neighbouring lanes, the same bits in each: within sixteen lanes the operand comes straight from a
+// neighbour's register (quads, then halves and rows mirrored: what is met there is the same in a quad, in
+// eight lanes), beyond by exchanging rows of sixteen and halves; with an LDS exchange per step
+// short rows wait for LDS (500,000 rows of 64 bf16 classes and entries: 826 us; 257 this way).
+template <int CTRL>
+__device__ __forceinline__ float ds_dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+template <bool MAX>
+__device__ __forceinline__ float ds_join(float a, float b) { return MAX ? fmaxf(a, b) : a + b; }
+template <int G, bool MAX>
+__device__ __forceinline__ float ds_lanes(float v) {
+    static_assert(G >= 8 && G <= 64);
+    v = ds_join<MAX>(v, ds_dpp<0xB1>(v));              // lanes 1 0 3 2
+    v = ds_join<MAX>(v, ds_dpp<0x4E>(v));              // lanes 2 3 0 1
+    v = ds_join<MAX>(v, ds_dpp<0x141>(v));             // eight mirrored
+    if constexpr (G >= 16) v = ds_join<MAX>(v, ds_dpp<0x140>(v));      // sixteen mirrored
+    if constexpr (G >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = ds_join<MAX>(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    if constexpr (G >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = ds_join<MAX>(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
     return v;
 }
-__device__ __forceinline__ float ds_wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
+__device__ __forceinline__ float ds_wave_max(float v) { return ds_lanes<64, true>(v); }
+__device__ __forceinline__ float ds_wave_sum(float v) { return ds_lanes<64, false>(v); }
 // over the workgroup, the same order for every thread; `sh` of BLOCK / 64 floats is used once per call
 template <int BLOCK, bool MAX>
 __device__ __forceinline__ float ds_block(float v, float* sh) {
@@ -272,6 +291,7 @@ __device__ __forceinline__ void ds_zero(T* grad, long long v0, long long v1, int
 // ---- rows of up to 64 classes and 64 entries: G lanes per row ------------------------------------------
 template <typename T, bool FORWARD, int G>
 __global__ void __launch_bounds__(256) distill_small_kernel(DsArgs a) {
+    __shared__ __attribute__((aligned(16))) float2 entry[256];        // label and p of a row's entries
     const int l = threadIdx.x & (G - 1), first = lane_id() & ~(G - 1);
     const long long row = (long long)blockIdx.x * (256 / G) + threadIdx.x / G;
     if (row >= a.rows) return;                         // whole groups of lanes leave
@@ -286,40 +306,31 @@ __global__ void __launch_bounds__(256) distill_small_kernel(DsArgs a) {
         t = ds_teacher_logit<T>(a, row * a.k + l) * inv_t;
         if (i >= 0 && i < a.V && !(t == ninf)) label = (int)i;
     }
-    float top = label >= 0 ? t : ninf, m = z;
-    int any = label >= 0;
-#pragma unroll
-    for (int d = G / 2; d; d >>= 1) {
-        top = fmaxf(top, __shfl_xor(top, d));
-        m = fmaxf(m, __shfl_xor(m, d));
-        any |= __shfl_xor(any, d);
-    }
+    const float top = ds_lanes<G, true>(label >= 0 ? t : ninf), m = ds_lanes<G, true>(z);
+    const bool any = (__ballot(label >= 0) >> first & (~0ull >> (64 - G))) != 0;
     const float te = label >= 0 ? __builtin_amdgcn_exp2f((t - top) * DS_LOG2E) : 0.f;
-    float ts = te, s = mine ? __builtin_amdgcn_exp2f((z - m) * (inv_t * DS_LOG2E)) : 0.f;
-#pragma unroll
-    for (int d = G / 2; d; d >>= 1) {
-        ts += __shfl_xor(ts, d);
-        s += __shfl_xor(s, d);
-    }
+    const float ts = ds_lanes<G, false>(te);
+    const float s = ds_lanes<G, false>(mine ? __builtin_amdgcn_exp2f((z - m) * (inv_t * DS_LOG2E)) : 0.f);
     const bool part = w != 0.f && any;
     const float log_sum = logf(ts), log_s = logf(s);
     const float log_p = t - top - log_sum, p = label >= 0 ? __builtin_amdgcn_exp2f(log_p * DS_LOG2E) : 0.f;
     const float zi = __shfl(z, first + (label >= 0 ? label : 0));
     if (FORWARD) {
-        float loss = label >= 0 && !(p == 0.f) ? p * (log_p - ((zi - m) * inv_t - log_s)) : 0.f;
-#pragma unroll
-        for (int d = G / 2; d; d >>= 1) loss += __shfl_xor(loss, d);
+        const float loss =
+            ds_lanes<G, false>(label >= 0 && !(p == 0.f) ? p * (log_p - ((zi - m) * inv_t - log_s)) : 0.f);
         if (l == 0) {
             a.loss[row] = part ? w * (a.temperature * a.temperature) * loss : 0.f;
             a.lse[row] = part ? m * inv_t + log_s : 0.f;
         }
         if (!a.grad) return;
     }
+    entry[threadIdx.x] = make_float2(__int_as_float(label), p);       // read by the same wave
+    __builtin_amdgcn_wave_barrier();
     float listed = 0.f;                                // the p of the entries that name this lane's class
-    for (int j = 0; j < a.k; ++j) {
-        const int i = __shfl(label, first + j);
-        const float pj = __shfl(p, first + j);
-        if (i == l) listed += pj;
+    for (int j = 0; j < a.k; j += 2) {
+        const float4 two = *reinterpret_cast<const float4*>(&entry[threadIdx.x - l + j]);
+        if (__float_as_int(two.x) == l) listed += two.y;
+        if (__float_as_int(two.z) == l) listed += two.w;
     }
     const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale);
     const float log_q = FORWARD ? (z - m) * inv_t - log_s : z * inv_t - a.lse_in[row];

@@ -19,7 +19,7 @@
 
 namespace frcnn {
 
-constexpr int DS_MAX_K = 1024;
+constexpr int DS_MAX_K = 1024, DS_SHORT_K = 64;
 constexpr float DS_LOG2E = 1.4426950408889634f;
 
 struct DsArgs {
@@ -205,16 +205,12 @@ __device__ __forceinline__ void ds_listed_sums(DsTeacher e, int k, float log_sum
         const int mine = lane < k ? e.label[lane] : -1;
         const float p = lane < k ? __builtin_amdgcn_exp2f((e.t[lane] - log_sum) * DS_LOG2E) : 0.f;
         float sum = 0.f;
-        bool first = mine >= 0;
         for (int n = 0; n < k; ++n) {
             const int other = __builtin_amdgcn_readlane(mine, n);
             const float q = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), n));
-            if (other == mine) {
-                sum += q;
-                if (n < lane) first = false;
-            }
+            sum += other == mine ? q : 0.f;
         }
-        if (lane < k) e.p[lane] = first ? sum : -1.0f;
+        if (lane < k) e.p[lane] = mine >= 0 ? sum : -1.0f;
         return;
     }
     const int tid = threadIdx.x, slots = ds_slots(k), shift = __builtin_clz(slots) + 1;
@@ -336,6 +332,129 @@ __global__ void __launch_bounds__(256) distill_small_kernel(DsArgs a) {
     const float log_q = FORWARD ? (z - m) * inv_t - log_s : z * inv_t - a.lse_in[row];
     if (mine)
         ((T*)a.grad)[row * a.ldg + l] = (T)(part ? c * (__builtin_amdgcn_exp2f(log_q * DS_LOG2E) - listed) : 0.f);
+}
+
+// ---- short rows with up to 64 entries: G lanes per row, NV pieces of 16 bytes per lane -------------------
+// What a row of 91 classes costs is latency: several rows per wave, its entries and weight loaded before anything
+// is decided, no barrier.  The piece that would end behind the row is the row's last 16 bytes instead: what it
+// shares with its neighbour is left out of the sums and stored twice with the same value.
+template <typename T, bool FORWARD, int G, int NV>
+__global__ void __launch_bounds__(256) distill_short_kernel(DsArgs a) {
+    constexpr int W = DsVec<T>::W, E = DS_SHORT_K / G;            // entries per lane
+    __shared__ __attribute__((aligned(16))) float2 entry[256 / G][DS_SHORT_K + 2];       // label and p
+    const int l = threadIdx.x & (G - 1), first = lane_id() & ~(G - 1), rl = threadIdx.x / G;
+    const long long row = (long long)blockIdx.x * (256 / G) + rl;
+    if (row >= a.rows) return;                         // whole groups of lanes leave
+    const float inv_t = 1.0f / a.temperature, ninf = -__builtin_inff(), f = inv_t * DS_LOG2E;
+    const float w = a.weight ? a.weight[row] : 1.0f;
+    const float up = a.d_loss ? a.d_loss[row] : a.scale, lse = FORWARD ? 0.f : a.lse_in[row];
+    const T* z = (const T*)a.z + row * a.ldz;
+    int label[E];
+    float t[E], zi[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        label[e] = -1;
+        t[e] = ninf;
+        zi[e] = 0.f;
+        if (G * e >= a.k) continue;
+        const int j = l + G * e, at = j < a.k ? j : a.k - 1;
+        const int64_t i = a.idx[row * a.k + at];
+        t[e] = ds_teacher_logit<T>(a, row * a.k + at) * inv_t;
+        if (j < a.k && i >= 0 && i < a.V && !(t[e] == ninf)) label[e] = (int)i;
+    }
+    DsVec<T> x[NV];
+    int from[NV], dup[NV];                             // the piece's place; how many of its values belong to others
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v = (l + G * i) * W;
+        from[i] = v + W <= a.V ? v : a.V - W;
+        dup[i] = v >= a.V ? W : v - from[i];
+        x[i].b = ds_u32x4{0, 0, 0, 0};
+        if (w != 0.f) x[i].load(z + from[i], W);
+    }
+    if (w != 0.f) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (label[e] >= 0) zi[e] = (float)z[label[e]];
+    }
+    float top = ninf, m = ninf;
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        any |= label[e] >= 0;
+        top = fmaxf(top, label[e] >= 0 ? t[e] : ninf);
+    }
+    top = ds_lanes<G, true>(top);
+    any = (__ballot(any) >> first & (~0ull >> (64 - G))) != 0;
+    auto value = [&](int i, int n) { return n < dup[i] ? ninf : x[i][n]; };
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int n = 0; n < W; ++n) m = fmaxf(m, value(i, n));
+    m = ds_lanes<G, true>(m);
+    float ts = 0.f, s = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ts += label[e] >= 0 ? __builtin_amdgcn_exp2f((t[e] - top) * DS_LOG2E) : 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int n = 0; n < W; ++n) s += __builtin_amdgcn_exp2f((value(i, n) - m) * f);
+    const float log_sum = logf(ds_lanes<G, false>(ts));
+    s = ds_lanes<G, false>(s);
+    const float log_s = logf(s);
+    const bool part = w != 0.f && any;
+    float p[E];
+    float loss = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float log_p = t[e] - top - log_sum;
+        p[e] = label[e] >= 0 ? __builtin_amdgcn_exp2f(log_p * DS_LOG2E) : 0.f;
+        if (label[e] >= 0 && !(p[e] == 0.f)) loss += p[e] * (log_p - ((zi[e] - m) * inv_t - log_s));
+    }
+    if (FORWARD) {
+        loss = ds_lanes<G, false>(loss);
+        if (l == 0) {
+            a.loss[row] = part ? w * (a.temperature * a.temperature) * loss : 0.f;
+            a.lse[row] = part ? m * inv_t + log_s : 0.f;
+        }
+        if (!a.grad) return;
+    }
+    T* grad = (T*)a.grad + row * a.ldg;
+    const float c = w * a.temperature * up, cq = FORWARD ? c / s : c;
+    auto relative = [&](float v) { return __builtin_amdgcn_exp2f(FORWARD ? (v - m) * f : (v * inv_t - lse) * DS_LOG2E); };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float q[W];
+#pragma unroll
+        for (int n = 0; n < W; ++n) q[n] = part ? cq * relative(x[i][n]) : 0.f;
+        x[i].set(q);
+        if (dup[i] < W) x[i].store(grad + from[i], W);
+    }
+    if (!part) return;                                 // whole groups of lanes
+    // entries of the same label add up the same values in the same order and store the same result, behind
+    // what the same wave stored above
+    float sum[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (G * e < a.k) entry[rl][l + G * e] = make_float2(__int_as_float(label[e]), p[e]);
+        sum[e] = 0.f;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    for (int j = 0; j < a.k; j += 2) {
+        const float4 two = *reinterpret_cast<const float4*>(&entry[rl][j]);
+        const int i0 = __float_as_int(two.x), i1 = __float_as_int(two.z);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (G * e >= a.k) continue;
+            sum[e] += i0 == label[e] ? two.y : 0.f;
+            sum[e] += i1 == label[e] ? two.w : 0.f;
+        }
+    }
+    const float scale = FORWARD ? 1.0f / s : 1.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (label[e] >= 0) grad[label[e]] = (T)(c * (relative(zi[e]) * scale - sum[e]));
 }
 
 // ---- a whole row in the registers of one workgroup: up to BLOCK * NV vectors ------------------------------
@@ -558,6 +677,8 @@ static int ds_group(int V, int k) {
     while (g < V || g < k) g *= 2;
     return g;
 }
+// rows of which a wave takes one or more
+static bool ds_short(int V, int k, int dtype) { return k <= DS_SHORT_K && ds_vectors(V, dtype) <= 512; }
 
 // rows r .. r + n - 1 of a call
 template <typename T>
@@ -582,6 +703,12 @@ static int ds_launch_small(const DsArgs& a, hipStream_t s) {
                  0, s, a);
     return FRCNN_OK;
 }
+template <typename T, bool FORWARD, int G, int NV>
+static int ds_launch_short(const DsArgs& a, hipStream_t s) {
+    FRCNN_LAUNCH((distill_short_kernel<T, FORWARD, G, NV>), dim3((unsigned)((a.rows + 256 / G - 1) / (256 / G))),
+                 dim3(256), 0, s, a);
+    return FRCNN_OK;
+}
 template <typename T, int BLOCK, int NV>
 static int ds_launch_row(const DsArgs& a, hipStream_t s) {
     FRCNN_LAUNCH((distill_row_kernel<T, BLOCK, NV>), dim3((unsigned)a.rows), dim3(BLOCK), ds_lds_bytes(a.k),
@@ -599,12 +726,22 @@ static int ds_launch_chunk(const DsArgs& a, hipStream_t s) {
 
 template <typename T, bool FORWARD>
 static int ds_run(const DsArgs& a, int dtype, hipStream_t s) {
-    const int g = ds_group(a.V, a.k);
-    if (g <= 8) return ds_launch_small<T, FORWARD, 8>(a, s);
-    if (g <= 16) return ds_launch_small<T, FORWARD, 16>(a, s);
-    if (g <= 32) return ds_launch_small<T, FORWARD, 32>(a, s);
-    if (g <= 64) return ds_launch_small<T, FORWARD, 64>(a, s);
     const long long n = ds_vectors(a.V, dtype);
+    if (ds_short(a.V, a.k, dtype)) {
+        // a value per lane up to 16 classes (300,000 x 12 f32 with 4 entries 23.7 us, 28.1 in pieces; 40 classes
+        // with 20 entries 112 us, 56 in pieces), and where a row is less than a piece
+        const int g = ds_group(a.V, a.k);
+        if (g <= 8) return ds_launch_small<T, FORWARD, 8>(a, s);
+        if (g <= 16) return ds_launch_small<T, FORWARD, 16>(a, s);
+        if (a.V < DsVec<T>::W)
+            return g <= 32 ? ds_launch_small<T, FORWARD, 32>(a, s) : ds_launch_small<T, FORWARD, 64>(a, s);
+        if (n <= 8) return ds_launch_short<T, FORWARD, 8, 1>(a, s);
+        if (n <= 16) return ds_launch_short<T, FORWARD, 16, 1>(a, s);
+        if (n <= 64) return ds_launch_short<T, FORWARD, 16, 4>(a, s);
+        if (n <= 128) return ds_launch_short<T, FORWARD, 32, 4>(a, s);
+        if (n <= 256) return ds_launch_short<T, FORWARD, 64, 4>(a, s);
+        return ds_launch_short<T, FORWARD, 64, 8>(a, s);
+    }
     if constexpr (FORWARD) {
         if (!a.part) {
             if (n <= 64) return ds_launch_row<T, 64, 1>(a, s);
@@ -630,7 +767,7 @@ static int ds_run(const DsArgs& a, int dtype, hipStream_t s) {
 // workgroups of up to 1,024 threads (fewer than 2^32 threads in a launch)
 template <bool FORWARD>
 static int ds_dispatch(DsArgs a, int dtype, hipStream_t s) {
-    const bool chunked = ds_group(a.V, a.k) > 64 && (!FORWARD || ds_split(a.rows, a.V, dtype));
+    const bool chunked = !ds_short(a.V, a.k, dtype) && (!FORWARD || ds_split(a.rows, a.V, dtype));
     if (!chunked) a.part = nullptr;
     a.nv = ds_chunk_vectors(a.rows, a.V, dtype);
     a.chunks = (int)ds_chunks(a.rows, a.V, dtype);
@@ -666,7 +803,7 @@ static int ds_check(const void* z, int64_t ldz, int dtype, const void* t, int t_
 using namespace frcnn;
 
 extern "C" size_t frcnn_distill_workspace_bytes(int64_t rows, int V, int k, int dtype) {
-    if (rows <= 0 || V <= 0 || k <= 0 || ds_group(V, k) <= 64 || !ds_split(rows, V, dtype)) return 0;
+    if (rows <= 0 || V <= 0 || k <= 0 || !ds_split(rows, V, dtype)) return 0;
     return (size_t)rows * (size_t)ds_chunks(rows, V, dtype) * sizeof(float2);
 }
 

@@ -297,3 +297,34 @@ def test_many_entries_with_the_same_labels(dev, V, k, labels):
     for _ in range(3):
         assert torch.equal(ops.distill_loss(z, t, idx, temperature=1.5)["d_logits"], got["d_logits"])
         assert torch.equal(ops.distill_bwd(g, z, t, idx, got["lse"], None, 1.5), d)
+
+
+@pytest.mark.parametrize("rows,V,k", [(9, 3, 40), (6, 1, 17), (70, 17, 17), (33, 21, 40), (5, 129, 64), (65, 511, 63), (3, 2049, 64),
+                                      (7, 4096, 20), (5, 1024, 1), (40, 92, 33), (3, 2048, 2), (17, 8, 31)])
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+def test_short_rows(dev, rows, V, k, name):
+    """Several rows per wave: row ends inside a piece, entries that do not fill their lanes, labels listed twice."""
+    from objectdetection_amd import ops
+    dt = TYPES[name]
+    for pad, tdt in ((False, None), (True, torch.float32)):
+        z, t, idx, wt = make(rows * V + k, dev, rows, V, k, dt, tdt, pad)
+        idx[:, k // 2:] = torch.where(idx[:, k // 2:] >= 0, idx[:, :k - k // 2], idx[:, k // 2:])
+        got = ops.distill_loss(z, t, idx, weight=wt, temperature=1.5)
+        check(got, z, t, idx, wt, 1.5)
+        g = torch.linspace(-1.5, 2.0, rows, device=dev)
+        check({"d_logits": ops.distill_bwd(g, z, t, idx, got["lse"], wt, 1.5)}, z, t, idx, wt, 1.5, g.double().cpu())
+
+
+def test_short_rows_write_nothing_behind_their_end(dev):
+    """A strided gradient: what lies between the rows keeps its bytes (the C entry takes the stride)."""
+    from objectdetection_amd import _lib
+    for V, k, ldg in ((21, 8, 24), (91, 8, 100), (9, 20, 9), (5, 20, 7), (1203, 32, 1210)):
+        z, t, idx, _ = make(V, dev, 37, V, k, torch.bfloat16, torch.float32)
+        buf = torch.full((37 * ldg + 64,), 7.0, dtype=torch.bfloat16, device=dev)
+        loss, lse = torch.empty(37, device=dev), torch.empty(37, device=dev)
+        s = torch.cuda.current_stream().cuda_stream
+        assert _lib.lib.frcnn_distill_loss(z.data_ptr(), V, _lib.DT_BF16, t.data_ptr(), _lib.DT_F32, idx.data_ptr(), None, 37, V, k, 2.0,
+                                           1.0, loss.data_ptr(), lse.data_ptr(), buf.data_ptr(), ldg, None, 0, s) == _lib.OK
+        rows = buf[:37 * ldg].view(37, ldg)
+        check(dict(loss=loss, lse=lse, d_logits=rows[:, :V]), z, t, idx, None, 2.0)
+        assert (rows[:, V:] == 7).all() and (buf[37 * ldg:] == 7).all()

@@ -415,14 +415,14 @@ int frcnn_fc1_fwd(const float* x, const float* w, const float* bias, int64_t M, 
  *   out_dtype  dtype or FRCNN_DT_F32;   d_dtype likewise for d_out;
  *   ld*        elements between rows, at least the row's length; any alignment is taken: an operand
  *              of a product whose rows are not whole 16-byte pieces starting on 16 bytes is copied
- *              to the workspace first (not for calls of up to 32 rows);
+ *              to the workspace first (not for W in calls of up to 32 rows);
  *   aligned    of the workspace sizes: bit 0 x, bit 1 W starts on 16 bytes with a row stride of a
  *              multiple of 8 up to 2,097,152; bit 2 (backward) d_out does, is of type dtype and act
  *              is FRCNN_ACT_NONE.  A bit left out asks for more than needed;
  *   bias, residual, pre may be NULL (pre: the pre-activations, rounded, which the backward needs
  *              for an activation other than FRCNN_ACT_NONE).
  * M = 0 is allowed (no forward output; d_w and d_bias become 0); M up to 1,073,741,760,
- * K and N up to 2,097,152 (a call of up to 32 rows: as memory allows); what needs a launch of 2^32
+ * K and N up to 2,097,152 (a forward of up to 32 rows: as memory allows); what needs a launch of 2^32
  * threads is refused (FRCNN_E_UNSUPPORTED).  Results overlap neither the inputs nor one another;
  * only `out` may be the residual (the same type, rows and stride).  A workspace serves one call at
  * a time: calls on two streams, or two captured graphs, have one each.

@@ -347,10 +347,13 @@ __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&a
 // while the fragments of step s, already in registers, are multiplied, those of step s + 1 are read from
 // LDS and later ones are in flight.  An outer-contiguous operand is copied a step at a time into a ring of
 // four, at step s that of s + 4; a k-contiguous one two steps at a time (64 k: whole 128-byte lines, copies
-// of half lines took L2 twice the requests: 1,282 -> TFLOP/s) into a ring of two, at every odd s those of
+// of half lines took L2 twice the requests: 1,282 TFLOP/s at 8,192 cubed, 1,444 this way) into a ring of two, at every odd s those of
 // s + 3 and s + 4.  A handover says that the copies step s + 1 needs have arrived (the newer ones stay in
 // flight) and that every wave has read step s, whose place is then filled again.  Rows outside the
 // operand repeat its last row (their results are not stored); k outside reads a page of zeros.
+// What bounds it: the clock (1.83 GHz under this load) and the matrix cores, busy 75 % of its cycles.  8,192 cubed
+// in bf16: 1,450 TFLOP/s with W as [N,K], 1,550 as Keras kernel and for d_weight.  A ring of eight for small products
+// costs 1.2 us more to fill than it saves.
 constexpr int DN_SK = 32, DN_RING = 4;
 __device__ const __attribute__((aligned(16))) uint32_t dn_zeros[4] = {0, 0, 0, 0};
 
@@ -590,20 +593,25 @@ dense_gemm_kernel(DnGemm p, int tiles) {
 // Up to 32 rows (I): the product reads B once and little else, so what counts is how soon and how wide the
 // loads of B leave.  A workgroup owns 16 (k contiguous) or 32 (outer contiguous) columns and its eight waves
 // share out the reduction in pieces of 64 k: a wave's load covers whole 128-byte lines of 16 rows of B, or
-// 64-byte pieces of 16 k, and the next piece is loaded while the present one is multiplied.  A fragment of A
-// comes straight from memory (every workgroup reads the same few rows: L2).  An outer-contiguous piece is
-// turned round by the transposing LDS read in the wave's own LDS.  The eight sums are added in wave order.
-// The MFMA's k order is free as long as both operands agree: lane group g takes k 16 g .. 16 g + 15 of a
-// piece in two instructions (k contiguous), or 8 g .. 8 g + 7 of each half.
-constexpr int DN_FEW = 32, DN_FW = 8;           // most rows; waves
+// 64-byte pieces of 16 k (neighbouring workgroups on the same XCD share the lines), and three pieces are on their
+// way while one is multiplied.  A fragment of A comes straight from memory (every workgroup reads the same few
+// rows: L2).  An outer-contiguous piece is turned round by the transposing LDS read in the wave's own LDS.
+// The eight sums are added in wave order.  The MFMA's k order is free as long as both operands agree: lane
+// group g takes k 16 g .. 16 g + 15 of a piece in two instructions (k contiguous), or 8 g .. 8 g + 7 of each half.
+// One row x 4,096 x 4,096 bf16, W as [N,K]: 8.6 us, 3.9 TB/s; Keras kernel of 4,096 x 84: 9 us.
+constexpr int DN_FEW = 32, DN_FW = 8, DN_FS = 3;   // most rows; waves; pieces on their way
 
 template <typename T, bool BKC, int MB>
 __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
     constexpr int JB = BKC ? 1 : 2, NL = BKC ? 2 : 4;             // 16-column blocks; loads of B per piece and lane
     __shared__ dn_f32x4 sums[DN_FW][JB * MB][64];
     __shared__ dn_s16x8 turn[BKC ? 1 : DN_FW][BKC ? 1 : 256];     // [64 k][4 pieces of 8 columns] per wave
-    const int lane = lane_id(), wave = wave_id(), g = lane >> 4, l = lane & 15;
-    const long long j0 = (long long)blockIdx.x * (16 * JB);
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), g = lane >> 4, l = lane & 15;
+    // the last columns are the row's last ones: what they share with their neighbour is not stored
+    const unsigned xcd = blockIdx.x & 7, per = gridDim.x >> 3, rest = gridDim.x & 7;
+    const long long jw = (long long)(!BKC && gridDim.x >= 128 ? xcd * per + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3)
+                                                              : blockIdx.x) * (16 * JB);
+    const long long j0 = !BKC && jw > p.J - 32 && p.J >= 32 ? p.J - 32 : jw;
     const int slice = blockIdx.y;
     const long long k0 = slice * p.k_slice, k_end = k0 + p.k_slice < p.K ? k0 + p.k_slice : p.K;
     const T* A = (const T*)p.a;
@@ -618,22 +626,21 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
     const bool inner = BKC || j0 + 16 * JB <= p.J;                // whole pieces in every lane
     const int jv = (int)(p.J - j0 - 8 * (lane & 3) < 8 ? p.J - j0 - 8 * (lane & 3) : 8);
 
-    dn_s16x8 b[NL], a[MB][2], nb[NL], na[MB][2];
+    dn_s16x8 b[DN_FS][NL], a[DN_FS][MB][2];
     auto load = [&](long long k, dn_s16x8 (&rb)[NL], dn_s16x8 (&ra)[MB][2]) {
-        if (k + 64 <= k_end && inner) {                // no guard at all: the loads leave back to back
 #pragma unroll
-            for (int h = 0; h < NL; ++h) {
-                const T* q = BKC ? B + jl * p.ldb + k + 16 * g + 8 * h
-                                 : B + (k + 16 * h + (lane >> 2)) * p.ldb + j0 + 8 * (lane & 3);
-                __builtin_memcpy(&rb[h], q, 16);
-            }
-#pragma unroll
-            for (int m = 0; m < MB; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    __builtin_memcpy(&ra[m][h], rows[m] + k + (BKC ? 16 * g + 8 * h : 32 * h + 8 * g), 16);
-            return;
+        for (int h = 0; h < NL; ++h) {
+            const T* q = BKC ? B + jl * p.ldb + k + 16 * g + 8 * h
+                             : B + (k + 16 * h + (lane >> 2)) * p.ldb + j0 + 8 * (lane & 3);
+            __builtin_memcpy(&rb[h], q, 16);
         }
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                __builtin_memcpy(&ra[m][h], rows[m] + k + (BKC ? 16 * g + 8 * h : 32 * h + 8 * g), 16);
+    };
+    auto load_some = [&](long long k, dn_s16x8 (&rb)[NL], dn_s16x8 (&ra)[MB][2]) {
         auto at = [&](const T* q, long long kk) {
             const long long left = k_end - kk;
             return dn_load8(q + kk, left > 8 ? 8 : (int)left);
@@ -687,20 +694,36 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
                 }
         }
     };
+    constexpr long long STEP = 64 * DN_FW;
     long long k = k0 + 64 * wave;
-    if (k < k_end) load(k, b, a);
+    const int n = inner && k + 64 <= k_end ? (int)((k_end - k - 64) / STEP) + 1 : 0;     // whole pieces
+#pragma unroll
+    for (int u = 0; u < DN_FS; ++u)
+        if (u < n) load(k + u * STEP, b[u], a[u]);
+    int s = 0;
 #pragma unroll 1
-    while (k < k_end) {
-        const long long next = k + 64 * DN_FW;
-        if (next < k_end) load(next, nb, na);
-        multiply(b, a);
+    for (; s + 2 * DN_FS <= n; s += DN_FS) {
 #pragma unroll
-        for (int h = 0; h < NL; ++h) b[h] = nb[h];
+        for (int u = 0; u < DN_FS; ++u) {
+            multiply(b[u], a[u]);
+            load(k + DN_FS * STEP, b[u], a[u]);
+            k += STEP;
+        }
+    }
+#pragma unroll 1
+    for (; s < n; s += DN_FS) {
 #pragma unroll
-        for (int m = 0; m < MB; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) a[m][h] = na[m][h];
-        k = next;
+        for (int u = 0; u < DN_FS; ++u)
+            if (s + u < n) {
+                multiply(b[u], a[u]);
+                if (s + u + DN_FS < n) load(k + DN_FS * STEP, b[u], a[u]);
+                k += STEP;
+            }
+    }
+#pragma unroll 1
+    for (; k < k_end; k += STEP) {                     // a piece that is cut short, columns of a narrow B
+        load_some(k, b[0], a[0]);
+        multiply(b[0], a[0]);
     }
 #pragma unroll
     for (int j = 0; j < JB; ++j)
@@ -716,13 +739,19 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
         for (int r = 0; r < 4; ++r) v[r] += o[r];
     }
     const long long i = 16 * (wave % MB) + l, j = j0 + 16 * (wave / MB) + 4 * g, left = p.J - j;
-    if (i >= p.I || left <= 0) return;
+    if (i >= p.I || left <= 0 || j + 4 <= jw) return;
+    float o[4] = {v[0], v[1], v[2], v[3]};
     if (p.partial) {
-        const long long Jp = (p.J + 3) / 4 * 4;
-        *reinterpret_cast<dn_f32x4*>(p.partial + (slice * p.I + i) * Jp + j) = v;
-    } else {
-        float o[4] = {v[0], v[1], v[2], v[3]};
+        float* to = p.partial + (slice * p.I + i) * ((p.J + 3) / 4 * 4) + j;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (j + r >= jw && r < left) to[r] = o[r];
+    } else if (j >= jw) {
         dn_epilogue<T, 4>(p.e, i, j, left > 4 ? 4 : (int)left, o);
+    } else {                                           // the first of them belong to the neighbour
+#pragma unroll
+        for (int r = 1; r < 4; ++r)
+            if (j + r >= jw) dn_epilogue<T, 1>(p.e, i, j + r, 1, &o[r]);
     }
 }
 
@@ -731,7 +760,8 @@ __device__ __forceinline__ long long dn_divide(long long a, long long b) {
     return a < 0x80000000ll && b < 0x80000000ll ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
-// sums of a split product's slices, in slice order, and the epilogue; four outputs per thread
+// sums of a split product's slices, in slice order, and the epilogue; four outputs per thread.  Bound by the
+// partial sums' way from memory: sixteen slices of 128 x 4,096 (33.5 MB) 8.2 us, two of 2,000 x 4,096 13.7 us (4.8 TB/s)
 template <typename T>
 __global__ void __launch_bounds__(64)
 dense_join_kernel(const float* __restrict__ partial, int splits, long long I, long long J, DnEpilogue e) {
@@ -761,7 +791,7 @@ dense_join_kernel(const float* __restrict__ partial, int splits, long long I, lo
 
 // ---- operands whose rows are not whole 16-byte pieces --------------------------------------------------
 // are copied once to rows that are, with zeros behind their end: a piece per thread, in one launch for all
-// of a call's operands
+// of a call's operands (777 x 1,003 and 1,003 x 531 f16: 4.6 us, latency; 25,088 x 4,099: 68 us, 6 TB/s)
 struct DnPack { const void* src; void* dst; long long rows, cols, ld, pieces; };   // pieces of 8 per row of dst
 struct DnPacks { DnPack of[2]; long long blocks_first, blocks; };                  // workgroups of 256 pieces
 
@@ -784,7 +814,8 @@ __global__ void __launch_bounds__(256) dense_pack_kernel(DnPacks packs) {
 // A workgroup takes `rows` rows of 8 * cg columns; a thread 8 neighbouring columns of every (256 / cg)-th
 // row.  dz (may be null) has rows of ldz elements, a multiple of 8; its columns N .. ldz-1 become 0.  The
 // sums of the unrounded values go to d_bias where one workgroup has all rows, else to `sums`, a row per
-// block of rows.  The workgroups behind the first `blocks` pack the products' operands.
+// block of rows.  The workgroups behind the first `blocks` pack the products' operands.  16,000 x 84 bf16: 7 us;
+// 1,111 x 333 f16 with SiLU, packing 779 x 333 and 1,111 x 779: 8.5 us (latency both)
 struct DnDz {
     const void *d_out, *pre;
     void *dz, *d_bias;
@@ -852,7 +883,7 @@ __global__ void __launch_bounds__(256) dense_dz_kernel(DnDz p, DnPacks packs) {
 }
 
 // column sums of `blocks` rows of float32 partial sums: 16 columns per workgroup, 64 threads each, four
-// rows on their way per thread
+// rows on their way per thread (16,000 rows of 84: 4 us)
 template <typename T>
 __global__ void __launch_bounds__(1024)
 dense_bias_grad_kernel(const float* __restrict__ sums, int blocks, int N, T* __restrict__ d_bias) {
@@ -888,28 +919,36 @@ struct DnPlan { int bi, bj, splits; long long k_slice, tiles_i, tiles_j; size_t 
 
 // Workgroup tiles: what a step of 32 k takes in us on a compute unit that is full of such workgroups (with
 // W as [N,K], both operands k-contiguous: step_kc), and for one alone; the rest of a workgroup (start, first
-// copies, results) and how many are resident.  Measured with every tile and split on products from 300 x 512 x
-// 512 to 16,000 x 25,088 x 4,096; what follows takes the pair with the shortest sum: rounds over the chip, at
-// least the operands' bytes at 4.6 TB/s and what tiles copy again at 20 TB/s (all compute units), plus the
-// join of a split.  Large products want the large tile (1.45 PFLOP/s; 1.2 from 128 x 128), 2,000 x 25,088 x
-// 4,096 two slices of it (295 us; 391 from 128 x 128 unsplit), 128 x 25,088 x 4,096 eight slices of 128 x 128
-// (51 us; 67 from four of 64 x 128), 1,024 cubed the small one (10.5 us; 15.6 from 128 x 256).
+// copies, results) and how many are resident.  What follows takes the pair of tile and split with the shortest
+// sum: rounds over the chip, or what the operands take at 3.81 TB/s and what tiles copy again at 25.2 TB/s (all
+// compute units) if that is longer, plus 0.3 of the latter, plus the join of a split.  The constants are fitted to
+// 132 products from 40 x 1,024 x 1,024 to 25,088 x 4,096 x 2,000, each measured with every tile and split: what is
+// taken is 2.1 % slower than the best of them in the mean.  4,000 x 4,096 x 4,096 wants the large tile (103 us; 119
+// and 130 from the next two), 2,000 x 25,088 x 4,096 two slices of it (307; 330 from 128 x 256 unsplit), 128 x 25,088
+// x 4,096 eight slices of 128 x 128 (53.5; 55.9 from sixteen of 128 x 256), 16,000 x 4,096 x 24 three of them (33;
+// 44.7 from 256 x 256), 1,024 cubed the small tile (10.7; 13.1).
 struct DnTile { int bi, bj; double step, step_kc, alone, fixed; int resident; };
-constexpr DnTile DN_TILES[] = {{256, 256, 0.69, 0.69, 0.69, 5.5, 1},
-                               {128, 256, 0.374, 0.50, 0.374, 5.0, 1},
-                               {128, 128, 0.215, 0.215, 0.26, 4.0, 2},
-                               {64, 128, 0.18, 0.18, 0.22, 3.0, 3}};
+constexpr DnTile DN_TILES[] = {{256, 256, 0.70, 0.69, 0.69, 6.8, 1},
+                               {128, 256, 0.388, 0.459, 0.374, 4.9, 1},
+                               {128, 128, 0.236, 0.307, 0.27, 4.3, 2},
+                               {64, 128, 0.18, 0.153, 0.22, 3.0, 3}};
 
+constexpr long long DN_MAX_LD = 1ll << 21;             // a tile's rows lie within 2 GiB of each other
 // a launch has fewer than 2^32 threads
 static bool dn_grid(long long blocks, int threads) { return blocks * threads < 1ll << 32; }
 
-// a product of few rows reads its operands as they are
-static bool dn_few(long long rows) { return rows <= DN_FEW; }
+// Whether a product of I rows reads its operands as they are.  Large weights of whole pieces are left to the
+// tiles: the few rows' kernel reads half lines of an outer-contiguous B (1 x 4,096 x 4,096 as Keras kernel 17.4 us,
+// 13.0 by tiles; 1 x 25,088 x 4,096 59 and 42; 1 x 1,024 x 1,024 4.7 and 7.7), and A again for every 16 columns
+// (W as [N,K], 32 x 25,088 x 4,096: 86 us, 60 by tiles; 16 x 4,096 x 4,096: 11.8 and 15.7).
+static bool dn_few(long long I, long long J, long long K, bool bkc, bool whole_b) {
+    return I <= DN_FEW && !(whole_b && K <= DN_MAX_LD && (bkc ? I : 1) * J * K >= (bkc ? 1ll << 30 : 1ll << 23));
+}
 
 // akc: A is k-contiguous (the forward and d_x); only those products have few rows
-static DnPlan dn_plan(long long I, long long J, long long K, bool akc, bool bkc) {
+static DnPlan dn_plan(long long I, long long J, long long K, bool akc, bool bkc, bool few) {
     DnPlan p{};
-    if (akc && dn_few(I)) {
+    if (akc && few) {
         // one workgroup per 16 or 32 columns; a long reduction is split where that leaves compute units idle
         p.bi = 0;
         p.bj = bkc ? 16 : 32;
@@ -941,12 +980,11 @@ static DnPlan dn_plan(long long I, long long J, long long K, bool akc, bool bkc)
             // (rows outside the operand repeat one row: counted half)
             const double copied = groups * per * ((I < t.bi ? (I + t.bi) / 2 : t.bi) +
                                                   (J < t.bj ? (J + t.bj) / 2 : t.bj)) * (2.0 * DN_SK);
-            const double stream = (bytes / 4.6e6 + (copied > bytes ? copied - bytes : 0.0) / 2.0e7) *
+            const double stream = (bytes / 3.81e6 + (copied > bytes ? copied - bytes : 0.0) / 2.52e7) *
                                   (groups < DN_CUS ? DN_CUS / groups : 1.0);
-            if (us < stream) us = stream;
-            if (splits > 1) us += 3.0 + 0.3 * splits + (double)splits * I * J * 8.0 / 1.0e7;
-            // in doubt the larger tile and fewer slices
-            if (p.bi && us > 0.97 * best) continue;
+            us = (us < stream ? stream : us) + 0.3 * stream;
+            if (splits > 1) us += 2.35 + 0.35 * splits + (double)splits * I * J * 8.0 / 9.1e6;
+            if (p.bi && us > best) continue;
             best = us;
             p.bi = t.bi; p.bj = t.bj;
             p.tiles_i = ti; p.tiles_j = tj;
@@ -1017,7 +1055,6 @@ static size_t dn_up(size_t b) { return (b + 255) / 256 * 256; }
 
 // A matrix in memory as rows of `cols` values.  padded: its rows are whole pieces with zeros behind `cols`.
 struct DnMatrix { const void* p; long long rows, cols, ld; bool padded; };
-constexpr long long DN_MAX_LD = 1ll << 21;             // a tile's rows lie within 2 GiB of each other
 static long long dn_pieces(long long n) { return (n + 7) / 8; }
 // rows that start on 16 bytes, of whole 16-byte pieces
 static bool dn_whole(const DnMatrix& m) {
@@ -1054,10 +1091,10 @@ static int dn_launch_packs(const DnPacks& packs, hipStream_t stream) {
 // D = A B^T: `a` holds A as [I][K] (akc) or [K][I], `b` B as [J][K] (bkc) or [K][J], packed where they have
 // to be; the workspace holds the partial sums of a split reduction
 template <typename T>
-static int dn_product(const DnMatrix& a, bool akc, const DnMatrix& b, bool bkc, const DnEpilogue& e, void* ws,
-                      hipStream_t stream) {
+static int dn_product(const DnMatrix& a, bool akc, const DnMatrix& b, bool bkc, bool few, const DnEpilogue& e,
+                      void* ws, hipStream_t stream) {
     const long long I = akc ? a.rows : a.cols, K = akc ? a.cols : a.rows, J = bkc ? b.rows : b.cols;
-    const DnPlan pl = dn_plan(I, J, K, akc, bkc);
+    const DnPlan pl = dn_plan(I, J, K, akc, bkc, few);
     if (pl.tiles_i > 0xFFFFFFF || pl.tiles_j > 0xFFFFFFF) return FRCNN_E_UNSUPPORTED;
     DnGemm g{};
     g.a = a.p; g.b = b.p; g.lda = a.ld; g.ldb = b.ld; g.I = I; g.J = J; g.K = K;
@@ -1085,8 +1122,8 @@ enum DnRows { DN_ANY, DN_ALIGNED, DN_PADDED };
 static size_t dn_copy_bytes(long long rows, long long cols, DnRows r) {
     return r == DN_PADDED || (r == DN_ALIGNED && cols % 8 == 0) ? 0 : dn_pack_bytes(rows, cols);
 }
-static size_t dn_partial_bytes(long long I, long long J, long long K, bool akc, bool bkc) {
-    return dn_up(dn_plan(I, J, K, akc, bkc).partial_bytes);
+static size_t dn_partial_bytes(long long I, long long J, long long K, bool akc, bool bkc, bool few) {
+    return dn_up(dn_plan(I, J, K, akc, bkc, few).partial_bytes);
 }
 
 // the backward's workspace: dz, its column sums, then what one product at a time needs
@@ -1135,13 +1172,14 @@ static int dn_zero(void* p, long long rows, long long cols, long long ld, hipStr
 
 template <typename T>
 static int dn_forward(DnMatrix x, DnMatrix w, bool bkc, const DnEpilogue& e, char* ws, hipStream_t s) {
-    if (!dn_few(x.rows)) {
+    const bool few = dn_few(x.rows, bkc ? w.rows : w.cols, x.cols, bkc, dn_whole(w));
+    if (!few) {
         DnPacks packs;
         int rc = dn_pack(&x, &w, ws, packs);
         if (rc == FRCNN_OK) rc = dn_launch_packs<T>(packs, s);
         if (rc != FRCNN_OK) return rc;
     }
-    return dn_product<T>(x, true, w, bkc, e, ws, s);
+    return dn_product<T>(x, true, w, bkc, few, e, ws, s);
 }
 
 template <typename T>
@@ -1161,8 +1199,9 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
     char* rest = ws + p.dz_bytes + p.sum_bytes;
     const DnMatrix z = dz ? DnMatrix{dz, M, N, p.ldz, true} : DnMatrix{d_out, M, N, ldd, false};
     DnMatrix mx{x, M, K, ldx, false}, mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
+    const bool few = dn_few(M, K, N, kn, dn_whole(mw));
     DnPacks packs;
-    rc = dn_pack(d_x && !dn_few(M) ? &mw : nullptr, d_w ? &mx : nullptr, rest, packs);
+    rc = dn_pack(d_x && !few ? &mw : nullptr, d_w ? &mx : nullptr, rest, packs);
     if (rc != FRCNN_OK) return rc;
     if (d_bias || dz) {
         DnDz q{};
@@ -1187,12 +1226,12 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
     DnEpilogue e{};
     if (d_x) {
         e.out = d_x; e.ldo = lddx;
-        rc = dn_product<T>(z, true, mw, kn, e, rest, s);
+        rc = dn_product<T>(z, true, mw, kn, few, e, rest, s);
         if (rc != FRCNN_OK) return rc;
     }
     if (d_w) {
         e.out = d_w; e.ldo = lddw;
-        rc = kn ? dn_product<T>(mx, false, z, false, e, rest, s) : dn_product<T>(z, false, mx, false, e, rest, s);
+        rc = kn ? dn_product<T>(mx, false, z, false, false, e, rest, s) : dn_product<T>(z, false, mx, false, false, e, rest, s);
     }
     return rc;
 }
@@ -1201,13 +1240,21 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
 
 using namespace frcnn;
 
-extern "C" size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
-    if (!dn_sizes(M, K, N) || M == 0 || M > DN_MAX_ROWS) return 0;
+// the largest need of a call whose operands are as aligned as said, or more
+static size_t dn_fwd_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
     const DnRows x = aligned & 1 ? DN_ALIGNED : DN_ANY, w = aligned & 2 ? DN_ALIGNED : DN_ANY;
     const bool kn = w_layout == FRCNN_W_KN;
-    const size_t partial = dn_partial_bytes(M, N, K, true, !kn);
-    if (dn_few(M)) return partial;
-    return dn_copy_bytes(M, K, x) + (kn ? dn_copy_bytes(K, N, w) : dn_copy_bytes(N, K, w)) + partial;
+    const size_t copy_w = kn ? dn_copy_bytes(K, N, w) : dn_copy_bytes(N, K, w);
+    const bool few = dn_few(M, N, K, !kn, copy_w == 0), few_whole = dn_few(M, N, K, !kn, true);
+    size_t need = dn_partial_bytes(M, N, K, true, !kn, few) + (few ? 0 : dn_copy_bytes(M, K, x) + copy_w);
+    if (few != few_whole) {                            // W may be whole after all
+        const size_t other = dn_partial_bytes(M, N, K, true, !kn, few_whole) + dn_copy_bytes(M, K, x);
+        if (need < other) need = other;
+    }
+    return need;
+}
+extern "C" size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
+    return !dn_sizes(M, K, N) || M == 0 || M > DN_MAX_ROWS ? 0 : dn_fwd_bytes(M, K, N, w_layout, aligned);
 }
 
 static int dn_aligned(const void* x, int64_t ldx, const void* w, int64_t ldw) {
@@ -1246,10 +1293,15 @@ extern "C" size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N, int w
     const DnBwdPlan p = dn_bwd_plan(M, N, !(aligned & 4) || N % 8 != 0);
     const bool kn = w_layout == FRCNN_W_KN;
     const DnRows x = aligned & 1 ? DN_ALIGNED : DN_ANY, w = aligned & 2 ? DN_ALIGNED : DN_ANY;
-    const size_t dx = dn_partial_bytes(M, K, N, true, kn);
-    const size_t dw = kn ? dn_partial_bytes(K, N, M, false, false) : dn_partial_bytes(N, K, M, false, false);
-    const size_t packed = dn_copy_bytes(M, K, x) + (dn_few(M) ? 0 : kn ? dn_copy_bytes(K, N, w) : dn_copy_bytes(N, K, w));
-    return p.dz_bytes + p.sum_bytes + packed + (dx > dw ? dx : dw);
+    const size_t copy_w = kn ? dn_copy_bytes(K, N, w) : dn_copy_bytes(N, K, w);
+    const bool few = dn_few(M, K, N, kn, copy_w == 0), few_whole = dn_few(M, K, N, kn, true);
+    size_t dx = dn_partial_bytes(M, K, N, true, kn, few);
+    if (few != few_whole) {                            // W may be whole after all
+        const size_t other = dn_partial_bytes(M, K, N, true, kn, few_whole);
+        if (dx < other) dx = other;
+    }
+    const size_t dw = kn ? dn_partial_bytes(K, N, M, false, false, false) : dn_partial_bytes(N, K, M, false, false, false);
+    return p.dz_bytes + p.sum_bytes + dn_copy_bytes(M, K, x) + (few ? 0 : copy_w) + (dx > dw ? dx : dw);
 }
 
 extern "C" int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, const void* x, int64_t ldx, const void* w,

@@ -770,7 +770,7 @@ def dense_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
         pre = xx.new_empty((*lead, N))
         pp = pre.data_ptr()
     px, pw = xx.data_ptr(), w.data_ptr()
-    aligned = 3 if M <= 32 else _aligned(px, ldx) + 2 * _aligned(pw, ldw)
+    aligned = _aligned(px, ldx) + 2 * _aligned(pw, ldw)
     pws, nws, ws = _scratch(workspace, dense_fwd_workspace_bytes(M, K, N, layout, aligned), xx, dev)
     _call("frcnn_dense_fwd", lib.frcnn_dense_fwd, dev, (
         px, ldx, pw, ldw, layout, pb, pr, ldr, M, K, N, _DT[dt], code, out.data_ptr(), N,

@@ -371,7 +371,7 @@ def test_refusals(dev):
 def test_the_output_may_be_the_residual_and_nothing_else(dev):
     from objectdetection_amd import ops
     rng = np.random.default_rng(15)
-    for M, K, N in ((5, 40, 13), (300, 136, 136), (3000, 64, 520), (60, 8200, 84)):
+    for M, K, N in ((5, 40, 13), (5, 40, 45), (20, 9000, 47), (300, 136, 136), (3000, 64, 520), (60, 8200, 84)):
         x, w, b, d = make(rng, dev, M, K, N, torch.bfloat16, "nk", True, True)
         ref = ops.dense_fwd(x, w, b, "silu", residual=d)
         assert ops.dense_fwd(x, w, b, "silu", residual=d, out=d) is d and torch.equal(d, ref)
@@ -437,3 +437,21 @@ def test_two_streams_at_once(dev):
     torch.cuda.synchronize()
     for n, r in got:
         assert all(torch.equal(a, b) for a, b in zip(r, want[n])), n
+
+
+@pytest.mark.parametrize("M,K,N", [(3, 4104, 2056), (17, 4104, 2056), (32, 8200, 4104)])
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+def test_few_rows_of_large_weights(dev, M, K, N, layout):
+    """Up to 32 rows: weights in whole pieces go through the tiles when they are large, others as they are."""
+    from objectdetection_amd import ops
+    x, w, b, d = make(np.random.default_rng(M), dev, M, K, N, torch.bfloat16, layout, True, True)
+    odd = torch.zeros((K * N + 1,), dtype=torch.bfloat16, device=dev)[1:]
+    odd = odd.view(w.t().shape).t() if layout == "nk" else odd.view(w.shape)
+    odd.copy_(w)
+    lay = 0 if layout == "kn" else 1
+    for ww in (w, odd):
+        out, pre = ops.dense_fwd(x, ww, b, "gelu", residual=d, want_pre=True)
+        check_fwd(x, w, b, d, "gelu", out, pre)
+        most = torch.empty(max(16, ops.dense_fwd_workspace_bytes(M, K, N, lay)), dtype=torch.uint8, device=dev)
+        assert torch.equal(ops.dense_fwd(x, ww, b, "gelu", residual=d, workspace=most), out)
+        check_bwd(x, w, d, pre, "silu", ops.dense_bwd(d, x, ww, pre, "silu"))

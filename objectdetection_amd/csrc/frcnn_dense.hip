@@ -189,8 +189,8 @@ __device__ __forceinline__ void dn_epilogue(const DnEpilogue& e, long long i, lo
 template <bool KC, int R, int BK>
 __device__ __forceinline__ int dn_swizzle(int r, int c) {
     if constexpr (KC) return c ^ ((r >> 1) & 7);                              // [R][8 pieces of 8 k]
-    constexpr int m = R >= 128 ? 7 : R / 16 - 1;                              // [BK][R / 8 pieces]
-    return c ^ ((((r & 3) | ((r >> 1) & 4)) & m) << 1);
+    else if constexpr (R == 64) return c ^ ((((r >> 1) & 1) | ((r >> 2) & 2)) << 1);      // [BK][8 pieces]
+    else return c ^ (((r & 3) | ((r >> 1) & 4)) << 1);                        // [BK][R / 8 pieces]
 }
 
 // tile number -> tile: every XCD (number % 8) gets a contiguous run of tiles, and a run walks groups of eight
@@ -761,7 +761,7 @@ __device__ __forceinline__ long long dn_divide(long long a, long long b) {
 }
 
 // sums of a split product's slices, in slice order, and the epilogue; four outputs per thread.  Bound by the
-// partial sums' way from memory: sixteen slices of 128 x 4,096 (33.5 MB) 8.2 us, two of 2,000 x 4,096 13.7 us (4.8 TB/s)
+// partial sums' way from memory: eight slices of 128 x 4,096 4.9 us, two of 2,000 x 4,096 (65.5 MB, 16.4 written) 13.4 us
 template <typename T>
 __global__ void __launch_bounds__(64)
 dense_join_kernel(const float* __restrict__ partial, int splits, long long I, long long J, DnEpilogue e) {
@@ -791,7 +791,7 @@ dense_join_kernel(const float* __restrict__ partial, int splits, long long I, lo
 
 // ---- operands whose rows are not whole 16-byte pieces --------------------------------------------------
 // are copied once to rows that are, with zeros behind their end: a piece per thread, in one launch for all
-// of a call's operands (777 x 1,003 and 1,003 x 531 f16: 4.6 us, latency; 25,088 x 4,099: 68 us, 6 TB/s)
+// of a call's operands (777 x 1,003 and 1,003 x 531 f16: 4.3 us, latency; 8,192 x 4,099 bf16 22 us, 6.1 TB/s)
 struct DnPack { const void* src; void* dst; long long rows, cols, ld, pieces; };   // pieces of 8 per row of dst
 struct DnPacks { DnPack of[2]; long long blocks_first, blocks; };                  // workgroups of 256 pieces
 

@@ -451,14 +451,12 @@ struct DnReader {
 };
 
 // FULL: with bias, pre, activation, residual or a float32 output in the epilogue (the forward).
-// STAY: the workgroup takes every gridDim.x-th tile; the first copies of the next tile leave before the
-// results of this one are written, and arrive meanwhile.  `tiles`: tiles and slices in all.
+// STAY: the workgroup takes tile `id` and every `stride`-th after it; the first copies of the next tile leave
+// before the results of this one are written, and arrive meanwhile.  `tiles`: tiles and slices in all.
 template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, bool FULL, bool STAY>
-__global__ void __launch_bounds__(64 * WI * WJ)
-dense_gemm_kernel(DnGemm p, int tiles) {
+__device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int stride, char* dn_lds) {
     constexpr int NT = 64 * WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
     constexpr int READS = FI * (AKC ? 1 : 2) + FJ * (BKC ? 1 : 2);  // LDS reads per wave and step
-    extern __shared__ __attribute__((aligned(16))) char dn_lds[];    // A's ring, B's, the turns (STAY)
     constexpr uint32_t RING_A = BI * DN_SK * 2 * DN_RING, RING_B = BJ * DN_SK * 2 * DN_RING;
     const int wave = __builtin_amdgcn_readfirstlane(wave_id());
     const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
@@ -512,7 +510,6 @@ dense_gemm_kernel(DnGemm p, int tiles) {
         issue(3, true, false);
     };
 
-    int id = (int)blockIdx.x;
     start(id);
 #pragma unroll 1
     while (true) {
@@ -581,12 +578,19 @@ dense_gemm_kernel(DnGemm p, int tiles) {
         dn_handover<0>();                              // every wave has read the last step: the ring is free
         const long long oi = i0 + wi, oj = j0 + wj;
         const int os = slice;
-        id += (int)gridDim.x;
+        id += stride;
         const bool more = STAY && id < tiles;
         if (more) start(id);
         dn_write_out<T, FI, FJ, FULL>(p, acc, os, oi, oj, turn);
         if (!more) return;
     }
+}
+
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, bool FULL, bool STAY>
+__global__ void __launch_bounds__(64 * WI * WJ)
+dense_gemm_kernel(DnGemm p, int tiles) {
+    extern __shared__ __attribute__((aligned(16))) char dn_lds[];    // A's ring, B's, the turns (STAY)
+    dn_gemm<T, AKC, BKC, BI, BJ, WI, WJ, FULL, STAY>(p, tiles, (int)blockIdx.x, (int)gridDim.x, dn_lds);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------
@@ -760,33 +764,37 @@ __device__ __forceinline__ long long dn_divide(long long a, long long b) {
     return a < 0x80000000ll && b < 0x80000000ll ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
-// sums of a split product's slices, in slice order, and the epilogue; four outputs per thread.  Bound by the
-// partial sums' way from memory: eight slices of 128 x 4,096 4.9 us, two of 2,000 x 4,096 (65.5 MB, 16.4 written) 13.4 us
+// sums of a split product's slices, in slice order, and the epilogue; four outputs per thread; of one product
+// or two.  Bound by the partial sums' way from memory: eight slices of 128 x 4,096 4.9 us, two of 2,000 x 4,096
+// (65.5 MB, 16.4 written) 13.4 us
+struct DnJoin { const float* partial; long long I, J, blocks; int splits; DnEpilogue e; };
+
 template <typename T>
-__global__ void __launch_bounds__(64)
-dense_join_kernel(const float* __restrict__ partial, int splits, long long I, long long J, DnEpilogue e) {
-    const long long q = (J + 3) / 4, id = (long long)blockIdx.x * 64 + threadIdx.x;
-    if (id >= I * q) return;
-    const long long i = dn_divide(id, q), j = (id - i * q) * 4, stride = I * q * 4;
-    dn_f32x4 v = *reinterpret_cast<const dn_f32x4*>(partial + id * 4);
+__global__ void __launch_bounds__(64) dense_join_kernel(DnJoin one, DnJoin two) {
+    const bool first = (long long)blockIdx.x < one.blocks;
+    const DnJoin p = first ? one : two;
+    const long long q = (p.J + 3) / 4, id = ((long long)blockIdx.x - (first ? 0 : one.blocks)) * 64 + threadIdx.x;
+    if (id >= p.I * q) return;
+    const long long i = dn_divide(id, q), j = (id - i * q) * 4, stride = p.I * q * 4;
+    dn_f32x4 v = *reinterpret_cast<const dn_f32x4*>(p.partial + id * 4);
     int s = 1;
-    for (; s + 8 <= splits; s += 8) {                  // eight slices on their way at once
+    for (; s + 8 <= p.splits; s += 8) {                // eight slices on their way at once
         dn_f32x4 w[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) w[q] = *reinterpret_cast<const dn_f32x4*>(partial + (s + q) * stride + id * 4);
+        for (int q = 0; q < 8; ++q) w[q] = *reinterpret_cast<const dn_f32x4*>(p.partial + (s + q) * stride + id * 4);
 #pragma unroll
         for (int q = 0; q < 8; ++q)
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] += w[q][r];
     }
-    for (; s < splits; ++s) {
-        const dn_f32x4 w = *reinterpret_cast<const dn_f32x4*>(partial + s * stride + id * 4);
+    for (; s < p.splits; ++s) {
+        const dn_f32x4 w = *reinterpret_cast<const dn_f32x4*>(p.partial + s * stride + id * 4);
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] += w[r];
     }
-    const long long left = J - j;
+    const long long left = p.J - j;
     float o[4] = {v[0], v[1], v[2], v[3]};
-    dn_epilogue<T, 4>(e, i, j, left > 4 ? 4 : (int)left, o);
+    dn_epilogue<T, 4>(p.e, i, j, left > 4 ? 4 : (int)left, o);
 }
 
 // ---- operands whose rows are not whole 16-byte pieces --------------------------------------------------
@@ -882,21 +890,24 @@ __global__ void __launch_bounds__(256) dense_dz_kernel(DnDz p, DnPacks packs) {
     }
 }
 
-// column sums of `blocks` rows of float32 partial sums: 16 columns per workgroup, 64 threads each, four
+// column sums of `blocks` rows of float32 partial sums: 16 columns per workgroup, NT / 16 threads each, four
 // rows on their way per thread (16,000 rows of 84: 4 us)
-template <typename T>
-__global__ void __launch_bounds__(1024)
-dense_bias_grad_kernel(const float* __restrict__ sums, int blocks, int N, T* __restrict__ d_bias) {
-    __shared__ float part[64][17];
+struct DnBiasGrad { const float* sums; void* d_bias; int blocks, N; };
+
+template <typename T, int NT>
+__device__ __forceinline__ void dn_bias_grad(const DnBiasGrad& p, int block, float (*part)[17]) {
     const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
-    const int col = blockIdx.x * 16 + c;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (col < N)
-        for (int b = q; b < blocks; b += 256)
+    const int col = block * 16 + c;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (b + 64 * u < blocks) s[u] += sums[(long long)(b + 64 * u) * N + col];
-    part[q][c] = (s[0] + s[1]) + (s[2] + s[3]);
+    for (int g = q; g < 64; g += NT / 16) {            // the same 64 sums however many threads there are
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (col < p.N)
+            for (int b = g; b < p.blocks; b += 256)
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (b + 64 * u < p.blocks) s[u] += p.sums[(long long)(b + 64 * u) * p.N + col];
+        part[g][c] = (s[0] + s[1]) + (s[2] + s[3]);
+    }
     __syncthreads();
     if (q < 4) {                                       // 16 rows each
         float v = part[16 * q][c];
@@ -904,8 +915,25 @@ dense_bias_grad_kernel(const float* __restrict__ sums, int blocks, int N, T* __r
         for (int r = 1; r < 16; ++r) v += part[16 * q + r][c];
         v += __shfl_xor(v, 16);
         v += __shfl_xor(v, 32);
-        if (q == 0 && col < N) d_bias[col] = (T)v;
+        if (q == 0 && col < p.N) ((T*)p.d_bias)[col] = (T)v;
     }
+}
+template <typename T>
+__global__ void __launch_bounds__(1024) dense_bias_grad_kernel(DnBiasGrad p) {
+    __shared__ float part[64][17];
+    dn_bias_grad<T, 1024>(p, (int)blockIdx.x, part);
+}
+
+// ---- the products of a small backward, and the rest of its bias gradient, in one launch -------------------
+// d_x and d_w leave most of the chip idle each, and a launch takes longer on the host than such a product on
+// the GPU: workgroups of d_x, then of d_w, then of the bias gradient.
+template <typename T, bool BKC>
+__global__ void __launch_bounds__(256) dense_pair_kernel(DnGemm x, int tiles_x, DnGemm w, int tiles_w, DnBiasGrad b) {
+    extern __shared__ __attribute__((aligned(16))) char dn_lds[];
+    const int id = (int)blockIdx.x;
+    if (id < tiles_x) dn_gemm<T, true, BKC, 64, 128, 1, 4, false, false>(x, tiles_x, id, 0, dn_lds);
+    else if (id < tiles_x + tiles_w) dn_gemm<T, false, false, 64, 128, 1, 4, false, false>(w, tiles_w, id - tiles_x, 0, dn_lds);
+    else dn_bias_grad<T, 256>(b, id - tiles_x - tiles_w, reinterpret_cast<float(*)[17]>(dn_lds));
 }
 
 template <typename T>
@@ -1090,30 +1118,63 @@ static int dn_launch_packs(const DnPacks& packs, hipStream_t stream) {
 
 // D = A B^T: `a` holds A as [I][K] (akc) or [K][I], `b` B as [J][K] (bkc) or [K][J], packed where they have
 // to be; the workspace holds the partial sums of a split reduction
-template <typename T>
-static int dn_product(const DnMatrix& a, bool akc, const DnMatrix& b, bool bkc, bool few, const DnEpilogue& e,
-                      void* ws, hipStream_t stream) {
-    const long long I = akc ? a.rows : a.cols, K = akc ? a.cols : a.rows, J = bkc ? b.rows : b.cols;
-    const DnPlan pl = dn_plan(I, J, K, akc, bkc, few);
-    if (pl.tiles_i > 0xFFFFFFF || pl.tiles_j > 0xFFFFFFF) return FRCNN_E_UNSUPPORTED;
+static DnGemm dn_arguments(const DnPlan& pl, const DnMatrix& a, bool akc, const DnMatrix& b, bool bkc, const DnEpilogue& e,
+                           void* ws) {
     DnGemm g{};
-    g.a = a.p; g.b = b.p; g.lda = a.ld; g.ldb = b.ld; g.I = I; g.J = J; g.K = K;
-    g.outer_a = a.padded ? dn_pieces(I) * 8 : I;
-    g.outer_b = b.padded ? dn_pieces(J) * 8 : J;
+    g.I = akc ? a.rows : a.cols; g.J = bkc ? b.rows : b.cols; g.K = akc ? a.cols : a.rows;
+    g.a = a.p; g.b = b.p; g.lda = a.ld; g.ldb = b.ld;
+    g.outer_a = a.padded ? dn_pieces(g.I) * 8 : g.I;
+    g.outer_b = b.padded ? dn_pieces(g.J) * 8 : g.J;
     g.k_slice = pl.k_slice; g.splits = pl.splits;
     g.tiles_i = (int)pl.tiles_i; g.tiles_j = (int)pl.tiles_j;
     g.partial = pl.splits > 1 ? (float*)ws : nullptr;
     g.e = e;
+    return g;
+}
+// joins what is split of one product or two
+template <typename T>
+static int dn_join(const DnGemm* a, const DnGemm* b, hipStream_t stream) {
+    DnJoin j[2] = {};
+    int n = 0;
+    for (const DnGemm* g : {a, b})
+        if (g && g->partial) j[n++] = DnJoin{g->partial, g->I, g->J, (g->I * ((g->J + 3) / 4) + 63) / 64, g->splits, g->e};
+    if (n == 0) return FRCNN_OK;
+    const long long blocks = j[0].blocks + j[1].blocks;
+    if (!dn_grid(blocks, 64)) return FRCNN_E_UNSUPPORTED;
+    FRCNN_LAUNCH(dense_join_kernel<T>, dim3((unsigned)blocks), dim3(64), 0, stream, j[0], j[1]);
+    return FRCNN_OK;
+}
+template <typename T>
+static int dn_product(const DnMatrix& a, bool akc, const DnMatrix& b, bool bkc, bool few, const DnEpilogue& e,
+                      void* ws, hipStream_t stream) {
+    const DnPlan pl = dn_plan(akc ? a.rows : a.cols, bkc ? b.rows : b.cols, akc ? a.cols : a.rows, akc, bkc, few);
+    if (pl.tiles_i > 0xFFFFFFF || pl.tiles_j > 0xFFFFFFF) return FRCNN_E_UNSUPPORTED;
+    const DnGemm g = dn_arguments(pl, a, akc, b, bkc, e, ws);
     int rc;
     if (akc && bkc) rc = dn_launch_gemm<T, true, true>(pl, g, stream);
     else if (akc) rc = dn_launch_gemm<T, true, false>(pl, g, stream);
     else rc = dn_launch_gemm<T, false, false>(pl, g, stream);
-    if (rc != FRCNN_OK || pl.splits == 1) return rc;
-    const long long groups = (I * ((J + 3) / 4) + 63) / 64;
-    if (!dn_grid(groups, 64)) return FRCNN_E_UNSUPPORTED;
-    FRCNN_LAUNCH(dense_join_kernel<T>, dim3((unsigned)groups), dim3(64), 0, stream, (const float*)g.partial, pl.splits,
-                 I, J, e);
-    return FRCNN_OK;
+    return rc != FRCNN_OK ? rc : dn_join<T>(&g, nullptr, stream);
+}
+
+// the plans of a backward's two products; whether they share a launch: both of small tiles, few enough workgroups to be
+// on the chip at once (1,111 x 779 x 333 f16 with SiLU: 21.8 us for the call; 29.1 one after the other)
+struct DnPair { DnPlan x, w; bool together; };
+static DnPair dn_pair(int64_t M, int K, int N, bool kn, bool few) {
+    DnPair p{dn_plan(M, K, N, true, kn, few), kn ? dn_plan(K, N, M, false, false, false) : dn_plan(N, K, M, false, false, false), false};
+    auto small = [](const DnPlan& q) { return q.bi == 64 && q.tiles_i * q.tiles_j * q.splits <= 2 * DN_CUS; };
+    p.together = small(p.x) && small(p.w);
+    return p;
+}
+template <typename T, bool BKC>
+static int dn_launch_pair(const DnGemm& x, const DnGemm& w, const DnBiasGrad& b, hipStream_t stream) {
+    constexpr int lds = DN_RING * (64 + 128) * DN_SK * 2;
+    static std::atomic<uint64_t> raised{0};
+    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_pair_kernel<T, BKC>), lds, raised)) return FRCNN_E_LAUNCH;
+    const int tx = x.tiles_i * x.tiles_j * x.splits, tw = w.tiles_i * w.tiles_j * w.splits;
+    const int tb = b.sums ? (b.N + 15) / 16 : 0;
+    FRCNN_LAUNCH((dense_pair_kernel<T, BKC>), dim3((unsigned)(tx + tw + tb)), dim3(256), lds, stream, x, tx, w, tw, b);
+    return dn_join<T>(&x, &w, stream);
 }
 
 // Whether the operands of a product have to be whole pieces, and what its partial sums and its packed
@@ -1203,6 +1264,9 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
     DnPacks packs;
     rc = dn_pack(d_x && !few ? &mw : nullptr, d_w ? &mx : nullptr, rest, packs);
     if (rc != FRCNN_OK) return rc;
+    DnPair pair{};
+    if (d_x && d_w) pair = dn_pair(M, K, N, kn, few);
+    DnBiasGrad bias{};
     if (d_bias || dz) {
         DnDz q{};
         q.d_out = d_out; q.ldd = ldd; q.pre = pre; q.ldp = ldp; q.dz = dz; q.ldz = p.ldz;
@@ -1216,14 +1280,25 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
             FRCNN_LAUNCH((dense_dz_kernel<T, float>), dim3((unsigned)blocks), dim3(256), 0, s, q, packs);
         else
             FRCNN_LAUNCH((dense_dz_kernel<T, T>), dim3((unsigned)blocks), dim3(256), 0, s, q, packs);
-        if (q.sums)
-            FRCNN_LAUNCH(dense_bias_grad_kernel<T>, dim3((unsigned)((N + 15) / 16)), dim3(1024), 0, s, q.sums,
-                         (int)p.blocks, N, (T*)d_bias);
+        if (q.sums) {
+            bias = DnBiasGrad{q.sums, d_bias, (int)p.blocks, N};
+            if (!pair.together)
+                FRCNN_LAUNCH(dense_bias_grad_kernel<T>, dim3((unsigned)((N + 15) / 16)), dim3(1024), 0, s, bias);
+        }
     } else {
         rc = dn_launch_packs<T>(packs, s);
         if (rc != FRCNN_OK) return rc;
     }
     DnEpilogue e{};
+    if (pair.together) {
+        e.out = d_x; e.ldo = lddx;
+        const DnGemm gx = dn_arguments(pair.x, z, true, mw, kn, e, rest);
+        e.out = d_w; e.ldo = lddw;
+        char* behind = rest + dn_up(pair.x.partial_bytes);
+        const DnGemm gw = kn ? dn_arguments(pair.w, mx, false, z, false, e, behind)
+                             : dn_arguments(pair.w, z, false, mx, false, e, behind);
+        return kn ? dn_launch_pair<T, true>(gx, gw, bias, s) : dn_launch_pair<T, false>(gx, gw, bias, s);
+    }
     if (d_x) {
         e.out = d_x; e.ldo = lddx;
         rc = dn_product<T>(z, true, mw, kn, few, e, rest, s);
@@ -1295,13 +1370,17 @@ extern "C" size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N, int w
     const DnRows x = aligned & 1 ? DN_ALIGNED : DN_ANY, w = aligned & 2 ? DN_ALIGNED : DN_ANY;
     const size_t copy_w = kn ? dn_copy_bytes(K, N, w) : dn_copy_bytes(N, K, w);
     const bool few = dn_few(M, K, N, kn, copy_w == 0), few_whole = dn_few(M, K, N, kn, true);
-    size_t dx = dn_partial_bytes(M, K, N, true, kn, few);
+    auto partial = [&](bool few) {                     // one product's at a time, or both
+        const DnPair q = dn_pair(M, K, N, kn, few);
+        const size_t dx = dn_up(q.x.partial_bytes), dw = dn_up(q.w.partial_bytes);
+        return q.together ? dx + dw : dx > dw ? dx : dw;
+    };
+    size_t most = partial(few);
     if (few != few_whole) {                            // W may be whole after all
-        const size_t other = dn_partial_bytes(M, K, N, true, kn, few_whole);
-        if (dx < other) dx = other;
+        const size_t other = partial(few_whole);
+        if (most < other) most = other;
     }
-    const size_t dw = kn ? dn_partial_bytes(K, N, M, false, false, false) : dn_partial_bytes(N, K, M, false, false, false);
-    return p.dz_bytes + p.sum_bytes + dn_copy_bytes(M, K, x) + (few ? 0 : copy_w) + (dx > dw ? dx : dw);
+    return p.dz_bytes + p.sum_bytes + dn_copy_bytes(M, K, x) + (few ? 0 : copy_w) + most;
 }
 
 extern "C" int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, const void* x, int64_t ldx, const void* w,

@@ -455,3 +455,23 @@ def test_few_rows_of_large_weights(dev, M, K, N, layout):
         most = torch.empty(max(16, ops.dense_fwd_workspace_bytes(M, K, N, lay)), dtype=torch.uint8, device=dev)
         assert torch.equal(ops.dense_fwd(x, ww, b, "gelu", residual=d, workspace=most), out)
         check_bwd(x, w, d, pre, "silu", ops.dense_bwd(d, x, ww, pre, "silu"))
+
+
+@pytest.mark.parametrize("M,K,N", [(1111, 779, 333), (300, 203, 85), (64, 512, 512), (257, 16, 8), (40, 40, 40), (1000, 136, 1000)])
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+def test_small_backward_in_one_launch_gives_the_same_bits(dev, M, K, N, layout):
+    """Both products and the bias gradient of a small backward share launches; asked for one by one they do not."""
+    from objectdetection_amd import ops
+    x, w, b, d = make(np.random.default_rng(M), dev, M, K, N, torch.float16, layout, True, True)
+    pre = ops.dense_fwd(x, w, b, want_pre=True)[1]
+    for act in ("silu", "none"):
+        full = ops.dense_bwd(d, x, w, pre, act)
+        check_bwd(x, w, d, pre, act, full)
+        for key, want in (("d_x", (True, False, False)), ("d_weight", (False, True, False)), ("d_bias", (False, False, True))):
+            assert torch.equal(ops.dense_bwd(d, x, w, pre, act, *want)[key], full[key]), key
+        two = ops.dense_bwd(d, x, w, pre, act, want_db=False)
+        assert torch.equal(two["d_x"], full["d_x"]) and torch.equal(two["d_weight"], full["d_weight"])
+        lay = 0 if layout == "kn" else 1
+        ws = torch.full((ops.dense_bwd_workspace_bytes(M, K, N, lay) + 256,), 255, dtype=torch.uint8, device=dev)
+        g = ops.dense_bwd(d, x, w, pre, act, workspace=ws[:-256])
+        assert all(torch.equal(g[k], full[k]) for k in g) and (ws[-256:] == 255).all()

@@ -7,6 +7,7 @@ Layout
   module/    the reference's function names and argument order
              (Faster_RCNN/module/{anchor,data,model}.py)
   config.py  the sizes the reference hard-codes, as parameters
+  capture.py refusal of captures that would end the process
   shard.py   per-image sharding across ranks (one process per GPU)
 """
 from .config import PathConfig, REFERENCE, SHIP  # noqa: F401

@@ -351,9 +351,9 @@ __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&a
 // s + 3 and s + 4.  A handover says that the copies step s + 1 needs have arrived (the newer ones stay in
 // flight) and that every wave has read step s, whose place is then filled again.  Rows outside the
 // operand repeat its last row (their results are not stored); k outside reads a page of zeros.
-// What bounds it: the clock (1.83 GHz under this load) and the matrix cores, busy 75 % of its cycles.  8,192 cubed
-// in bf16: 1,450 TFLOP/s with W as [N,K], 1,550 as Keras kernel and for d_weight.  A ring of eight for small products
-// costs 1.2 us more to fill than it saves.
+// What bounds it: the clock (1.83 GHz under this load) and the matrix cores, busy 75 to 84 % of its cycles.  8,192
+// cubed in bf16: 1,430 to 1,450 TFLOP/s with W as [N,K], 1,460 to 1,550 as Keras kernel, 1,445 to 1,550 for d_weight
+// (from card to card).  A ring of eight for small products costs 1.2 us more to fill than it saves.
 constexpr int DN_SK = 32, DN_RING = 4;
 __device__ const __attribute__((aligned(16))) uint32_t dn_zeros[4] = {0, 0, 0, 0};
 

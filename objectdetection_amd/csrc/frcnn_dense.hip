@@ -627,7 +627,9 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
         rows[m] = A + (i < p.I ? i : p.I - 1) * p.lda;
     }
     const long long jl = j0 + l < p.J ? j0 + l : p.J - 1;         // k contiguous: this lane's row of B
-    const bool inner = BKC || j0 + 16 * JB <= p.J;                // whole pieces in every lane
+    // Columns outside B are loaded too, from the rows behind, and not stored; the last rows have none behind them.
+    const long long whole = BKC || j0 + 16 * JB <= p.J || p.K - 7 > k_end ? k_end : p.K - 7;
+    const int last = (int)(p.J - 1 - j0) / 8 * 8, c8 = 8 * (lane & 3) < last ? 8 * (lane & 3) : last;
     const int jv = (int)(p.J - j0 - 8 * (lane & 3) < 8 ? p.J - j0 - 8 * (lane & 3) : 8);
 
     dn_s16x8 b[DN_FS][NL], a[DN_FS][MB][2];
@@ -635,7 +637,7 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
 #pragma unroll
         for (int h = 0; h < NL; ++h) {
             const T* q = BKC ? B + jl * p.ldb + k + 16 * g + 8 * h
-                             : B + (k + 16 * h + (lane >> 2)) * p.ldb + j0 + 8 * (lane & 3);
+                             : B + (k + 16 * h + (lane >> 2)) * p.ldb + j0 + c8;
             __builtin_memcpy(&rb[h], q, 16);
         }
 #pragma unroll
@@ -700,7 +702,7 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
     };
     constexpr long long STEP = 64 * DN_FW;
     long long k = k0 + 64 * wave;
-    const int n = inner && k + 64 <= k_end ? (int)((k_end - k - 64) / STEP) + 1 : 0;     // whole pieces
+    const int n = k + 64 <= whole ? (int)((whole - k - 64) / STEP) + 1 : 0;              // whole pieces
 #pragma unroll
     for (int u = 0; u < DN_FS; ++u)
         if (u < n) load(k + u * STEP, b[u], a[u]);
@@ -725,7 +727,7 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
             }
     }
 #pragma unroll 1
-    for (; k < k_end; k += STEP) {                     // a piece that is cut short, columns of a narrow B
+    for (; k < k_end; k += STEP) {                     // pieces that are cut short or come last in a narrow B
         load_some(k, b[0], a[0]);
         multiply(b[0], a[0]);
     }

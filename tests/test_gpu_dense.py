@@ -475,3 +475,19 @@ def test_small_backward_in_one_launch_gives_the_same_bits(dev, M, K, N, layout):
         ws = torch.full((ops.dense_bwd_workspace_bytes(M, K, N, lay) + 256,), 255, dtype=torch.uint8, device=dev)
         g = ops.dense_bwd(d, x, w, pre, act, workspace=ws[:-256])
         assert all(torch.equal(g[k], full[k]) for k in g) and (ws[-256:] == 255).all()
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 4096, 21), (9, 4103, 5), (32, 2048, 31), (3, 70, 1), (20, 9000, 3), (2, 64, 30), (4, 71, 9)])
+def test_few_rows_of_a_narrow_kernel(dev, M, K, N):
+    """Fewer than 32 columns: what is loaded beside them never reaches a result (infinities and NaN around the matrix)."""
+    from objectdetection_amd import ops
+    x, w, b, d = make(np.random.default_rng(K), dev, M, K, N, torch.float16, "kn", True, True)
+    for ld in (N, N + 3, N + 40):
+        wide = torch.full((K * ld + 64,), math.nan, dtype=torch.float16, device=dev)
+        ww = torch.as_strided(wide, (K, N), (ld, 1), 32)
+        ww.copy_(w)
+        check_fwd(x, w, b, d, "relu", ops.dense_fwd(x, ww, b, "relu", residual=d))
+        end = torch.empty((K * ld,), dtype=torch.float16, device=dev)
+        last = torch.as_strided(end, (K, N), (ld, 1), ld - N)          # its last value is the buffer's
+        last.copy_(w)
+        assert torch.equal(ops.dense_fwd(x, last, b), ops.dense_fwd(x, w, b))

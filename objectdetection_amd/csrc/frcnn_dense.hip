@@ -1147,9 +1147,8 @@ static int dn_join(const DnGemm* a, const DnGemm* b, hipStream_t stream) {
     return FRCNN_OK;
 }
 template <typename T>
-static int dn_product(const DnMatrix& a, bool akc, const DnMatrix& b, bool bkc, bool few, const DnEpilogue& e,
+static int dn_product(const DnPlan& pl, const DnMatrix& a, bool akc, const DnMatrix& b, bool bkc, const DnEpilogue& e,
                       void* ws, hipStream_t stream) {
-    const DnPlan pl = dn_plan(akc ? a.rows : a.cols, bkc ? b.rows : b.cols, akc ? a.cols : a.rows, akc, bkc, few);
     if (pl.tiles_i > 0xFFFFFFF || pl.tiles_j > 0xFFFFFFF) return FRCNN_E_UNSUPPORTED;
     const DnGemm g = dn_arguments(pl, a, akc, b, bkc, e, ws);
     int rc;
@@ -1179,15 +1178,12 @@ static int dn_launch_pair(const DnGemm& x, const DnGemm& w, const DnBiasGrad& b,
     return dn_join<T>(&x, &w, stream);
 }
 
-// Whether the operands of a product have to be whole pieces, and what its partial sums and its packed
-// operands take.  DN_ANY: rows anywhere; DN_ALIGNED: on 16 bytes; DN_PADDED: padded to whole pieces as well
-enum DnRows { DN_ANY, DN_ALIGNED, DN_PADDED };
+// What a packed operand takes.  DN_ANY: rows anywhere; DN_ALIGNED: on 16 bytes
+enum DnRows { DN_ANY, DN_ALIGNED };
 static size_t dn_copy_bytes(long long rows, long long cols, DnRows r) {
-    return r == DN_PADDED || (r == DN_ALIGNED && cols % 8 == 0) ? 0 : dn_pack_bytes(rows, cols);
+    return r == DN_ALIGNED && cols % 8 == 0 ? 0 : dn_pack_bytes(rows, cols);
 }
-static size_t dn_partial_bytes(long long I, long long J, long long K, bool akc, bool bkc, bool few) {
-    return dn_up(dn_plan(I, J, K, akc, bkc, few).partial_bytes);
-}
+static size_t dn_copy_bytes(const DnMatrix& m) { return dn_whole(m) ? 0 : dn_pack_bytes(m.rows, m.cols); }
 
 // the backward's workspace: dz, its column sums, then what one product at a time needs
 struct DnBwdPlan { bool copy; long long ldz; int cg; long long rows, blocks; size_t dz_bytes, sum_bytes; };
@@ -1234,22 +1230,22 @@ static int dn_zero(void* p, long long rows, long long cols, long long ld, hipStr
 }
 
 template <typename T>
-static int dn_forward(DnMatrix x, DnMatrix w, bool bkc, const DnEpilogue& e, char* ws, hipStream_t s) {
-    const bool few = dn_few(x.rows, bkc ? w.rows : w.cols, x.cols, bkc, dn_whole(w));
+static int dn_forward(DnMatrix x, DnMatrix w, bool bkc, bool few, const DnPlan& plan, const DnEpilogue& e, char* ws,
+                      hipStream_t s) {
     if (!few) {
         DnPacks packs;
         int rc = dn_pack(&x, &w, ws, packs);
         if (rc == FRCNN_OK) rc = dn_launch_packs<T>(packs, s);
         if (rc != FRCNN_OK) return rc;
     }
-    return dn_product<T>(x, true, w, bkc, few, e, ws, s);
+    return dn_product<T>(plan, x, true, w, bkc, e, ws, s);
 }
 
 template <typename T>
 static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void* x, long long ldx, const void* w,
                        long long ldw, int w_layout, const void* pre, long long ldp, long long M, int K, int N,
                        int dtype, int act, void* d_x, long long lddx, void* d_w, long long lddw, void* d_bias,
-                       char* ws, const DnBwdPlan& p, hipStream_t s) {
+                       char* ws, const DnBwdPlan& p, bool few, const DnPair& pair, hipStream_t s) {
     const bool kn = w_layout == FRCNN_W_KN;
     int rc = FRCNN_OK;
     if (M == 0) {
@@ -1262,12 +1258,9 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
     char* rest = ws + p.dz_bytes + p.sum_bytes;
     const DnMatrix z = dz ? DnMatrix{dz, M, N, p.ldz, true} : DnMatrix{d_out, M, N, ldd, false};
     DnMatrix mx{x, M, K, ldx, false}, mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
-    const bool few = dn_few(M, K, N, kn, dn_whole(mw));
     DnPacks packs;
     rc = dn_pack(d_x && !few ? &mw : nullptr, d_w ? &mx : nullptr, rest, packs);
     if (rc != FRCNN_OK) return rc;
-    DnPair pair{};
-    if (d_x && d_w) pair = dn_pair(M, K, N, kn, few);
     DnBiasGrad bias{};
     if (d_bias || dz) {
         DnDz q{};
@@ -1303,12 +1296,12 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
     }
     if (d_x) {
         e.out = d_x; e.ldo = lddx;
-        rc = dn_product<T>(z, true, mw, kn, few, e, rest, s);
+        rc = dn_product<T>(pair.x, z, true, mw, kn, e, rest, s);
         if (rc != FRCNN_OK) return rc;
     }
     if (d_w) {
         e.out = d_w; e.ldo = lddw;
-        rc = kn ? dn_product<T>(mx, false, z, false, false, e, rest, s) : dn_product<T>(z, false, mx, false, false, e, rest, s);
+        rc = kn ? dn_product<T>(pair.w, mx, false, z, false, e, rest, s) : dn_product<T>(pair.w, z, false, mx, false, e, rest, s);
     }
     return rc;
 }
@@ -1317,26 +1310,20 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
 
 using namespace frcnn;
 
-// the largest need of a call whose operands are as aligned as said, or more
-static size_t dn_fwd_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
+// what a forward's packed operands and partial sums take
+static size_t dn_fwd_bytes(const DnPlan& plan, bool few, size_t copies) { return dn_up(plan.partial_bytes) + (few ? 0 : copies); }
+extern "C" size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
+    if (!dn_sizes(M, K, N) || M == 0 || M > DN_MAX_ROWS) return 0;
     const DnRows x = aligned & 1 ? DN_ALIGNED : DN_ANY, w = aligned & 2 ? DN_ALIGNED : DN_ANY;
     const bool kn = w_layout == FRCNN_W_KN;
-    const size_t copy_w = kn ? dn_copy_bytes(K, N, w) : dn_copy_bytes(N, K, w);
+    const size_t copy_x = dn_copy_bytes(M, K, x), copy_w = kn ? dn_copy_bytes(K, N, w) : dn_copy_bytes(N, K, w);
     const bool few = dn_few(M, N, K, !kn, copy_w == 0), few_whole = dn_few(M, N, K, !kn, true);
-    size_t need = dn_partial_bytes(M, N, K, true, !kn, few) + (few ? 0 : dn_copy_bytes(M, K, x) + copy_w);
+    size_t need = dn_fwd_bytes(dn_plan(M, N, K, true, !kn, few), few, copy_x + copy_w);
     if (few != few_whole) {                            // W may be whole after all
-        const size_t other = dn_partial_bytes(M, N, K, true, !kn, few_whole) + dn_copy_bytes(M, K, x);
+        const size_t other = dn_fwd_bytes(dn_plan(M, N, K, true, !kn, few_whole), few_whole, copy_x);
         if (need < other) need = other;
     }
     return need;
-}
-extern "C" size_t frcnn_dense_fwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
-    return !dn_sizes(M, K, N) || M == 0 || M > DN_MAX_ROWS ? 0 : dn_fwd_bytes(M, K, N, w_layout, aligned);
-}
-
-static int dn_aligned(const void* x, int64_t ldx, const void* w, int64_t ldw) {
-    return (dn_even(x, 16) && ldx % 8 == 0 && ldx <= DN_MAX_LD ? 1 : 0) |
-           (dn_even(w, 16) && ldw % 8 == 0 && ldw <= DN_MAX_LD ? 2 : 0);
 }
 
 extern "C" int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int w_layout, const void* bias,
@@ -1355,34 +1342,37 @@ extern "C" int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_
     if (!dn_even(x, 2) || !dn_even(w, 2) || !dn_even(bias, 2) || !dn_even(residual, 2) || !dn_even(pre, 2) ||
         !dn_even(out, out_dtype == FRCNN_DT_F32 ? 4 : 2))
         return FRCNN_E_BADARG;
-    const size_t need = frcnn_dense_fwd_workspace_bytes(M, K, N, w_layout, dn_aligned(x, ldx, w, ldw));
+    const DnMatrix mx{x, M, K, ldx, false}, mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
+    const bool few = dn_few(M, N, K, !kn, dn_whole(mw));
+    const DnPlan plan = dn_plan(M, N, K, true, !kn, few);
+    const size_t need = dn_fwd_bytes(plan, few, dn_copy_bytes(mx) + dn_copy_bytes(mw));
     if (need && (!workspace || workspace_bytes < need || !dn_even(workspace, 16))) return FRCNN_E_WORKSPACE;
     DnEpilogue e{};
     e.bias = bias; e.residual = residual; e.pre = pre; e.out = out;
     e.ldr = ldr; e.ldp = ldp; e.ldo = ldo; e.act = act; e.out_f32 = out_dtype == FRCNN_DT_F32;
-    const DnMatrix mx{x, M, K, ldx, false}, mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
-    return dtype == FRCNN_DT_BF16 ? dn_forward<__bf16>(mx, mw, !kn, e, (char*)workspace, (hipStream_t)stream)
-                                  : dn_forward<_Float16>(mx, mw, !kn, e, (char*)workspace, (hipStream_t)stream);
+    return dtype == FRCNN_DT_BF16
+               ? dn_forward<__bf16>(mx, mw, !kn, few, plan, e, (char*)workspace, (hipStream_t)stream)
+               : dn_forward<_Float16>(mx, mw, !kn, few, plan, e, (char*)workspace, (hipStream_t)stream);
 }
 
+// what a backward's dz, column sums, packed operands and partial sums (one product's at a time, or both) take
+static size_t dn_bwd_bytes(const DnBwdPlan& p, const DnPair& pair, size_t copies) {
+    const size_t x = dn_up(pair.x.partial_bytes), w = dn_up(pair.w.partial_bytes);
+    return p.dz_bytes + p.sum_bytes + copies + (pair.together ? x + w : x > w ? x : w);
+}
 extern "C" size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned) {
     if (!dn_sizes(M, K, N) || M == 0 || M > DN_MAX_ROWS) return 0;
     const DnBwdPlan p = dn_bwd_plan(M, N, !(aligned & 4) || N % 8 != 0);
     const bool kn = w_layout == FRCNN_W_KN;
     const DnRows x = aligned & 1 ? DN_ALIGNED : DN_ANY, w = aligned & 2 ? DN_ALIGNED : DN_ANY;
-    const size_t copy_w = kn ? dn_copy_bytes(K, N, w) : dn_copy_bytes(N, K, w);
+    const size_t copy_x = dn_copy_bytes(M, K, x), copy_w = kn ? dn_copy_bytes(K, N, w) : dn_copy_bytes(N, K, w);
     const bool few = dn_few(M, K, N, kn, copy_w == 0), few_whole = dn_few(M, K, N, kn, true);
-    auto partial = [&](bool few) {                     // one product's at a time, or both
-        const DnPair q = dn_pair(M, K, N, kn, few);
-        const size_t dx = dn_up(q.x.partial_bytes), dw = dn_up(q.w.partial_bytes);
-        return q.together ? dx + dw : dx > dw ? dx : dw;
-    };
-    size_t most = partial(few);
+    size_t need = dn_bwd_bytes(p, dn_pair(M, K, N, kn, few), copy_x + (few ? 0 : copy_w));
     if (few != few_whole) {                            // W may be whole after all
-        const size_t other = partial(few_whole);
-        if (most < other) most = other;
+        const size_t other = dn_bwd_bytes(p, dn_pair(M, K, N, kn, few_whole), copy_x);
+        if (need < other) need = other;
     }
-    return p.dz_bytes + p.sum_bytes + dn_copy_bytes(M, K, x) + (few ? 0 : copy_w) + most;
+    return need;
 }
 
 extern "C" int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, const void* x, int64_t ldx, const void* w,
@@ -1407,15 +1397,23 @@ extern "C" int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, cons
         if (act != FRCNN_ACT_NONE && (!pre || ldp < N)) return FRCNN_E_BADARG;
         if (d_x && (!w || ldw < (kn ? N : K) || lddx < K)) return FRCNN_E_BADARG;
         if (d_w && (!x || ldx < K)) return FRCNN_E_BADARG;
-        const int aligned = dn_aligned(d_x ? w : nullptr, d_x ? ldw : 0, d_w ? x : nullptr, d_w ? ldx : 0);
-        const size_t need = frcnn_dense_bwd_workspace_bytes(M, K, N, w_layout, (aligned & 1) * 2 | aligned >> 1 |
-                                                            (copy ? 0 : 4));
-        if (need && (!workspace || workspace_bytes < need || !dn_even(workspace, 16))) return FRCNN_E_WORKSPACE;
     }
     const DnBwdPlan p = dn_bwd_plan(M, N, copy);
+    bool few = false;
+    DnPair pair{};
+    if (M > 0) {
+        const DnMatrix mx{x, M, K, ldx, false}, mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
+        few = dn_few(M, K, N, kn, dn_whole(mw));
+        pair = dn_pair(M, K, N, kn, few);
+        pair.together = pair.together && d_x && d_w;
+        if (!d_x) pair.x.partial_bytes = 0;
+        if (!d_w) pair.w.partial_bytes = 0;
+        const size_t need = dn_bwd_bytes(p, pair, (d_w ? dn_copy_bytes(mx) : 0) + (d_x && !few ? dn_copy_bytes(mw) : 0));
+        if (need && (!workspace || workspace_bytes < need || !dn_even(workspace, 16))) return FRCNN_E_WORKSPACE;
+    }
     return dtype == FRCNN_DT_BF16
                ? dn_backward<__bf16>(d_out, ldd, d_dtype, x, ldx, w, ldw, w_layout, pre, ldp, M, K, N, dtype, act,
-                                     d_x, lddx, d_w, lddw, d_bias, (char*)workspace, p, (hipStream_t)stream)
+                                     d_x, lddx, d_w, lddw, d_bias, (char*)workspace, p, few, pair, (hipStream_t)stream)
                : dn_backward<_Float16>(d_out, ldd, d_dtype, x, ldx, w, ldw, w_layout, pre, ldp, M, K, N, dtype, act,
-                                       d_x, lddx, d_w, lddw, d_bias, (char*)workspace, p, (hipStream_t)stream);
+                                       d_x, lddx, d_w, lddw, d_bias, (char*)workspace, p, few, pair, (hipStream_t)stream);
 }

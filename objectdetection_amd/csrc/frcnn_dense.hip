@@ -345,16 +345,20 @@ __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&a
 // Tiles go from memory to LDS directly (global_load_lds, 16 bytes per lane, the swizzle applied to the
 // source address because the destination is linear in the lane).  The reduction is walked in steps of 32 k:
 // while the fragments of step s, already in registers, are multiplied, those of step s + 1 are read from
-// LDS and later ones are in flight.  An outer-contiguous operand is copied a step at a time into a ring of
-// four, at step s that of s + 4; a k-contiguous one two steps at a time (64 k: whole 128-byte lines, copies
-// of half lines took L2 twice the requests: 1,282 TFLOP/s at 8,192 cubed, 1,444 this way) into a ring of two, at every odd s those of
-// s + 3 and s + 4.  A handover says that the copies step s + 1 needs have arrived (the newer ones stay in
+// LDS and later ones are in flight, in a ring of RING steps.  An outer-contiguous operand is copied a step at a
+// time, at step s that of s + RING; a k-contiguous one two steps at a time (64 k: whole 128-byte lines, copies of
+// half lines took L2 twice the requests: 1,282 TFLOP/s at 8,192 cubed, 1,444 this way), at every odd s those of
+// s + RING - 1 and s + RING.  A handover says that the copies step s + 1 needs have arrived (the newer ones stay in
 // flight) and that every wave has read step s, whose place is then filled again.  Rows outside the
 // operand repeat its last row (their results are not stored); k outside reads a page of zeros.
+// RING is 4.  With both operands k-contiguous that is one copy of two steps in flight, which the steps of the smaller
+// tiles do not cover: there it is 6 where a compute unit holds one workgroup (1,000 x 4,096 x 4,096 54 -> 47 us
+// with the same tiles, 2,000 x 4,096 x 4,096 77 -> 60; with more workgroups the room is better used by a second one:
+// 50,000 x 64 x 64 6.6 us, 8.2 with 6).  Eight cost another 1.2 us to fill.
 // What bounds it: the clock (1.83 GHz under this load) and the matrix cores, busy 75 to 84 % of its cycles.  8,192
 // cubed in bf16: 1,430 to 1,450 TFLOP/s with W as [N,K], 1,460 to 1,550 as Keras kernel, 1,445 to 1,550 for d_weight
-// (from card to card).  A ring of eight for small products costs 1.2 us more to fill than it saves.
-constexpr int DN_SK = 32, DN_RING = 4;
+// (from card to card).
+constexpr int DN_SK = 32;
 __device__ const __attribute__((aligned(16))) uint32_t dn_zeros[4] = {0, 0, 0, 0};
 
 // (m0 is a reserved register: the compiler sets it before each use of its own)
@@ -421,7 +425,7 @@ struct DnCopy {
 // fragment f is a constant further where k is contiguous, and at the address with f in its swizzled
 // bits where it is not; the place in the ring is a constant offset of the instruction (an operand's ring
 // lies within 64 KB, its first byte on a multiple of 2 KB).
-template <bool KC, int R>
+template <bool KC, int R, int RING>
 struct DnReader {
     uint32_t at;
     __device__ __forceinline__ void init(uint32_t lds, int o0) {
@@ -437,7 +441,7 @@ struct DnReader {
     // keeps the compiler from holding an address per fragment in registers
     __device__ __forceinline__ void renew() { asm volatile("" : "+v"(at)); }
     __device__ __forceinline__ dn_s16x8 read(int f, int step) const {
-        const uint32_t ring = (uint32_t)(step % DN_RING);
+        const uint32_t ring = (uint32_t)(step % RING);
         if constexpr (KC) {     // the odd step is the second half of the row: pieces 4 .. 7
             const uint32_t a = (at ^ ((ring & 1u) * 64u)) + (ring >> 1) * (R * 128u);
             return *(dn_lds_s16x8*)(uintptr_t)(a + (uint32_t)f * 2048u);
@@ -453,11 +457,11 @@ struct DnReader {
 // FULL: with bias, pre, activation, residual or a float32 output in the epilogue (the forward).
 // STAY: the workgroup takes tile `id` and every `stride`-th after it; the first copies of the next tile leave
 // before the results of this one are written, and arrive meanwhile.  `tiles`: tiles and slices in all.
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, bool FULL, bool STAY>
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RING, bool FULL, bool STAY>
 __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int stride, char* dn_lds) {
     constexpr int NT = 64 * WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
     constexpr int READS = FI * (AKC ? 1 : 2) + FJ * (BKC ? 1 : 2);  // LDS reads per wave and step
-    constexpr uint32_t RING_A = BI * DN_SK * 2 * DN_RING, RING_B = BJ * DN_SK * 2 * DN_RING;
+    constexpr uint32_t RING_A = BI * DN_SK * 2 * RING, RING_B = BJ * DN_SK * 2 * RING;
     const int wave = __builtin_amdgcn_readfirstlane(wave_id());
     const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
     char* turn = dn_lds + (STAY ? RING_A + RING_B : 0) + wave * dn_turn_bytes<FJ>();
@@ -467,12 +471,14 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
     // copies per thread: of the operands that are copied every step, of those copied every other step
     constexpr int EVERY = (AKC ? 0 : CopyA::NP) + (BKC ? 0 : CopyB::NP);
     constexpr int OTHER = (AKC ? CopyA::NP : 0) + (BKC ? CopyB::NP : 0);
+    // newer ones that a handover before an even / an odd step leaves in flight
+    constexpr int EVEN = (RING / 2 - 1) * OTHER + (RING - 2) * EVERY, ODD = EVEN - OTHER;
     CopyA ca;
     CopyB cb;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dn_lds;
     const uint32_t la = lds0 + (uint32_t)wave * 1024u, lb = la + RING_A;
-    DnReader<AKC, BI> qa;
-    DnReader<BKC, BJ> qb;
+    DnReader<AKC, BI, RING> qa;
+    DnReader<BKC, BJ, RING> qb;
     qa.init(lds0, wi);
     qb.init(lds0 + RING_A, wj);
     auto read = [&](int s, dn_s16x8 (&ra)[FI], dn_s16x8 (&rb)[FJ]) {
@@ -490,7 +496,7 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
         if (s >= n) return;
         const long long left = k_end - k0 - (long long)s * DN_SK;
         const int valid = left < 2 * DN_SK ? (int)left : 2 * DN_SK;
-        const uint32_t ring = (uint32_t)(s % DN_RING);
+        const uint32_t ring = (uint32_t)(s % RING);
         if (AKC ? ot : ev) ca.issue(la + ring * (BI * 64u), valid);
         if (BKC ? ot : ev) cb.issue(lb + ring * (BJ * 64u), valid);
     };
@@ -504,10 +510,8 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
         n = (int)((k_end - k0 + DN_SK - 1) / DN_SK);
         ca.init((const T*)p.a, p.lda, i0, AKC ? p.I : p.outer_a, k0);
         cb.init((const T*)p.b, p.ldb, j0, BKC ? p.J : p.outer_b, k0);
-        issue(0, true, true);
-        issue(1, true, false);
-        issue(2, true, true);
-        issue(3, true, false);
+#pragma unroll
+        for (int s = 0; s < RING; ++s) issue(s, true, s % 2 == 0);
     };
 
     start(id);
@@ -526,21 +530,21 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
                 for (int j = 0; j < FJ; ++j) acc[i][j] = dn_mfma(rb[j], ra[i], acc[i][j], T());
         };
         // steps 0 and 1 (behind the last tile's results all but the newest are waited for: no harm)
-        if (n >= DN_RING) dn_handover<OTHER + 2 * EVERY>();
+        if (n >= RING) dn_handover<EVEN>();
         else dn_handover<0>();
         read(0, fa[0], fb[0]);
         int s = 0;
         // whole steps, four at a time so that every LDS address is a constant; no branch inside
 #pragma unroll 1
-        for (; s + 2 * DN_RING < n; s += DN_RING) {
+        for (; s + 2 * RING < n; s += RING) {
 #pragma unroll
-            for (int u = 0; u < DN_RING; ++u) {
+            for (int u = 0; u < RING; ++u) {
                 if (u & 1) {
-                    dn_handover<2 * EVERY>();
-                    if (AKC) ca.issue(la + ((u + 3) % DN_RING) * (BI * 64u));
-                    if (BKC) cb.issue(lb + ((u + 3) % DN_RING) * (BJ * 64u));
+                    dn_handover<ODD>();
+                    if (AKC) ca.issue(la + ((u + RING - 1) % RING) * (BI * 64u));
+                    if (BKC) cb.issue(lb + ((u + RING - 1) % RING) * (BJ * 64u));
                 } else if (EVERY) {
-                    dn_handover<OTHER + 2 * EVERY>();
+                    dn_handover<EVEN>();
                 }
                 if (!AKC) ca.issue(la + u * (BI * 64u));
                 if (!BKC) cb.issue(lb + u * (BJ * 64u));
@@ -560,11 +564,11 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
         // the last steps: up to eight, the last one maybe cut short
         auto step = [&](const dn_s16x8 (&ra)[FI], const dn_s16x8 (&rb)[FJ], dn_s16x8 (&na)[FI], dn_s16x8 (&nb)[FJ]) {
             if (s + 1 < n) {
-                if (s + 3 >= n) dn_handover<0>();
-                else if (s & 1) dn_handover<2 * EVERY>();
-                else dn_handover<OTHER + 2 * EVERY>();
-                if (s & 1) issue(s + 3, false, true);
-                issue(s + 4, true, false);
+                if (s + RING - 1 >= n) dn_handover<0>();
+                else if (s & 1) dn_handover<ODD>();
+                else dn_handover<EVEN>();
+                if (s & 1) issue(s + RING - 1, false, true);
+                issue(s + RING, true, false);
                 read(s + 1, na, nb);
             }
             multiply(ra, rb);
@@ -586,11 +590,11 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
     }
 }
 
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, bool FULL, bool STAY>
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RING, bool FULL, bool STAY>
 __global__ void __launch_bounds__(64 * WI * WJ)
 dense_gemm_kernel(DnGemm p, int tiles) {
     extern __shared__ __attribute__((aligned(16))) char dn_lds[];    // A's ring, B's, the turns (STAY)
-    dn_gemm<T, AKC, BKC, BI, BJ, WI, WJ, FULL, STAY>(p, tiles, (int)blockIdx.x, (int)gridDim.x, dn_lds);
+    dn_gemm<T, AKC, BKC, BI, BJ, WI, WJ, RING, FULL, STAY>(p, tiles, (int)blockIdx.x, (int)gridDim.x, dn_lds);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------
@@ -933,8 +937,8 @@ template <typename T, bool BKC>
 __global__ void __launch_bounds__(256) dense_pair_kernel(DnGemm x, int tiles_x, DnGemm w, int tiles_w, DnBiasGrad b) {
     extern __shared__ __attribute__((aligned(16))) char dn_lds[];
     const int id = (int)blockIdx.x;
-    if (id < tiles_x) dn_gemm<T, true, BKC, 64, 128, 1, 4, false, false>(x, tiles_x, id, 0, dn_lds);
-    else if (id < tiles_x + tiles_w) dn_gemm<T, false, false, 64, 128, 1, 4, false, false>(w, tiles_w, id - tiles_x, 0, dn_lds);
+    if (id < tiles_x) dn_gemm<T, true, BKC, 64, 128, 1, 4, BKC ? 6 : 4, false, false>(x, tiles_x, id, 0, dn_lds);
+    else if (id < tiles_x + tiles_w) dn_gemm<T, false, false, 64, 128, 1, 4, 4, false, false>(w, tiles_w, id - tiles_x, 0, dn_lds);
     else dn_bias_grad<T, 256>(b, id - tiles_x - tiles_w, reinterpret_cast<float(*)[17]>(dn_lds));
 }
 
@@ -947,21 +951,21 @@ __global__ void __launch_bounds__(256) dense_zero_kernel(T* p, long long rows, l
 // ---- host ------------------------------------------------------------------------------------------
 struct DnPlan { int bi, bj, splits; long long k_slice, tiles_i, tiles_j; size_t partial_bytes; };
 
-// Workgroup tiles: what a step of 32 k takes in us on a compute unit that is full of such workgroups (with
-// W as [N,K], both operands k-contiguous: step_kc), and for one alone; the rest of a workgroup (start, first
-// copies, results) and how many are resident.  What follows takes the pair of tile and split with the shortest
-// sum: rounds over the chip, or what the operands take at 3.81 TB/s and what tiles copy again at 25.2 TB/s (all
-// compute units) if that is longer, plus 0.3 of the latter, plus the join of a split.  The constants are fitted to
-// 132 products from 40 x 1,024 x 1,024 to 25,088 x 4,096 x 2,000, each measured with every tile and split: what is
-// taken is 2.1 % slower than the best of them in the mean.  4,000 x 4,096 x 4,096 wants the large tile (103 us; 119
-// and 130 from the next two), 2,000 x 25,088 x 4,096 two slices of it (307; 330 from 128 x 256 unsplit), 128 x 25,088
-// x 4,096 eight slices of 128 x 128 (53.5; 55.9 from sixteen of 128 x 256), 16,000 x 4,096 x 24 three of them (33;
-// 44.7 from 256 x 256), 1,024 cubed the small tile (10.7; 13.1).
-struct DnTile { int bi, bj; double step, step_kc, alone, fixed; int resident; };
-constexpr DnTile DN_TILES[] = {{256, 256, 0.70, 0.69, 0.69, 6.8, 1},
-                               {128, 256, 0.388, 0.459, 0.374, 4.9, 1},
-                               {128, 128, 0.236, 0.307, 0.27, 4.3, 2},
-                               {64, 128, 0.18, 0.153, 0.22, 3.0, 3}};
+// Workgroup tiles: what a step of 32 k takes in us per round over the chip, and where one round is all (alone); the
+// same with both operands k-contiguous (W as [N,K]); the rest of a workgroup (start, first copies, results) and how many
+// are resident.  What follows takes the pair of tile and split with the shortest sum: steps and rounds, or what the
+// operands take at 3.81 TB/s and what tiles copy again at 26.2 TB/s (all compute units) if that is longer, plus 0.3 of
+// the latter, plus the join of a split.  The constants are fitted to 132 products from 40 x 1,024 x 1,024 to 25,088 x
+// 4,096 x 2,000, each measured with every tile and split: what is taken is 1.4 % slower than the best of them in the
+// mean.  4,000 x 4,096 x 4,096 wants the large tile (103 us; 119 and 130 from the next two), 2,000 x 25,088 x 4,096 two
+// slices of it (307; 330 from 128 x 256 unsplit), 128 x 25,088 x 4,096 eight slices of 128 x 128 (53.5; 55.9 from
+// sixteen of 128 x 256), 16,000 x 4,096 x 24 three of them (33; 44.7 from 256 x 256), 1,024 cubed the small tile (9.6;
+// 12.5).
+struct DnTile { int bi, bj; double step, alone, step_kc, alone_kc, fixed; int resident; };
+constexpr DnTile DN_TILES[] = {{256, 256, 0.70, 0.595, 0.77, 0.69, 6.8, 1},
+                               {128, 256, 0.388, 0.411, 0.44, 0.38, 4.9, 1},
+                               {128, 128, 0.236, 0.28, 0.312, 0.25, 4.3, 2},
+                               {64, 128, 0.18, 0.22, 0.153, 0.145, 3.18, 3}};
 
 constexpr long long DN_MAX_LD = 1ll << 21;             // a tile's rows lie within 2 GiB of each other
 // a launch has fewer than 2^32 threads
@@ -999,21 +1003,21 @@ static DnPlan dn_plan(long long I, long long J, long long K, bool akc, bool bkc,
     double best = 0.0;
     for (const DnTile& t : DN_TILES) {
         const long long ti = (I + t.bi - 1) / t.bi, tj = (J + t.bj - 1) / t.bj;
-        const double sat = bkc && akc ? t.step_kc : t.step;
+        const double step = bkc && akc ? t.step_kc : t.step, alone = bkc && akc ? t.alone_kc : t.alone;
         for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
             if (want > 1 && steps < 8 * want) break;       // eight steps per slice at least
             const long long per = ((steps + want - 1) / want + 1) / 2 * 2, splits = (steps + per - 1) / per;
             const double groups = (double)(ti * tj) * (double)splits;
             const double waves = groups <= DN_CUS ? 1.0 : __builtin_ceil(groups / DN_CUS);
-            double us = per * (waves * sat > t.alone ? waves * sat : t.alone) + t.fixed * __builtin_ceil(waves / t.resident);
+            double us = per * (waves > 1.0 ? waves * step : alone) + t.fixed * __builtin_ceil(waves / t.resident);
             // what memory gives, and what L2 gives again
             // (rows outside the operand repeat one row: counted half)
             const double copied = groups * per * ((I < t.bi ? (I + t.bi) / 2 : t.bi) +
                                                   (J < t.bj ? (J + t.bj) / 2 : t.bj)) * (2.0 * DN_SK);
-            const double stream = (bytes / 3.81e6 + (copied > bytes ? copied - bytes : 0.0) / 2.52e7) *
+            const double stream = (bytes / 3.81e6 + (copied > bytes ? copied - bytes : 0.0) / 2.62e7) *
                                   (groups < DN_CUS ? DN_CUS / groups : 1.0);
             us = (us < stream ? stream : us) + 0.3 * stream;
-            if (splits > 1) us += 2.35 + 0.35 * splits + (double)splits * I * J * 8.0 / 9.1e6;
+            if (splits > 1) us += 2.35 + 0.349 * splits + (double)splits * I * J * 8.0 / 8.92e6;
             if (p.bi && us > best) continue;
             best = us;
             p.bi = t.bi; p.bj = t.bj;
@@ -1036,30 +1040,38 @@ static bool dn_raise_lds(const void* kernel, int bytes, std::atomic<uint64_t>& r
     return true;
 }
 
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, bool FULL>
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RING, bool FULL>
 static int dn_launch_kernel(const DnGemm& g, unsigned tiles, hipStream_t stream) {
     // One workgroup of the large tile is all that a compute unit holds: it stays for the tiles of its XCD
     // (16,384 x 64 x 4,096: 32.8 us; 36.5 with a workgroup per tile).  Not with the full epilogue and not where
     // both operands are outer-contiguous: there the next tile's addresses do not fit beside the sums in 256
     // registers, and what is parked in memory costs the products 20 %.
     constexpr bool STAY = BI == 256 && BJ == 256 && AKC && !FULL;
-    constexpr int lds = DN_RING * (BI + BJ) * DN_SK * 2 + (STAY ? WI * WJ * dn_turn_bytes<BJ / WJ / 16>() : 0);
+    constexpr int lds = RING * (BI + BJ) * DN_SK * 2 + (STAY ? WI * WJ * dn_turn_bytes<BJ / WJ / 16>() : 0);
     static_assert(lds <= 160 * 1024, "LDS of a compute unit");
     const unsigned blocks = STAY && tiles > DN_CUS ? DN_CUS : tiles;
     static std::atomic<uint64_t> raised{0};
-    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, FULL, STAY>), lds, raised))
+    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, FULL, STAY>), lds, raised))
         return FRCNN_E_LAUNCH;
-    FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, FULL, STAY>), dim3(blocks), dim3(64 * WI * WJ), lds, stream, g,
+    FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, FULL, STAY>), dim3(blocks), dim3(64 * WI * WJ), lds, stream, g,
                  (int)tiles);
     return FRCNN_OK;
 }
 
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
-static int dn_launch_tiles(const DnGemm& g, unsigned blocks, hipStream_t stream) {
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RING>
+static int dn_launch_ring(const DnGemm& g, unsigned blocks, hipStream_t stream) {
     const bool full = !g.partial && (g.e.bias || g.e.pre || g.e.residual || g.e.act != FRCNN_ACT_NONE || g.e.out_f32);
     if constexpr (AKC)          // d_weight's product has none of it
-        if (full) return dn_launch_kernel<T, AKC, BKC, BI, BJ, WI, WJ, true>(g, blocks, stream);
-    return dn_launch_kernel<T, AKC, BKC, BI, BJ, WI, WJ, false>(g, blocks, stream);
+        if (full) return dn_launch_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, true>(g, blocks, stream);
+    return dn_launch_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, false>(g, blocks, stream);
+}
+
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
+static int dn_launch_tiles(const DnGemm& g, unsigned blocks, hipStream_t stream) {
+    if constexpr (AKC && BKC && BI < 256)       // of 128 x 256 a compute unit holds one in any case
+        if (BJ == 256 || blocks <= DN_CUS) return dn_launch_ring<T, AKC, BKC, BI, BJ, WI, WJ, 6>(g, blocks, stream);
+    if constexpr (!(AKC && BKC && BJ == 256 && BI < 256)) return dn_launch_ring<T, AKC, BKC, BI, BJ, WI, WJ, 4>(g, blocks, stream);
+    return FRCNN_E_UNSUPPORTED;
 }
 
 template <typename T, bool AKC, bool BKC>
@@ -1169,7 +1181,7 @@ static DnPair dn_pair(int64_t M, int K, int N, bool kn, bool few) {
 }
 template <typename T, bool BKC>
 static int dn_launch_pair(const DnGemm& x, const DnGemm& w, const DnBiasGrad& b, hipStream_t stream) {
-    constexpr int lds = DN_RING * (64 + 128) * DN_SK * 2;
+    constexpr int lds = (BKC ? 6 : 4) * (64 + 128) * DN_SK * 2;
     static std::atomic<uint64_t> raised{0};
     if (!dn_raise_lds(reinterpret_cast<const void*>(dense_pair_kernel<T, BKC>), lds, raised)) return FRCNN_E_LAUNCH;
     const int tx = x.tiles_i * x.tiles_j * x.splits, tw = w.tiles_i * w.tiles_j * w.splits;

@@ -130,8 +130,8 @@ __device__ __forceinline__ float ds_block(float v, float* sh) {
 
 // ---- the teacher's side of a row, by one wave ----------------------------------------------------------
 // LDS: per entry its label (-1: not there), t / T relative to the largest one, the student's logit there,
-// and what its label gets: the sum of its entries' p at the first of them, -1 at the others; with more than
-// 64 entries also a table of twice as many places or more, in which entries with the same label meet
+// and what its label gets: the sum of its entries' p, or a negative number where another entry of the label has
+// it; with more than 64 entries also a table of twice as many places or more, in which entries of a label meet
 constexpr int ds_slots(int k) {
     int n = 0;
     if (k > 64)
@@ -153,7 +153,7 @@ __device__ __forceinline__ float ds_teacher_logit(const DsArgs& a, long long at)
 }
 
 template <typename T>
-__device__ DsTeacherSum ds_teacher(const DsArgs& a, long long row, DsTeacher e, float inv_t, bool want_z) {
+__device__ DsTeacherSum ds_teacher(const DsArgs& a, long long row, DsTeacher e, float inv_t) {
     const int lane = lane_id();
     const T* z = (const T*)a.z + row * a.ldz;
     float top = -__builtin_inff();
@@ -167,7 +167,7 @@ __device__ DsTeacherSum ds_teacher(const DsArgs& a, long long row, DsTeacher e, 
         if (there) {
             any = true;
             top = fmaxf(top, t);
-            if (want_z) e.z[j] = (float)z[i];
+            e.z[j] = (float)z[i];
         }
     }
     top = ds_wave_max(top);
@@ -196,8 +196,9 @@ __device__ __forceinline__ float ds_row_loss(const DsArgs& a, DsTeacher e, float
 
 // e.p for the labels in [v0, v1), by the whole workgroup.  Up to 64 entries: one wave compares each with all
 // of them one by one (from a register of another lane: an LDS read per comparison costs the whole row its
-// latency).  More: that would be the square of their number, so each looks for its label's place in
-// the table; the first entry of a label adds up the later ones, in their order.  (4,096 rows x 65,536, 1,024 entries: 416 us; 1,917 by comparing all with all.)
+// latency), and entries of the same label come to the same sum.  More: that would be the square of their number, so
+// each looks for its label's place in the table, and the first entry of a label adds up the later ones, in their
+// order (4,096 rows x 65,536, 1,024 entries: 416 us; 1,917 by comparing all with all).
 template <int BLOCK>
 __device__ __forceinline__ void ds_listed_sums(DsTeacher e, int k, float log_sum, long long v0, long long v1) {
     if (k <= 64) {
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
     const DsTeacher e(ds_lds, a.k);
     DsTeacherSum te{0.f, false};
     if (wave_id() == 0) {                              // while the row arrives
-        te = ds_teacher<T>(a, row, e, inv_t, true);
+        te = ds_teacher<T>(a, row, e, inv_t);
         if (tid == 0) { sh_t = te.log_sum; sh_any = te.any; }
     }
     float m = -__builtin_inff();
@@ -613,7 +614,7 @@ __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
     const DsTeacher e(ds_lds, a.k);
     DsTeacherSum te{0.f, false};
     if (wave_id() == 0) {
-        te = ds_teacher<T>(a, row, e, inv_t, true);
+        te = ds_teacher<T>(a, row, e, inv_t);
         if (tid == 0) { sh_t = te.log_sum; sh_any = te.any; }
     }
     if constexpr (FORWARD) {

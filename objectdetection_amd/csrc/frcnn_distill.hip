@@ -128,7 +128,7 @@ __device__ __forceinline__ float ds_block(float v, float* sh) {
     }
 }
 
-// ---- the teacher's side of a row, by one wave ----------------------------------------------------------
+// ---- the teacher's side of a row -----------------------------------------------------------------------
 // LDS: per entry its label (-1: not there), t / T relative to the largest one, the student's logit there,
 // and what its label gets: the sum of its entries' p, or a negative number where another entry of the label has
 // it; with more than 64 entries also a table of twice as many places or more, in which entries of a label meet
@@ -145,20 +145,18 @@ struct DsTeacher {
           first(key + ds_slots(k)) {}
 };
 static size_t ds_lds_bytes(int k) { return (size_t)k * 16 + (size_t)ds_slots(k) * 8; }
-struct DsTeacherSum { float log_sum; bool any; };      // log of the sum of e^t; whether an entry is there
 
 template <typename T>
 __device__ __forceinline__ float ds_teacher_logit(const DsArgs& a, long long at) {
     return a.t_f32 ? ((const float*)a.t)[at] : (float)((const T*)a.t)[at];
 }
 
-template <typename T>
-__device__ DsTeacherSum ds_teacher(const DsArgs& a, long long row, DsTeacher e, float inv_t) {
-    const int lane = lane_id();
+// label, t / T and the student's logit of the row's entries, by the whole workgroup; whether this wave met one
+template <typename T, int BLOCK>
+__device__ __forceinline__ bool ds_teacher_load(const DsArgs& a, long long row, DsTeacher e, float inv_t) {
     const T* z = (const T*)a.z + row * a.ldz;
-    float top = -__builtin_inff();
     bool any = false;
-    for (int j = lane; j < a.k; j += 64) {
+    for (int j = threadIdx.x; j < a.k; j += BLOCK) {
         const int64_t i = a.idx[row * a.k + j];
         const float t = ds_teacher_logit<T>(a, row * a.k + j) * inv_t;
         const bool there = i >= 0 && i < a.V && !(t == -__builtin_inff());
@@ -166,19 +164,31 @@ __device__ DsTeacherSum ds_teacher(const DsArgs& a, long long row, DsTeacher e, 
         e.t[j] = t;
         if (there) {
             any = true;
-            top = fmaxf(top, t);
             e.z[j] = (float)z[i];
         }
     }
+    return __ballot(any) != 0;
+}
+// makes t relative to the largest one and returns the log of the sum of e^t, by one wave
+__device__ __forceinline__ float ds_teacher_sum(DsTeacher e, int k) {
+    const int lane = lane_id();
+    float top = -__builtin_inff(), s = 0.f;
+    for (int j = lane; j < k; j += 64) top = fmaxf(top, e.label[j] >= 0 ? e.t[j] : -__builtin_inff());
     top = ds_wave_max(top);
-    any = __ballot(any) != 0;
-    float s = 0.f;
-    for (int j = lane; j < a.k; j += 64) {
+    for (int j = lane; j < k; j += 64) {
         const float t = e.t[j] - top;
         e.t[j] = t;
         if (e.label[j] >= 0) s += __builtin_amdgcn_exp2f(t * DS_LOG2E);
     }
-    return {logf(ds_wave_sum(s)), any};
+    return logf(ds_wave_sum(s));
+}
+// over the workgroup, behind a barrier after sh[wave] was set
+template <int BLOCK>
+__device__ __forceinline__ bool ds_any(const int* sh) {
+    int any = sh[0];
+#pragma unroll
+    for (int w = 1; w < BLOCK / 64; ++w) any |= sh[w];
+    return any != 0;
 }
 
 // sum_j p_j (log p_j - log q_j) with log q = (z - z_max) / T - log_s, by the same wave
@@ -198,11 +208,12 @@ __device__ __forceinline__ float ds_row_loss(const DsArgs& a, DsTeacher e, float
 // of them one by one (from a register of another lane: an LDS read per comparison costs the whole row its
 // latency), and entries of the same label come to the same sum.  More: that would be the square of their number, so
 // each looks for its label's place in the table, and the first entry of a label adds up the later ones, in their
-// order (4,096 rows x 65,536, 1,024 entries: 416 us; 1,917 by comparing all with all).
+// order (4,096 rows x 65,536, 1,024 entries: 313 us; 1,917 by comparing all with all).
 template <int BLOCK>
-__device__ __forceinline__ void ds_listed_sums(DsTeacher e, int k, float log_sum, long long v0, long long v1) {
+__device__ __forceinline__ void ds_listed_sums(DsTeacher e, int k, const float* sh_log_sum, long long v0, long long v1) {
     if (k <= 64) {
         if (wave_id() != 0) return;
+        const float log_sum = *sh_log_sum;             // this wave's own
         const int lane = lane_id();
         const int mine = lane < k ? e.label[lane] : -1;
         const float p = lane < k ? __builtin_amdgcn_exp2f((e.t[lane] - log_sum) * DS_LOG2E) : 0.f;
@@ -221,6 +232,7 @@ __device__ __forceinline__ void ds_listed_sums(DsTeacher e, int k, float log_sum
         e.first[n] = k;
     }
     __syncthreads();
+    const float log_sum = *sh_log_sum;
     for (int j = tid; j < k; j += BLOCK) {             // places; e.p: the entry's place
         const int label = e.label[j];
         if (label < v0 || label >= v1) {
@@ -469,7 +481,7 @@ template <typename T, int BLOCK, int NV>
 __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
     extern __shared__ __attribute__((aligned(16))) char ds_lds[];
     __shared__ float sh_m[BLOCK / 64], sh_s[BLOCK / 64], sh_t;
-    __shared__ int sh_any;
+    __shared__ int sh_any[BLOCK / 64];
     constexpr int W = DsVec<T>::W;
     const int tid = threadIdx.x;
     const long long row = blockIdx.x;
@@ -488,11 +500,8 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
         x[i].load(z + v, a.V - v);
     }
     const DsTeacher e(ds_lds, a.k);
-    DsTeacherSum te{0.f, false};
-    if (wave_id() == 0) {                              // while the row arrives
-        te = ds_teacher<T>(a, row, e, inv_t);
-        if (tid == 0) { sh_t = te.log_sum; sh_any = te.any; }
-    }
+    const bool some = ds_teacher_load<T, BLOCK>(a, row, e, inv_t);        // while the row arrives
+    if (lane_id() == 0) sh_any[wave_id()] = some;
     float m = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -500,10 +509,15 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
         for (int j = 0; j < W; ++j) m = fmaxf(m, x[i][j]);
     m = ds_block<BLOCK, true>(m, sh_m);
     if constexpr (BLOCK == 64) __syncthreads();
-    if (!sh_any) {
+    if (!ds_any<BLOCK>(sh_any)) {
         if (tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
         if (grad) ds_zero(grad, 0, a.V, tid, BLOCK);
         return;
+    }
+    float log_sum = 0.f;
+    if (wave_id() == 0) {
+        log_sum = ds_teacher_sum(e, a.k);
+        if (tid == 0) sh_t = log_sum;
     }
     const float f = inv_t * DS_LOG2E;
     float s = 0.f;
@@ -515,11 +529,11 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
         for (int j = 0; j < W; ++j) part += __builtin_amdgcn_exp2f((x[i][j] - m) * f);
         s += part;
     }
-    if (grad) ds_listed_sums<BLOCK>(e, a.k, sh_t, 0, a.V);
+    if (grad) ds_listed_sums<BLOCK>(e, a.k, &sh_t, 0, a.V);
     s = ds_block<BLOCK, false>(s, sh_s);
     const float log_s = logf(s);
     if (wave_id() == 0) {
-        const float l = ds_row_loss(a, e, te.log_sum, inv_t, m, log_s);
+        const float l = ds_row_loss(a, e, log_sum, inv_t, m, log_s);
         if (tid == 0) {
             a.loss[row] = w * (a.temperature * a.temperature) * l;
             a.lse[row] = m * inv_t + log_s;
@@ -590,7 +604,7 @@ template <typename T, bool FORWARD, int BLOCK, int NV>
 __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
     extern __shared__ __attribute__((aligned(16))) char ds_lds[];
     __shared__ float sh_t, sh_m, sh_s;
-    __shared__ int sh_any;
+    __shared__ int sh_any[BLOCK / 64];
     constexpr int W = DsVec<T>::W;
     const int tid = threadIdx.x, chunk = blockIdx.x;
     const long long row = blockIdx.y;
@@ -612,11 +626,8 @@ __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
         }
     }
     const DsTeacher e(ds_lds, a.k);
-    DsTeacherSum te{0.f, false};
-    if (wave_id() == 0) {
-        te = ds_teacher<T>(a, row, e, inv_t);
-        if (tid == 0) { sh_t = te.log_sum; sh_any = te.any; }
-    }
+    const bool some = ds_teacher_load<T, BLOCK>(a, row, e, inv_t);
+    if (lane_id() == 0) sh_any[wave_id()] = some;
     if constexpr (FORWARD) {
         if (wave_id() == 1) {                          // every workgroup joins the chunks in the same order
             float m = -__builtin_inff(), s = 0.f;
@@ -632,21 +643,26 @@ __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
         }
     }
     __syncthreads();
-    if (!sh_any) {
+    if (!ds_any<BLOCK>(sh_any)) {
         if (FORWARD && chunk == 0 && tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
         if (grad) ds_zero(grad, v0, v1, tid, BLOCK);
         return;
     }
+    float log_sum = 0.f;
+    if (wave_id() == 0) {
+        log_sum = ds_teacher_sum(e, a.k);
+        if (tid == 0) sh_t = log_sum;
+    }
     const float m = FORWARD ? sh_m : 0.f, s = FORWARD ? sh_s : 1.f, lse = FORWARD ? 0.f : a.lse_in[row];
     if (FORWARD && chunk == 0 && wave_id() == 0) {
-        const float log_s = logf(s), l = ds_row_loss(a, e, te.log_sum, inv_t, m, log_s);
+        const float log_s = logf(s), l = ds_row_loss(a, e, log_sum, inv_t, m, log_s);
         if (tid == 0) {
             a.loss[row] = w * (a.temperature * a.temperature) * l;
             a.lse[row] = m * inv_t + log_s;
         }
     }
     if (!grad) return;
-    ds_listed_sums<BLOCK>(e, a.k, sh_t, v0, v1);
+    ds_listed_sums<BLOCK>(e, a.k, &sh_t, v0, v1);
     const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale), cq = FORWARD ? c / s : c;
     const float f = inv_t * DS_LOG2E;
     auto relative = [&](float zi) {
@@ -751,10 +767,14 @@ static int ds_run(const DsArgs& a, int dtype, hipStream_t s) {
         if (n <= 256) return ds_launch_short<T, FORWARD, 64, 4>(a, s);
         return ds_launch_short<T, FORWARD, 64, 8>(a, s);
     }
+    // a short row with more entries is one wave's up to 192 of them (16,384 x 1,000: with 100 entries 35 us, 50 by
+    // four waves; with 1,000 entries 755 and 307)
+    const bool one_wave = a.k <= 192;
     if constexpr (FORWARD) {
         if (!a.part) {
-            if (n <= 64) return ds_launch_row<T, 64, 1>(a, s);
-            if (n <= 256) return ds_launch_row<T, 64, 4>(a, s);
+            if (n <= 64 && one_wave) return ds_launch_row<T, 64, 1>(a, s);
+            if (n <= 256 && one_wave) return ds_launch_row<T, 64, 4>(a, s);
+            if (n <= 256) return ds_launch_row<T, 256, 1>(a, s);
             if (n <= 1024) return ds_launch_row<T, 256, 4>(a, s);
             if (n <= 2048) return ds_launch_row<T, 256, 8>(a, s);
             if (n <= 4096) return ds_launch_row<T, 512, 8>(a, s);
@@ -764,11 +784,10 @@ static int ds_run(const DsArgs& a, int dtype, hipStream_t s) {
         return a.nv == 1 ? ds_launch_chunk<T, true, DS_CHUNK_BLOCK, 1>(a, s)
                          : ds_launch_chunk<T, true, DS_CHUNK_BLOCK, 4>(a, s);
     } else {
-        // short rows: a wave each
-        if (n <= 64) return ds_launch_chunk<T, false, 64, 1>(a, s);
-        if (n <= 256) return ds_launch_chunk<T, false, 64, 4>(a, s);
-        return a.nv == 1 ? ds_launch_chunk<T, false, DS_CHUNK_BLOCK, 1>(a, s)
-                         : ds_launch_chunk<T, false, DS_CHUNK_BLOCK, 4>(a, s);
+        if (n <= 64 && one_wave) return ds_launch_chunk<T, false, 64, 1>(a, s);
+        if (n <= 256 && one_wave) return ds_launch_chunk<T, false, 64, 4>(a, s);
+        return a.nv == 1 || n <= DS_CHUNK_BLOCK ? ds_launch_chunk<T, false, DS_CHUNK_BLOCK, 1>(a, s)
+                                                : ds_launch_chunk<T, false, DS_CHUNK_BLOCK, 4>(a, s);
     }
 }
 

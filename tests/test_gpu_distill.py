@@ -277,7 +277,7 @@ def test_rows_further_apart_than_32_bits(dev):
 
 
 @pytest.mark.parametrize("V,k,labels", [(5000, 65, 30), (5000, 1024, 1), (5000, 1024, 5), (70000, 1024, 400), (300, 700, 300),
-                                        (1000, 130, 129), (40000, 1024, 1024)])
+                                        (1000, 130, 129), (40000, 1024, 1024), (3, 193, 3), (1024, 192, 150), (1024, 193, 190)])
 def test_many_entries_with_the_same_labels(dev, V, k, labels):
     """More than 64 entries: every label in the list once, a few times, or in all of it; the same bits each time."""
     rng = np.random.default_rng(V + k + labels)

@@ -186,3 +186,18 @@ def test_training_step_with_a_teacher_and_a_16_bit_head(dev, dtype):
     for p, q in zip(frcn.parameters(), before):
         assert p.grad.isfinite().all() and p.grad.any() and not torch.equal(p, q)
     assert all(p.grad is None for p in teacher.parameters())
+
+
+def test_a_head_served_from_16_bit_parameters_gives_the_same(dev):
+    """FRCNModel(dtype=bf16).to(bf16): the same bits without a cast per call, also for one RoI."""
+    from objectdetection_amd.train import FRCNModel
+    torch.manual_seed(5)
+    m = FRCNModel(16, 7, 136, 21, dtype=torch.bfloat16).to(dev)
+    served = FRCNModel(16, 7, 136, 21, dtype=torch.bfloat16).to(dev)
+    served.load_state_dict(m.state_dict())
+    served.to(torch.bfloat16)
+    for B, R in ((1, 1), (2, 100)):
+        x = torch.randn((B, R, 7, 7, 16), device=dev)
+        with torch.no_grad():
+            for a, b in zip(m.logits(x), served.logits(x)):
+                assert a.dtype == torch.float32 and torch.equal(a, b)

@@ -287,6 +287,7 @@ def test_many_entries_with_the_same_labels(dev, V, k, labels):
     idx[1, ::3] = -1
     idx[2, 1:] = V
     idx[3, :] = idx[3, 0]
+    idx[4, :] = -1 if k % 2 else V + 7
     idx = torch.from_numpy(idx).to(dev)
     from objectdetection_amd import ops
     got = ops.distill_loss(z, t, idx, temperature=1.5)

@@ -601,12 +601,14 @@ dense_gemm_kernel(DnGemm p, int tiles) {
 // Up to 32 rows (I): the product reads B once and little else, so what counts is how soon and how wide the
 // loads of B leave.  A workgroup owns 16 (k contiguous) or 32 (outer contiguous) columns and its eight waves
 // share out the reduction in pieces of 64 k: a wave's load covers whole 128-byte lines of 16 rows of B, or
-// 64-byte pieces of 16 k (neighbouring workgroups on the same XCD share the lines), and three pieces are on their
-// way while one is multiplied.  A fragment of A comes straight from memory (every workgroup reads the same few
-// rows: L2).  An outer-contiguous piece is turned round by the transposing LDS read in the wave's own LDS.
-// The eight sums are added in wave order.  The MFMA's k order is free as long as both operands agree: lane
-// group g takes k 16 g .. 16 g + 15 of a piece in two instructions (k contiguous), or 8 g .. 8 g + 7 of each half.
-// One row x 4,096 x 4,096 bf16, W as [N,K]: 8.6 us, 3.9 TB/s; Keras kernel of 4,096 x 84: 9 us.
+// 64-byte pieces of 16 k (neighbouring workgroups on the same XCD share the lines), and three pieces are loaded
+// ahead (waiting for the oldest alone takes as long as for the three together).  A fragment of A comes straight
+// from memory (every workgroup reads the same few rows: L2).  An outer-contiguous piece is turned round by the
+// transposing LDS read in the wave's own LDS.  The eight sums are added in wave order.  The MFMA's k order is free as
+// long as both operands agree: lane group g takes k 16 g .. 16 g + 15 of a piece in two instructions (k contiguous),
+// or 8 g .. 8 g + 7 of each half.
+// One row x 4,096 x 4,096 bf16, W as [N,K]: 8.6 us, 3.9 TB/s; Keras kernel of 4,096 x 84: 9 us.  An outer-contiguous B
+// of 4,096 rows costs every workgroup all of its pages: 17 us at 4,096 x 4,096, half the rate.
 constexpr int DN_FEW = 32, DN_FW = 8, DN_FS = 3;   // most rows; waves; pieces on their way
 
 template <typename T, bool BKC, int MB>

@@ -155,6 +155,8 @@ struct DnGemm {
     long long k_slice;        // k per slice: an even number of steps
     int splits, tiles_i, tiles_j;
     float* partial;           // [splits][I][Jp], Jp = J rounded up to 4, when splits > 1
+    long long low_a, low_b;   // TWO: elements from the operand that is dz to its low part, 0 for the other one
+    float low_scale, scale;   // TWO: factors of the low part's product and of the result
     DnEpilogue e;
 };
 
@@ -457,7 +459,9 @@ struct DnReader {
 // FULL: with bias, pre, activation, residual or a float32 output in the epilogue (the forward).
 // STAY: the workgroup takes tile `id` and every `stride`-th after it; the first copies of the next tile leave
 // before the results of this one are written, and arrive meanwhile.  `tiles`: tiles and slices in all.
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RING, bool FULL, bool STAY>
+// TWO: the operand that is dz comes as the sum of two values of its type (dense_dz_kernel); the reduction is walked
+// twice over the same other operand, the low part first, with the sums in the same registers.
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RING, bool FULL, bool STAY, bool TWO>
 __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int stride, char* dn_lds) {
     constexpr int NT = 64 * WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
     constexpr int READS = FI * (AKC ? 1 : 2) + FJ * (BKC ? 1 : 2);  // LDS reads per wave and step
@@ -508,21 +512,24 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
         k0 = slice * p.k_slice;
         k_end = k0 + p.k_slice < p.K ? k0 + p.k_slice : p.K;
         n = (int)((k_end - k0 + DN_SK - 1) / DN_SK);
-        ca.init((const T*)p.a, p.lda, i0, AKC ? p.I : p.outer_a, k0);
-        cb.init((const T*)p.b, p.ldb, j0, BKC ? p.J : p.outer_b, k0);
+        ca.init((const T*)p.a + (TWO ? p.low_a : 0), p.lda, i0, AKC ? p.I : p.outer_a, k0);
+        cb.init((const T*)p.b + (TWO ? p.low_b : 0), p.ldb, j0, BKC ? p.J : p.outer_b, k0);
 #pragma unroll
         for (int s = 0; s < RING; ++s) issue(s, true, s % 2 == 0);
     };
 
     start(id);
+    dn_f32x4 acc[FI][FJ];
+    bool low = TWO;                                    // the low part is being multiplied
 #pragma unroll 1
     while (true) {
-        dn_f32x4 acc[FI][FJ];
         dn_s16x8 fa[2][FI], fb[2][FJ];
+        if (!TWO || low) {
 #pragma unroll
-        for (int i = 0; i < FI; ++i)
+            for (int i = 0; i < FI; ++i)
 #pragma unroll
-            for (int j = 0; j < FJ; ++j) acc[i][j] = dn_f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < FJ; ++j) acc[i][j] = dn_f32x4{0.f, 0.f, 0.f, 0.f};
+        }
         auto multiply = [&](const dn_s16x8 (&ra)[FI], const dn_s16x8 (&rb)[FJ]) {
 #pragma unroll
             for (int i = 0; i < FI; ++i)
@@ -580,6 +587,24 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
             if (s < n) step(fa[1], fb[1], fa[0], fb[0]);
         }
         dn_handover<0>();                              // every wave has read the last step: the ring is free
+        if constexpr (TWO) {
+            const float f = low ? p.low_scale : p.scale;
+#pragma unroll
+            for (int i = 0; i < FI; ++i)
+#pragma unroll
+                for (int j = 0; j < FJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] *= f;
+            __builtin_amdgcn_sched_barrier(0);
+            low = !low;
+            if (!low) {                                // back to the first step, of the high part
+                ca.base -= (AKC ? (n + 1) / 2 : n) * ca.step + 2 * p.low_a;
+                cb.base -= (BKC ? (n + 1) / 2 : n) * cb.step + 2 * p.low_b;
+#pragma unroll
+                for (int s = 0; s < RING; ++s) issue(s, true, s % 2 == 0);
+                continue;
+            }
+        }
         const long long oi = i0 + wi, oj = j0 + wj;
         const int os = slice;
         id += stride;
@@ -590,11 +615,11 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
     }
 }
 
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RING, bool FULL, bool STAY>
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RING, bool FULL, bool STAY, bool TWO>
 __global__ void __launch_bounds__(64 * WI * WJ)
 dense_gemm_kernel(DnGemm p, int tiles) {
     extern __shared__ __attribute__((aligned(16))) char dn_lds[];    // A's ring, B's, the turns (STAY)
-    dn_gemm<T, AKC, BKC, BI, BJ, WI, WJ, RING, FULL, STAY>(p, tiles, (int)blockIdx.x, (int)gridDim.x, dn_lds);
+    dn_gemm<T, AKC, BKC, BI, BJ, WI, WJ, RING, FULL, STAY, TWO>(p, tiles, (int)blockIdx.x, (int)gridDim.x, dn_lds);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------
@@ -611,7 +636,7 @@ dense_gemm_kernel(DnGemm p, int tiles) {
 // of 4,096 rows costs every workgroup all of its pages: 17 us at 4,096 x 4,096, half the rate.
 constexpr int DN_FEW = 32, DN_FW = 8, DN_FS = 3;   // most rows; waves; pieces on their way
 
-template <typename T, bool BKC, int MB>
+template <typename T, bool BKC, int MB, bool TWO>
 __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
     constexpr int JB = BKC ? 1 : 2, NL = BKC ? 2 : 4;             // 16-column blocks; loads of B per piece and lane
     __shared__ dn_f32x4 sums[DN_FW][JB * MB][64];
@@ -638,8 +663,9 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
     const int last = (int)(p.J - 1 - j0) / 8 * 8, c8 = 8 * (lane & 3) < last ? 8 * (lane & 3) : last;
     const int jv = (int)(p.J - j0 - 8 * (lane & 3) < 8 ? p.J - j0 - 8 * (lane & 3) : 8);
 
-    dn_s16x8 b[DN_FS][NL], a[DN_FS][MB][2];
-    auto load = [&](long long k, dn_s16x8 (&rb)[NL], dn_s16x8 (&ra)[MB][2]) {
+    constexpr int NA = TWO ? 4 : 2;                               // loads of A per row: 2 and 2 of the low part
+    dn_s16x8 b[DN_FS][NL], a[DN_FS][MB][NA];
+    auto load = [&](long long k, dn_s16x8 (&rb)[NL], dn_s16x8 (&ra)[MB][NA]) {
 #pragma unroll
         for (int h = 0; h < NL; ++h) {
             const T* q = BKC ? B + jl * p.ldb + k + 16 * g + 8 * h
@@ -649,10 +675,11 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                __builtin_memcpy(&ra[m][h], rows[m] + k + (BKC ? 16 * g + 8 * h : 32 * h + 8 * g), 16);
+            for (int h = 0; h < NA; ++h)
+                __builtin_memcpy(&ra[m][h], rows[m] + (h < 2 ? 0 : p.low_a) + k +
+                                                (BKC ? 16 * g + 8 * (h & 1) : 32 * (h & 1) + 8 * g), 16);
     };
-    auto load_some = [&](long long k, dn_s16x8 (&rb)[NL], dn_s16x8 (&ra)[MB][2]) {
+    auto load_some = [&](long long k, dn_s16x8 (&rb)[NL], dn_s16x8 (&ra)[MB][NA]) {
         auto at = [&](const T* q, long long kk) {
             const long long left = k_end - kk;
             return dn_load8(q + kk, left > 8 ? 8 : (int)left);
@@ -669,19 +696,23 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) ra[m][h] = at(rows[m], k + (BKC ? 16 * g + 8 * h : 32 * h + 8 * g));
+            for (int h = 0; h < NA; ++h)
+                ra[m][h] = at(rows[m] + (h < 2 ? 0 : p.low_a), k + (BKC ? 16 * g + 8 * (h & 1) : 32 * (h & 1) + 8 * g));
     };
-    dn_f32x4 acc[JB][MB];
+    dn_f32x4 acc[JB][MB], acc_low[JB][MB];
 #pragma unroll
     for (int j = 0; j < JB; ++j)
 #pragma unroll
-        for (int m = 0; m < MB; ++m) acc[j][m] = dn_f32x4{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](dn_s16x8 (&rb)[NL], dn_s16x8 (&ra)[MB][2]) {
+        for (int m = 0; m < MB; ++m) acc[j][m] = acc_low[j][m] = dn_f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](dn_s16x8 (&rb)[NL], dn_s16x8 (&ra)[MB][NA]) {
         if constexpr (BKC) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int m = 0; m < MB; ++m) acc[0][m] = dn_mfma(rb[h], ra[m][h], acc[0][m], T());
+                for (int m = 0; m < MB; ++m) {
+                    acc[0][m] = dn_mfma(rb[h], ra[m][h], acc[0][m], T());
+                    if constexpr (TWO) acc_low[0][m] = dn_mfma(rb[h], ra[m][2 + h], acc_low[0][m], T());
+                }
         } else {
             // row k, 32-byte half c / 2 exchanged where k has bit 3: two lane groups meet no bank twice
             dn_s16x8* lds = turn[wave];
@@ -702,7 +733,10 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
                     const dn_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((dn_lds_s16x4*)(q + 4 * 32));
                     const dn_s16x8 f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-                    for (int m = 0; m < MB; ++m) acc[j][m] = dn_mfma(f, ra[m][h], acc[j][m], T());
+                    for (int m = 0; m < MB; ++m) {
+                        acc[j][m] = dn_mfma(f, ra[m][h], acc[j][m], T());
+                        if constexpr (TWO) acc_low[j][m] = dn_mfma(f, ra[m][2 + h], acc_low[j][m], T());
+                    }
                 }
         }
     };
@@ -736,6 +770,15 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
     for (; k < k_end; k += STEP) {                     // pieces that are cut short or come last in a narrow B
         load_some(k, b[0], a[0]);
         multiply(b[0], a[0]);
+    }
+    if constexpr (TWO) {
+#pragma unroll
+        for (int j = 0; j < JB; ++j)
+#pragma unroll
+            for (int m = 0; m < MB; ++m)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    acc[j][m][r] = (acc[j][m][r] + acc_low[j][m][r] * p.low_scale) * p.scale;
     }
 #pragma unroll
     for (int j = 0; j < JB; ++j)
@@ -828,7 +871,10 @@ __global__ void __launch_bounds__(256) dense_pack_kernel(DnPacks packs) {
 
 // ---- dz = d_out * act'(pre) and its column sums ---------------------------------------------------------
 // A workgroup takes `rows` rows of 8 * cg columns; a thread 8 neighbouring columns of every (256 / cg)-th
-// row.  dz (may be null) has rows of ldz elements, a multiple of 8; its columns N .. ldz-1 become 0.  The
+// row.  dz (may be null) has rows of ldz elements, a multiple of 8; its columns N .. ldz-1 become 0.  Where dz is
+// no value of the type (GELU, SiLU, a float32 d_out) it is kept as the sum of two that are, for two products:
+// scale dz = high + low / low_up with high the nearest value and low what is left of it.  That is 2^-16 relative
+// in bfloat16 and 2^-22 in float16 (2^-8 and 2^-11 in one value), and costs no more than its own two products.  The
 // sums of the unrounded values go to d_bias where one workgroup has all rows, else to `sums`, a row per
 // block of rows.  The workgroups behind the first `blocks` pack the products' operands.  16,000 x 84 bf16: 7 us;
 // 1,111 x 333 f16 with SiLU, packing 779 x 333 and 1,111 x 779: 8.5 us (latency both)
@@ -836,9 +882,19 @@ struct DnDz {
     const void *d_out, *pre;
     void *dz, *d_bias;
     float* sums;
-    long long ldd, ldp, ldz, M, rows, row_blocks, blocks;
+    long long ldd, ldp, ldz, M, rows, row_blocks, blocks, low;    // low: elements from dz to its low part, or 0
+    float scale, low_up;
     int N, act, cg;
 };
+// the nearest value of T, and the rest of v times up (0 behind infinities and NaN; a finite v that rounds to an
+// infinity leaves the largest finite value and the rest)
+template <typename T>
+__device__ __forceinline__ void dn_two(float v, float up, float& high, float& low) {
+    const float most = std::is_same<T, __bf16>::value ? 3.3895313892515355e38f : 65504.0f;
+    high = (float)(T)v;
+    if (fabsf(v) < __builtin_inff()) high = fabsf(high) <= most ? high : __builtin_copysignf(most, v);
+    low = fabsf(v) < __builtin_inff() ? (v - high) * up : 0.f;
+}
 template <typename T, typename D>
 __global__ void __launch_bounds__(256) dense_dz_kernel(DnDz p, DnPacks packs) {
     __shared__ float part[4][32][9];
@@ -855,9 +911,17 @@ __global__ void __launch_bounds__(256) dense_dz_kernel(DnDz p, DnPacks packs) {
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = e < valid ? dn_act_grad(d[e], z[e], p.act) : 0.f;
-        if (dz) dn_store<T, 8>(dz + r * p.ldz + col, 8, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] += v[e];
+        if (dz && p.low) {
+            float h[8], l[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dn_two<T>(v[e] * p.scale, p.low_up, h[e], l[e]);
+            dn_store<T, 8>(dz + r * p.ldz + col, 8, h);
+            dn_store<T, 8>(dz + p.low + r * p.ldz + col, 8, l);
+        } else if (dz) {
+            dn_store<T, 8>(dz + r * p.ldz + col, 8, v);
+        }
     };
     if (valid > 0) {
         const bool act_any = p.act != FRCNN_ACT_NONE;
@@ -935,12 +999,13 @@ __global__ void __launch_bounds__(1024) dense_bias_grad_kernel(DnBiasGrad p) {
 // ---- the products of a small backward, and the rest of its bias gradient, in one launch -------------------
 // d_x and d_w leave most of the chip idle each, and a launch takes longer on the host than such a product on
 // the GPU: workgroups of d_x, then of d_w, then of the bias gradient.
-template <typename T, bool BKC>
+template <typename T, bool BKC, bool TWO>
 __global__ void __launch_bounds__(256) dense_pair_kernel(DnGemm x, int tiles_x, DnGemm w, int tiles_w, DnBiasGrad b) {
     extern __shared__ __attribute__((aligned(16))) char dn_lds[];
     const int id = (int)blockIdx.x;
-    if (id < tiles_x) dn_gemm<T, true, BKC, 64, 128, 1, 4, BKC ? 6 : 4, false, false>(x, tiles_x, id, 0, dn_lds);
-    else if (id < tiles_x + tiles_w) dn_gemm<T, false, false, 64, 128, 1, 4, 4, false, false>(w, tiles_w, id - tiles_x, 0, dn_lds);
+    if (id < tiles_x) dn_gemm<T, true, BKC, 64, 128, 1, 4, BKC ? 6 : 4, false, false, TWO>(x, tiles_x, id, 0, dn_lds);
+    else if (id < tiles_x + tiles_w)
+        dn_gemm<T, false, false, 64, 128, 1, 4, 4, false, false, TWO>(w, tiles_w, id - tiles_x, 0, dn_lds);
     else dn_bias_grad<T, 256>(b, id - tiles_x - tiles_w, reinterpret_cast<float(*)[17]>(dn_lds));
 }
 
@@ -1042,7 +1107,7 @@ static bool dn_raise_lds(const void* kernel, int bytes, std::atomic<uint64_t>& r
     return true;
 }
 
-template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RING, bool FULL>
+template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RING, bool FULL, bool TWO>
 static int dn_launch_kernel(const DnGemm& g, unsigned tiles, hipStream_t stream) {
     // One workgroup of the large tile is all that a compute unit holds: it stays for the tiles of its XCD
     // (16,384 x 64 x 4,096: 32.8 us; 36.5 with a workgroup per tile).  Not with the full epilogue and not where
@@ -1054,9 +1119,9 @@ static int dn_launch_kernel(const DnGemm& g, unsigned tiles, hipStream_t stream)
     static_assert(lds <= 160 * 1024, "LDS of a compute unit");
     const unsigned blocks = STAY && tiles > DN_CUS ? DN_CUS : tiles;
     static std::atomic<uint64_t> raised{0};
-    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, FULL, STAY>), lds, raised))
+    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, FULL, STAY, TWO>), lds, raised))
         return FRCNN_E_LAUNCH;
-    FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, FULL, STAY>), dim3(blocks), dim3(64 * WI * WJ), lds, stream, g,
+    FRCNN_LAUNCH((dense_gemm_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, FULL, STAY, TWO>), dim3(blocks), dim3(64 * WI * WJ), lds, stream, g,
                  (int)tiles);
     return FRCNN_OK;
 }
@@ -1065,8 +1130,9 @@ template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RI
 static int dn_launch_ring(const DnGemm& g, unsigned blocks, hipStream_t stream) {
     const bool full = !g.partial && (g.e.bias || g.e.pre || g.e.residual || g.e.act != FRCNN_ACT_NONE || g.e.out_f32);
     if constexpr (AKC)          // d_weight's product has none of it
-        if (full) return dn_launch_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, true>(g, blocks, stream);
-    return dn_launch_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, false>(g, blocks, stream);
+        if (full) return dn_launch_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, true, false>(g, blocks, stream);
+    if (g.low_a || g.low_b) return dn_launch_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, false, true>(g, blocks, stream);
+    return dn_launch_kernel<T, AKC, BKC, BI, BJ, WI, WJ, RING, false, false>(g, blocks, stream);
 }
 
 template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ>
@@ -1083,8 +1149,14 @@ static int dn_launch_gemm(const DnPlan& pl, const DnGemm& g, hipStream_t stream)
         if (!dn_grid(pl.tiles_j, 64 * DN_FW)) return FRCNN_E_UNSUPPORTED;
         if constexpr (AKC) {
             const dim3 grid((unsigned)pl.tiles_j, (unsigned)pl.splits);
-            if (g.I <= 16) FRCNN_LAUNCH((dense_few_rows_kernel<T, BKC, 1>), grid, dim3(64 * DN_FW), 0, stream, g);
-            else FRCNN_LAUNCH((dense_few_rows_kernel<T, BKC, 2>), grid, dim3(64 * DN_FW), 0, stream, g);
+            const dim3 block(64 * DN_FW);
+            if (g.low_a) {
+                if (g.I <= 16) FRCNN_LAUNCH((dense_few_rows_kernel<T, BKC, 1, true>), grid, block, 0, stream, g);
+                else FRCNN_LAUNCH((dense_few_rows_kernel<T, BKC, 2, true>), grid, block, 0, stream, g);
+            } else {
+                if (g.I <= 16) FRCNN_LAUNCH((dense_few_rows_kernel<T, BKC, 1, false>), grid, block, 0, stream, g);
+                else FRCNN_LAUNCH((dense_few_rows_kernel<T, BKC, 2, false>), grid, block, 0, stream, g);
+            }
         }
         return FRCNN_OK;
     }
@@ -1099,7 +1171,8 @@ static int dn_launch_gemm(const DnPlan& pl, const DnGemm& g, hipStream_t stream)
 static size_t dn_up(size_t b) { return (b + 255) / 256 * 256; }
 
 // A matrix in memory as rows of `cols` values.  padded: its rows are whole pieces with zeros behind `cols`.
-struct DnMatrix { const void* p; long long rows, cols, ld; bool padded; };
+// low: elements to the low part of a dz in two parts, scale and low_scale what undoes their factors
+struct DnMatrix { const void* p; long long rows, cols, ld; bool padded; long long low = 0; float scale = 1.f, low_scale = 1.f; };
 static long long dn_pieces(long long n) { return (n + 7) / 8; }
 // rows that start on 16 bytes, of whole 16-byte pieces
 static bool dn_whole(const DnMatrix& m) {
@@ -1145,6 +1218,9 @@ static DnGemm dn_arguments(const DnPlan& pl, const DnMatrix& a, bool akc, const 
     g.k_slice = pl.k_slice; g.splits = pl.splits;
     g.tiles_i = (int)pl.tiles_i; g.tiles_j = (int)pl.tiles_j;
     g.partial = pl.splits > 1 ? (float*)ws : nullptr;
+    g.low_a = a.low; g.low_b = b.low;
+    const DnMatrix& dz = a.low ? a : b;
+    g.scale = dz.scale; g.low_scale = dz.low_scale;
     g.e = e;
     return g;
 }
@@ -1182,14 +1258,14 @@ static DnPair dn_pair(int64_t M, int K, int N, bool kn, bool few) {
     p.together = small(p.x) && small(p.w);
     return p;
 }
-template <typename T, bool BKC>
+template <typename T, bool BKC, bool TWO>
 static int dn_launch_pair(const DnGemm& x, const DnGemm& w, const DnBiasGrad& b, hipStream_t stream) {
     constexpr int lds = (BKC ? 6 : 4) * (64 + 128) * DN_SK * 2;
     static std::atomic<uint64_t> raised{0};
-    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_pair_kernel<T, BKC>), lds, raised)) return FRCNN_E_LAUNCH;
+    if (!dn_raise_lds(reinterpret_cast<const void*>(dense_pair_kernel<T, BKC, TWO>), lds, raised)) return FRCNN_E_LAUNCH;
     const int tx = x.tiles_i * x.tiles_j * x.splits, tw = w.tiles_i * w.tiles_j * w.splits;
     const int tb = b.sums ? (b.N + 15) / 16 : 0;
-    FRCNN_LAUNCH((dense_pair_kernel<T, BKC>), dim3((unsigned)(tx + tw + tb)), dim3(256), lds, stream, x, tx, w, tw, b);
+    FRCNN_LAUNCH((dense_pair_kernel<T, BKC, TWO>), dim3((unsigned)(tx + tw + tb)), dim3(256), lds, stream, x, tx, w, tw, b);
     return dn_join<T>(&x, &w, stream);
 }
 
@@ -1226,7 +1302,7 @@ static DnBwdPlan dn_bwd_plan(long long M, int N, bool copy) {
         p.rows = walk * walks;
         p.blocks = (M + p.rows - 1) / p.rows;
     }
-    p.dz_bytes = copy ? dn_up((size_t)M * (size_t)p.ldz * 2) : 0;
+    p.dz_bytes = copy ? 2 * dn_up((size_t)M * (size_t)p.ldz * 2) : 0;        // both parts
     p.sum_bytes = p.blocks > 1 ? dn_up((size_t)p.blocks * (size_t)N * 4) : 0;
     return p;
 }
@@ -1271,7 +1347,17 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
     if ((d_x || d_w) && dn_pieces(N) * 8 > DN_MAX_LD) return FRCNN_E_UNSUPPORTED;
     void* dz = p.copy && (d_x || d_w) ? ws : nullptr;
     char* rest = ws + p.dz_bytes + p.sum_bytes;
-    const DnMatrix z = dz ? DnMatrix{dz, M, N, p.ldz, true} : DnMatrix{d_out, M, N, ldd, false};
+    // d_out's values or 0 are dz where d_out has the products' type and act is none or ReLU; else dz is in two parts,
+    // in float16 with the low part up by 2^11 (its own 11 bits also below the normal range) and both down by two (act'
+    // reaches 1.13: no overflow)
+    const bool two = dz && (d_dtype != dtype || act > FRCNN_ACT_RELU), f16 = dtype == FRCNN_DT_F16;
+    const float scale = f16 ? 0.5f : 1.0f, low_up = f16 ? 2048.0f : 1.0f;
+    DnMatrix z = dz ? DnMatrix{dz, M, N, p.ldz, true} : DnMatrix{d_out, M, N, ldd, false};
+    if (two) {
+        z.low = (long long)(p.dz_bytes / 4);
+        z.scale = 1.0f / scale;
+        z.low_scale = 1.0f / low_up;
+    }
     DnMatrix mx{x, M, K, ldx, false}, mw = kn ? DnMatrix{w, K, N, ldw, false} : DnMatrix{w, N, K, ldw, false};
     DnPacks packs;
     rc = dn_pack(d_x && !few ? &mw : nullptr, d_w ? &mx : nullptr, rest, packs);
@@ -1281,6 +1367,7 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
         DnDz q{};
         q.d_out = d_out; q.ldd = ldd; q.pre = pre; q.ldp = ldp; q.dz = dz; q.ldz = p.ldz;
         q.M = M; q.N = N; q.act = act; q.cg = p.cg; q.rows = p.rows; q.row_blocks = p.blocks;
+        q.low = z.low; q.scale = scale; q.low_up = low_up;
         if (p.blocks == 1) q.d_bias = d_bias;
         else q.sums = d_bias ? reinterpret_cast<float*>(ws + p.dz_bytes) : nullptr;
         q.blocks = p.blocks * ((dn_pieces(N) + p.cg - 1) / p.cg);
@@ -1307,7 +1394,8 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
         char* behind = rest + dn_up(pair.x.partial_bytes);
         const DnGemm gw = kn ? dn_arguments(pair.w, mx, false, z, false, e, behind)
                              : dn_arguments(pair.w, z, false, mx, false, e, behind);
-        return kn ? dn_launch_pair<T, true>(gx, gw, bias, s) : dn_launch_pair<T, false>(gx, gw, bias, s);
+        if (two) return kn ? dn_launch_pair<T, true, true>(gx, gw, bias, s) : dn_launch_pair<T, false, true>(gx, gw, bias, s);
+        return kn ? dn_launch_pair<T, true, false>(gx, gw, bias, s) : dn_launch_pair<T, false, false>(gx, gw, bias, s);
     }
     if (d_x) {
         e.out = d_x; e.ldo = lddx;

@@ -446,9 +446,11 @@ int frcnn_dense_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int 
 /* dz = d_out * act'(pre) in float32 (the ReLU's is d_out where pre > 0, else 0);  d_x = dz W^T,
  * d_w = x^T dz in W's layout,  d_bias = sum of dz over the rows.  Where dz is no value of dtype
  * (GELU, SiLU, a float32 d_out) the products take it as the sum of two, within 2^-16 of it in
- * bfloat16 and 2^-22 in float16 (absolutely 2^-35), and cost twice as many matrix operations; an
- * infinity of W or x may then give NaN where one value would give an infinity.  d_x, d_w, d_bias:
- * NULL where not wanted, not all three.  The residual's gradient is d_out itself. */
+ * bfloat16 and 2^-22 in float16 (absolutely 2^-35, for a float32 d_out 2^-50 of its largest finite
+ * value, by whose power of two it is scaled for the products), and cost twice as many matrix
+ * operations; an infinity of W or x may then give NaN where one value would give an infinity.
+ * d_x, d_w, d_bias: NULL where not wanted, not all three.  The residual's gradient is d_out
+ * itself. */
 size_t frcnn_dense_bwd_workspace_bytes(int64_t M, int K, int N, int w_layout, int aligned);
 int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, const void* x, int64_t ldx,
                     const void* w, int64_t ldw, int w_layout, const void* pre, int64_t ldp,

@@ -156,7 +156,8 @@ struct DnGemm {
     int splits, tiles_i, tiles_j;
     float* partial;           // [splits][I][Jp], Jp = J rounded up to 4, when splits > 1
     long long low_a, low_b;   // TWO: elements from the operand that is dz to its low part, 0 for the other one
-    float low_scale, scale;   // TWO: factors of the low part's product and of the result
+    float low_scale, scale;   // TWO: factors of the low part's product and of the result,
+    const float* scale_at;    // the latter in memory where it comes from the values (or null)
     DnEpilogue e;
 };
 
@@ -588,7 +589,7 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
         }
         dn_handover<0>();                              // every wave has read the last step: the ring is free
         if constexpr (TWO) {
-            const float f = low ? p.low_scale : p.scale;
+            const float f = low ? p.low_scale : p.scale_at ? *p.scale_at : p.scale;
 #pragma unroll
             for (int i = 0; i < FI; ++i)
 #pragma unroll
@@ -772,13 +773,14 @@ __global__ void __launch_bounds__(64 * DN_FW) dense_few_rows_kernel(DnGemm p) {
         multiply(b[0], a[0]);
     }
     if constexpr (TWO) {
+        const float scale = p.scale_at ? *p.scale_at : p.scale;
 #pragma unroll
         for (int j = 0; j < JB; ++j)
 #pragma unroll
             for (int m = 0; m < MB; ++m)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    acc[j][m][r] = (acc[j][m][r] + acc_low[j][m][r] * p.low_scale) * p.scale;
+                    acc[j][m][r] = (acc[j][m][r] + acc_low[j][m][r] * p.low_scale) * scale;
     }
 #pragma unroll
     for (int j = 0; j < JB; ++j)
@@ -884,7 +886,9 @@ struct DnDz {
     float* sums;
     long long ldd, ldp, ldz, M, rows, row_blocks, blocks, low;    // low: elements from dz to its low part, or 0
     float scale, low_up;
-    int N, act, cg;
+    const float* most;        // largest |d_out| by the workgroups of dense_most_kernel, or null: `scale` is taken
+    float* back;              // where workgroup 0 leaves the inverse of the scale
+    int n_most, N, act, cg;
 };
 // the nearest value of T, and the rest of v times up (0 behind infinities and NaN; a finite v that rounds to an
 // infinity leaves the largest finite value and the rest)
@@ -895,10 +899,42 @@ __device__ __forceinline__ void dn_two(float v, float up, float& high, float& lo
     if (fabsf(v) < __builtin_inff()) high = fabsf(high) <= most ? high : __builtin_copysignf(most, v);
     low = fabsf(v) < __builtin_inff() ? (v - high) * up : 0.f;
 }
+// The largest finite |d_out|: a float32 gradient need not lie in float16's range, so for float16 it is brought there by
+// a power of two (of the largest value's exponent: 2^14 .. 2^15) that the products take off again.
+// At most 256 workgroups, each leaves one value.
+__global__ void __launch_bounds__(256) dense_most_kernel(const float* d_out, long long ldd, long long M, int N, float* most) {
+    __shared__ float part[4];
+    const long long pieces = (N + 7) / 8, step = (long long)gridDim.x * 256;
+    float m = 0.f;
+    for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < M * pieces; id += step) {
+        const long long r = dn_divide(id, pieces), c = 8 * (id - r * pieces), left = N - c;
+        float d[8];
+        dn_load<float, 8>(d_out + r * ldd + c, left > 8 ? 8 : (int)left, d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(d[e]) < __builtin_inff() ? fabsf(d[e]) : 0.f);
+    }
+    for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+    if (lane_id() == 0) part[wave_id()] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) most[blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+}
+
 template <typename T, typename D>
 __global__ void __launch_bounds__(256) dense_dz_kernel(DnDz p, DnPacks packs) {
-    __shared__ float part[4][32][9];
+    __shared__ float part[4][32][9], top[4];
     if ((long long)blockIdx.x >= p.blocks) return dn_pack_piece<T>(packs, blockIdx.x - p.blocks);
+    float scale = p.scale;
+    if (p.most) {
+        float m = (int)threadIdx.x < p.n_most ? p.most[threadIdx.x] : 0.f;
+        for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+        if (lane_id() == 0) top[wave_id()] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        int e = 14 + 127 - (int)(__float_as_uint(m) >> 23);          // below the normal range as at its end
+        e = m == 0.f ? 0 : e < 126 ? e : 126;
+        scale = __uint_as_float((unsigned)(127 + e) << 23);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *p.back = __uint_as_float((unsigned)(127 - e) << 23);
+    }
     const D* d_out = (const D*)p.d_out;
     const T* pre = (const T*)p.pre;
     T* dz = (T*)p.dz;
@@ -916,7 +952,7 @@ __global__ void __launch_bounds__(256) dense_dz_kernel(DnDz p, DnPacks packs) {
         if (dz && p.low) {
             float h[8], l[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dn_two<T>(v[e] * p.scale, p.low_up, h[e], l[e]);
+            for (int e = 0; e < 8; ++e) dn_two<T>(v[e] * scale, p.low_up, h[e], l[e]);
             dn_store<T, 8>(dz + r * p.ldz + col, 8, h);
             dn_store<T, 8>(dz + p.low + r * p.ldz + col, 8, l);
         } else if (dz) {
@@ -1172,7 +1208,7 @@ static size_t dn_up(size_t b) { return (b + 255) / 256 * 256; }
 
 // A matrix in memory as rows of `cols` values.  padded: its rows are whole pieces with zeros behind `cols`.
 // low: elements to the low part of a dz in two parts, scale and low_scale what undoes their factors
-struct DnMatrix { const void* p; long long rows, cols, ld; bool padded; long long low = 0; float scale = 1.f, low_scale = 1.f; };
+struct DnMatrix { const void* p; long long rows, cols, ld; bool padded; long long low = 0; float scale = 1.f, low_scale = 1.f; const float* scale_at = nullptr; };
 static long long dn_pieces(long long n) { return (n + 7) / 8; }
 // rows that start on 16 bytes, of whole 16-byte pieces
 static bool dn_whole(const DnMatrix& m) {
@@ -1220,7 +1256,7 @@ static DnGemm dn_arguments(const DnPlan& pl, const DnMatrix& a, bool akc, const 
     g.partial = pl.splits > 1 ? (float*)ws : nullptr;
     g.low_a = a.low; g.low_b = b.low;
     const DnMatrix& dz = a.low ? a : b;
-    g.scale = dz.scale; g.low_scale = dz.low_scale;
+    g.scale = dz.scale; g.low_scale = dz.low_scale; g.scale_at = dz.scale_at;
     g.e = e;
     return g;
 }
@@ -1276,8 +1312,10 @@ static size_t dn_copy_bytes(long long rows, long long cols, DnRows r) {
 }
 static size_t dn_copy_bytes(const DnMatrix& m) { return dn_whole(m) ? 0 : dn_pack_bytes(m.rows, m.cols); }
 
-// the backward's workspace: dz, its column sums, then what one product at a time needs
-struct DnBwdPlan { bool copy; long long ldz; int cg; long long rows, blocks; size_t dz_bytes, sum_bytes; };
+// the backward's workspace: both parts of dz, the largest |d_out| and the scale, the column sums, then what one product at
+// a time needs
+struct DnBwdPlan { bool copy; long long ldz; int cg; long long rows, blocks; size_t part_bytes, dz_bytes, sum_bytes; };
+constexpr int DN_MOST = 256;                           // workgroups of dense_most_kernel
 
 static DnBwdPlan dn_bwd_plan(long long M, int N, bool copy) {
     DnBwdPlan p{};
@@ -1302,7 +1340,8 @@ static DnBwdPlan dn_bwd_plan(long long M, int N, bool copy) {
         p.rows = walk * walks;
         p.blocks = (M + p.rows - 1) / p.rows;
     }
-    p.dz_bytes = copy ? 2 * dn_up((size_t)M * (size_t)p.ldz * 2) : 0;        // both parts
+    p.part_bytes = dn_up((size_t)M * (size_t)p.ldz * 2);
+    p.dz_bytes = copy ? 2 * p.part_bytes + dn_up((DN_MOST + 1) * 4) : 0;
     p.sum_bytes = p.blocks > 1 ? dn_up((size_t)p.blocks * (size_t)N * 4) : 0;
     return p;
 }
@@ -1349,12 +1388,12 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
     char* rest = ws + p.dz_bytes + p.sum_bytes;
     // d_out's values or 0 are dz where d_out has the products' type and act is none or ReLU; else dz is in two parts,
     // in float16 with the low part up by 2^11 (its own 11 bits also below the normal range) and both down by two (act'
-    // reaches 1.13: no overflow)
+    // reaches 1.13: no overflow), or by what brings a float32 d_out into range
     const bool two = dz && (d_dtype != dtype || act > FRCNN_ACT_RELU), f16 = dtype == FRCNN_DT_F16;
     const float scale = f16 ? 0.5f : 1.0f, low_up = f16 ? 2048.0f : 1.0f;
     DnMatrix z = dz ? DnMatrix{dz, M, N, p.ldz, true} : DnMatrix{d_out, M, N, ldd, false};
     if (two) {
-        z.low = (long long)(p.dz_bytes / 4);
+        z.low = (long long)(p.part_bytes / 2);
         z.scale = 1.0f / scale;
         z.low_scale = 1.0f / low_up;
     }
@@ -1362,12 +1401,21 @@ static int dn_backward(const void* d_out, long long ldd, int d_dtype, const void
     DnPacks packs;
     rc = dn_pack(d_x && !few ? &mw : nullptr, d_w ? &mx : nullptr, rest, packs);
     if (rc != FRCNN_OK) return rc;
+    float* most = two && f16 && d_dtype == FRCNN_DT_F32 ? reinterpret_cast<float*>(ws + 2 * p.part_bytes) : nullptr;
+    int n_most = 0;
+    if (most) {
+        z.scale_at = most + DN_MOST;
+        const long long blocks = (M * dn_pieces(N) + 255) / 256;
+        n_most = blocks < DN_MOST ? (int)blocks : DN_MOST;
+        FRCNN_LAUNCH(dense_most_kernel, dim3((unsigned)n_most), dim3(256), 0, s, (const float*)d_out, ldd, M, N, most);
+    }
     DnBiasGrad bias{};
     if (d_bias || dz) {
         DnDz q{};
         q.d_out = d_out; q.ldd = ldd; q.pre = pre; q.ldp = ldp; q.dz = dz; q.ldz = p.ldz;
         q.M = M; q.N = N; q.act = act; q.cg = p.cg; q.rows = p.rows; q.row_blocks = p.blocks;
         q.low = z.low; q.scale = scale; q.low_up = low_up;
+        q.most = most; q.n_most = n_most; q.back = most ? most + DN_MOST : nullptr;
         if (p.blocks == 1) q.d_bias = d_bias;
         else q.sums = d_bias ? reinterpret_cast<float*>(ws + p.dz_bytes) : nullptr;
         q.blocks = p.blocks * ((dn_pieces(N) + p.cg - 1) / p.cg);

@@ -124,6 +124,48 @@ def test_infinities_and_nan_reach_their_own_rows(dev):
             assert g["d_bias"].isnan().nonzero().flatten().tolist() == [1]
 
 
+@pytest.mark.parametrize("power", [-30, -20, -14, 12, 20])
+@pytest.mark.parametrize("M,K,N", [(20, 264, 100), (300, 203, 85), (2000, 1024, 264), (4097, 264, 2051)])
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_float32_gradients_outside_the_range_of_float16(dev, power, M, K, N, act):
+    """The gradients are in range (W and x make up for it as far as they can), d_out is not; infinities and zeros
+    in it do not move its scale."""
+    from objectdetection_amd import ops
+    x, w, d, pre = make(power + M, dev, M, K, N, torch.float16, "nk", torch.float32)
+    f = 2.0 ** max(-13, min(-power, 13))
+    x, w, d = (x.float() * f).half(), (w.float() * f).half(), d * 2.0 ** power
+    d[:, 1] = 0
+    g = ops.dense_bwd(d, x, w, None if act == "none" else pre, act)
+    dz = f64(d) * grad64(f64(pre), act)
+    for key, ref in (("d_x", dz @ f64(w).t()), ("d_weight", f64(x).t() @ dz)):
+        assert float(ref.abs().max()) < 60000
+        once = float((ref.half().double() - ref).norm())
+        assert float((f64(g[key]) - ref).norm()) <= 1.02 * once, key
+    d[3, 7] = math.inf
+    h = ops.dense_bwd(d, x, w, None if act == "none" else pre, act)
+    keep = torch.arange(M, device=dev) != 3
+    assert torch.equal(h["d_x"][keep], g["d_x"][keep]) and not h["d_x"][3].isfinite().any()
+    keep = torch.arange(N, device=dev) != 7
+    assert torch.equal(h["d_weight"][:, keep], g["d_weight"][:, keep])
+
+
+def test_a_scaled_gradient_gives_scaled_gradients(dev):
+    """A power of two in a float32 d_out is one in the results: the same bits, from float32's smallest values on."""
+    from objectdetection_amd import ops
+    x, w, d, _ = make(9, dev, 70, 96, 40, torch.float16, "kn", torch.float32)
+    ref = ops.dense_bwd(d, x, w)
+    for power in (-9, -5, 3):
+        g = ops.dense_bwd(d * 2.0 ** power, x, w)
+        for key in ("d_x", "d_weight"):
+            normal = ref[key].abs() >= 2.0 ** (-14 - min(power, 0))
+            assert torch.equal(g[key][normal].float(), ref[key][normal].float() * 2.0 ** power)
+    for up in (torch.zeros_like(d), torch.full_like(d, 2.0 ** -149)):
+        g = ops.dense_bwd(up, x, w)
+        assert not g["d_x"].any() and not g["d_weight"].any()
+    only = torch.full_like(d, math.nan)
+    assert ops.dense_bwd(only, x, w)["d_x"].isnan().all()
+
+
 @pytest.mark.parametrize("layout", ["kn", "nk"])
 def test_weight_gradients_lie_as_the_weights_do(dev, layout):
     from objectdetection_amd import ops

@@ -70,13 +70,67 @@ class RPNModel(nn.Module):
         return nhwc(f), nhwc(reg), nhwc(obj)
 
 
+class _GradRange:
+    """What one backward pass of a float16 head is scaled by: `up` and its inverse `down`, powers of two
+    on the device, set where the pass enters the head (_EnterHead) and taken off where it leaves it
+    (_To16)."""
+
+    SUM = 7                       # the rows' largest gradients add up to 2^7 .. 2^8 inside the head
+
+    def set(self, *grads: torch.Tensor) -> None:
+        """The sum bounds what a bias collects; a weight collects that many times its largest input,
+        far from float16's 65,504.  Spread evenly over 16,000 rows it is 2^-6 a row, 2^8 above
+        float16's normal range.  Sums of 256 values at a time stay inside a workgroup: no cleared counters
+        in a captured graph."""
+        rows = None
+        for g in grads:
+            m = g.float().abs().flatten(0, -2).amax(-1)
+            rows = m if rows is None else torch.maximum(rows, m)
+        if rows.numel() == 0:
+            rows = rows.new_zeros(1)
+        while rows.numel() > 1:
+            rows = nn.functional.pad(rows, (0, -rows.numel() % 256)).view(-1, 256).sum(-1)
+        e = (rows.view(torch.int32) >> 23 & 255) - 127      # the exponent, 128: not finite
+        k = torch.where(e < 128, (self.SUM - e).clamp(-100, 100), torch.zeros_like(e))
+        self.up, self.down = (((127 + n) << 23).view(torch.float32) for n in (k, -k))
+
+
+class _EnterHead(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, held, reg, cls):
+        ctx.held = held
+        return reg.view_as(reg), cls.view_as(cls)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_reg, g_cls):
+        ctx.held.set(g_reg, g_cls)
+        return None, g_reg * ctx.held.up, g_cls * ctx.held.up
+
+
+class _To16(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, held, t, dtype):
+        ctx.held, ctx.dtype = held, t.dtype
+        return t.to(dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        return None, (g.float() * ctx.held.down).to(ctx.dtype), None
+
+
 class FRCNModel(nn.Module):
     """construct_frcn (module/model.py:29-41) without its first layer (the 2x2 max-pool is fused
     into the crop): flatten (h,w,c) -> fc -> fc -> softmax classes, 4 x classes box deltas.
 
     dtype float16 / bfloat16: the four layers run on the fused dense kernels (module.model.dense)
     in that type, from the same float32 parameters; class logits and box deltas come out in
-    float32.  None (default): plain float32 modules."""
+    float32.  None (default): plain float32 modules.
+
+    The losses are means over thousands of rows, so the gradients between the layers would lie
+    below float16's normal range: a float16 head scales each backward pass by a power of two taken
+    from its upstream gradients and takes it off the float32 gradients again (bfloat16 has float32's range)."""
 
     def __init__(self, channels: int = 512, pooled: int = 7, hidden: int = 4096,
                  num_classes: int = 21, dtype: Optional[torch.dtype] = None):
@@ -89,23 +143,29 @@ class FRCNModel(nn.Module):
         self.cls = nn.Linear(hidden, num_classes)
         self.reg = nn.Linear(hidden, 4 * num_classes)
 
-    def _layer(self, m: nn.Linear, x: torch.Tensor, act: str, out_dtype=None) -> torch.Tensor:
+    def _to16(self, held: Optional[_GradRange], t: torch.Tensor) -> torch.Tensor:
+        return t.to(self.dtype) if held is None else _To16.apply(held, t, self.dtype)
+
+    def _layer(self, held, m: nn.Linear, x: torch.Tensor, act: str, out_dtype=None) -> torch.Tensor:
         from .module.model import dense
-        return dense(x, m.weight.to(self.dtype).t(), m.bias.to(self.dtype), act, out_dtype=out_dtype)
+        return dense(x, self._to16(held, m.weight).t(), self._to16(held, m.bias), act, out_dtype=out_dtype)
 
     def logits(self, pooled: torch.Tensor):
         """pooled [B,R,ph,pw,C] -> pred_reg [B,R,4K], class logits [B,R,K]."""
         B, R = pooled.shape[:2]
-        x = pooled.reshape(B * R, -1)
+        x = pooled.reshape(B * R, self.fc1.in_features)
         if self.dtype is None:
             x = torch.relu(self.fc2(torch.relu(self.fc1(x))))
             reg, cls = self.reg(x), self.cls(x)
         else:
-            x = self._layer(self.fc1, x.to(self.dtype), "relu")
-            x = self._layer(self.fc2, x, "relu")
-            reg = self._layer(self.reg, x, "none", torch.float32)
-            cls = self._layer(self.cls, x, "none", torch.float32)
-        return reg.reshape(B, R, -1), cls.reshape(B, R, -1)
+            held = _GradRange() if self.dtype == torch.float16 and torch.is_grad_enabled() else None
+            x = self._layer(held, self.fc1, self._to16(held, x), "relu")
+            x = self._layer(held, self.fc2, x, "relu")
+            reg = self._layer(held, self.reg, x, "none", torch.float32)
+            cls = self._layer(held, self.cls, x, "none", torch.float32)
+            if held is not None:
+                reg, cls = _EnterHead.apply(held, reg, cls)
+        return reg.reshape(B, R, self.reg.out_features), cls.reshape(B, R, self.cls.out_features)
 
     def forward(self, pooled: torch.Tensor):
         """pooled [B,R,ph,pw,C] -> pred_reg [B,R,4K], pred_obj [B,R,K]."""

@@ -129,7 +129,7 @@ __device__ __forceinline__ float ds_block(float v, float* sh) {
 }
 
 // ---- the teacher's side of a row -----------------------------------------------------------------------
-// LDS: per entry its label (-1: not there), t / T relative to the largest one, the student's logit there,
+// LDS: per entry its label (-1: not there), its logit, then that relative to the largest one and over T, the student's logit there,
 // and what its label gets: the sum of its entries' p, or a negative number where another entry of the label has
 // it; with more than 64 entries also a table of twice as many places or more, in which entries of a label meet
 constexpr int ds_slots(int k) {
@@ -151,14 +151,15 @@ __device__ __forceinline__ float ds_teacher_logit(const DsArgs& a, long long at)
     return a.t_f32 ? ((const float*)a.t)[at] : (float)((const T*)a.t)[at];
 }
 
-// label, t / T and the student's logit of the row's entries, by the whole workgroup; whether this wave met one
+// label, logit (as stored: dividing by T first would round what the maximum cancels, or overflow) and the student's
+// logit of the row's entries, by the whole workgroup; whether this wave met one
 template <typename T, int BLOCK>
-__device__ __forceinline__ bool ds_teacher_load(const DsArgs& a, long long row, DsTeacher e, float inv_t) {
+__device__ __forceinline__ bool ds_teacher_load(const DsArgs& a, long long row, DsTeacher e) {
     const T* z = (const T*)a.z + row * a.ldz;
     bool any = false;
     for (int j = threadIdx.x; j < a.k; j += BLOCK) {
         const int64_t i = a.idx[row * a.k + j];
-        const float t = ds_teacher_logit<T>(a, row * a.k + j) * inv_t;
+        const float t = ds_teacher_logit<T>(a, row * a.k + j);
         const bool there = i >= 0 && i < a.V && !(t == -__builtin_inff());
         e.label[j] = there ? (int)i : -1;
         e.t[j] = t;
@@ -169,14 +170,14 @@ __device__ __forceinline__ bool ds_teacher_load(const DsArgs& a, long long row, 
     }
     return __ballot(any) != 0;
 }
-// makes t relative to the largest one and returns the log of the sum of e^t, by one wave
-__device__ __forceinline__ float ds_teacher_sum(DsTeacher e, int k) {
+// makes t relative to the largest one, over T, and returns the log of the sum of e^t, by one wave
+__device__ __forceinline__ float ds_teacher_sum(DsTeacher e, int k, float inv_t) {
     const int lane = lane_id();
     float top = -__builtin_inff(), s = 0.f;
     for (int j = lane; j < k; j += 64) top = fmaxf(top, e.label[j] >= 0 ? e.t[j] : -__builtin_inff());
     top = ds_wave_max(top);
     for (int j = lane; j < k; j += 64) {
-        const float t = e.t[j] - top;
+        const float t = (e.t[j] - top) * inv_t;
         e.t[j] = t;
         if (e.label[j] >= 0) s += __builtin_amdgcn_exp2f(t * DS_LOG2E);
     }
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(256) distill_small_kernel(DsArgs a) {
     const int l = threadIdx.x & (G - 1), first = lane_id() & ~(G - 1);
     const long long row = (long long)blockIdx.x * (256 / G) + threadIdx.x / G;
     if (row >= a.rows) return;                         // whole groups of lanes leave
-    const float inv_t = 1.0f / a.temperature, ninf = -__builtin_inff();
+    const float inv_t = 1.0f / a.temperature, ninf = -__builtin_inff(), f = inv_t * DS_LOG2E;
     const float w = a.weight ? a.weight[row] : 1.0f;
     const bool mine = l < a.V;
     const float z = mine && w != 0.f ? (float)((const T*)a.z)[row * a.ldz + l] : ninf;
@@ -315,17 +316,17 @@ __global__ void __launch_bounds__(256) distill_small_kernel(DsArgs a) {
     float t = ninf;
     if (l < a.k) {
         const int64_t i = a.idx[row * a.k + l];
-        t = ds_teacher_logit<T>(a, row * a.k + l) * inv_t;
+        t = ds_teacher_logit<T>(a, row * a.k + l);
         if (i >= 0 && i < a.V && !(t == ninf)) label = (int)i;
     }
     const float top = ds_lanes<G, true>(label >= 0 ? t : ninf), m = ds_lanes<G, true>(z);
     const bool any = (__ballot(label >= 0) >> first & (~0ull >> (64 - G))) != 0;
-    const float te = label >= 0 ? __builtin_amdgcn_exp2f((t - top) * DS_LOG2E) : 0.f;
+    const float te = label >= 0 ? __builtin_amdgcn_exp2f((t - top) * f) : 0.f;
     const float ts = ds_lanes<G, false>(te);
-    const float s = ds_lanes<G, false>(mine ? __builtin_amdgcn_exp2f((z - m) * (inv_t * DS_LOG2E)) : 0.f);
+    const float s = ds_lanes<G, false>(mine ? __builtin_amdgcn_exp2f((z - m) * f) : 0.f);
     const bool part = w != 0.f && any;
     const float log_sum = logf(ts), log_s = logf(s);
-    const float log_p = t - top - log_sum, p = label >= 0 ? __builtin_amdgcn_exp2f(log_p * DS_LOG2E) : 0.f;
+    const float log_p = (t - top) * inv_t - log_sum, p = label >= 0 ? __builtin_amdgcn_exp2f(log_p * DS_LOG2E) : 0.f;
     const float zi = __shfl(z, first + (label >= 0 ? label : 0));
     if (FORWARD) {
         const float loss =
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DsArgs a) {
         if (G * e >= a.k) continue;
         const int j = l + G * e, at = j < a.k ? j : a.k - 1;
         const int64_t i = a.idx[row * a.k + at];
-        t[e] = ds_teacher_logit<T>(a, row * a.k + at) * inv_t;
+        t[e] = ds_teacher_logit<T>(a, row * a.k + at);
         if (j < a.k && i >= 0 && i < a.V && !(t[e] == ninf)) label[e] = (int)i;
     }
     DsVec<T> x[NV];
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DsArgs a) {
     m = ds_lanes<G, true>(m);
     float ts = 0.f, s = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) ts += label[e] >= 0 ? __builtin_amdgcn_exp2f((t[e] - top) * DS_LOG2E) : 0.f;
+    for (int e = 0; e < E; ++e) ts += label[e] >= 0 ? __builtin_amdgcn_exp2f((t[e] - top) * f) : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DsArgs a) {
     float loss = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const float log_p = t[e] - top - log_sum;
+        const float log_p = (t[e] - top) * inv_t - log_sum;
         p[e] = label[e] >= 0 ? __builtin_amdgcn_exp2f(log_p * DS_LOG2E) : 0.f;
         if (label[e] >= 0 && !(p[e] == 0.f)) loss += p[e] * (log_p - ((zi[e] - m) * inv_t - log_s));
     }
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
         x[i].load(z + v, a.V - v);
     }
     const DsTeacher e(ds_lds, a.k);
-    const bool some = ds_teacher_load<T, BLOCK>(a, row, e, inv_t);        // while the row arrives
+    const bool some = ds_teacher_load<T, BLOCK>(a, row, e);        // while the row arrives
     if (lane_id() == 0) sh_any[wave_id()] = some;
     float m = -__builtin_inff();
 #pragma unroll
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
     }
     float log_sum = 0.f;
     if (wave_id() == 0) {
-        log_sum = ds_teacher_sum(e, a.k);
+        log_sum = ds_teacher_sum(e, a.k, inv_t);
         if (tid == 0) sh_t = log_sum;
     }
     const float f = inv_t * DS_LOG2E;
@@ -626,7 +627,7 @@ __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
         }
     }
     const DsTeacher e(ds_lds, a.k);
-    const bool some = ds_teacher_load<T, BLOCK>(a, row, e, inv_t);
+    const bool some = ds_teacher_load<T, BLOCK>(a, row, e);
     if (lane_id() == 0) sh_any[wave_id()] = some;
     if constexpr (FORWARD) {
         if (wave_id() == 1) {                          // every workgroup joins the chunks in the same order
@@ -650,7 +651,7 @@ __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
     }
     float log_sum = 0.f;
     if (wave_id() == 0) {
-        log_sum = ds_teacher_sum(e, a.k);
+        log_sum = ds_teacher_sum(e, a.k, inv_t);
         if (tid == 0) sh_t = log_sum;
     }
     const float m = FORWARD ? sh_m : 0.f, s = FORWARD ? sh_s : 1.f, lse = FORWARD ? 0.f : a.lse_in[row];

@@ -470,10 +470,13 @@ int frcnn_dense_bwd(const void* d_out, int64_t ldd, int d_dtype, const void* x, 
  * has q = 0: the loss is +inf where the teacher gives that label weight; a row of -inf alone is NaN.
  *   dtype   of logits and d_logits: F32, F16 or BF16; t_dtype of top_values: dtype or F32;
  *   temperature  1e-18 .. 1e18;
- *   weight  [rows] or NULL (1);  loss, lse [rows] f32, lse = log sum_v e^(z_v / T) for the backward;
- *   frcnn_distill_loss: d_logits may be NULL, g = grad_scale; frcnn_distill_bwd: g = d_loss [rows].
+ *   weight  [rows] or NULL (1);  loss, lse [rows] f32, lse = log sum_v e^(z_v / T);
+ *   frcnn_distill_loss: d_logits may be NULL, g = grad_scale; frcnn_distill_bwd: g = d_loss [rows],
+ *   lse as the forward gave it (required; q is taken from the logits' own maximum and sum, as in
+ *   the forward: a float32 lse of large logits has lost what their differences need).
  * d_logits must not overlap logits.  The workspace (0 bytes for most sizes) joins the parts of few
- * or very long rows. */
+ * or very long rows; frcnn_distill_bwd_ws without one, which is frcnn_distill_bwd, reads such rows
+ * once more and takes up to twice as long. */
 size_t frcnn_distill_workspace_bytes(int64_t rows, int V, int k, int dtype);
 int frcnn_distill_loss(const void* logits, int64_t ldz, int dtype, const void* top_values,
                        int t_dtype, const int64_t* top_index, const float* weight, int64_t rows,
@@ -484,6 +487,11 @@ int frcnn_distill_bwd(const float* d_loss, const void* logits, int64_t ldz, int 
                       const void* top_values, int t_dtype, const int64_t* top_index,
                       const float* lse, const float* weight, int64_t rows, int V, int k,
                       float temperature, void* d_logits, int64_t ldg, frcnn_stream_t stream);
+int frcnn_distill_bwd_ws(const float* d_loss, const void* logits, int64_t ldz, int dtype,
+                         const void* top_values, int t_dtype, const int64_t* top_index,
+                         const float* lse, const float* weight, int64_t rows, int V, int k,
+                         float temperature, void* d_logits, int64_t ldg, void* workspace,
+                         size_t workspace_bytes, frcnn_stream_t stream);
 
 #ifdef __cplusplus
 }

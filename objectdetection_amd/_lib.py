@@ -94,6 +94,8 @@ _SIGS = {
                                 _i64, _p, _sz, _p]),
     "frcnn_distill_bwd": (_i, [_p, _p, _i64, _i, _p, _i, _p, _p, _p, _i64, _i, _i, _f, _p, _i64,
                                _p]),
+    "frcnn_distill_bwd_ws": (_i, [_p, _p, _i64, _i, _p, _i, _p, _p, _p, _i64, _i, _i, _f, _p, _i64,
+                                  _p, _sz, _p]),
 }
 
 for _name, (_res, _args) in _SIGS.items():

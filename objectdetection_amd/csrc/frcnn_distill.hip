@@ -8,14 +8,15 @@
 // (with w = 0 they are not read).
 //
 // All sums are float32, relative to the row's maximum; log q is kept as (z - max) / T - log(sum), so the
-// two large terms of z - lse never cancel.  The gradient is written as c q first and the few listed labels
-// are written again with their p subtracted; a label listed twice gets both.
+// two large terms of z - lse never cancel: the backward takes maximum and sum from the logits again instead of the
+// forward's lse, whose rounding would be in every q (2^-24 of lse: 2e-4 at logits of 1e4).  The gradient is written
+// as c q first and the few listed labels are written again with their p subtracted; a label listed twice gets both.
 //
 // Memory is the bound: a logit is read once and its gradient written once.  A row stays in registers, as it
 // lies in memory, between the three walks over it (maximum, sum, gradient): in those of a wave or a part of one
 // (up to 512 pieces of 16 bytes, 64 entries), of a workgroup (up to 16,384 pieces).  Longer rows, and few long
 // rows, are split: one launch leaves a maximum and a sum per chunk, a second one joins them in every workgroup
-// and writes the chunk's gradient.
+// and writes the chunk's gradient; in a backward without a workspace every workgroup walks its row itself.
 #include "frcnn_common.h"
 
 namespace frcnn {
@@ -29,11 +30,10 @@ struct DsArgs {
     const int64_t* idx;                  // [rows,k]
     const float* weight;                 // [rows] or null
     const float* d_loss;                 // [rows] or null: the backward's upstream gradient
-    const float* lse_in;                 // [rows]: the backward's
     float scale;                         // factor of the gradient when d_loss is null
     float temperature;
     long long rows; int V, k;
-    float* loss; float* lse; void* grad; long long ldg;
+    float* loss; float* lse; void* grad; long long ldg;      // loss and lse: null in the backward
     float2* part; int chunks, nv;        // maximum and sum of each chunk of a split row; its vectors per thread
 };
 
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(256) distill_small_kernel(DsArgs a) {
         if (__float_as_int(two.z) == l) listed += two.w;
     }
     const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale);
-    const float log_q = FORWARD ? (z - m) * inv_t - log_s : z * inv_t - a.lse_in[row];
+    const float log_q = (z - m) * inv_t - log_s;
     if (mine)
         ((T*)a.grad)[row * a.ldg + l] = (T)(part ? c * (__builtin_amdgcn_exp2f(log_q * DS_LOG2E) - listed) : 0.f);
 }
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DsArgs a) {
     if (row >= a.rows) return;                         // whole groups of lanes leave
     const float inv_t = 1.0f / a.temperature, ninf = -__builtin_inff(), f = inv_t * DS_LOG2E;
     const float w = a.weight ? a.weight[row] : 1.0f;
-    const float up = a.d_loss ? a.d_loss[row] : a.scale, lse = FORWARD ? 0.f : a.lse_in[row];
+    const float up = a.d_loss ? a.d_loss[row] : a.scale;
     const T* z = (const T*)a.z + row * a.ldz;
     int label[E];
     float t[E], zi[E];
@@ -439,8 +439,8 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DsArgs a) {
         if (!a.grad) return;
     }
     T* grad = (T*)a.grad + row * a.ldg;
-    const float c = w * a.temperature * up, cq = FORWARD ? c / s : c;
-    auto relative = [&](float v) { return __builtin_amdgcn_exp2f(FORWARD ? (v - m) * f : (v * inv_t - lse) * DS_LOG2E); };
+    const float c = w * a.temperature * up, cq = c / s;
+    auto relative = [&](float v) { return __builtin_amdgcn_exp2f((v - m) * f); };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         float q[W];
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DsArgs a) {
             sum[e] += i1 == label[e] ? two.w : 0.f;
         }
     }
-    const float scale = FORWARD ? 1.0f / s : 1.0f;
+    const float scale = 1.0f / s;
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if (label[e] >= 0) grad[label[e]] = (T)(c * (relative(zi[e]) * scale - sum[e]));
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
     T* grad = a.grad ? (T*)a.grad + row * a.ldg : nullptr;
     const float w = a.weight ? a.weight[row] : 1.0f, inv_t = 1.0f / a.temperature;
     if (w == 0.f) {
-        if (tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
+        if (tid == 0 && a.loss) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
         if (grad) ds_zero(grad, 0, a.V, tid, BLOCK);
         return;
     }
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
     m = ds_block<BLOCK, true>(m, sh_m);
     if constexpr (BLOCK == 64) __syncthreads();
     if (!ds_any<BLOCK>(sh_any)) {
-        if (tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
+        if (tid == 0 && a.loss) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
         if (grad) ds_zero(grad, 0, a.V, tid, BLOCK);
         return;
     }
@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
     if (grad) ds_listed_sums<BLOCK>(e, a.k, &sh_t, 0, a.V);
     s = ds_block<BLOCK, false>(s, sh_s);
     const float log_s = logf(s);
-    if (wave_id() == 0) {
+    if (wave_id() == 0 && a.loss) {
         const float l = ds_row_loss(a, e, log_sum, inv_t, m, log_s);
         if (tid == 0) {
             a.loss[row] = w * (a.temperature * a.temperature) * l;
@@ -563,8 +563,7 @@ __global__ void __launch_bounds__(BLOCK) distill_row_kernel(DsArgs a) {
 
 // ---- a chunk of a row per workgroup --------------------------------------------------------------------
 // of 4 vectors per thread, of one where the rows are few and their chunks would not fill the chip (one row of
-// 131,072 f32: 8.7 us for the two launches, latency of loads and sums).  The backward of every longer row is the
-// second launch alone: 1,027 x 32,003 f16 24 us, 5.5 TB/s
+// 131,072 f32: 8.7 us for the two launches, latency of loads and sums)
 constexpr int DS_CHUNK_BLOCK = 256;
 template <typename T, int BLOCK, int NV> constexpr int ds_chunk() { return BLOCK * NV * DsVec<T>::W; }
 
@@ -600,8 +599,8 @@ __global__ void __launch_bounds__(DS_CHUNK_BLOCK) distill_part_kernel(DsArgs a) 
     if (tid == 0) a.part[row * a.chunks + chunk] = float2{m, s};
 }
 
-// FORWARD: joins the row's partial sums; chunk 0 writes loss and lse; else q comes from the forward's lse
-template <typename T, bool FORWARD, int BLOCK, int NV>
+// joins the row's partial sums; in the forward chunk 0 writes loss and lse
+template <typename T, int BLOCK, int NV>
 __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
     extern __shared__ __attribute__((aligned(16))) char ds_lds[];
     __shared__ float sh_t, sh_m, sh_s;
@@ -614,7 +613,7 @@ __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
     const long long v0 = (long long)chunk * ds_chunk<T, BLOCK, NV>(), v1 = v0 + ds_chunk<T, BLOCK, NV>() < a.V ? v0 + ds_chunk<T, BLOCK, NV>() : a.V;
     const float w = a.weight ? a.weight[row] : 1.0f, inv_t = 1.0f / a.temperature;
     if (w == 0.f) {
-        if (FORWARD && chunk == 0 && tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
+        if (chunk == 0 && tid == 0 && a.loss) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
         if (grad) ds_zero(grad, v0, v1, tid, BLOCK);
         return;
     }
@@ -629,23 +628,21 @@ __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
     const DsTeacher e(ds_lds, a.k);
     const bool some = ds_teacher_load<T, BLOCK>(a, row, e);
     if (lane_id() == 0) sh_any[wave_id()] = some;
-    if constexpr (FORWARD) {
-        if (wave_id() == 1) {                          // every workgroup joins the chunks in the same order
-            float m = -__builtin_inff(), s = 0.f;
-            for (int c = lane_id(); c < a.chunks; c += 64) m = fmaxf(m, a.part[row * a.chunks + c].x);
-            m = ds_wave_max(m);
-            for (int c = lane_id(); c < a.chunks; c += 64) {
-                const float2 q = a.part[row * a.chunks + c];
-                const float d = q.x == m ? 0.f : q.x - m;      // also where both are infinite
-                s += q.y * __builtin_amdgcn_exp2f(d * (inv_t * DS_LOG2E));
-            }
-            s = ds_wave_sum(s);
-            if (lane_id() == 0) { sh_m = m; sh_s = m == -__builtin_inff() ? __builtin_nanf("") : s; }
+    if (wave_id() == 1) {                              // every workgroup joins the chunks in the same order
+        float m = -__builtin_inff(), s = 0.f;
+        for (int c = lane_id(); c < a.chunks; c += 64) m = fmaxf(m, a.part[row * a.chunks + c].x);
+        m = ds_wave_max(m);
+        for (int c = lane_id(); c < a.chunks; c += 64) {
+            const float2 q = a.part[row * a.chunks + c];
+            const float d = q.x == m ? 0.f : q.x - m;  // also where both are infinite
+            s += q.y * __builtin_amdgcn_exp2f(d * (inv_t * DS_LOG2E));
         }
+        s = ds_wave_sum(s);
+        if (lane_id() == 0) { sh_m = m; sh_s = m == -__builtin_inff() ? __builtin_nanf("") : s; }
     }
     __syncthreads();
     if (!ds_any<BLOCK>(sh_any)) {
-        if (FORWARD && chunk == 0 && tid == 0) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
+        if (chunk == 0 && tid == 0 && a.loss) { a.loss[row] = 0.f; a.lse[row] = 0.f; }
         if (grad) ds_zero(grad, v0, v1, tid, BLOCK);
         return;
     }
@@ -654,8 +651,8 @@ __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
         log_sum = ds_teacher_sum(e, a.k, inv_t);
         if (tid == 0) sh_t = log_sum;
     }
-    const float m = FORWARD ? sh_m : 0.f, s = FORWARD ? sh_s : 1.f, lse = FORWARD ? 0.f : a.lse_in[row];
-    if (FORWARD && chunk == 0 && wave_id() == 0) {
+    const float m = sh_m, s = sh_s;
+    if (chunk == 0 && wave_id() == 0 && a.loss) {
         const float log_s = logf(s), l = ds_row_loss(a, e, log_sum, inv_t, m, log_s);
         if (tid == 0) {
             a.loss[row] = w * (a.temperature * a.temperature) * l;
@@ -664,11 +661,9 @@ __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
     }
     if (!grad) return;
     ds_listed_sums<BLOCK>(e, a.k, &sh_t, v0, v1);
-    const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale), cq = FORWARD ? c / s : c;
+    const float c = w * a.temperature * (a.d_loss ? a.d_loss[row] : a.scale), cq = c / s;
     const float f = inv_t * DS_LOG2E;
-    auto relative = [&](float zi) {
-        return __builtin_amdgcn_exp2f(FORWARD ? (zi - m) * f : (zi * inv_t - lse) * DS_LOG2E);
-    };
+    auto relative = [&](float zi) { return __builtin_amdgcn_exp2f((zi - m) * f); };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const long long v = v0 + (tid + BLOCK * i) * W, left = a.V - v;
@@ -679,6 +674,82 @@ __global__ void __launch_bounds__(BLOCK) distill_chunk_kernel(DsArgs a) {
         x[i].store(grad + v, left > W ? W : (int)left);
     }
     __syncthreads();
+    ds_listed(e, a.k, c, grad, v0, v1, tid, BLOCK, [&](float zi) { return relative(zi) / s; });
+}
+
+// ---- the same backward without a workspace ---------------------------------------------------------------
+// There is nowhere to leave sums: every workgroup walks the whole row for them, 4 vectors per thread at a time with a
+// running maximum and the sum relative to it, and writes the gradient of its chunk, reading that again.  Bound by the
+// walk's latency where rows are few (one of 131,072 f32 15.6 us, 9 in two launches with a workspace; 64 of 131,072 bf16
+// 30 and 16), by memory else (2,048 of 131,072 f32 624 and 565).
+constexpr int DS_WALK_BLOCK = 512, DS_WALK_VECTORS = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(DS_WALK_BLOCK) distill_walk_kernel(DsArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char ds_lds[];
+    __shared__ float sh_t, sh_m[DS_WALK_BLOCK / 64], sh_s[DS_WALK_BLOCK / 64];
+    __shared__ int sh_any[DS_WALK_BLOCK / 64];
+    constexpr int W = DsVec<T>::W, BLOCK = DS_WALK_BLOCK, NV = DS_WALK_VECTORS;
+    const int tid = threadIdx.x;
+    const long long row = blockIdx.y, per = (long long)a.nv * (BLOCK * NV * W), v0 = blockIdx.x * per;
+    const long long v1 = v0 + per < a.V ? v0 + per : a.V;
+    const T* z = (const T*)a.z + row * a.ldz;
+    T* grad = (T*)a.grad + row * a.ldg;
+    const float w = a.weight ? a.weight[row] : 1.0f, inv_t = 1.0f / a.temperature, f = inv_t * DS_LOG2E;
+    if (w == 0.f) return ds_zero(grad, v0, v1, tid, BLOCK);
+    const DsTeacher e(ds_lds, a.k);
+    const bool some = ds_teacher_load<T, BLOCK>(a, row, e);
+    if (lane_id() == 0) sh_any[wave_id()] = some;
+    __syncthreads();
+    if (!ds_any<BLOCK>(sh_any)) return ds_zero(grad, v0, v1, tid, BLOCK);
+    if (wave_id() == 0) {
+        const float log_sum = ds_teacher_sum(e, a.k, inv_t);
+        if (tid == 0) sh_t = log_sum;
+    }
+    DsVec<T> x[NV];
+    auto load = [&](long long at, long long end) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const long long v = at + (tid + BLOCK * i) * W, left = end - v;
+            x[i].load(z + v, left > W ? W : (int)left);
+        }
+    };
+    // A maximum of -inf is taken as 0: nothing but -inf was met, and its sum is 0.
+    float m = -__builtin_inff(), s = 0.f;
+    for (long long at = 0; at < a.V; at += BLOCK * NV * W) {
+        load(at, a.V);
+        float top = m, part = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) top = fmaxf(top, x[i][j]);
+        const float base = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) part += __builtin_amdgcn_exp2f((x[i][j] - base) * f);
+        s = s * __builtin_amdgcn_exp2f((m - base) * f) + part;
+        m = top;
+    }
+    const float most = ds_block<BLOCK, true>(m, sh_m);
+    s = ds_block<BLOCK, false>(s * __builtin_amdgcn_exp2f(m == most ? 0.f : (m - most) * f), sh_s);
+    if (most == -__builtin_inff()) s = __builtin_nanf("");
+    ds_listed_sums<BLOCK>(e, a.k, &sh_t, v0, v1);
+    const float c = w * a.temperature * a.d_loss[row], cq = c / s;
+    auto relative = [&](float zi) { return __builtin_amdgcn_exp2f((zi - most) * f); };
+    for (long long at = v0; at < v1; at += BLOCK * NV * W) {
+        load(at, v1);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const long long v = at + (tid + BLOCK * i) * W, left = v1 - v;
+            float q[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) q[j] = cq * relative(x[i][j]);
+            x[i].set(q);
+            x[i].store(grad + v, left > W ? W : (int)left);
+        }
+    }
+    __syncthreads();                                   // the stores of c q come before those of the listed labels
     ds_listed(e, a.k, c, grad, v0, v1, tid, BLOCK, [&](float zi) { return relative(zi) / s; });
 }
 
@@ -716,7 +787,6 @@ static DsArgs ds_rows(const DsArgs& a, long long r, long long n) {
     b.idx = a.idx + r * a.k;
     if (a.weight) b.weight = a.weight + r;
     if (a.d_loss) b.d_loss = a.d_loss + r;
-    if (a.lse_in) b.lse_in = a.lse_in + r;
     if (a.loss) { b.loss = a.loss + r; b.lse = a.lse + r; }
     if (a.grad) b.grad = (T*)a.grad + r * a.ldg;
     if (a.part) b.part = a.part + r * a.chunks;
@@ -741,12 +811,17 @@ static int ds_launch_row(const DsArgs& a, hipStream_t s) {
                  s, a);
     return FRCNN_OK;
 }
-template <typename T, bool FORWARD, int BLOCK, int NV>
+template <typename T, int BLOCK, int NV>
 static int ds_launch_chunk(const DsArgs& a, hipStream_t s) {
-    if constexpr (FORWARD)
-        FRCNN_LAUNCH((distill_part_kernel<T, NV>), dim3((unsigned)a.chunks, (unsigned)a.rows), dim3(BLOCK), 0, s, a);
+    FRCNN_LAUNCH((distill_part_kernel<T, NV>), dim3((unsigned)a.chunks, (unsigned)a.rows), dim3(BLOCK), 0, s, a);
     const dim3 grid(a.grad ? (unsigned)a.chunks : 1u, (unsigned)a.rows);           // without a gradient: the loss alone
-    FRCNN_LAUNCH((distill_chunk_kernel<T, FORWARD, BLOCK, NV>), grid, dim3(BLOCK), ds_lds_bytes(a.k), s, a);
+    FRCNN_LAUNCH((distill_chunk_kernel<T, BLOCK, NV>), grid, dim3(BLOCK), ds_lds_bytes(a.k), s, a);
+    return FRCNN_OK;
+}
+template <typename T>
+static int ds_launch_walk(const DsArgs& a, hipStream_t s) {
+    FRCNN_LAUNCH(distill_walk_kernel<T>, dim3((unsigned)a.chunks, (unsigned)a.rows), dim3(DS_WALK_BLOCK), ds_lds_bytes(a.k),
+                 s, a);
     return FRCNN_OK;
 }
 
@@ -771,38 +846,38 @@ static int ds_run(const DsArgs& a, int dtype, hipStream_t s) {
     // a short row with more entries is one wave's up to 192 of them (16,384 x 1,000: with 100 entries 35 us, 50 by
     // four waves; with 1,000 entries 755 and 307)
     const bool one_wave = a.k <= 192;
-    if constexpr (FORWARD) {
-        if (!a.part) {
-            if (n <= 64 && one_wave) return ds_launch_row<T, 64, 1>(a, s);
-            if (n <= 256 && one_wave) return ds_launch_row<T, 64, 4>(a, s);
-            if (n <= 256) return ds_launch_row<T, 256, 1>(a, s);
-            if (n <= 1024) return ds_launch_row<T, 256, 4>(a, s);
-            if (n <= 2048) return ds_launch_row<T, 256, 8>(a, s);
-            if (n <= 4096) return ds_launch_row<T, 512, 8>(a, s);
-            if (n <= 8192) return ds_launch_row<T, 512, 16>(a, s);
-            return ds_launch_row<T, 1024, 16>(a, s);
-        }
-        return a.nv == 1 ? ds_launch_chunk<T, true, DS_CHUNK_BLOCK, 1>(a, s)
-                         : ds_launch_chunk<T, true, DS_CHUNK_BLOCK, 4>(a, s);
-    } else {
-        if (n <= 64 && one_wave) return ds_launch_chunk<T, false, 64, 1>(a, s);
-        if (n <= 256 && one_wave) return ds_launch_chunk<T, false, 64, 4>(a, s);
-        return a.nv == 1 || n <= DS_CHUNK_BLOCK ? ds_launch_chunk<T, false, DS_CHUNK_BLOCK, 1>(a, s)
-                                                : ds_launch_chunk<T, false, DS_CHUNK_BLOCK, 4>(a, s);
+    if (a.chunks) {
+        if (!a.part) return ds_launch_walk<T>(a, s);
+        return a.nv == 1 ? ds_launch_chunk<T, DS_CHUNK_BLOCK, 1>(a, s) : ds_launch_chunk<T, DS_CHUNK_BLOCK, 4>(a, s);
     }
+    if (n <= 64 && one_wave) return ds_launch_row<T, 64, 1>(a, s);
+    if (n <= 256 && one_wave) return ds_launch_row<T, 64, 4>(a, s);
+    if (n <= 256) return ds_launch_row<T, 256, 1>(a, s);
+    if (n <= 1024) return ds_launch_row<T, 256, 4>(a, s);
+    if (n <= 2048) return ds_launch_row<T, 256, 8>(a, s);
+    if (n <= 4096) return ds_launch_row<T, 512, 8>(a, s);
+    if (n <= 8192) return ds_launch_row<T, 512, 16>(a, s);
+    return ds_launch_row<T, 1024, 16>(a, s);
 }
 
 // a launch at a time: rows are the grid's second dimension where rows have chunks (65,535 at most), else
 // workgroups of up to 1,024 threads (fewer than 2^32 threads in a launch)
 template <bool FORWARD>
 static int ds_dispatch(DsArgs a, int dtype, hipStream_t s) {
-    const bool chunked = !ds_short(a.V, a.k, dtype) && (!FORWARD || ds_split(a.rows, a.V, dtype));
+    const bool chunked = !ds_short(a.V, a.k, dtype) && ds_split(a.rows, a.V, dtype);
     if (!chunked) a.part = nullptr;
-    a.nv = ds_chunk_vectors(a.rows, a.V, dtype);
-    a.chunks = (int)ds_chunks(a.rows, a.V, dtype);
-    const long long most = chunked ? 65535 : 1 << 21;
-    for (long long r = 0; r < a.rows; r += most) {
-        const long long n = a.rows - r < most ? a.rows - r : most;
+    if (chunked && a.part) {
+        a.nv = ds_chunk_vectors(a.rows, a.V, dtype);
+        a.chunks = (int)ds_chunks(a.rows, a.V, dtype);
+    } else if (chunked) {                              // nv: steps of the walk per chunk; up to 512 workgroups for few rows
+        const long long step = DS_WALK_BLOCK * DS_WALK_VECTORS, steps = (ds_vectors(a.V, dtype) + step - 1) / step;
+        const long long most = a.rows < 512 ? 512 / a.rows : 1;
+        a.nv = (int)((steps + most - 1) / most);
+        a.chunks = (int)((steps + a.nv - 1) / a.nv);
+    }
+    const long long at_once = chunked ? 65535 : 1 << 21;
+    for (long long r = 0; r < a.rows; r += at_once) {
+        const long long n = a.rows - r < at_once ? a.rows - r : at_once;
         const int rc = dtype == FRCNN_DT_F32   ? ds_run<float, FORWARD>(ds_rows<float>(a, r, n), dtype, s)
                        : dtype == FRCNN_DT_F16 ? ds_run<_Float16, FORWARD>(ds_rows<_Float16>(a, r, n), dtype, s)
                                                : ds_run<__bf16, FORWARD>(ds_rows<__bf16>(a, r, n), dtype, s);
@@ -854,16 +929,29 @@ extern "C" int frcnn_distill_loss(const void* logits, int64_t ldz, int dtype, co
     return ds_dispatch<true>(a, dtype, (hipStream_t)stream);
 }
 
+extern "C" int frcnn_distill_bwd_ws(const float* d_loss, const void* logits, int64_t ldz, int dtype,
+                                    const void* top_values, int t_dtype, const int64_t* top_index, const float* lse,
+                                    const float* weight, int64_t rows, int V, int k, float temperature,
+                                    void* d_logits, int64_t ldg, void* workspace, size_t workspace_bytes,
+                                    frcnn_stream_t stream) {
+    const int rc = ds_check(logits, ldz, dtype, top_values, t_dtype, top_index, rows, V, k, temperature);
+    if (rc != FRCNN_OK || rows == 0) return rc;
+    if (!d_loss || !lse || !d_logits || ldg < V) return FRCNN_E_BADARG;
+    const size_t need = frcnn_distill_workspace_bytes(rows, V, k, dtype);
+    if (workspace && need && (workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8))
+        return FRCNN_E_WORKSPACE;
+    DsArgs a{};
+    a.z = logits; a.ldz = ldz; a.t = top_values; a.idx = top_index; a.weight = weight; a.d_loss = d_loss;
+    a.temperature = temperature; a.rows = rows; a.V = V; a.k = k;
+    a.grad = d_logits; a.ldg = ldg; a.t_f32 = t_dtype == FRCNN_DT_F32;
+    a.part = (float2*)workspace;
+    return ds_dispatch<false>(a, dtype, (hipStream_t)stream);
+}
+
 extern "C" int frcnn_distill_bwd(const float* d_loss, const void* logits, int64_t ldz, int dtype,
                                  const void* top_values, int t_dtype, const int64_t* top_index, const float* lse,
                                  const float* weight, int64_t rows, int V, int k, float temperature, void* d_logits,
                                  int64_t ldg, frcnn_stream_t stream) {
-    const int rc = ds_check(logits, ldz, dtype, top_values, t_dtype, top_index, rows, V, k, temperature);
-    if (rc != FRCNN_OK || rows == 0) return rc;
-    if (!d_loss || !lse || !d_logits || ldg < V) return FRCNN_E_BADARG;
-    DsArgs a{};
-    a.z = logits; a.ldz = ldz; a.t = top_values; a.idx = top_index; a.weight = weight; a.d_loss = d_loss;
-    a.lse_in = lse; a.temperature = temperature; a.rows = rows; a.V = V; a.k = k;
-    a.grad = d_logits; a.ldg = ldg; a.t_f32 = t_dtype == FRCNN_DT_F32;
-    return ds_dispatch<false>(a, dtype, (hipStream_t)stream);
+    return frcnn_distill_bwd_ws(d_loss, logits, ldz, dtype, top_values, t_dtype, top_index, lse, weight, rows, V, k,
+                                temperature, d_logits, ldg, nullptr, 0, stream);
 }

@@ -901,9 +901,10 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_index: torc
 
 def distill_bwd(d_loss: torch.Tensor, logits: torch.Tensor, top_values: torch.Tensor,
                 top_index: torch.Tensor, lse: torch.Tensor, weight: Optional[torch.Tensor] = None,
-                temperature: float = 1.0) -> torch.Tensor:
-    """Gradient of distill_loss in logits for upstream gradients d_loss [...] (frcnn_distill_bwd);
-    lse [...] as distill_loss returned it."""
+                temperature: float = 1.0, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of distill_loss in logits for upstream gradients d_loss [...] (frcnn_distill_bwd_ws);
+    lse [...] as distill_loss returned it (the softmax is taken from the logits again, as precisely as
+    there).  workspace: uint8 of distill_workspace_bytes(rows, V, k, dtype)."""
     head, pw, lead, rows, V, k, dev, kept = _distill_args(logits, top_values, top_index, weight, temperature)
     for t, name in ((d_loss, "d_loss"), (lse, "lse")):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
@@ -914,6 +915,7 @@ def distill_bwd(d_loss: torch.Tensor, logits: torch.Tensor, top_values: torch.Te
             raise ValueError(f"{name} must be {list(lead)}")
     d_loss, lse = d_loss.contiguous(), lse.contiguous()
     grad = kept[0].new_empty(logits.shape)
-    _call("frcnn_distill_bwd", lib.frcnn_distill_bwd, dev, (
-        d_loss.data_ptr(), *head, lse.data_ptr(), pw, rows, V, k, temperature, grad.data_ptr(), V))
+    pws, nws, ws = _scratch(workspace, distill_workspace_bytes(rows, V, k, grad.dtype), grad, dev)
+    _call("frcnn_distill_bwd_ws", lib.frcnn_distill_bwd_ws, dev, (
+        d_loss.data_ptr(), *head, lse.data_ptr(), pw, rows, V, k, temperature, grad.data_ptr(), V, pws, nws))
     return grad

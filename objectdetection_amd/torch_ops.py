@@ -45,13 +45,13 @@ OP_ENTRY_POINTS = {
     "dense": ("frcnn_dense_fwd",),
     "dense_backward": ("frcnn_dense_bwd",),
     "distill_loss": ("frcnn_distill_loss",),
-    "distill_loss_backward": ("frcnn_distill_bwd",),
+    "distill_loss_backward": ("frcnn_distill_bwd_ws",),
 }
 HELPER_ENTRY_POINTS = (
     "frcnn_abi_version", "frcnn_status_string", "frcnn_set_tuning", "frcnn_get_tuning",
     "frcnn_topk_sort_workspace_bytes", "frcnn_nms_workspace_bytes", "frcnn_roi_fwd_workspace_bytes",
     "frcnn_roi_fwd_plan", "frcnn_topk_sort_plan", "frcnn_dense_fwd_workspace_bytes",
-    "frcnn_dense_bwd_workspace_bytes", "frcnn_distill_workspace_bytes",
+    "frcnn_dense_bwd_workspace_bytes", "frcnn_distill_workspace_bytes", "frcnn_distill_bwd",
     # stream-ordered halves / allocation-free variants used by RegionProposalPath and serving
     # loops directly; as operators they would be the ones above
     "frcnn_roi_fwd_prepare", "frcnn_roi_crop_pool_fwd_prepared", "frcnn_nms_static",

@@ -47,6 +47,19 @@ def make(seed, dev, rows, V, k, spread):
     return z.to(dev), t.to(dev), idx.to(dev)
 
 
+def without_workspace(g, z, t, idx, lse, w, T):
+    """frcnn_distill_bwd: rows that ops.distill_bwd splits with a workspace are walked instead."""
+    from objectdetection_amd import _lib
+    dts = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
+    (rows, V), k = z.shape, t.shape[1]
+    t, idx, g, lse = t.contiguous(), idx.contiguous(), g.contiguous(), lse.contiguous()
+    grad = torch.empty((rows, V), dtype=z.dtype, device=z.device)
+    assert _lib.lib.frcnn_distill_bwd(g.data_ptr(), z.data_ptr(), z.stride(0), dts[z.dtype], t.data_ptr(), dts[t.dtype], idx.data_ptr(),
+                                      lse.data_ptr(), None if w is None else w.data_ptr(), rows, V, k, T, grad.data_ptr(), V,
+                                      torch.cuda.current_stream().cuda_stream) == _lib.OK
+    return grad
+
+
 def check(got, ref, what):
     loss, grad, tol_l, tol_g = ref
     if "loss" in got:
@@ -89,3 +102,89 @@ def test_entries_of_the_lowest_value_are_entries(dev, V, k, name):
         got = ops.distill_loss(z, td, idx, temperature=T)
         check(got, reference(z, td, idx, T), T)
         assert (got["loss"][0] > 0) and got["loss"].isfinite().all()
+
+
+@pytest.mark.parametrize("rows,V,k", SHAPES + [(1, 70001, 64), (1, 131072, 5), (700, 17000, 3), (2, 300001, 1024), (513, 70001, 2)])
+@pytest.mark.parametrize("offset,T,spread", OFFSETS)
+def test_the_backward_is_as_precise_as_the_fused_gradient(dev, rows, V, k, offset, T, spread):
+    """The offset in the student's logits; both gradients are within the bounds, and each row of q sums to 1."""
+    from objectdetection_amd import ops
+    rows = min(rows, 40) if V > 5000 and rows < 200 else rows
+    z, t, idx = make(V + k, dev, rows, V, k, spread)
+    z = z + offset
+    got = ops.distill_loss(z, t, idx, temperature=T)
+    back = ops.distill_bwd(torch.ones(rows, device=dev), z, t, idx, got["lse"], temperature=T)
+    some = torch.arange(0, rows, max(1, rows // 40))                # the reference of all would take minutes
+    at = some.to(dev)
+    ref = reference(z[at], t[at], idx[at], T)
+    check({"loss": got["loss"][at], "d_logits": got["d_logits"][at]}, ref, (offset, T))
+    walk = without_workspace(torch.ones(rows, device=dev), z, t, idx, got["lse"], None, T)
+    for d in (back, walk):
+        check({"d_logits": d[at]}, ref, (offset, T, "backward"))
+        # sum_v (q_v - p_v) = 0: V roundings and the bounds above on either side
+        assert (d.double().sum(1).abs() <= T * (2.0 ** -20 * 30 + 2 * (V / 256 + k + 32) * 2.0 ** -23 + V * 2.0 ** -126)).all()
+
+
+@pytest.mark.parametrize("rows,V", [(1, 70001), (3, 40000), (2, 300001), (5, 131073)])
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("split", [True, False])
+def test_backward_of_long_rows(dev, rows, V, name, split):
+    """A row by one workgroup, by several, masked rows, rows without entries, -inf, NaN and +inf logits, strided rows, a captured
+    call; rows alone give what they give among others."""
+    from objectdetection_amd import ops
+    bwd = ops.distill_bwd if split else without_workspace
+    dt = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+    z, t, idx = make(V, dev, 600, V, 70, 2.0) if rows == 3 else make(V, dev, 30, V, 70, 2.0)
+    z, n = z.to(dt), z.shape[0]
+    w = torch.ones(n, device=dev)
+    idx[0, 3:9] = idx[0, :1]                       # a label listed often
+    g = torch.linspace(-1.0, 2.0, n, device=dev)
+    lse = torch.zeros(n, device=dev)
+    every = bwd(g, z, t, idx, lse, w, 1.5)
+    _, grad, _, tol = reference(z[:1], t[:1], idx[:1], 1.5)        # g[0] is -1
+    off = (every[:1].double().cpu() + grad).abs()
+    assert (off <= tol + torch.finfo(dt).eps / 2 * grad.abs() + (2.0 ** -25 if dt == torch.float16 else 1e-37)).all()
+    for r in range(0, n - rows, max(1, n // 4)):
+        s = slice(r, r + rows)
+        assert torch.allclose(bwd(g[s], z[s], t[s], idx[s], lse[s], w[s], 1.5).float(), every[s].float(),
+                              rtol=2 * torch.finfo(dt).eps, atol=2.0 ** -24)
+    z, t, idx, g, lse, w = z[:6].clone(), t[:6], idx[:6].clone(), g[:6], lse[:6], w[:6].clone()
+    w[0] = 0
+    z[0] = math.nan
+    idx[1] = -1
+    z[2, 7] = math.nan
+    z[3, 9] = math.inf
+    z[4] = -math.inf
+    z[5, ::2] = -math.inf
+    got = bwd(g, z, t, idx, lse, w, 1.5)
+    assert not got[:2].any()
+    for r in (2, 3, 4):
+        assert got[r].isnan().any()
+    assert got[5].isfinite().all()
+    wide = torch.zeros((6, V + 13), dtype=dt, device=dev)
+    wide[:, 5:5 + V] = z
+    same = lambda a, b: torch.equal(a.nan_to_num(nan=-77.0), b.nan_to_num(nan=-77.0))
+    assert same(bwd(g, wide[:, 5:5 + V], t, idx, lse, w, 1.5), got)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        held = bwd(g, z, t, idx, lse, w, 1.5)
+    for _ in range(3):
+        held.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(held, got)
+
+
+def test_the_backwards_workspace(dev):
+    from objectdetection_amd import ops
+    z, t, idx = make(1, dev, 3, 70001, 9, 2.0)
+    one = torch.ones(3, device=dev)
+    need = ops.distill_workspace_bytes(3, 70001, 9, torch.float32)
+    ws = torch.full((need + 256,), 255, dtype=torch.uint8, device=dev)
+    assert torch.equal(ops.distill_bwd(one, z, t, idx, one, workspace=ws[:need]), ops.distill_bwd(one, z, t, idx, one))
+    assert need > 0 and (ws[need:] == 255).all()
+    with pytest.raises(ValueError):
+        ops.distill_bwd(one, z, t, idx, one, workspace=ws[:need - 1])
+    with pytest.raises(RuntimeError):
+        ops.distill_bwd(one, z, t, idx, one, workspace=ws[4:need + 4])

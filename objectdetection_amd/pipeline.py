@@ -214,6 +214,10 @@ class RegionProposalPath:
             prop.wait_event(ready)
         elif inputs_ready is not None:
             main.wait_event(ready)                     # inputs may come from another stream
+            if self.train:
+                # the one set is in use until the caller's stream stands here: `ready` says nothing of that
+                ready = ev[0]
+                ready.record(main)
         if self.topk == "sort":
             check("frcnn_topk_sort", lib.frcnn_topk_sort(
                 _p(score), B, N, cfg.pre_k, _p(self.anchor), _p(coord), _p(d["top_scores"]),

@@ -99,9 +99,9 @@ def making_frcnn_input(gt_box: torch.Tensor, label: torch.Tensor, fmap: torch.Te
     [1,128].  For B == 1 the two agree; the joint branch for B >= 3 is not reproduced.
 
     cache=True (default) with counter keys (keys=None): the call runs on a buffer set kept per
-    (cfg, B, C, device), see process_fmap -- crop_fmap is overwritten by the next call of the same
-    dimensions, proposed / tindex by the one after it; the three gathered targets are new
-    tensors.  Injected keys (parity runs) and cache=False take the allocate-per-call route.
+    (cfg, B, C, device), see process_fmap -- crop_fmap, proposed and tindex are kept for what is
+    queued to read them before the next call of the same dimensions; the three gathered targets are
+    new tensors.  Injected keys (parity runs) and cache=False take the allocate-per-call route.
     """
     if anchor_box is None:
         raise ValueError("anchor_box is required (the reference reads an undefined global here)")

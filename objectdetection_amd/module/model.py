@@ -57,9 +57,9 @@ def process_fmap(fmap: torch.Tensor, score: torch.Tensor, coord: torch.Tensor,
 
     cache=True (default): the call runs on a buffer set kept per (cfg, B, C, device) --
     radix-sort top-k, NMS and band-resident RoI kernel with their workspaces, nothing allocated
-    per call.  The returned tensors belong to that set: `crop_fmap` is overwritten by the next
-    call with the same dimensions, `proposed` by the one after it; clone what must live longer
-    (pipeline.clear_path_cache() frees the sets).  `inputs_ready`: an event after which the inputs
+    per call.  The returned tensors belong to that set and are kept for what is queued to read
+    them before the next call with the same dimensions, on the stream of this call or of that one;
+    clone what must live longer (pipeline.clear_path_cache() frees the sets).  `inputs_ready`: an event after which the inputs
     may be read -- with it the proposals of this call are computed beside the RoI kernel of the
     call before.  cache=False allocates every output per call, as TensorFlow does.
     """

@@ -20,7 +20,9 @@ With `depth=2` consecutive batches are software-pipelined: stages 3-4 (latency-b
 dozen small launches) go to a proposal stream and write one of two buffer sets, so the
 proposals of batch i+1 are computed while the RoI kernel of batch i (bandwidth-bound, fills
 the chip) is still running on the caller's stream.  Results of a run() are valid on the
-caller's stream as before; the set they live in is reused two calls later.  The proposal
+caller's stream as before; reads of them are queued before the next call (on its stream or on
+that of the next call), for which they are kept although the set is rewritten two calls later.
+A call on another stream than the one before is ordered behind what that stream holds.  The proposal
 stream has normal priority on purpose: a high-priority stream in this wait pattern stopped
 making progress on MI355X (ROCm 7.2) once earlier streams of the process shared the hardware
 queues.
@@ -80,6 +82,7 @@ class RegionProposalPath:
         # the RoI geometry (frcnn_roi_fwd_prepare) is computed on the proposal stream right behind
         # the NMS, not in front of the RoI kernel (a stream of its own for it measured the same)
         self._calls = 0
+        self._last, self._order = None, torch.cuda.Event()   # the stream of the call before
         dev, B, N = self.device, batch, cfg.N
         f32, i32, i64, u8 = torch.float32, torch.int32, torch.int64, torch.uint8
         e = lambda shape, dt: torch.empty(shape, dtype=dt, device=dev)
@@ -191,6 +194,15 @@ class RegionProposalPath:
         if self.pooled is None and not skip_roi:
             raise ValueError("this path was built with alloc_pooled=False: call run(skip_roi=True)")
         main = torch.cuda.current_stream(self.device)
+        last = self._last
+        if (last is None or last.cuda_stream != main.cuda_stream) and \
+                not torch.cuda.is_current_stream_capturing():
+            # `pooled` and, one batch at a time, everything else is shared by all streams, and the
+            # call before and what was queued to read it are on its stream alone
+            if last is not None:
+                self._order.record(last)
+                main.wait_event(self._order)
+            self._last = main
         if self.depth == 2 and self._calls:
             # what the caller queued behind the call before may still read that call's results:
             # its set may be rewritten once the caller's stream has passed this point

@@ -1,5 +1,6 @@
-"""One batch at a time with inputs that are ready before the call: the training targets, which have a stream
-of their own, do not overwrite what the caller has queued to read of the call before."""
+"""What the caller has queued to read of a call is not overwritten: with one batch at a time and inputs that
+are ready before the call by the training targets, which have a stream of their own, and by calls made
+on another stream."""
 import numpy as np
 import pytest
 import torch
@@ -49,3 +50,37 @@ def test_late_reads_with_one_batch_at_a_time(dev):
         torch.cuda.synchronize()
         for i, (a, b) in enumerate(zip(got, ref)):
             assert all(torch.equal(x, y) for x, y in zip(a, b)), i
+
+
+@pytest.mark.parametrize("depth", [1, 2])
+def test_calls_on_two_streams_in_turn(dev, depth):
+    """The caller orders nothing between them, also through the function that keeps its buffers by itself."""
+    from objectdetection_amd import pipeline
+    from objectdetection_amd.module import process_fmap
+    cfg, data = batches(dev, 6)
+    ref = expected(cfg, data, dev)
+    path, got = pipeline.RegionProposalPath(cfg, 2, 32, dev, train=True, depth=depth), []
+    pipeline.clear_path_cache()
+    torch.cuda.synchronize()
+    ready = torch.cuda.Event()
+    ready.record()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i, x in enumerate(data):
+        with torch.cuda.stream(streams[i % 2]):
+            path.run(*x, seed=i, inputs_ready=ready)
+            torch.cuda._sleep(2_000_000)
+            got.append(results(path))
+    torch.cuda.synchronize()
+    for i, (a, b) in enumerate(zip(got, ref)):
+        assert all(torch.equal(x, y) for x, y in zip(a, b)), i
+    got = []
+    for i, (fmap, score, coord, _, _) in enumerate(data):
+        with torch.cuda.stream(streams[i % 2]):
+            crop, proposed = process_fmap(fmap, score, coord, path.anchor.view(cfg.H, cfg.W, cfg.A, 4), cfg, fuse_pool=True,
+                                          inputs_ready=ready)
+            torch.cuda._sleep(2_000_000)
+            got.append((crop.clone(), proposed.clone()))
+    torch.cuda.synchronize()
+    for i, ((crop, proposed), b) in enumerate(zip(got, ref)):
+        assert torch.equal(proposed, b[2]) and torch.equal(crop, b[5]), i
+    pipeline.clear_path_cache()

@@ -131,7 +131,7 @@ def read(path, names, stream):
 @pytest.mark.parametrize("depth", [1, 2])
 @pytest.mark.parametrize("train,rpn", [(True, True), (True, False), (False, False)])
 @pytest.mark.parametrize("given", [True, False])
-@pytest.mark.parametrize("streams", [1])
+@pytest.mark.parametrize("streams", [1, 2, 3])
 def test_every_two_uses_are_ordered(account, depth, train, rpn, given, streams):
     """Calls on one stream or on several in turn (which the caller does not order), with inputs that are ready
     from the start or where the caller's stream stands; the results are read before the next call, on the stream of the call."""
@@ -143,6 +143,19 @@ def test_every_two_uses_are_ordered(account, depth, train, rpn, given, streams):
         acc.current = callers[n % streams]
         path.run(*ins, seed=n, inputs_ready=ready if given else None)
         read(path, names, acc.current)
+
+
+@pytest.mark.parametrize("depth", [1, 2])
+def test_reads_on_the_next_calls_stream(account, depth):
+    """The results are read by the stream that makes the next call, which waits for the one before."""
+    acc, names = account
+    path, ins = build(names, depth=depth, train=True)
+    ready, callers = Event(), [acc.current, Stream()]
+    for n in range(7):
+        acc.current = callers[n % 2]
+        path.run(*ins, inputs_ready=ready)
+        callers[(n + 1) % 2].wait_stream(callers[n % 2])
+        read(path, names, callers[(n + 1) % 2])
 
 
 def test_the_account_sees_an_order_that_is_missing(account):

@@ -205,6 +205,8 @@ class HipPathOps:
         return dict(
             rpn_label=p.rpn["label"], rpn_pos=p.rpn["pos"], rpn_reg=p.rpn["reg"],
             proposed=p.proposed, tindex=ti,
+            # 1 for a RoI that the NMS kept, 0 for the zero boxes that fill the image's rows up
+            roi_weight=(torch.arange(cfg.post_n, device=ti.device) < p.keep_count[:, None]).float(),
             gt_label2=torch.gather(p.gt_onehot, 1, ti.unsqueeze(-1).expand(-1, -1, cfg.num_classes)),
             gt_mask2=torch.gather(p.gt_mask, 1, ti),
             gt_coord2=torch.gather(p.gt_coord, 1, ti.unsqueeze(-1).expand(-1, -1, 4)))
@@ -230,9 +232,11 @@ class HipPathOps:
                                           out["d_cls"], out["d_reg"].reshape(reg.shape))
         return two_cls, lreg, out["partial"][:, 2].sum()
 
-    def distill_loss(self, logits, top_values, top_index, temperature):
+    def distill_loss(self, logits, top_values, top_index, temperature, weight=None):
+        """The mean over the rows, each counted `weight` [B,R] times."""
         from .module.loss import distill_loss
-        return distill_loss(logits, top_values, top_index, None, temperature).mean()
+        loss = distill_loss(logits, top_values, top_index, weight, temperature)
+        return loss.mean() if weight is None else loss.sum() / weight.sum().clamp(min=1.0)
 
 
 class GradBuckets:
@@ -317,7 +321,8 @@ class TrainStep:
                  distill_k: int = 8, distill_temperature: float = 2.0, distill_weight: float = 1.0):
         """teacher: a trained head (its `logits(pooled)` is called without gradients) whose
         distill_k largest class logits per RoI the head also learns from: the mean distillation
-        loss at distill_temperature is added, times distill_weight."""
+        loss over the RoIs of all ranks (those the NMS kept, where the path's targets tell:
+        `roi_weight`) at distill_temperature is added, times distill_weight."""
         self.rpn, self.frcn, self.cfg, self.ops = rpn, frcn, cfg, path_ops
         self.teacher, self.distill_k = teacher, min(distill_k, cfg.num_classes)
         self.distill_temperature, self.distill_weight = distill_temperature, distill_weight
@@ -356,23 +361,27 @@ class TrainStep:
             with torch.no_grad():
                 _, t_logits = self.teacher.logits(pooled.detach())
                 top_values, top_index = torch.topk(t_logits.float(), self.distill_k, -1)
+            counted = (t["roi_weight"],) if "roi_weight" in t else ()
             distill = self.distill_weight * self.ops.distill_loss(
-                head_logits, top_values, top_index, self.distill_temperature)
+                head_logits, top_values, top_index, self.distill_temperature, *counted)
         head_cls2, head_reg, head_pos = self.ops.head_loss(head_cls_out, head_reg_out, t)
         # global normalisation: the class terms are means over world*B*S samples, the box terms
-        # means over the positives of ALL ranks
-        pos = torch.stack([rpn_pos, head_pos]).float()
+        # means over the positives of ALL ranks, the distillation one over all ranks' RoIs
+        pos = [rpn_pos, head_pos]
+        if distill is not None:
+            pos.append(counted[0].sum() if counted else torch.ones_like(head_pos))
+        pos = torch.stack([p.float() for p in pos])
         gpos = self._global(pos)
         w_reg = torch.where(gpos > 0, pos / gpos.clamp(min=1.0), torch.zeros_like(pos))
         local = (rpn_cls2 + head_cls2) / self.world + w_reg[0] * rpn_reg + w_reg[1] * head_reg
         if distill is not None:
-            local = local + distill / self.world
+            local = local + w_reg[2] * distill
         local.backward()
         self.buckets.finish()
         terms = [rpn_cls2 / self.world, w_reg[0] * rpn_reg, head_cls2 / self.world,
                  w_reg[1] * head_reg]
         if distill is not None:
-            terms.append(distill / self.world)
+            terms.append(w_reg[2] * distill)
         # [2*rpn_cls, rpn_reg, 2*head_cls, head_reg (, distillation)], global
         return self._global(torch.stack(terms).detach())
 

@@ -427,7 +427,7 @@ int frcnn_fc1_fwd(const float* x, const float* w, const float* bias, int64_t M, 
  * only `out` may be the residual (the same type, rows and stride).  A workspace serves one call at
  * a time: calls on two streams, or two captured graphs, have one each.
  * Activations: ReLU max(z, 0); GELU z Phi(z), Phi the normal distribution function (relative error
- * 1.3e-6); SiLU z / (1 + e^-z). */
+ * below 2e-6 as far as it is a normal number); SiLU z / (1 + e^-z). */
 #define FRCNN_DT_F32   0
 #define FRCNN_DT_F16   1
 #define FRCNN_DT_BF16  2

@@ -174,3 +174,67 @@ def test_weight_gradients_lie_as_the_weights_do(dev, layout):
         for act in ("none", "gelu"):
             g = ops.dense_bwd(d, x, w, pre, act)["d_weight"]
             assert g.shape == w.shape and g.stride() == w.stride()
+
+
+def test_a_strided_float32_gradient_and_a_dirty_workspace(dev):
+    """Between the rows of d_out, and in the workspace before the call, stand NaN and infinities."""
+    from objectdetection_amd import ops
+    for M, K, N in ((20, 264, 21), (300, 203, 85), (5000, 40, 84)):
+        x, w, d, pre = make(M, dev, M, K, N, torch.float16, "nk", torch.float32)
+        d = d * 1e-7
+        wide = torch.full((M, N + 11), math.inf, device=dev)
+        wide[:, 4] = math.nan
+        wide[:, 5:5 + N] = d
+        for act in ("none", "silu"):
+            z = None if act == "none" else pre
+            need = ops.dense_bwd_workspace_bytes(M, K, N, 1)
+            ws = torch.full((need + 256,), 255, dtype=torch.uint8, device=dev)
+            g, h = ops.dense_bwd(d, x, w, z, act), ops.dense_bwd(wide[:, 5:5 + N], x, w, z, act, workspace=ws[:need])
+            assert all(torch.equal(g[k], h[k]) for k in g) and (ws[need:] == 255).all() and g["d_x"].any()
+
+
+def test_captured_with_the_scale_of_each_replay(dev):
+    """A float16 layer's float32 gradient of another size in every replay; two graphs with a workspace each."""
+    from objectdetection_amd import ops
+    for M, K, N in ((700, 4096, 84), (24, 520, 21), (1111, 779, 333)):
+        x, w, d, pre = make(M, dev, M, K, N, torch.float16, "kn", torch.float32)
+        side, graphs = torch.cuda.Stream(), []
+        for _ in range(2):
+            side.wait_stream(torch.cuda.current_stream())
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                graphs.append((graph, ops.dense_bwd(d, x, w, pre, "silu")))
+        for f in (1.0, 1e-9, 3e5, 1e-4):
+            d.copy_(f * torch.randn_like(d))
+            for graph, _ in graphs:
+                graph.replay()
+            torch.cuda.synchronize()
+            want = ops.dense_bwd(d, x, w, pre, "silu")
+            assert all(torch.equal(got[k], want[k]) for _, got in graphs for k in want), f
+
+
+def test_parts_of_dz_beyond_4_gib(dev):
+    """600,000 rows of 4,096: each part of dz takes 4.9 GB."""
+    from objectdetection_amd import ops
+    M, K, N = 600_000, 8, 4096
+    g = torch.Generator(device=dev).manual_seed(2)
+    x = torch.randn((M, K), generator=g, device=dev).bfloat16()
+    w = torch.randn((K, N), generator=g, device=dev).bfloat16()
+    d = torch.randn((M, N), generator=g, device=dev, dtype=torch.bfloat16)
+    pre = torch.randn((M, N), generator=g, device=dev, dtype=torch.bfloat16)
+    got = ops.dense_bwd(d, x, w, pre, "silu")
+    dw, db = torch.zeros((K, N), dtype=torch.float64, device=dev), torch.zeros(N, dtype=torch.float64, device=dev)
+    for r in range(0, M, 50_000):
+        s = slice(r, r + 50_000)
+        z = pre[s].double()
+        q = torch.sigmoid(z)
+        dz = d[s].double() * q * (1 + z * (1 - q))
+        dw += x[s].double().t().contiguous() @ dz
+        db += dz.sum(0)
+        ref = dz[-3000:] @ w.double().t().contiguous()
+        once = float((ref.bfloat16().double() - ref).norm())
+        assert float((got["d_x"][r + 47_000:r + 50_000].double() - ref).norm()) <= 1.02 * once
+    # float32 sums of 600,000 terms: relative to the sums of their sizes 2^-24 a step of 32 and a slice, sqrt of their number
+    for key, ref in (("d_weight", dw), ("d_bias", db)):
+        once = float((ref.bfloat16().double() - ref).norm())
+        assert float((got[key].double() - ref).norm()) <= 1.02 * once + 2.0 ** -24 * math.sqrt(M / 32) * math.sqrt(M) * math.sqrt(ref.numel()), key

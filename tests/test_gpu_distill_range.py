@@ -188,3 +188,17 @@ def test_the_backwards_workspace(dev):
         ops.distill_bwd(one, z, t, idx, one, workspace=ws[:need - 1])
     with pytest.raises(RuntimeError):
         ops.distill_bwd(one, z, t, idx, one, workspace=ws[4:need + 4])
+
+
+def test_backward_of_rows_further_apart_than_32_bits(dev):
+    from objectdetection_amd import ops
+    for rows, V, ld in ((3, 70001, 1 << 31), (5, 40000, 1 << 30)):
+        z, t, idx = make(rows, dev, rows, V, 5, 2.0)
+        z = z.bfloat16()
+        buf = torch.empty(((rows - 1) * ld + V,), dtype=torch.bfloat16, device=dev)
+        far = torch.as_strided(buf, (rows, V), (ld, 1))
+        far.copy_(z)
+        g = torch.linspace(-1.0, 2.0, rows, device=dev)
+        for bwd in (ops.distill_bwd, without_workspace):
+            assert torch.equal(bwd(g, far, t, idx, g, None, 2.0), bwd(g, z, t, idx, g, None, 2.0))
+        del buf, far

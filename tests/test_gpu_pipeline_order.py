@@ -84,3 +84,27 @@ def test_calls_on_two_streams_in_turn(dev, depth):
     for i, ((crop, proposed), b) in enumerate(zip(got, ref)):
         assert torch.equal(proposed, b[2]) and torch.equal(crop, b[5]), i
     pipeline.clear_path_cache()
+
+
+def test_captures_between_calls_on_other_streams(dev):
+    """A path that has run on two streams is captured, replayed and run again."""
+    from objectdetection_amd.pipeline import RegionProposalPath
+    cfg, data = batches(dev, 3)
+    ref = expected(cfg, data, dev)
+    path = RegionProposalPath(cfg, 2, 32, dev, train=True, depth=1)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for i in range(2):
+        with torch.cuda.stream(streams[i]):
+            path.run(*data[i], seed=i)
+            torch.cuda._sleep(1_000_000)
+    graph = path.capture(*data[2], seed=2)
+    for i in (0, 1, 0):
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(results(path), ref[2]))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[i]):
+            path.run(*data[i], seed=i)
+            got = results(path)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, ref[i])), i

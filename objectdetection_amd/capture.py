@@ -5,7 +5,9 @@ uses the leaf was built, for as long as any such graph is alive.  A backward pas
 another stream meanwhile waits for that stream, which is not part of the capture: the capture is
 invalidated and the process ends inside the runtime.  guard_leaves notes the stream of the eager
 graphs that the differentiable functions of this package build on their leaves (also through a few
-views and casts, as `weight.to(dtype).t()`) and refuses the capture instead.
+views and casts, as `weight.to(dtype).t()`) and refuses the capture instead: when a graph is built
+during it, whether or not a backward follows (a forward alone is captured under torch.no_grad()).
+Graphs that other functions build on the same leaves are not seen.
 """
 from __future__ import annotations
 

@@ -362,8 +362,8 @@ __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&a
 // tiles do not cover: there it is 6 where a compute unit holds one workgroup (1,000 x 4,096 x 4,096 54 -> 47 us
 // with the same tiles, 2,000 x 4,096 x 4,096 77 -> 60; with more workgroups the room is better used by a second one:
 // 50,000 x 64 x 64 6.6 us, 8.2 with 6).  Eight cost another 1.2 us to fill.
-// What bounds it: the clock (1.83 GHz under this load) and the matrix cores, busy 75 to 84 % of its cycles.  8,192
-// cubed in bf16: 1,430 to 1,450 TFLOP/s with W as [N,K], 1,460 to 1,550 as Keras kernel, 1,445 to 1,550 for d_weight
+// What bounds it: the clock (1.83 GHz under this load) and the matrix cores, busy 74 (W as [N,K]) to 84 % (d_weight of
+// 16,000 x 25,088 x 4,096) of its cycles.  8,192 cubed in bf16: 1,430 to 1,450 TFLOP/s with W as [N,K], 1,460 to 1,550 as Keras kernel, 1,445 to 1,550 for d_weight
 // (from card to card).
 constexpr int DN_SK = 32;
 __device__ const __attribute__((aligned(16))) uint32_t dn_zeros[4] = {0, 0, 0, 0};
@@ -546,7 +546,7 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
         else dn_handover<0>();
         read(0, fa[0], fb[0]);
         int s = 0;
-        // whole steps, four at a time so that every LDS address is a constant; no branch inside
+        // whole steps, a ring's length at a time so that every LDS address is a constant; no branch inside
 #pragma unroll 1
         for (; s + 2 * RING < n; s += RING) {
 #pragma unroll
@@ -573,7 +573,7 @@ __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int 
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        // the last steps: up to eight, the last one maybe cut short
+        // the last steps: up to two rings' lengths, the last one maybe cut short
         auto step = [&](const dn_s16x8 (&ra)[FI], const dn_s16x8 (&rb)[FJ], dn_s16x8 (&na)[FI], dn_s16x8 (&nb)[FJ]) {
             if (s + 1 < n) {
                 if (s + RING - 1 >= n) dn_handover<0>();
@@ -637,8 +637,9 @@ dense_gemm_kernel(DnGemm p, int tiles) {
 // transposing LDS read in the wave's own LDS.  The eight sums are added in wave order.  The MFMA's k order is free as
 // long as both operands agree: lane group g takes k 16 g .. 16 g + 15 of a piece in two instructions (k contiguous),
 // or 8 g .. 8 g + 7 of each half.
-// One row x 4,096 x 4,096 bf16, W as [N,K]: 8.6 us, 3.9 TB/s; Keras kernel of 4,096 x 84: 9 us.  An outer-contiguous B
-// of 4,096 rows costs every workgroup all of its pages: 17 us at 4,096 x 4,096, half the rate.
+// One row x 4,096 x 4,096 bf16, W as [N,K]: 8.3 us, 4.0 TB/s; Keras kernel of 4,096 x 84: 8.6 us.  An outer-contiguous B
+// of 4,096 rows, read in half lines, comes at half the rate: 17.5 us at 4,096 x 4,096 (what holds it up is not known).
+// Both parts of a dz are multiplied against each load of B.
 constexpr int DN_FEW = 32, DN_FW = 8, DN_FS = 3;   // most rows; waves; pieces on their way
 
 template <typename T, bool BKC, int MB, bool TWO>
@@ -1079,9 +1080,10 @@ constexpr long long DN_MAX_LD = 1ll << 21;             // a tile's rows lie with
 static bool dn_grid(long long blocks, int threads) { return blocks * threads < 1ll << 32; }
 
 // Whether a product of I rows reads its operands as they are.  Large weights of whole pieces are left to the
-// tiles: the few rows' kernel reads half lines of an outer-contiguous B (1 x 4,096 x 4,096 as Keras kernel 17.4 us,
-// 13.0 by tiles; 1 x 25,088 x 4,096 59 and 42; 1 x 1,024 x 1,024 4.7 and 7.7), and A again for every 16 columns
-// (W as [N,K], 32 x 25,088 x 4,096: 86 us, 60 by tiles; 16 x 4,096 x 4,096: 11.8 and 15.7).
+// tiles: the few rows' kernel reads half lines of an outer-contiguous B (1 x 4,096 x 4,096 as Keras kernel 17.5 us,
+// 13.2 by tiles; 1 x 25,088 x 4,096 56 and 39; 1 x 1,024 x 1,024 4.6 and 8.0), and A again for every 16 columns
+// (W as [N,K], 32 x 25,088 x 4,096: 78 us, 43 by tiles; 16 x 25,088 x 4,096 54 and 42; 16 x 4,096 x 4,096 10.8 and 13.9).
+// Weights from memory, not from the last-level cache, in all of these.
 static bool dn_few(long long I, long long J, long long K, bool bkc, bool whole_b) {
     return I <= DN_FEW && !(whole_b && K <= DN_MAX_LD && (bkc ? I : 1) * J * K >= (bkc ? 1ll << 30 : 1ll << 23));
 }

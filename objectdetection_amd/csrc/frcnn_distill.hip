@@ -352,8 +352,9 @@ __global__ void __launch_bounds__(256) distill_small_kernel(DsArgs a) {
 }
 
 // ---- short rows with up to 64 entries: G lanes per row, NV pieces of 16 bytes per lane -------------------
-// What such a row costs is latency and issued instructions: several rows per wave, its entries and weight loaded
-// before anything is decided, no barrier.  1,000,000 x 21 f32 with 8 entries 83 us (156 with a lane per class),
+// What such a row costs is latency and issued instructions (1,000,000 x 21: vector instructions issue in 0.8 of the
+// cycles, memory at 3.0 TB/s): several rows per wave, its entries and weight loaded before anything is decided, no
+// barrier.  1,000,000 x 21 f32 with 8 entries 83 us (156 with a lane per class),
 // 300,000 x 91 bf16 50 us (203 with a workgroup per row), 100,000 x 1,203 f32 with 32 entries 190 us, 5.3 TB/s
 // (351).  The piece that would end behind the row is the row's last 16 bytes instead: what it
 // shares with its neighbour is left out of the sums and stored twice with the same value.

@@ -150,8 +150,12 @@ def dense(x: torch.Tensor, kernel: torch.Tensor, bias: Optional[torch.Tensor] = 
 
     x [..., K] or the pooled tensor [B,R,7,7,C]; kernel [K, units] in the Keras layout, or a
     Linear module's weight as `weight.t()` (read as it lies); activation "none", "relu", "gelu",
-    "silu"; out_dtype float32 for class logits.  fc1 is the float32 layer.  Under graph capture no
-    autograd graph of the same leaves that was built on another stream may be alive (refused)."""
+    "silu"; out_dtype float32 for class logits.  Gradients have their tensors' types: in float16
+    the loss has to be scaled (FRCNModel does it by itself).  fc1 is the float32 layer.
+
+    Under graph capture no autograd graph of the same leaves that this function (or distill_loss)
+    built on another stream may be alive: refused, also where only the forward is captured, unless
+    under torch.no_grad()."""
     held = guard_leaves(x, kernel, bias, residual)
     out = _Dense.apply(x, kernel, bias, residual, activation, out_dtype)
     del held

@@ -363,8 +363,8 @@ __device__ __forceinline__ void dn_write_out(const DnGemm& p, const dn_f32x4 (&a
 // with the same tiles, 2,000 x 4,096 x 4,096 77 -> 60; with more workgroups the room is better used by a second one:
 // 50,000 x 64 x 64 6.6 us, 8.2 with 6).  Eight cost another 1.2 us to fill.
 // What bounds it: the clock (1.83 GHz under this load) and the matrix cores, busy 74 (W as [N,K]) to 84 % (d_weight of
-// 16,000 x 25,088 x 4,096) of its cycles.  8,192 cubed in bf16: 1,430 to 1,450 TFLOP/s with W as [N,K], 1,460 to 1,550 as Keras kernel, 1,445 to 1,550 for d_weight
-// (from card to card).
+// 16,000 x 25,088 x 4,096) of its cycles.  8,192 cubed in bf16: 1,430 to 1,450 TFLOP/s with W as [N,K], 1,460 to 1,550
+// as Keras kernel, 1,445 to 1,550 for d_weight (from card to card).
 constexpr int DN_SK = 32;
 __device__ const __attribute__((aligned(16))) uint32_t dn_zeros[4] = {0, 0, 0, 0};
 
@@ -465,7 +465,8 @@ struct DnReader {
 // STAY: the workgroup takes tile `id` and every `stride`-th after it; the first copies of the next tile leave
 // before the results of this one are written, and arrive meanwhile.  `tiles`: tiles and slices in all.
 // TWO: the operand that is dz comes as the sum of two values of its type (dense_dz_kernel); the reduction is walked
-// twice over the same other operand, the low part first, with the sums in the same registers.
+// twice over the same other operand, the low part first, with the sums in the same registers (d_weight of 16,000 x
+// 4,096 x 4,096: 746 us, 1,440 TFLOP/s of the two products).
 template <typename T, bool AKC, bool BKC, int BI, int BJ, int WI, int WJ, int RING, bool FULL, bool STAY, bool TWO>
 __device__ __forceinline__ void dn_gemm(const DnGemm& p, int tiles, int id, int stride, char* dn_lds) {
     constexpr int NT = 64 * WI * WJ, FI = BI / WI / 16, FJ = BJ / WJ / 16;
@@ -879,12 +880,12 @@ __global__ void __launch_bounds__(256) dense_pack_kernel(DnPacks packs) {
 // ---- dz = d_out * act'(pre) and its column sums ---------------------------------------------------------
 // A workgroup takes `rows` rows of 8 * cg columns; a thread 8 neighbouring columns of every (256 / cg)-th
 // row.  dz (may be null) has rows of ldz elements, a multiple of 8; its columns N .. ldz-1 become 0.  Where dz is
-// no value of the type (GELU, SiLU, a float32 d_out) it is kept as the sum of two that are, for two products:
+// no value of the type (GELU, SiLU, a float32 d_out) it is kept as the sum of two that are:
 // scale dz = high + low / low_up with high the nearest value and low what is left of it.  That is 2^-16 relative
-// in bfloat16 and 2^-22 in float16 (2^-8 and 2^-11 in one value), and costs no more than its own two products.  The
-// sums of the unrounded values go to d_bias where one workgroup has all rows, else to `sums`, a row per
-// block of rows.  The workgroups behind the first `blocks` pack the products' operands.  16,000 x 84 bf16: 7 us;
-// 1,111 x 333 f16 with SiLU, packing 779 x 333 and 1,111 x 779: 8.5 us (latency both)
+// in bfloat16 and 2^-22 in float16, for twice the matrix operations; one value (2^-8 and 2^-11) makes the gradients
+// 1.4 times as wrong as their own rounding does.  The sums of the unrounded values go to d_bias where one workgroup
+// has all rows, else to `sums`, a row per block of rows.  The workgroups behind the first `blocks` pack the products'
+// operands.  16,000 x 84 bf16: 7 us; 1,111 x 333 f16 with SiLU, packing 779 x 333 and 1,111 x 779: 9 us (latency both)
 struct DnDz {
     const void *d_out, *pre;
     void *dz, *d_bias;
@@ -906,7 +907,7 @@ __device__ __forceinline__ void dn_two(float v, float up, float& high, float& lo
 }
 // The largest finite |d_out|: a float32 gradient need not lie in float16's range, so for float16 it is brought there by
 // a power of two (of the largest value's exponent: 2^14 .. 2^15) that the products take off again.
-// At most 256 workgroups, each leaves one value.
+// At most 256 workgroups, each leaves one value (16,000 x 21: 4.7 us, latency).
 __global__ void __launch_bounds__(256) dense_most_kernel(const float* d_out, long long ldd, long long M, int N, float* most) {
     __shared__ float part[4];
     const long long pieces = (N + 7) / 8, step = (long long)gridDim.x * 256;
@@ -1292,7 +1293,7 @@ static int dn_product(const DnPlan& pl, const DnMatrix& a, bool akc, const DnMat
 }
 
 // the plans of a backward's two products; whether they share a launch: both of small tiles, few enough workgroups to be
-// on the chip at once (1,111 x 779 x 333 f16 with SiLU: 21.8 us for the call; 29.1 one after the other)
+// on the chip at once (1,111 x 779 x 333 f16, dz in one part: 21.8 us for the call, 29.1 one after the other; 27.4 in two)
 struct DnPair { DnPlan x, w; bool together; };
 static DnPair dn_pair(int64_t M, int K, int N, bool kn, bool few) {
     DnPair p{dn_plan(M, K, N, true, kn, few), kn ? dn_plan(K, N, M, false, false, false) : dn_plan(N, K, M, false, false, false), false};
